@@ -82,6 +82,22 @@ class DecodeArgs(ctypes.Structure):
                 ("head_v_dim", _i64), ("scale", _dbl), ("params", ctypes.POINTER(LayerParams))]
 
 
+class GatedScanArgs(ctypes.Structure):
+    _fields_ = [("g", _fp), ("v", _fp), ("w", _fp), ("state_in", _fp), ("state_out", _fp), ("out", _fp),
+                ("cu_seqlens", _fp),
+                ("batch", _i64), ("num_heads", _i64), ("seq_len", _i64), ("head_v_dim", _i64), ("num_seqs", _i64),
+                ("g_per_head", ctypes.c_int32),
+                ("stride_g_b", _i64), ("stride_g_h", _i64), ("stride_g_t", _i64),
+                ("stride_vw_b", _i64), ("stride_vw_h", _i64), ("stride_vw_t", _i64),
+                ("stride_o_b", _i64), ("stride_o_h", _i64), ("stride_o_t", _i64),
+                ("workspace", _fp), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class GatedScanBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", GatedScanArgs), ("d_out", _fp), ("d_state_out", _fp), ("dg", _fp), ("dv", _fp), ("dw", _fp),
+                ("d_state0", _fp), ("workspace", _fp), ("workspace_bytes", ctypes.c_size_t)]
+
+
 class Config(ctypes.Structure):
     """gdn2_config (include/gdn2_layer.h) = Gdn2Config (src/config.rs:23-58)."""
     _fields_ = [("hidden_size", _i64), ("num_heads", _i64), ("head_dim", _i64), ("expand_v", ctypes.c_float),
@@ -104,6 +120,8 @@ EXPORTS = ("gdn2_last_error", "gdn2_hip_available", "gdn2_recurrent_step_f32", "
            "gdn2_stream_copy_f32", "gdn2_short_conv_f32", "gdn2_l2_normalize_f32", "gdn2_rms_norm_gate_f32",
            "gdn2_chunk_bwd_workspace_bytes", "gdn2_chunk_bwd_f32", "gdn2_chunk_fwd_train_f32",
            "gdn2_chunk_bwd_saved_f32", "gdn2_recurrent_bwd_workspace_bytes",
+           "gdn2_gated_scan_workspace_bytes", "gdn2_gated_scan_fwd_f32", "gdn2_gated_scan_fwd_bf16",
+           "gdn2_gated_scan_bwd_workspace_bytes", "gdn2_gated_scan_bwd_f32", "gdn2_gated_scan_bwd_bf16",
            "gdn2_recurrent_bwd_f32", "gdn2_decode_fused_f32",
            "gdn2_config_default", "gdn2_config_validate", "gdn2_config_dims", "gdn2_param_count",
            "gdn2_param_name", "gdn2_param_shape", "gdn2_param_init", "gdn2_layer_create", "gdn2_layer_destroy",
@@ -166,9 +184,19 @@ def lib():
         L.gdn2_chunk_bwd_workspace_bytes.restype = ctypes.c_size_t
         L.gdn2_recurrent_bwd_workspace_bytes.argtypes = [ctypes.POINTER(RecurrentBwdArgs)]
         L.gdn2_recurrent_bwd_workspace_bytes.restype = ctypes.c_size_t
+        _declare_mixer(L)
         _declare_layer(L)
         _lib = L
     return _lib
+
+
+def _declare_mixer(L):
+    for name, st in (("gdn2_gated_scan", GatedScanArgs), ("gdn2_gated_scan_bwd", GatedScanBwdArgs)):
+        fn = getattr(L, name + "_workspace_bytes")
+        fn.argtypes, fn.restype = [ctypes.POINTER(st)], ctypes.c_size_t
+        for ty in ("_f32", "_bf16"):
+            fn = getattr(L, (name if "_bwd" in name else name + "_fwd") + ty)
+            fn.argtypes, fn.restype = [ctypes.POINTER(st), ctypes.c_void_p], ctypes.c_int
 
 
 def _declare_layer(L):

@@ -1,0 +1,191 @@
+"""Operators of a gated recurrent mixer beside the GDN-2 layer, over the C ABI
+of include/gdn2_mixer.h (no reference counterpart):
+
+  gated_scan, gated_scan_backward   h_t = e^{g_t} h_{t-1} + w_t v_t per channel
+
+Tensors as in ops.py: [B, H, T, V] of any strides with contiguous channels, in
+float32 or bfloat16; log decays, states, weights and their gradients are
+float32.  A call runs on its tensors' device, on torch's current stream there;
+workspaces come from torch's allocator, so a call may be captured into a graph.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+
+from . import _capi as C
+
+_SUFFIX = {torch.float32: "_f32", torch.bfloat16: "_bf16"}
+
+
+def _p(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
+    """The device of every operand; TypeError off the GPU, ValueError for several devices."""
+    for t in (first, *others):
+        if t is not None:
+            if not t.is_cuda:
+                raise TypeError("gdn2_amd operators take device tensors")
+            if t.device != first.device:
+                raise ValueError("the operands are on several devices")
+    return first.device
+
+
+def _f32(name: str, t: Optional[torch.Tensor]) -> None:
+    if t is not None and t.dtype != torch.float32:
+        raise TypeError(f"{name} must be float32")
+
+
+def _call(fn, args, device: torch.device) -> None:
+    if torch.cuda.current_device() == device.index:
+        status = fn(ctypes.byref(args), torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(device):
+            status = fn(ctypes.byref(args), torch.cuda.current_stream().cuda_stream)
+    C.check(status)
+
+
+def _workspace(workspace: Optional[torch.Tensor], need: int, device: torch.device) -> Optional[torch.Tensor]:
+    if need == 0:
+        return workspace
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        return torch.empty(need, dtype=torch.uint8, device=device)
+    return workspace
+
+
+def _dense_rows(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy of it, with contiguous channels and no element of memory in
+    two places (what the gradients are laid out like)."""
+    if t.shape[-1] != 1 and t.stride(-1) != 1:
+        return t.contiguous()
+    if t.is_contiguous():
+        return t
+    span = 1
+    for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda x: x[1]):
+        if s < span:
+            return t.contiguous()
+        span = s * n
+    return t
+
+
+def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    return torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=t.device)
+
+
+def _in_layout(t: torch.Tensor, ref: torch.Tensor) -> torch.Tensor:
+    if t.stride() == ref.stride():
+        return t
+    return _empty_like(ref).copy_(t)
+
+
+# -- gated scan -----------------------------------------------------------------
+
+def _scan_check(g, v, w, state, cu_seqlens, more=()):
+    """The checks of both directions; the number of states."""
+    if v.dim() != 4:
+        raise ValueError("v must be [B, H, T, V]")
+    if v.dtype not in _SUFFIX:
+        raise TypeError("v must be float32 or bfloat16")
+    _f32("g", g)
+    if g.dim() != 4 or g.shape[:3] != v.shape[:3] or g.shape[3] not in (1, v.shape[3]):
+        raise ValueError("g must be [B, H, T, V] or [B, H, T, 1]")
+    for name, t in (("w", w), *more):
+        if t is not None and t.dtype != v.dtype:
+            raise TypeError(f"{name} must have v's type")
+        if t is not None and t.shape != v.shape:
+            raise ValueError(f"{name} must have v's shape")
+    n = v.shape[0]
+    if cu_seqlens is not None:
+        if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or not cu_seqlens.is_contiguous():
+            raise TypeError("cu_seqlens must be a contiguous int32 vector")
+        if v.shape[0] != 1:
+            raise ValueError("packed sequences need a batch of 1")
+        n = cu_seqlens.shape[0] - 1
+        if n < 0:
+            raise ValueError("cu_seqlens needs at least one offset")
+    _state_check("state", state, n, v)
+    return n
+
+
+def _state_check(name, state, n, v):
+    _f32(name, state)
+    if state is not None and tuple(state.shape) != (n, v.shape[1], v.shape[3]):
+        raise ValueError(f"{name} must be [{n}, H, V]")
+
+
+def _scan_args(g, v, w, state, new_state, out, cu_seqlens, n):
+    B, H, T, V = v.shape
+    sg, sv, so = g.stride(), v.stride(), out.stride()
+    return C.GatedScanArgs(_p(g), _p(v), _p(w), _p(state), _p(new_state), _p(out), _p(cu_seqlens), B, H, T, V, n,
+                           int(g.shape[3] != V or V == 1), sg[0], sg[1], sg[2], sv[0], sv[1], sv[2], so[0], so[1], so[2],
+                           None, 0)
+
+
+def _channels(t: torch.Tensor) -> torch.Tensor:
+    return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
+
+
+def gated_scan(g, v, w=None, state=None, cu_seqlens=None, out=None, new_state=None,
+               workspace=None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """h_t = e^{g_t} h_{t-1} + w_t v_t for every channel; returns (h [B, H, T, V],
+    the state after the last token [N, H, V]).
+
+    g [B, H, T, V], or [B, H, T, 1] for one log decay per head and token; w None
+    means 1, state None zeros.  With cu_seqlens (int32 on the device, N + 1 token
+    offsets) the one row of the batch holds N sequences, each with its own state;
+    rows of out outside all of them are left as they were.  Otherwise N = B.
+    T = 1 is the serving step.  `out` and `new_state` (which may be `state`) take
+    the results where given."""
+    n = _scan_check(g, v, w, state, cu_seqlens, (("out", out),))
+    _state_check("new_state", new_state, n, v)
+    dev = _device(v, g, w, state, cu_seqlens, out, new_state)
+    v, g = _channels(v), _channels(g)
+    if w is not None:
+        w = _in_layout(w, v)
+    if state is not None:
+        state = state.contiguous()
+    if out is None:
+        out = torch.empty_like(v)
+    if new_state is None:
+        new_state = torch.empty((n, v.shape[1], v.shape[3]), dtype=torch.float32, device=dev)
+    elif not new_state.is_contiguous() or (out.shape[3] != 1 and out.stride(3) != 1):
+        raise ValueError("new_state must be contiguous, and out's channels")
+    a = _scan_args(g, v, w, state, new_state, out, cu_seqlens, n)
+    L = C.lib()
+    if v.shape[2] > 8 or cu_seqlens is not None:  # (up to 8 tokens never need one)
+        workspace = _workspace(workspace, L.gdn2_gated_scan_workspace_bytes(ctypes.byref(a)), dev)
+        if workspace is not None:
+            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _call(L.gdn2_gated_scan_fwd_f32 if v.dtype == torch.float32 else L.gdn2_gated_scan_fwd_bf16, a, dev)
+    return out, new_state
+
+
+def gated_scan_backward(g, v, w, out, d_out, state=None, d_state=None, cu_seqlens=None, workspace=None) -> dict:
+    """The gradients of L = <d_out, out> + <d_state, new_state> for gated_scan's
+    arguments and its `out`: dict dg (g's shape), dv, dw (v's; dw None without w)
+    and dS0 (the state's gradient, also for state None).  Rows outside every
+    sequence of cu_seqlens have no gradient: dg, dv and dw are zero there."""
+    n = _scan_check(g, v, w, state, cu_seqlens, (("out", out), ("d_out", d_out)))
+    _state_check("d_state", d_state, n, v)
+    dev = _device(v, g, w, state, cu_seqlens, out, d_out, d_state)
+    v, g = _dense_rows(v), _dense_rows(g)
+    if w is not None:
+        w = _in_layout(w, v)
+    out = _channels(out)
+    d_out = _in_layout(d_out, out)
+    state = None if state is None else state.contiguous()
+    d_state = None if d_state is None else d_state.contiguous()
+    dg, dv, dw = _empty_like(g), _empty_like(v), None if w is None else _empty_like(v)
+    dS0 = torch.empty((n, v.shape[1], v.shape[3]), dtype=torch.float32, device=dev)
+    a = C.GatedScanBwdArgs(_scan_args(g, v, w, state, None, out, cu_seqlens, n), _p(d_out), _p(d_state), _p(dg), _p(dv),
+                           _p(dw), _p(dS0), None, 0)
+    L = C.lib()
+    workspace = _workspace(workspace, L.gdn2_gated_scan_bwd_workspace_bytes(ctypes.byref(a)), dev)
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _call(L.gdn2_gated_scan_bwd_f32 if v.dtype == torch.float32 else L.gdn2_gated_scan_bwd_bf16, a, dev)
+    return {"dg": dg, "dv": dv, "dw": dw, "dS0": dS0}

@@ -1,0 +1,117 @@
+"""The mixer operators without a GPU: their 64-bit forms against differences,
+and what they refuse."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import mixer_testutil as M
+
+
+@pytest.mark.parametrize("bounds", [None, [0, 3, 3, 7], [1, 4, 6]])
+@pytest.mark.parametrize("w", [False, True])
+def test_scan_gradients_against_differences(bounds, w):
+    """The plain backward against central differences of the plain forward."""
+    r = np.random.default_rng(3)
+    B, T, C = (1, 7, 2) if bounds else (2, 7, 2)
+    N = len(bounds) - 1 if bounds else B
+    x = {"g": -r.uniform(0.01, 1.5, (B, T, C)), "v": r.standard_normal((B, T, C)), "w": r.standard_normal((B, T, C)),
+         "h0": r.standard_normal((N, C))}
+    dy, ds = r.standard_normal((B, T, C)), r.standard_normal((N, C))
+
+    def loss(y):
+        h, last, _, _ = M.scan64(y["g"], y["v"] * (y["w"] if w else 1), y["h0"], bounds)
+        return np.nansum(h * dy) + (last * ds).sum()
+
+    h = M.scan64(x["g"], x["v"] * (x["w"] if w else 1), x["h0"], bounds)[0]
+    got, _ = M.scan_bwd64(x["g"], x["v"], x["w"] if w else None, h, dy, x["h0"], ds, bounds)
+    for name, key in (("g", "dg"), ("v", "dv"), ("w", "dw"), ("h0", "dS0")):
+        if name == "w" and not w:
+            continue
+        for i in np.ndindex(x[name].shape):
+            up, down = dict(x, **{name: x[name].copy()}), dict(x, **{name: x[name].copy()})
+            up[name][i] += 1e-6
+            down[name][i] -= 1e-6
+            d = (loss(up) - loss(down)) / 2e-6
+            assert abs(d - got[key][i]) <= 1e-7 * (1 + abs(d)), (name, i)
+
+
+def _scan_struct(**kw):
+    from gdn2_amd import _capi as C
+
+    a = C.GatedScanArgs()
+    for k, v in dict(g=256, v=256, out=256, batch=1, num_heads=2, seq_len=4, head_v_dim=8).items():
+        setattr(a, k, v)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_scan_refusals_of_the_c_entry():
+    """Invalid arguments come back as a status with a message, before any launch."""
+    from gdn2_amd import _capi as C
+
+    L = C.lib()
+    for fn in (L.gdn2_gated_scan_fwd_f32, L.gdn2_gated_scan_fwd_bf16):
+        assert fn(None, None) == C.GDN2_EINVAL
+        for bad in (dict(batch=-1), dict(seq_len=-1), dict(g=None), dict(v=None), dict(out=None),
+                    dict(cu_seqlens=256, num_seqs=2, batch=2), dict(num_seqs=-1), dict(seq_len=5000),
+                    dict(seq_len=5000, workspace=256, workspace_bytes=8),
+                    dict(seq_len=5000, workspace=264, workspace_bytes=1 << 40),
+                    dict(cu_seqlens=256, num_seqs=2)):
+            assert fn(ctypes.byref(_scan_struct(**bad)), None) == C.GDN2_EINVAL, bad
+            assert b"gdn2_gated_scan_fwd" in L.gdn2_last_error()
+        for big in (dict(seq_len=1 << 30), dict(num_heads=1 << 30), dict(head_v_dim=1 << 20, num_heads=1 << 20),
+                    dict(batch=1 << 29, head_v_dim=1 << 10), dict(batch=1 << 20, seq_len=1 << 20)):
+            assert fn(ctypes.byref(_scan_struct(**big)), None) == C.GDN2_NOT_APPLICABLE, big
+        for nothing in (dict(batch=0), dict(num_heads=0), dict(head_v_dim=0), dict(cu_seqlens=256, num_seqs=0)):
+            assert fn(ctypes.byref(_scan_struct(**nothing)), None) == C.GDN2_OK, nothing
+    for fn in (L.gdn2_gated_scan_bwd_f32, L.gdn2_gated_scan_bwd_bf16):
+        assert fn(None, None) == C.GDN2_EINVAL
+        b = C.GatedScanBwdArgs(_scan_struct(), 256, None, 256, 256, None, None, None, 0)
+        b.fwd.w = 256  # dw missing
+        assert fn(ctypes.byref(b), None) == C.GDN2_EINVAL
+        b.fwd.w, b.dw = None, 256  # dw without w
+        assert fn(ctypes.byref(b), None) == C.GDN2_EINVAL
+        b.dw, b.dv = None, None
+        assert fn(ctypes.byref(b), None) == C.GDN2_EINVAL
+        b.dv, b.fwd.seq_len = 256, 5000  # workspace missing
+        assert fn(ctypes.byref(b), None) == C.GDN2_EINVAL
+
+
+def test_scan_workspace_sizes():
+    from gdn2_amd import _capi as C
+
+    size = lambda **kw: C.lib().gdn2_gated_scan_workspace_bytes(ctypes.byref(_scan_struct(**kw)))  # noqa: E731
+    assert size(seq_len=1) == size(seq_len=8) == size(seq_len=0) == size(batch=0) == size(batch=-1) == 0
+    assert C.lib().gdn2_gated_scan_workspace_bytes(None) == 0 and C.lib().gdn2_gated_scan_bwd_workspace_bytes(None) == 0
+    assert 0 < size(seq_len=5000) <= 4 * 5000 * 16  # less than one operand
+    assert size(seq_len=5, cu_seqlens=256, num_seqs=1) >= 4 * 7
+
+
+def test_scan_refusals_in_python():
+    torch = pytest.importorskip("torch")
+    import gdn2_amd as G
+
+    v = torch.zeros(2, 3, 5, 8)
+    g1 = torch.zeros(2, 3, 5, 1)
+    st = torch.zeros(2, 3, 8)
+    cu = torch.tensor([0, 5], dtype=torch.int32)
+    for err, args, kw in [
+        (TypeError, (v, v), {}),  # not on a device
+        (TypeError, (v, v.half()), {}), (TypeError, (v.bfloat16(), v.bfloat16()), {}),
+        (ValueError, (v, v[0]), {}), (ValueError, (v[:, :, :4], v), {}), (ValueError, (torch.zeros(2, 3, 5, 2), v), {}),
+        (TypeError, (g1, v, v.bfloat16()), {}), (ValueError, (g1, v, v[:1]), {}),
+        (ValueError, (g1, v, None, st[:1]), {}), (TypeError, (g1, v, None, st.double()), {}),
+        (ValueError, (g1, v, None, None, cu), {}), (TypeError, (g1[:1], v[:1], None, None, cu.long()), {}),
+        (ValueError, (g1[:1], v[:1], None, st, cu), {}), (ValueError, (g1[:1], v[:1], None, None, cu[:0]), {}),
+        (ValueError, (g1, v), {"out": v[:1]}), (TypeError, (g1, v), {"out": v.bfloat16()}),
+        (ValueError, (g1, v), {"new_state": st[:1]}),
+    ]:
+        with pytest.raises(err):
+            G.gated_scan(*args, **kw)
+    for err, args, kw in [(TypeError, (g1, v, None, v, v), {}), (ValueError, (g1, v, None, v[:1], v), {}),
+                          (TypeError, (g1, v, None, v, v.bfloat16()), {}),
+                          (ValueError, (g1, v, None, v, v), {"d_state": st[:1]})]:
+        with pytest.raises(err):
+            G.gated_scan_backward(*args, **kw)
