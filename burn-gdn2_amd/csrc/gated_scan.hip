@@ -33,11 +33,10 @@
 
 #include "common.hpp"
 #include "gdn2_mixer.h"
+#include "vec_io.hpp"
 
 namespace gdn2 {
 namespace {
-
-typedef __bf16 bf16;
 
 constexpr unsigned kNaN = 0x7FC00000u;
 
@@ -62,26 +61,6 @@ struct GatedScanParams {
     unsigned *pre;           // [chain][tile][CH] final states
     unsigned long long *agg; // [chain][tile][CH] (G, X)
 };
-
-template <typename T, int N> struct Vec {
-    typedef T type __attribute__((ext_vector_type(N)));
-};
-// N consecutive values as they lie in memory; nothing waits for the load
-template <typename T, int N> using Raw = typename Vec<T, N>::type;
-template <typename T, int N> __device__ __forceinline__ Raw<T, N> raw_n(const T *p) {
-    return *reinterpret_cast<const Raw<T, N> *>(p);
-}
-template <typename T, int N> __device__ __forceinline__ void load_n(const T *p, float *x) {
-    const Raw<T, N> v = raw_n<T, N>(p);
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = (float)v[j];
-}
-template <typename T, int N> __device__ __forceinline__ void store_n(T *p, const float *x) {
-    Raw<T, N> v;
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = (T)x[j];
-    *reinterpret_cast<Raw<T, N> *>(p) = v;
-}
 
 // A token's decay in a register.  Sign bit set: expm1(g), for -0.34 < g <= 0, by
 // seven terms of its series (the rest is below 2^-26 of it).  Clear: e^g.

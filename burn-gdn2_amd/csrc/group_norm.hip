@@ -1,0 +1,827 @@
+// gdn2_group_norm_act_*: group norm over channels-last rows with an activation
+// (or an activated gate) in the same pass, and its adjoint.
+//   n = (x - mean) rstd,  z = n weight + bias,  y = act(z) or z act(gate)
+//   dz = dy act'(z) or dy act(gate),  dgate = dy z act'(gate),  dn = dz weight
+//   dx = rstd (dn - mean(dn) - n mean(dn n)),  dweight = sum dz n,  dbias = sum dz
+//
+// S = 1 (a token's heads): L lanes hold a group in registers, so that everything
+// is read once; the variance is taken about the mean.  Other groups are too large
+// for one wave: a first pass leaves sums for every channel and chunk of rows, a
+// second joins them, a third reads x again and writes.  Every sum runs in a
+// fixed order.
+//
+// Bound: HBM.
+#include <algorithm>
+#include <cmath>
+#include <exception>
+#include <string>
+
+#include "common.hpp"
+#include "gdn2_mixer.h"
+#include "vec_io.hpp"
+
+namespace gdn2 {
+namespace {
+
+struct GroupNormParams {
+    const void *x, *gate, *dy;
+    const float *weight, *bias;
+    void *y; // forward: y; backward: dx
+    void *dgate;
+    float *stats; // [N][G] (mean, rstd); forward: NULL if not wanted
+    float *dweight, *dbias;
+    float *part;  // see the kernels
+    float *sums;  // backward, S > 1: [N][G] means of dn and dn n
+    int64_t sxn, sxs, sgn, sgs;
+    int64_t N, S;
+    int C, G, D, act;
+    float eps;
+    int log_l;         // rows kernels: lanes a group, as a power of two
+    int row_blocks;    // backward rows kernel
+    int lc;            // tile kernels: lanes along the channels (a power of two)
+    int chunks, chunk; // row chunks of a sample, rows in one
+};
+
+__device__ __forceinline__ float sigmoid_f(float z) { return 1.f / (1.f + fast_exp2(-kLog2e * z)); }
+
+template <int N> __device__ __forceinline__ void act_n(int act, const float *z, float *a) {
+    if (act == GDN2_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) a[j] = z[j] * sigmoid_f(z[j]);
+    } else if (act == GDN2_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) a[j] = 0.5f * z[j] * (1.f + erff(z[j] * 0.70710678118654752f));
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) a[j] = z[j];
+    }
+}
+// a = act(z), d = act'(z)
+template <int N> __device__ __forceinline__ void act_grad_n(int act, const float *z, float *a, float *d) {
+    if (act == GDN2_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float s = sigmoid_f(z[j]);
+            a[j] = z[j] * s;
+            d[j] = s * __builtin_fmaf(z[j], 1.f - s, 1.f);
+        }
+    } else if (act == GDN2_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const float c = 0.5f * (1.f + erff(z[j] * 0.70710678118654752f));
+            a[j] = z[j] * c;
+            d[j] = __builtin_fmaf(z[j] * 0.3989422804014327f, fast_exp2(-0.5f * kLog2e * z[j] * z[j]), c);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) a[j] = z[j], d[j] = 1.f;
+    }
+}
+
+// Sum over the 2^log_l lanes of a group, to all of them.
+__device__ __forceinline__ float lanes_sum(float v, int log_l) {
+    for (int o = 1; o < 1 << log_l; o <<= 1) v += __shfl_xor(v, o, kWave);
+    return v;
+}
+
+// The place of a lane: VEC channels from c of the wave's groups, chunk k of NV.
+template <int VEC, int NV> struct Lanes {
+    int g, c[NV];
+    bool ok[NV];
+    __device__ Lanes(const GroupNormParams &p, int set, int lane) {
+        const int l = 1 << p.log_l;
+        g = set * (kWave >> p.log_l) + (lane >> p.log_l);
+        const int first = lane & (l - 1);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            const int e = (k * l + first) * VEC;
+            ok[k] = g < p.G && e < p.D; // (VEC divides D)
+            c[k] = ok[k] ? g * p.D + e : 0;
+        }
+    }
+};
+
+// S = 1.  A wave takes U rows at a time of its groups.
+template <typename T, int VEC, int NV, int U, bool GATE>
+__global__ __launch_bounds__(256) void norm_rows_kernel(GroupNormParams p) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Lanes<VEC, NV> at(p, blockIdx.y, lane);
+    const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * U;
+    if (n0 >= p.N) return;
+    Raw<T, VEC> rx[U][NV], rg[U][GATE ? NV : 1];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int64_t n = min(n0 + u, p.N - 1);
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            rx[u][k] = raw_n<T, VEC>(static_cast<const T *>(p.x) + n * p.sxn + at.c[k]);
+            if constexpr (GATE) rg[u][k] = raw_n<T, VEC>(static_cast<const T *>(p.gate) + n * p.sgn + at.c[k]);
+        }
+    }
+    float wt[NV][VEC], bs[NV][VEC];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) wt[k][j] = 1.f, bs[k][j] = 0.f;
+        if (p.weight) load_n<float, VEC>(p.weight + at.c[k], wt[k]);
+        if (p.bias) load_n<float, VEC>(p.bias + at.c[k], bs[k]);
+    }
+    const float inv_d = 1.f / p.D;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        float x[NV][VEC], sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                x[k][j] = at.ok[k] ? (float)rx[u][k][j] : 0.f;
+                sum += x[k][j];
+            }
+        const float mean = lanes_sum(sum, p.log_l) * inv_d;
+        float sq = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                x[k][j] -= mean;
+                sq = at.ok[k] ? __builtin_fmaf(x[k][j], x[k][j], sq) : sq;
+            }
+        const float rstd = 1.f / sqrtf(__builtin_fmaf(lanes_sum(sq, p.log_l), inv_d, p.eps));
+        const int64_t n = n0 + u;
+        if (n >= p.N) break;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float z[VEC], a[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) z[j] = __builtin_fmaf(x[k][j] * rstd, wt[k][j], bs[k][j]);
+            if constexpr (GATE) {
+                float gt[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) gt[j] = (float)rg[u][k][j];
+                act_n<VEC>(p.act, gt, a);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) a[j] *= z[j];
+            } else {
+                act_n<VEC>(p.act, z, a);
+            }
+            if (at.ok[k]) store_n<T, VEC>(static_cast<T *>(p.y) + n * p.sxn + at.c[k], a);
+        }
+        if (p.stats && at.g < p.G && (lane & ((1 << p.log_l) - 1)) == 0) {
+            p.stats[(n * p.G + at.g) * 2] = mean;
+            p.stats[(n * p.G + at.g) * 2 + 1] = rstd;
+        }
+    }
+}
+
+// S = 1, adjoint.  A wave walks rows wave, wave + 4, ... of its workgroup's
+// block of them and keeps dweight and dbias of its channels in registers; the
+// workgroup's go to part [row_blocks][2][C].
+template <typename T, int VEC, int NV, bool GATE>
+__global__ __launch_bounds__(256) void norm_rows_bwd_kernel(GroupNormParams p) {
+    __shared__ float red[2][4][kWave * VEC * NV];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Lanes<VEC, NV> at(p, blockIdx.y, lane);
+    const int64_t n0 = p.N * blockIdx.x / p.row_blocks, n1 = p.N * (blockIdx.x + 1) / p.row_blocks;
+    float wt[NV][VEC], bs[NV][VEC], dwt[NV][VEC], dbs[NV][VEC];
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) wt[k][j] = 1.f, bs[k][j] = dwt[k][j] = dbs[k][j] = 0.f;
+        if (p.weight) load_n<float, VEC>(p.weight + at.c[k], wt[k]);
+        if (p.bias) load_n<float, VEC>(p.bias + at.c[k], bs[k]);
+    }
+    const float inv_d = 1.f / p.D;
+    const int gs = min(at.g, p.G - 1);
+    struct Row {
+        Raw<T, VEC> x[NV], dy[NV], gate[GATE ? NV : 1];
+        float mean, rstd;
+    };
+    auto load = [&](int64_t n, Row &r) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            r.x[k] = raw_n<T, VEC>(static_cast<const T *>(p.x) + n * p.sxn + at.c[k]);
+            r.dy[k] = raw_n<T, VEC>(static_cast<const T *>(p.dy) + n * p.sxn + at.c[k]);
+            if constexpr (GATE) r.gate[k] = raw_n<T, VEC>(static_cast<const T *>(p.gate) + n * p.sgn + at.c[k]);
+        }
+        r.mean = p.stats[(n * p.G + gs) * 2];
+        r.rstd = p.stats[(n * p.G + gs) * 2 + 1];
+    };
+    Row next;
+    if (n0 + wave < n1) load(n0 + wave, next);
+    for (int64_t n = n0 + wave; n < n1; n += 4) {
+        const Row r = next;
+        load(min(n + 4, n1 - 1), next);
+        float nn[NV][VEC], dn[NV][VEC], s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float z[VEC], a[VEC], d[VEC], dz[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                nn[k][j] = ((float)r.x[k][j] - r.mean) * r.rstd;
+                z[j] = __builtin_fmaf(nn[k][j], wt[k][j], bs[k][j]);
+            }
+            if constexpr (GATE) {
+                float gt[VEC], dg[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) gt[j] = (float)r.gate[k][j];
+                act_grad_n<VEC>(p.act, gt, a, d);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    dg[j] = (float)r.dy[k][j] * z[j] * d[j];
+                    dz[j] = (float)r.dy[k][j] * a[j];
+                }
+                if (at.ok[k]) store_n<T, VEC>(static_cast<T *>(p.dgate) + n * p.sgn + at.c[k], dg);
+            } else {
+                act_grad_n<VEC>(p.act, z, a, d);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) dz[j] = (float)r.dy[k][j] * d[j];
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                dwt[k][j] = __builtin_fmaf(dz[j], nn[k][j], dwt[k][j]);
+                dbs[k][j] += dz[j];
+                dn[k][j] = dz[j] * wt[k][j];
+                s1 += at.ok[k] ? dn[k][j] : 0.f;
+                s2 = at.ok[k] ? __builtin_fmaf(dn[k][j], nn[k][j], s2) : s2;
+            }
+        }
+        s1 = lanes_sum(s1, p.log_l) * inv_d;
+        s2 = lanes_sum(s2, p.log_l) * inv_d;
+#pragma unroll
+        for (int k = 0; k < NV; ++k) {
+            float dx[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) dx[j] = r.rstd * (dn[k][j] - s1 - nn[k][j] * s2);
+            if (at.ok[k]) store_n<T, VEC>(static_cast<T *>(p.y) + n * p.sxn + at.c[k], dx);
+        }
+    }
+    if (!p.part) return;
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            red[0][wave][(k * VEC + j) * kWave + lane] = dwt[k][j];
+            red[1][wave][(k * VEC + j) * kWave + lane] = dbs[k][j];
+        }
+    __syncthreads();
+    if (wave == 0) {
+        float *out = p.part + (int64_t)blockIdx.x * 2 * p.C;
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+            if (at.ok[k]) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const int i = (k * VEC + j) * kWave + lane;
+                    out[at.c[k] + j] = (red[0][0][i] + red[0][1][i]) + (red[0][2][i] + red[0][3][i]);
+                    out[p.C + at.c[k] + j] = (red[1][0][i] + red[1][1][i]) + (red[1][2][i] + red[1][3][i]);
+                }
+            }
+    }
+}
+
+// dweight and dbias from the blocks' sums: part [blocks][2][C].  A workgroup
+// takes 16 columns (of 2 C), 16 threads a column.
+__global__ __launch_bounds__(256) void column_sum_kernel(const float *part, int64_t blocks, int C, float *dweight, float *dbias) {
+    __shared__ float red[16][17];
+    const int col = threadIdx.x & 15, r = threadIdx.x >> 4;
+    const int64_t i = (int64_t)blockIdx.x * 16 + col;
+    float sum = 0.f;
+    if (i < 2 * (int64_t)C)
+#pragma unroll 4
+        for (int64_t b = r; b < blocks; b += 16) sum += part[b * 2 * C + i];
+    red[r][col] = sum;
+    __syncthreads();
+    if (r == 0 && i < 2 * (int64_t)C) {
+        sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sum += red[k][col];
+        float *out = i < C ? dweight : dbias;
+        if (out) out[i < C ? i : i - C] = sum;
+    }
+}
+
+// A workgroup's tile of the general form: lc lanes of VEC channels, 256 / lc rows
+// at a time of a chunk of rows of sample n.
+template <int VEC> struct TileAt {
+    int c, rl, rows;
+    bool ok;
+    int64_t n, s0, s1;
+    __device__ explicit TileAt(const GroupNormParams &p) {
+        const int cl = threadIdx.x & (p.lc - 1);
+        rl = threadIdx.x / p.lc;
+        rows = 256 / p.lc;
+        c = (blockIdx.y * p.lc + cl) * VEC;
+        ok = c < p.C; // (VEC divides C)
+        c = ok ? c : 0;
+        n = blockIdx.x / p.chunks;
+        s0 = (int64_t)(blockIdx.x % p.chunks) * p.chunk;
+        s1 = min(s0 + p.chunk, p.S);
+    }
+};
+
+// Sums over a chunk's rows of a pair of values a channel: every thread's over
+// its rows are joined in LDS and go to part [N][chunks][2][C].
+template <int VEC, typename F>
+__device__ __forceinline__ void tile_pairs(const GroupNormParams &p, const TileAt<VEC> &at, const float *a, const float *b, F join) {
+    __shared__ float red[2][VEC][256];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        red[0][j][threadIdx.x] = a[j];
+        red[1][j][threadIdx.x] = b[j];
+    }
+    __syncthreads();
+    if (at.rl == 0 && at.ok) {
+        float *out = p.part + (int64_t)blockIdx.x * 2 * p.C + at.c;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            float x, y;
+            join(red[0][j], red[1][j], &x, &y);
+            out[j] = x;
+            out[p.C + j] = y;
+        }
+    }
+}
+
+// First pass, forward: the mean and the sum of squares about it of every channel
+// over the chunk's rows.  A thread sums about its first row's value, so that a
+// large mean costs no digits.
+template <typename T, int VEC> __global__ __launch_bounds__(256) void norm_moments_kernel(GroupNormParams p) {
+    const TileAt<VEC> at(p);
+    float first[VEC], sum[VEC], sq[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) first[j] = sum[j] = sq[j] = 0.f;
+    const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c;
+    int count = 0;
+    if (at.s0 + at.rl < at.s1) {
+        load_n<T, VEC>(x + (at.s0 + at.rl) * p.sxs, first);
+        count = 1;
+#pragma unroll 8
+        for (int64_t s = at.s0 + at.rl + at.rows; s < at.s1; s += at.rows) {
+            float v[VEC];
+            load_n<T, VEC>(x + s * p.sxs, v);
+            ++count;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                v[j] -= first[j];
+                sum[j] += v[j];
+                sq[j] = __builtin_fmaf(v[j], v[j], sq[j]);
+            }
+        }
+    }
+    const float inv = count ? 1.f / count : 0.f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) { // mean, and squares about it
+        const float m = sum[j] * inv;
+        sq[j] = fmaxf(__builtin_fmaf(-m, sum[j], sq[j]), 0.f);
+        sum[j] = first[j] + m;
+    }
+    const int64_t total = at.s1 - at.s0;
+    tile_pairs<VEC>(p, at, sum, sq, [&](const float *m, const float *q, float *mean, float *m2) {
+        const int cl = threadIdx.x & (p.lc - 1);
+        float s = 0.f;
+        for (int r = 0; r < at.rows; ++r) {
+            const int64_t k = (total - r + at.rows - 1) / at.rows; // rows of thread r
+            if (k > 0) s += (float)k * (m[r * p.lc + cl] - m[cl]);
+        }
+        *mean = m[cl] + s / (float)total;
+        float t = 0.f;
+        for (int r = 0; r < at.rows; ++r) {
+            const int64_t k = (total - r + at.rows - 1) / at.rows;
+            const float d = m[r * p.lc + cl] - *mean;
+            if (k > 0) t += q[r * p.lc + cl] + (float)k * d * d;
+        }
+        *m2 = t;
+    });
+}
+
+__device__ __forceinline__ float block_sum(float v, float *red) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// Second pass, forward: a group's mean and rstd from its channels' and chunks'.
+__global__ __launch_bounds__(256) void norm_join_kernel(GroupNormParams p) {
+    __shared__ float red[4];
+    const int64_t n = blockIdx.x / p.G;
+    const int g = (int)(blockIdx.x % p.G), entries = p.chunks * p.D;
+    const float *part = p.part + n * p.chunks * 2 * p.C + g * p.D;
+    auto rows = [&](int k) { return (float)min((int64_t)p.chunk, p.S - (int64_t)k * p.chunk); };
+    const float base = part[0]; // a mean to sum about
+    float s = 0.f;
+    for (int i = threadIdx.x; i < entries; i += 256) {
+        const int k = i / p.D;
+        s += rows(k) * (part[(int64_t)k * 2 * p.C + i % p.D] - base);
+    }
+    const float size = (float)p.S * (float)p.D;
+    const float mean = base + block_sum(s, red) / size;
+    float t = 0.f;
+    for (int i = threadIdx.x; i < entries; i += 256) {
+        const int k = i / p.D;
+        const float *e = part + (int64_t)k * 2 * p.C + i % p.D;
+        const float d = e[0] - mean;
+        t += e[p.C] + rows(k) * d * d;
+    }
+    const float var = block_sum(t, red) / size;
+    if (threadIdx.x == 0) {
+        p.stats[blockIdx.x * 2] = mean;
+        p.stats[blockIdx.x * 2 + 1] = 1.f / sqrtf(var + p.eps);
+    }
+}
+
+template <int VEC> struct Channels {
+    float mean[VEC], rstd[VEC], wt[VEC], bs[VEC];
+    __device__ Channels(const GroupNormParams &p, int64_t n, int c) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const int64_t g = n * p.G + (c + j) / p.D;
+            mean[j] = p.stats[g * 2];
+            rstd[j] = p.stats[g * 2 + 1];
+            wt[j] = 1.f;
+            bs[j] = 0.f;
+        }
+        if (p.weight) load_n<float, VEC>(p.weight + c, wt);
+        if (p.bias) load_n<float, VEC>(p.bias + c, bs);
+    }
+};
+
+// Third pass, forward.
+template <typename T, int VEC, bool GATE> __global__ __launch_bounds__(256) void norm_apply_kernel(GroupNormParams p) {
+    const TileAt<VEC> at(p);
+    if (!at.ok) return;
+    const Channels<VEC> ch(p, at.n, at.c);
+    const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c;
+    const T *gate = static_cast<const T *>(p.gate) + at.n * p.sgn + at.c;
+    T *y = static_cast<T *>(p.y) + at.n * p.sxn + at.c;
+#pragma unroll 4
+    for (int64_t s = at.s0 + at.rl; s < at.s1; s += at.rows) {
+        float z[VEC], a[VEC];
+        load_n<T, VEC>(x + s * p.sxs, z);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) z[j] = __builtin_fmaf((z[j] - ch.mean[j]) * ch.rstd[j], ch.wt[j], ch.bs[j]);
+        if constexpr (GATE) {
+            float gt[VEC];
+            load_n<T, VEC>(gate + s * p.sgs, gt);
+            act_n<VEC>(p.act, gt, a);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) a[j] *= z[j];
+        } else {
+            act_n<VEC>(p.act, z, a);
+        }
+        store_n<T, VEC>(y + s * p.sxs, a);
+    }
+}
+
+// One element's adjoint up to dz and n.
+template <typename T, int VEC, bool GATE>
+__device__ __forceinline__ void dz_n(const GroupNormParams &p, const Channels<VEC> &ch, const float *x, const float *dy,
+                                     const float *gt, float *n, float *dz, float *dg) {
+    float z[VEC], a[VEC], d[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        n[j] = (x[j] - ch.mean[j]) * ch.rstd[j];
+        z[j] = __builtin_fmaf(n[j], ch.wt[j], ch.bs[j]);
+    }
+    act_grad_n<VEC>(p.act, GATE ? gt : z, a, d);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        dz[j] = dy[j] * (GATE ? a[j] : d[j]);
+        if constexpr (GATE) dg[j] = dy[j] * z[j] * d[j];
+    }
+}
+
+// First pass, adjoint: sums of dz n and dz of every channel over the chunk's rows.
+template <typename T, int VEC, bool GATE> __global__ __launch_bounds__(256) void norm_bwd_sums_kernel(GroupNormParams p) {
+    const TileAt<VEC> at(p);
+    const Channels<VEC> ch(p, at.n, at.c);
+    const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c;
+    const T *dy = static_cast<const T *>(p.dy) + at.n * p.sxn + at.c;
+    const T *gate = static_cast<const T *>(p.gate) + at.n * p.sgn + at.c;
+    float a[VEC], b[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) a[j] = b[j] = 0.f;
+#pragma unroll 4
+    for (int64_t s = at.s0 + at.rl; s < at.s1; s += at.rows) {
+        float vx[VEC], vd[VEC], vg[VEC], n[VEC], dz[VEC], dg[VEC];
+        load_n<T, VEC>(x + s * p.sxs, vx);
+        load_n<T, VEC>(dy + s * p.sxs, vd);
+        if constexpr (GATE) load_n<T, VEC>(gate + s * p.sgs, vg);
+        dz_n<T, VEC, GATE>(p, ch, vx, vd, vg, n, dz, dg);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            a[j] = __builtin_fmaf(dz[j], n[j], a[j]);
+            b[j] += dz[j];
+        }
+    }
+    tile_pairs<VEC>(p, at, a, b, [&](const float *u, const float *v, float *x0, float *x1) {
+        const int cl = threadIdx.x & (p.lc - 1);
+        float s = 0.f, t = 0.f;
+        for (int r = 0; r < at.rows; ++r) {
+            s += u[r * p.lc + cl];
+            t += v[r * p.lc + cl];
+        }
+        *x0 = s;
+        *x1 = t;
+    });
+}
+
+// Second pass, adjoint: a group's means of dn n and dn.
+__global__ __launch_bounds__(256) void norm_bwd_join_kernel(GroupNormParams p) {
+    __shared__ float red[4];
+    const int64_t n = blockIdx.x / p.G;
+    const int g = (int)(blockIdx.x % p.G), entries = p.chunks * p.D;
+    const float *part = p.part + n * p.chunks * 2 * p.C + g * p.D;
+    float s = 0.f, t = 0.f;
+    for (int i = threadIdx.x; i < entries; i += 256) {
+        const float *e = part + (int64_t)(i / p.D) * 2 * p.C + i % p.D;
+        const float w = p.weight ? p.weight[g * p.D + i % p.D] : 1.f;
+        s = __builtin_fmaf(e[0], w, s);
+        t = __builtin_fmaf(e[p.C], w, t);
+    }
+    s = block_sum(s, red);
+    t = block_sum(t, red);
+    if (threadIdx.x == 0) {
+        const float size = (float)p.S * (float)p.D;
+        p.sums[blockIdx.x * 2] = s / size;
+        p.sums[blockIdx.x * 2 + 1] = t / size;
+    }
+}
+
+// Third pass, adjoint.
+template <typename T, int VEC, bool GATE> __global__ __launch_bounds__(256) void norm_bwd_apply_kernel(GroupNormParams p) {
+    const TileAt<VEC> at(p);
+    if (!at.ok) return;
+    const Channels<VEC> ch(p, at.n, at.c);
+    float s2[VEC], s1[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const int64_t g = at.n * p.G + (at.c + j) / p.D;
+        s2[j] = p.sums[g * 2];
+        s1[j] = p.sums[g * 2 + 1];
+    }
+    const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c;
+    const T *dy = static_cast<const T *>(p.dy) + at.n * p.sxn + at.c;
+    T *dx = static_cast<T *>(p.y) + at.n * p.sxn + at.c;
+    const T *gate = static_cast<const T *>(p.gate) + at.n * p.sgn + at.c;
+    T *dgate = static_cast<T *>(p.dgate) + at.n * p.sgn + at.c;
+#pragma unroll 4
+    for (int64_t s = at.s0 + at.rl; s < at.s1; s += at.rows) {
+        float vx[VEC], vd[VEC], vg[VEC], n[VEC], dz[VEC], dg[VEC], o[VEC];
+        load_n<T, VEC>(x + s * p.sxs, vx);
+        load_n<T, VEC>(dy + s * p.sxs, vd);
+        if constexpr (GATE) load_n<T, VEC>(gate + s * p.sgs, vg);
+        dz_n<T, VEC, GATE>(p, ch, vx, vd, vg, n, dz, dg);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = ch.rstd[j] * (dz[j] * ch.wt[j] - s1[j] - n[j] * s2[j]);
+        store_n<T, VEC>(dx + s * p.sxs, o);
+        if constexpr (GATE) store_n<T, VEC>(dgate + s * p.sgs, dg);
+    }
+}
+
+// -- host ---------------------------------------------------------------------
+
+size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+struct Plan {
+    bool rows; // S = 1 with groups that a wave holds
+    int vec, nv, u, log_l, sets;
+    int row_blocks;
+    int lc, tiles, chunks, chunk;
+    size_t o_stats, o_sums, bytes; // workspace: part, then these
+};
+
+int up_log2(int64_t n) {
+    int k = 0;
+    while ((int64_t(1) << k) < n) ++k;
+    return k;
+}
+
+Plan plan_of(const gdn2_group_norm_args &a, bool bwd, bool vec4, bool sums_wanted) {
+    Plan q{};
+    const int64_t C = a.channels, D = C / a.groups, N = a.samples, S = a.rows;
+    q.vec = vec4 && D % 4 == 0 ? 4 : 1;
+    const int64_t lanes = (D + q.vec - 1) / q.vec;
+    q.log_l = std::min(6, up_log2(lanes));
+    const int64_t nv = (lanes + (1 << q.log_l) - 1) >> q.log_l;
+    q.rows = S == 1 && nv <= (bwd && q.vec == 4 ? 8 : 16);
+    if (q.rows) {
+        q.nv = nv == 1 ? 1 : nv <= 4 ? 4 : bwd && q.vec == 4 ? 8 : 16;
+        q.u = q.nv == 1 ? 4 : 1;
+        const int gpw = 64 >> q.log_l;
+        q.sets = (int)((a.groups + gpw - 1) / gpw);
+        if (bwd) {
+            // 2048 workgroups, eight a compute unit, of at least two rows a wave
+            q.row_blocks = (int)std::max<int64_t>(1, std::min<int64_t>((2048 + q.sets - 1) / q.sets, (N + 7) / 8));
+            q.bytes = sums_wanted ? up256(8 * (size_t)q.row_blocks * C) : 0;
+        }
+        return q;
+    }
+    q.vec = vec4 && C % 4 == 0 ? 4 : 1;
+    // the widest tile that wastes at most an eighth of its lanes, or the one that wastes least
+    const int64_t need = (C + q.vec - 1) / q.vec;
+    int64_t best = 0;
+    for (int lc = 64; lc >= 8; lc /= 2) {
+        const int64_t padded = (need + lc - 1) / lc * lc;
+        if (best == 0 || padded < best) {
+            best = padded;
+            q.lc = lc;
+        }
+        if (8 * (padded - need) <= need) break;
+    }
+    q.tiles = (int)((need + q.lc - 1) / q.lc);
+    // about 2048 workgroups, of at least four rows a thread
+    const int64_t rows = 256 / q.lc;
+    const int64_t most = std::max<int64_t>(1, S / (4 * rows)), want = std::max<int64_t>(1, 2048 / (N * q.tiles));
+    const int64_t chunks = std::min(most, want);
+    q.chunk = (int)((S + chunks - 1) / chunks);
+    q.chunks = (int)((S + q.chunk - 1) / q.chunk);
+    size_t at = up256(8 * (size_t)(N * q.chunks) * C);
+    q.o_stats = at;
+    if (!bwd) at += up256(8 * (size_t)(N * a.groups));
+    q.o_sums = at;
+    if (bwd) at += up256(8 * (size_t)(N * a.groups));
+    q.bytes = at;
+    return q;
+}
+
+const char *check(const gdn2_group_norm_args &a, bool *nothing, bool *limits) {
+    *nothing = *limits = false;
+    if (a.samples < 0 || a.rows < 0 || a.channels < 0 || a.groups < 0) return "negative dimension";
+    if (a.activation < GDN2_ACT_NONE || a.activation > GDN2_ACT_GELU) return "unknown activation";
+    if (!(a.eps >= 0.0) || !std::isfinite(a.eps)) return "eps must be finite and not negative";
+    if (a.groups == 0 ? a.channels != 0 : a.channels % a.groups != 0) return "channels must be a multiple of groups";
+    if (a.samples == 0 || a.rows == 0 || a.channels == 0) {
+        *nothing = true;
+        return nullptr;
+    }
+    const int64_t most = int64_t(1) << 30;
+    // 2^24 workgroups of 256 threads, and 2^16 of them along the channels
+    if (a.channels >= (1 << 24) || a.samples >= most || a.rows >= most || a.samples * a.groups >= (1 << 24) ||
+        a.samples >= (1 << 24)) {
+        *limits = true;
+        return "sizes above the kernels' limits";
+    }
+    return nullptr;
+}
+
+bool mult4(int64_t s) { return s % 4 == 0; }
+bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+template <typename T> bool can_vec(const gdn2_group_norm_args &a) {
+    const size_t e = 4 * sizeof(T);
+    return aligned(a.x, e) && aligned(a.gate, e) && aligned(a.y, e) && aligned(a.weight, 16) && aligned(a.bias, 16) &&
+           mult4(a.stride_x_n) && mult4(a.stride_x_s) && (!a.gate || (mult4(a.stride_gate_n) && mult4(a.stride_gate_s)));
+}
+
+GroupNormParams fill(const gdn2_group_norm_args &a, const Plan &q, void *ws) {
+    GroupNormParams p{};
+    p.x = a.x; p.gate = a.gate; p.weight = a.weight; p.bias = a.bias; p.y = a.y; p.stats = a.stats;
+    p.sxn = a.stride_x_n; p.sxs = a.stride_x_s; p.sgn = a.stride_gate_n; p.sgs = a.stride_gate_s;
+    p.N = a.samples; p.S = a.rows; p.C = (int)a.channels; p.G = (int)a.groups; p.D = p.C / p.G;
+    p.act = a.activation; p.eps = (float)a.eps;
+    p.log_l = q.log_l; p.row_blocks = q.row_blocks; p.lc = q.lc; p.chunks = q.chunks; p.chunk = q.chunk;
+    char *w = static_cast<char *>(ws);
+    if (q.bytes) p.part = reinterpret_cast<float *>(w);
+    return p;
+}
+
+template <typename T, int VEC, bool GATE> hipError_t run_rows(const Plan &q, const GroupNormParams &p, hipStream_t s) {
+    const dim3 grid((unsigned)((p.N + 4 * q.u - 1) / (4 * q.u)), (unsigned)q.sets);
+    if (q.nv == 1) hipLaunchKernelGGL((norm_rows_kernel<T, VEC, 1, 4, GATE>), grid, dim3(256), 0, s, p);
+    else if (q.nv == 4) hipLaunchKernelGGL((norm_rows_kernel<T, VEC, 4, 1, GATE>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((norm_rows_kernel<T, VEC, 16, 1, GATE>), grid, dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+template <typename T, int VEC, bool GATE> hipError_t run_rows_bwd(const Plan &q, const GroupNormParams &p, hipStream_t s) {
+    const dim3 grid((unsigned)q.row_blocks, (unsigned)q.sets);
+    if (q.nv == 1) hipLaunchKernelGGL((norm_rows_bwd_kernel<T, VEC, 1, GATE>), grid, dim3(256), 0, s, p);
+    else if (q.nv == 4) hipLaunchKernelGGL((norm_rows_bwd_kernel<T, VEC, 4, GATE>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((norm_rows_bwd_kernel<T, VEC, VEC == 4 ? 8 : 16, GATE>), grid, dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
+gdn2_status refuse(const char *who, const char *what, gdn2_status st = GDN2_EINVAL) {
+    return fail(st, std::string(who) + ": " + what);
+}
+
+template <typename T, int VEC> hipError_t run_forward(const Plan &q, const GroupNormParams &p, hipStream_t s) {
+    if (q.rows) return p.gate ? run_rows<T, VEC, true>(q, p, s) : run_rows<T, VEC, false>(q, p, s);
+    const dim3 grid((unsigned)(p.N * q.chunks), (unsigned)q.tiles);
+    hipLaunchKernelGGL((norm_moments_kernel<T, VEC>), grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)(p.N * p.G)), dim3(256), 0, s, p);
+    if (p.gate) hipLaunchKernelGGL((norm_apply_kernel<T, VEC, true>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((norm_apply_kernel<T, VEC, false>), grid, dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+template <typename T, int VEC, bool GATE> hipError_t run_backward(const Plan &q, const GroupNormParams &p, hipStream_t s) {
+    const bool sums = p.dweight || p.dbias;
+    int64_t blocks = q.row_blocks;
+    if (q.rows) {
+        if (const hipError_t e = run_rows_bwd<T, VEC, GATE>(q, p, s); e != hipSuccess) return e;
+    } else {
+        const dim3 grid((unsigned)(p.N * q.chunks), (unsigned)q.tiles);
+        hipLaunchKernelGGL((norm_bwd_sums_kernel<T, VEC, GATE>), grid, dim3(256), 0, s, p);
+        hipLaunchKernelGGL(norm_bwd_join_kernel, dim3((unsigned)(p.N * p.G)), dim3(256), 0, s, p);
+        hipLaunchKernelGGL((norm_bwd_apply_kernel<T, VEC, GATE>), grid, dim3(256), 0, s, p);
+        blocks = p.N * q.chunks;
+    }
+    if (sums)
+        hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)((2 * (int64_t)p.C + 15) / 16)), dim3(256), 0, s, p.part, blocks,
+                           p.C, p.dweight, p.dbias);
+    return hipGetLastError();
+}
+
+bool grid_fits(const gdn2_group_norm_args &a, const Plan &q) {
+    if (q.rows) return q.sets < 65536;
+    return (double)a.samples * q.chunks < 16777216.0 && q.tiles < 65536;
+}
+
+template <typename T> gdn2_status forward(const char *who, const gdn2_group_norm_args *a, hipStream_t s) {
+    if (!a) return refuse(who, "null args");
+    bool nothing, limits;
+    if (const char *e = check(*a, &nothing, &limits)) return refuse(who, e, limits ? GDN2_NOT_APPLICABLE : GDN2_EINVAL);
+    if (nothing) return GDN2_OK;
+    if (!a->x || !a->y) return refuse(who, "null tensor pointer");
+    const Plan q = plan_of(*a, false, can_vec<T>(*a), false);
+    if (!grid_fits(*a, q)) return refuse(who, "sizes above the kernels' limits", GDN2_NOT_APPLICABLE);
+    if (q.bytes > 0 && (!a->workspace || a->workspace_bytes < q.bytes || !aligned(a->workspace, 256)))
+        return refuse(who, "workspace missing, too small or not 256-byte aligned");
+    GroupNormParams p = fill(*a, q, a->workspace);
+    if (!q.rows && !p.stats) p.stats = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + q.o_stats);
+    GDN2_HIP_CHECK((q.vec == 4 ? run_forward<T, 4>(q, p, s) : run_forward<T, 1>(q, p, s)));
+    return GDN2_OK;
+}
+
+template <typename T> gdn2_status backward(const char *who, const gdn2_group_norm_bwd_args *a, hipStream_t s) {
+    if (!a) return refuse(who, "null args");
+    const gdn2_group_norm_args &f = a->fwd;
+    bool nothing, limits;
+    if (const char *e = check(f, &nothing, &limits)) return refuse(who, e, limits ? GDN2_NOT_APPLICABLE : GDN2_EINVAL);
+    if (!nothing) {
+        if (!f.x || !f.stats || !a->d_y || !a->dx) return refuse(who, "null tensor pointer");
+        if (!f.gate != !a->dgate) return refuse(who, "dgate must be given exactly where gate is");
+    }
+    const bool sums = a->dweight || a->dbias;
+    if (nothing) { // no rows: zero gradients of the weights
+        if (sums && f.channels > 0) {
+            if (f.channels >= (1 << 24)) return refuse(who, "sizes above the kernels' limits", GDN2_NOT_APPLICABLE);
+            hipLaunchKernelGGL(column_sum_kernel, dim3((unsigned)((2 * f.channels + 15) / 16)), dim3(256), 0, s, nullptr,
+                               (int64_t)0, (int)f.channels, a->dweight, a->dbias);
+            GDN2_HIP_CHECK(hipGetLastError());
+        }
+        return GDN2_OK;
+    }
+    const size_t e = 4 * sizeof(T);
+    const bool vec4 = can_vec<T>(f) && aligned(a->d_y, e) && aligned(a->dx, e) && aligned(a->dgate, e);
+    const Plan q = plan_of(f, true, vec4, sums);
+    if (!grid_fits(f, q)) return refuse(who, "sizes above the kernels' limits", GDN2_NOT_APPLICABLE);
+    if (q.bytes > 0 && (!a->workspace || a->workspace_bytes < q.bytes || !aligned(a->workspace, 256)))
+        return refuse(who, "workspace missing, too small or not 256-byte aligned");
+    GroupNormParams p = fill(f, q, a->workspace);
+    p.dy = a->d_y; p.y = a->dx; p.dgate = a->dgate; p.dweight = a->dweight; p.dbias = a->dbias;
+    p.sums = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + q.o_sums);
+    if (f.gate)
+        GDN2_HIP_CHECK((q.vec == 4 ? run_backward<T, 4, true>(q, p, s) : run_backward<T, 1, true>(q, p, s)));
+    else
+        GDN2_HIP_CHECK((q.vec == 4 ? run_backward<T, 4, false>(q, p, s) : run_backward<T, 1, false>(q, p, s)));
+    return GDN2_OK;
+}
+
+size_t workspace_of(const gdn2_group_norm_args *a, bool bwd) {
+    bool nothing, limits;
+    if (!a || check(*a, &nothing, &limits) || nothing) return 0;
+    return std::max(plan_of(*a, bwd, true, true).bytes, plan_of(*a, bwd, false, true).bytes);
+}
+
+// No exception leaves a C entry.
+template <typename F> gdn2_status guarded(F f) {
+    try {
+        return f();
+    } catch (const std::exception &) {
+        return GDN2_EHIP;
+    }
+}
+
+}  // namespace
+}  // namespace gdn2
+
+using namespace gdn2;
+
+extern "C" size_t gdn2_group_norm_act_workspace_bytes(const gdn2_group_norm_args *a) { return workspace_of(a, false); }
+extern "C" size_t gdn2_group_norm_act_bwd_workspace_bytes(const gdn2_group_norm_bwd_args *a) {
+    return a ? workspace_of(&a->fwd, true) : 0;
+}
+extern "C" gdn2_status gdn2_group_norm_act_f32(const gdn2_group_norm_args *a, gdn2_stream_t s) {
+    return guarded([&] { return forward<float>("gdn2_group_norm_act_f32", a, (hipStream_t)s); });
+}
+extern "C" gdn2_status gdn2_group_norm_act_bf16(const gdn2_group_norm_args *a, gdn2_stream_t s) {
+    return guarded([&] { return forward<bf16>("gdn2_group_norm_act_bf16", a, (hipStream_t)s); });
+}
+extern "C" gdn2_status gdn2_group_norm_act_bwd_f32(const gdn2_group_norm_bwd_args *a, gdn2_stream_t s) {
+    return guarded([&] { return backward<float>("gdn2_group_norm_act_bwd_f32", a, (hipStream_t)s); });
+}
+extern "C" gdn2_status gdn2_group_norm_act_bwd_bf16(const gdn2_group_norm_bwd_args *a, gdn2_stream_t s) {
+    return guarded([&] { return backward<bf16>("gdn2_group_norm_act_bwd_bf16", a, (hipStream_t)s); });
+}

@@ -98,6 +98,21 @@ class GatedScanBwdArgs(ctypes.Structure):
                 ("d_state0", _fp), ("workspace", _fp), ("workspace_bytes", ctypes.c_size_t)]
 
 
+class GroupNormArgs(ctypes.Structure):
+    _fields_ = [("x", _fp), ("gate", _fp), ("weight", _fp), ("bias", _fp), ("y", _fp), ("stats", _fp),
+                ("samples", _i64), ("rows", _i64), ("channels", _i64), ("groups", _i64),
+                ("stride_x_n", _i64), ("stride_x_s", _i64), ("stride_gate_n", _i64), ("stride_gate_s", _i64),
+                ("eps", _dbl), ("activation", ctypes.c_int32), ("workspace", _fp), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class GroupNormBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", GroupNormArgs), ("d_y", _fp), ("dx", _fp), ("dgate", _fp), ("dweight", _fp), ("dbias", _fp),
+                ("workspace", _fp), ("workspace_bytes", ctypes.c_size_t)]
+
+
+ACT_NONE, ACT_SILU, ACT_GELU = 0, 1, 2
+
+
 class Config(ctypes.Structure):
     """gdn2_config (include/gdn2_layer.h) = Gdn2Config (src/config.rs:23-58)."""
     _fields_ = [("hidden_size", _i64), ("num_heads", _i64), ("head_dim", _i64), ("expand_v", ctypes.c_float),
@@ -122,6 +137,8 @@ EXPORTS = ("gdn2_last_error", "gdn2_hip_available", "gdn2_recurrent_step_f32", "
            "gdn2_chunk_bwd_saved_f32", "gdn2_recurrent_bwd_workspace_bytes",
            "gdn2_gated_scan_workspace_bytes", "gdn2_gated_scan_fwd_f32", "gdn2_gated_scan_fwd_bf16",
            "gdn2_gated_scan_bwd_workspace_bytes", "gdn2_gated_scan_bwd_f32", "gdn2_gated_scan_bwd_bf16",
+           "gdn2_group_norm_act_workspace_bytes", "gdn2_group_norm_act_f32", "gdn2_group_norm_act_bf16",
+           "gdn2_group_norm_act_bwd_workspace_bytes", "gdn2_group_norm_act_bwd_f32", "gdn2_group_norm_act_bwd_bf16",
            "gdn2_recurrent_bwd_f32", "gdn2_decode_fused_f32",
            "gdn2_config_default", "gdn2_config_validate", "gdn2_config_dims", "gdn2_param_count",
            "gdn2_param_name", "gdn2_param_shape", "gdn2_param_init", "gdn2_layer_create", "gdn2_layer_destroy",
@@ -191,11 +208,14 @@ def lib():
 
 
 def _declare_mixer(L):
-    for name, st in (("gdn2_gated_scan", GatedScanArgs), ("gdn2_gated_scan_bwd", GatedScanBwdArgs)):
-        fn = getattr(L, name + "_workspace_bytes")
+    for size, entry, st in (("gdn2_gated_scan", "gdn2_gated_scan_fwd", GatedScanArgs),
+                            ("gdn2_gated_scan_bwd", "gdn2_gated_scan_bwd", GatedScanBwdArgs),
+                            ("gdn2_group_norm_act", "gdn2_group_norm_act", GroupNormArgs),
+                            ("gdn2_group_norm_act_bwd", "gdn2_group_norm_act_bwd", GroupNormBwdArgs)):
+        fn = getattr(L, size + "_workspace_bytes")
         fn.argtypes, fn.restype = [ctypes.POINTER(st)], ctypes.c_size_t
         for ty in ("_f32", "_bf16"):
-            fn = getattr(L, (name if "_bwd" in name else name + "_fwd") + ty)
+            fn = getattr(L, entry + ty)
             fn.argtypes, fn.restype = [ctypes.POINTER(st), ctypes.c_void_p], ctypes.c_int
 
 

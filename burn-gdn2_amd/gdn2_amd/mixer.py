@@ -1,10 +1,12 @@
 """Operators of a gated recurrent mixer beside the GDN-2 layer, over the C ABI
 of include/gdn2_mixer.h (no reference counterpart):
 
-  gated_scan, gated_scan_backward   h_t = e^{g_t} h_{t-1} + w_t v_t per channel
+  gated_scan, gated_scan_backward           h_t = e^{g_t} h_{t-1} + w_t v_t per channel
+  group_norm_act, group_norm_act_backward   group norm over channels-last rows with
+                                            an activation or an activated gate
 
-Tensors as in ops.py: [B, H, T, V] of any strides with contiguous channels, in
-float32 or bfloat16; log decays, states, weights and their gradients are
+Tensors as in ops.py, of any strides with contiguous channels, in float32 or
+bfloat16; log decays, states, weights and their gradients are
 float32.  A call runs on its tensors' device, on torch's current stream there;
 workspaces come from torch's allocator, so a call may be captured into a graph.
 """
@@ -189,3 +191,102 @@ def gated_scan_backward(g, v, w, out, d_out, state=None, d_state=None, cu_seqlen
         a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     _call(L.gdn2_gated_scan_bwd_f32 if v.dtype == torch.float32 else L.gdn2_gated_scan_bwd_bf16, a, dev)
     return {"dg": dg, "dv": dv, "dw": dw, "dS0": dS0}
+
+
+# -- group norm -------------------------------------------------------------------
+
+_ACTS = {"none": C.ACT_NONE, "silu": C.ACT_SILU, "gelu": C.ACT_GELU}
+
+
+def _rows3(t: torch.Tensor) -> torch.Tensor:
+    """[N, ..., C] as [N, S, C]."""
+    return t if t.dim() == 3 else t.unsqueeze(1) if t.dim() == 2 else t.reshape(t.shape[0], -1, t.shape[-1])
+
+
+def _norm_check(x, groups, weight, bias, activation, gate, more=()):
+    if x.dim() < 2:
+        raise ValueError("x must be [N, C] or [N, ..., C]")
+    if x.dtype not in _SUFFIX:
+        raise TypeError("x must be float32 or bfloat16")
+    if activation not in _ACTS:
+        raise ValueError(f"activation must be one of {sorted(_ACTS)}, got {activation!r}")
+    if groups < 1 or x.shape[-1] % groups:
+        raise ValueError("the channels must be a multiple of groups")
+    for name, t in (("gate", gate), *more):
+        if t is not None and t.dtype != x.dtype:
+            raise TypeError(f"{name} must have x's type")
+        if t is not None and t.shape != x.shape:
+            raise ValueError(f"{name} must have x's shape")
+    for name, t in (("weight", weight), ("bias", bias)):
+        _f32(name, t)
+        if t is not None and tuple(t.shape) != (x.shape[-1],):
+            raise ValueError(f"{name} must be [C]")
+
+
+def _contig(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return None if t is None else t.contiguous()
+
+
+def _norm_args(x, groups, weight, bias, eps, activation, gate, y, stats):
+    N, S, Ch = x.shape
+    sx, sg = x.stride(), (0, 0) if gate is None else gate.stride()
+    one_n, one_s = N == 1, S == 1  # (a dimension of one has no stride to speak of)
+    return C.GroupNormArgs(_p(x), _p(gate), _p(weight), _p(bias), _p(y), _p(stats), N, S, Ch, groups,
+                           0 if one_n else sx[0], 0 if one_s else sx[1], 0 if one_n else sg[0], 0 if one_s else sg[1],
+                           eps, _ACTS[activation], None, 0)
+
+
+def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-5, activation: str = "silu", gate=None,
+                   return_stats: bool = False, out=None, workspace=None):
+    """act(z), or z act(gate) with a gate, of z = group_norm(x) weight + bias.
+
+    x [N, ..., C] with its channels in `groups` runs; a group is normalised over
+    the run and all of the dimensions between, for each of the N samples alone.
+    [M, C]: each row for itself, as a norm over the heads of a token takes it.
+    activation: "silu", "gelu" (with erf) or "none".  weight, bias [C].
+    With return_stats also stats [N, groups, 2] (mean, 1 / sqrt(variance + eps)),
+    which the backward takes.  `out` takes the result where given (it may be x)."""
+    _norm_check(x, groups, weight, bias, activation, gate, (("out", out),))
+    dev = _device(x, weight, bias, gate, out)
+    shape, x = x.shape, _dense_rows(_rows3(x))
+    gate = None if gate is None else _dense_rows(_rows3(gate))
+    weight, bias = _contig(weight), _contig(bias)
+    y = _empty_like(x) if out is None else _rows3(out)
+    if out is not None and (y.data_ptr() != out.data_ptr() or y.stride() != x.stride()):
+        raise ValueError("out must have x's layout")
+    stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=dev) if return_stats else None
+    a = _norm_args(x, groups, weight, bias, eps, activation, gate, y, stats)
+    L = C.lib()
+    workspace = _workspace(workspace, L.gdn2_group_norm_act_workspace_bytes(ctypes.byref(a)), dev)
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _call(L.gdn2_group_norm_act_f32 if x.dtype == torch.float32 else L.gdn2_group_norm_act_bf16, a, dev)
+    y = out if out is not None else y.view(shape) if len(shape) != 3 else y
+    return (y, stats) if return_stats else y
+
+
+def group_norm_act_backward(x, groups: int, stats, d_out, weight=None, bias=None, activation: str = "silu", gate=None,
+                            workspace=None) -> dict:
+    """The gradients of <d_out, y> for group_norm_act's arguments and the stats it
+    returned: dict dx, dgate (None without a gate), dweight and dbias [C] (also for
+    weight or bias None: of ones and zeros)."""
+    _norm_check(x, groups, weight, bias, activation, gate, (("d_out", d_out),))
+    _f32("stats", stats)
+    if tuple(stats.shape) != (x.shape[0], groups, 2):
+        raise ValueError("stats must be [N, groups, 2]")
+    dev = _device(x, weight, bias, gate, d_out, stats)
+    shape, x = x.shape, _dense_rows(_rows3(x))
+    gate = None if gate is None else _dense_rows(_rows3(gate))
+    d_out = _in_layout(_rows3(d_out), x)
+    weight, bias, stats = _contig(weight), _contig(bias), stats.contiguous()
+    dx, dgate = _empty_like(x), None if gate is None else _empty_like(gate)
+    dweight, dbias = torch.empty((2, shape[-1]), dtype=torch.float32, device=dev).unbind(0)
+    a = C.GroupNormBwdArgs(_norm_args(x, groups, weight, bias, 0.0, activation, gate, None, stats), _p(d_out), _p(dx),
+                           _p(dgate), _p(dweight), _p(dbias), None, 0)
+    L = C.lib()
+    workspace = _workspace(workspace, L.gdn2_group_norm_act_bwd_workspace_bytes(ctypes.byref(a)), dev)
+    if workspace is not None:
+        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _call(L.gdn2_group_norm_act_bwd_f32 if x.dtype == torch.float32 else L.gdn2_group_norm_act_bwd_bf16, a, dev)
+    return {"dx": dx.view(shape), "dgate": None if dgate is None else dgate.view(shape), "dweight": dweight,
+            "dbias": dbias}

@@ -1,7 +1,9 @@
 /*
  * gdn2_mixer.h -- C ABI of the operators of a gated recurrent mixer that
  * stands beside the GDN-2 layer: the diagonal gated recurrence with its
- * backward.  No reference counterpart.
+ * backward, and the group norm with an activation with its backward.  (The
+ * short conv in front of them is gdn2_short_conv_f32 of gdn2.h, its gradient
+ * gdn2_short_conv_bwd_f32.)  No reference counterpart.
  *
  * Status codes and gdn2_last_error() are those of gdn2.h, and so are its
  * rules: caller-owned device pointers of the current device, no allocation,
@@ -99,6 +101,67 @@ typedef struct gdn2_gated_scan_bwd_args {
 GDN2_API size_t gdn2_gated_scan_bwd_workspace_bytes(const gdn2_gated_scan_bwd_args *args);
 GDN2_API gdn2_status gdn2_gated_scan_bwd_f32(const gdn2_gated_scan_bwd_args *args, gdn2_stream_t stream);
 GDN2_API gdn2_status gdn2_gated_scan_bwd_bf16(const gdn2_gated_scan_bwd_args *args, gdn2_stream_t stream);
+
+/* ------------------------------------------------------------------------
+ * Group norm with an activation, channels last.  x [N, S, C] has its channels
+ * in `groups` runs of D = C / groups; a group's statistics are over the S rows
+ * and D channels of one sample (S = 1: each token and head by itself, as
+ * gdn2_rms_norm_gate_f32 normalises).
+ *   n = (x - mean) / sqrt(var + eps),  z = n weight + bias
+ *   y = act(z), or z act(gate) when a gate [N, S, C] is given
+ * weight, bias [C] f32, either NULL (1, 0).  Rows are C contiguous elements;
+ * strides in elements for (sample, row), one set for x and one for gate, y
+ * and x share theirs.  y may be x, or gate where their strides are equal, and
+ * must not overlap them otherwise.
+ * stats [N, groups, 2] f32 contiguous, or NULL: mean and 1 / sqrt(var + eps),
+ * what the backward takes.
+ * workspace: gdn2_group_norm_act_workspace_bytes(args) bytes (0 for S = 1 and
+ * ordinary groups), 256-byte aligned.
+ * Limits (else GDN2_NOT_APPLICABLE): C < 2^24, S < 2^30, N groups < 2^24, and at
+ * most 2^16 groups where a wave holds fewer than two of them.
+ * ---------------------------------------------------------------------- */
+typedef enum gdn2_activation {
+    GDN2_ACT_NONE = 0,
+    GDN2_ACT_SILU = 1, /* z / (1 + e^-z) */
+    GDN2_ACT_GELU = 2, /* z (1 + erf(z / sqrt 2)) / 2 */
+} gdn2_activation;
+
+typedef struct gdn2_group_norm_args {
+    const void *x, *gate;
+    const float *weight, *bias;
+    void *y;
+    float *stats;
+    int64_t samples, rows, channels, groups;
+    int64_t stride_x_n, stride_x_s;
+    int64_t stride_gate_n, stride_gate_s;
+    double eps;
+    int32_t activation; /* gdn2_activation */
+    void *workspace;
+    size_t workspace_bytes;
+} gdn2_group_norm_args;
+
+GDN2_API size_t gdn2_group_norm_act_workspace_bytes(const gdn2_group_norm_args *args);
+GDN2_API gdn2_status gdn2_group_norm_act_f32(const gdn2_group_norm_args *args, gdn2_stream_t stream);
+GDN2_API gdn2_status gdn2_group_norm_act_bf16(const gdn2_group_norm_args *args, gdn2_stream_t stream);
+
+/* The gradients of L = <d_y, y> of that call.  fwd: its arguments with the
+ * stats it wrote (y unused).  d_y and dx strided like x, dgate like gate (NULL
+ * iff gate is); dweight, dbias [C], either NULL (not wanted).  Every output is
+ * overwritten; dx may be d_y (equal strides), nothing else may overlap.  Sums
+ * over samples and rows run in a fixed order.
+ * workspace: gdn2_group_norm_act_bwd_workspace_bytes(args) bytes. */
+typedef struct gdn2_group_norm_bwd_args {
+    gdn2_group_norm_args fwd;
+    const void *d_y;
+    void *dx, *dgate;
+    float *dweight, *dbias;
+    void *workspace;
+    size_t workspace_bytes;
+} gdn2_group_norm_bwd_args;
+
+GDN2_API size_t gdn2_group_norm_act_bwd_workspace_bytes(const gdn2_group_norm_bwd_args *args);
+GDN2_API gdn2_status gdn2_group_norm_act_bwd_f32(const gdn2_group_norm_bwd_args *args, gdn2_stream_t stream);
+GDN2_API gdn2_status gdn2_group_norm_act_bwd_bf16(const gdn2_group_norm_bwd_args *args, gdn2_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -75,3 +75,86 @@ def worst(got, want, err, half):
         return 0.0
     bound = err + half * (np.abs(want) + err) + 1e-37  # (and the range of f32)
     return float(np.max(np.abs(got - want) / bound))
+
+
+# -- group norm -------------------------------------------------------------------
+
+def act64(z, act):
+    """act(z) and its first derivative."""
+    from scipy.special import erf, expit
+
+    if act == "silu":
+        s = expit(z)
+        return z * s, s * (1 + z * (1 - s))
+    if act == "gelu":
+        c = 0.5 * (1 + erf(z / np.sqrt(2)))
+        return z * c, c + z * np.exp(-z * z / 2) / np.sqrt(2 * np.pi)
+    return z, np.ones_like(z)
+
+
+def _act_err(z, z_err, a):
+    """The error of act(z) and of its derivative in f32: those of z (|act'| < 1.13,
+    |act''| < 0.8), the exponential's argument (2 |z| roundings of the factor it
+    makes), erf's two units in the last place of 1, and a few products."""
+    return 1.13 * z_err + (np.abs(a) * (2 * np.abs(z) + 8) + 4 * np.abs(z)) * EPS, 0.8 * z_err + (4 * np.abs(z) + 12) * EPS
+
+
+SUM = 80  # roundings of a sum of a group: 64 terms one after the other, then a tree
+
+
+def norm64(x, groups, weight, bias, eps, act, gate=None, stats=None):
+    """[N, S, C]: dict y, stats, and what the backward needs; *_err bounds on f32
+    errors.  With `stats` these are taken as given."""
+    N, S, C = x.shape
+    r = x.reshape(N, S, groups, C // groups)
+    full = lambda v: np.broadcast_to(v, r.shape).reshape(N, S, C)  # noqa: E731
+    if stats is None:
+        mean, var = r.mean((1, 3), keepdims=True), r.var((1, 3), keepdims=True)
+        rstd = 1 / np.sqrt(var + eps)
+        mean_err = SUM * EPS * np.abs(r).mean((1, 3), keepdims=True)
+        # the variance about a shifted point loses what the shift adds to the squares
+        spread = 1 + ((r - mean) ** 2).max((1, 3), keepdims=True) * rstd ** 2
+        rel = 0.5 * (SUM * EPS * spread + (mean_err * rstd) ** 2) + 4 * EPS
+    else:
+        mean, rstd = stats[:, None, :, 0:1], stats[:, None, :, 1:2]
+        mean_err, rel = np.zeros_like(mean), np.zeros_like(mean)
+    n = full((r - mean) * rstd)
+    n_err = np.abs(n) * full(rel + 3 * EPS) + full(mean_err * rstd)
+    w, b = (np.ones(C) if weight is None else weight), (np.zeros(C) if bias is None else bias)
+    z = n * w + b
+    z_err = np.abs(w) * n_err + 2 * EPS * (np.abs(n * w) + np.abs(b))
+    p = z if gate is None else gate  # what the activation is of
+    a, d = act64(p, act)
+    a_err, d_err = _act_err(p, z_err if gate is None else 0.0, a)
+    y, y_err = (a, a_err) if gate is None else (z * a, z_err * np.abs(a) + np.abs(z) * a_err + EPS * np.abs(z * a))
+    st = np.concatenate([mean, rstd], -1).reshape(N, groups, 2)
+    st_err = np.concatenate([mean_err, rel * rstd], -1).reshape(N, groups, 2)
+    return dict(y=y, y_err=y_err, stats=st, stats_err=st_err, n=n, n_err=n_err, z=z, z_err=z_err, a=a, a_err=a_err, d=d,
+                d_err=d_err, w=w, rstd=full(rstd))
+
+
+def norm_bwd64(x, groups, weight, bias, act, gate, stats, dy, sum_terms=200):
+    """The gradients for given stats, and the bounds on their errors.  sum_terms:
+    roundings of a sum over samples and rows (a thread's rows one after the other,
+    then its workgroup's and the others')."""
+    N, S, C = x.shape
+    f = norm64(x, groups, weight, bias, 0.0, act, gate, stats)
+    k, k_err = (f["d"], f["d_err"]) if gate is None else (f["a"], f["a_err"])
+    dz = dy * k
+    dz_err = np.abs(dy) * k_err + EPS * np.abs(dz)
+    dn, dn_err = dz * f["w"], np.abs(f["w"]) * dz_err + EPS * np.abs(dz * f["w"])
+    grp = lambda v: np.broadcast_to(v.reshape(N, S, groups, -1).mean((1, 3), keepdims=True),  # noqa: E731
+                                    (N, S, groups, C // groups)).reshape(N, S, C)
+    n, n_err = f["n"], f["n_err"]
+    s1, s2 = grp(dn), grp(dn * n)
+    s1_err = grp(dn_err + (SUM + sum_terms) * EPS * np.abs(dn))
+    s2_err = grp(dn_err * np.abs(n) + np.abs(dn) * n_err + (SUM + sum_terms) * EPS * np.abs(dn * n))
+    out = {"dx": f["rstd"] * (dn - s1 - n * s2), "dweight": (dz * n).sum((0, 1)), "dbias": dz.sum((0, 1)), "dgate": None}
+    err = {"dx": f["rstd"] * (dn_err + s1_err + n_err * np.abs(s2) + np.abs(n) * s2_err
+                              + 4 * EPS * (np.abs(dn) + np.abs(s1) + np.abs(n * s2))),
+           "dweight": (dz_err * np.abs(n) + np.abs(dz) * n_err + sum_terms * EPS * np.abs(dz * n)).sum((0, 1)),
+           "dbias": (dz_err + sum_terms * EPS * np.abs(dz)).sum((0, 1)), "dgate": None}
+    if gate is not None:
+        out["dgate"] = dy * f["z"] * f["d"]
+        err["dgate"] = np.abs(dy) * (f["z_err"] * np.abs(f["d"]) + np.abs(f["z"]) * f["d_err"]) + 2 * EPS * np.abs(out["dgate"])
+    return out, err

@@ -115,3 +115,95 @@ def test_scan_refusals_in_python():
                           (ValueError, (g1, v, None, v, v), {"d_state": st[:1]})]:
         with pytest.raises(err):
             G.gated_scan_backward(*args, **kw)
+
+
+@pytest.mark.parametrize("act", ["none", "silu", "gelu"])
+@pytest.mark.parametrize("gate", [False, True])
+def test_norm_gradients_against_differences(act, gate):
+    """The plain backward against central differences of the plain forward."""
+    r = np.random.default_rng(4)
+    N, S, C, groups = 2, 3, 6, 2
+    x = {"x": r.standard_normal((N, S, C)), "weight": r.uniform(0.5, 1.5, C), "bias": r.standard_normal(C),
+         "gate": r.standard_normal((N, S, C))}
+    dy = r.standard_normal((N, S, C))
+
+    def run(y):
+        return M.norm64(y["x"], groups, y["weight"], y["bias"], 1e-5, act, y["gate"] if gate else None)
+
+    got, _ = M.norm_bwd64(x["x"], groups, x["weight"], x["bias"], act, x["gate"] if gate else None, run(x)["stats"], dy)
+    for name in ("x", "weight", "bias") + (("gate",) if gate else ()):
+        for i in np.ndindex(x[name].shape):
+            up, down = dict(x, **{name: x[name].copy()}), dict(x, **{name: x[name].copy()})
+            up[name][i] += 1e-5
+            down[name][i] -= 1e-5
+            d = ((run(up)["y"] - run(down)["y"]) * dy).sum() / 2e-5
+            assert abs(d - got["d" + name][i]) <= 1e-7 * (1 + abs(d)), (name, i)
+
+
+def _norm_struct(**kw):
+    from gdn2_amd import _capi as C
+
+    a = C.GroupNormArgs()
+    for k, v in dict(x=256, y=256, samples=2, rows=3, channels=8, groups=2, eps=1e-5, activation=1, workspace=256,
+                     workspace_bytes=1 << 40).items():
+        setattr(a, k, v)
+    for k, v in kw.items():
+        setattr(a, k, v)
+    return a
+
+
+def test_norm_refusals_of_the_c_entry():
+    from gdn2_amd import _capi as C
+
+    L = C.lib()
+    for fn in (L.gdn2_group_norm_act_f32, L.gdn2_group_norm_act_bf16):
+        assert fn(None, None) == C.GDN2_EINVAL
+        for bad in (dict(samples=-1), dict(rows=-1), dict(channels=-8), dict(groups=3), dict(groups=0), dict(x=None),
+                    dict(y=None), dict(eps=-1.0), dict(eps=float("nan")), dict(eps=float("inf")), dict(activation=3),
+                    dict(activation=-1), dict(workspace=None), dict(workspace_bytes=8), dict(workspace=264)):
+            assert fn(ctypes.byref(_norm_struct(**bad)), None) == C.GDN2_EINVAL, bad
+            assert b"gdn2_group_norm_act" in L.gdn2_last_error()
+        for big in (dict(samples=1 << 24), dict(rows=1 << 30), dict(channels=1 << 24), dict(samples=1 << 20, groups=8, channels=8 * 4, rows=1) | dict(samples=1 << 22)):
+            assert fn(ctypes.byref(_norm_struct(**big)), None) == C.GDN2_NOT_APPLICABLE, big
+        for nothing in (dict(samples=0), dict(rows=0), dict(channels=0)):
+            assert fn(ctypes.byref(_norm_struct(**nothing)), None) == C.GDN2_OK, nothing
+    for fn in (L.gdn2_group_norm_act_bwd_f32, L.gdn2_group_norm_act_bwd_bf16):
+        assert fn(None, None) == C.GDN2_EINVAL
+        for bad in (dict(stats=None), dict(x=None), dict(gate=256), dict(activation=9)):
+            b = C.GroupNormBwdArgs(_norm_struct(**{"stats": 256, **bad}), 256, 256, None, None, None, 256, 1 << 40)
+            assert fn(ctypes.byref(b), None) == C.GDN2_EINVAL, bad
+        for bad in (dict(d_y=None), dict(dx=None), dict(dgate=256), dict(workspace=None), dict(workspace_bytes=8)):
+            b = C.GroupNormBwdArgs(_norm_struct(stats=256), 256, 256, None, None, None, 256, 1 << 40)
+            for k, v in bad.items():
+                setattr(b, k, v)
+            assert fn(ctypes.byref(b), None) == C.GDN2_EINVAL, bad
+
+
+def test_norm_workspace_sizes():
+    from gdn2_amd import _capi as C
+
+    size = lambda **kw: C.lib().gdn2_group_norm_act_workspace_bytes(ctypes.byref(_norm_struct(**kw)))  # noqa: E731
+    assert size(rows=1, channels=2048, groups=16) == size(samples=0) == size(groups=3) == 0
+    assert 0 < size(samples=8, rows=4096, channels=1024, groups=32) < 8 * 4096 * 1024
+    assert C.lib().gdn2_group_norm_act_workspace_bytes(None) == 0
+    assert C.lib().gdn2_group_norm_act_bwd_workspace_bytes(None) == 0
+
+
+def test_norm_refusals_in_python():
+    torch = pytest.importorskip("torch")
+    import gdn2_amd as G
+
+    x, w, st = torch.zeros(2, 3, 8), torch.ones(8), torch.zeros(2, 2, 2)
+    for err, args, kw in [
+        (TypeError, (x, 2), {}),  # not on a device
+        (TypeError, (x.half(), 2), {}), (ValueError, (x[0, 0], 2), {}), (ValueError, (x, 3), {}), (ValueError, (x, 0), {}),
+        (ValueError, (x, 2, w[:4]), {}), (TypeError, (x, 2, w.double()), {}), (ValueError, (x, 2, w, w[:4]), {}),
+        (ValueError, (x, 2), {"activation": "relu"}), (ValueError, (x, 2), {"gate": x[:1]}),
+        (TypeError, (x, 2), {"gate": x.bfloat16()}), (ValueError, (x, 2), {"out": x[:1]}),
+    ]:
+        with pytest.raises(err):
+            G.group_norm_act(*args, **kw)
+    for err, args in [(TypeError, (x, 2, st, x)), (ValueError, (x, 2, st[:1], x)), (TypeError, (x, 2, st.double(), x)),
+                      (ValueError, (x, 2, st, x[:1])), (TypeError, (x, 2, st, x.bfloat16()))]:
+        with pytest.raises(err):
+            G.group_norm_act_backward(*args)
