@@ -12,9 +12,9 @@ from .mixer import gated_scan, gated_scan_backward, group_norm_act, group_norm_a
 from .ops import (chunk_wy_backward, chunk_wy_forward, chunk_wy_forward_train, chunk_workspace_bytes, decode_fused,
                   fused_recurrent_backward,
                   fused_recurrent_forward, fused_recurrent_gdn2, fused_step, hip_available, l2_normalize,
-                  l2_normalize_4d, rms_norm_gate_per_head, short_conv_1d)
+                  l2_normalize_4d, rms_norm_gate_per_head, short_conv_1d, short_conv_1d_backward)
 
 __all__ = ["chunk_wy_backward", "chunk_wy_forward", "chunk_wy_forward_train", "chunk_workspace_bytes", "decode_fused", "fused_recurrent_backward", "fused_recurrent_forward",
            "fused_recurrent_gdn2", "fused_step", "hip_available", "l2_normalize", "l2_normalize_4d",
-           "rms_norm_gate_per_head", "short_conv_1d", "GatedDeltaNet2", "Gdn2Config", "Gdn2Grads", "Gdn2Saved", "Gdn2State", "init_param", "init_params",
+           "rms_norm_gate_per_head", "short_conv_1d", "short_conv_1d_backward", "GatedDeltaNet2", "Gdn2Config", "Gdn2Grads", "Gdn2Saved", "Gdn2State", "init_param", "init_params",
            "gated_scan", "gated_scan_backward", "group_norm_act", "group_norm_act_backward", "param_names", "param_shape", "_capi"]

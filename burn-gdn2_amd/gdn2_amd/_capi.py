@@ -133,6 +133,7 @@ EXPORTS = ("gdn2_last_error", "gdn2_hip_available", "gdn2_recurrent_step_f32", "
            "gdn2_chunk_segments", "gdn2_chunk_inter_pass_f32",
            "gdn2_chunk_fwd_states_f32", "gdn2_chunk_noalloc_scratch_bytes", "gdn2_chunk_fwd_noalloc_f32",
            "gdn2_stream_copy_f32", "gdn2_short_conv_f32", "gdn2_l2_normalize_f32", "gdn2_rms_norm_gate_f32",
+           "gdn2_short_conv_bwd_workspace_bytes", "gdn2_short_conv_bwd_f32",
            "gdn2_chunk_bwd_workspace_bytes", "gdn2_chunk_bwd_f32", "gdn2_chunk_fwd_train_f32",
            "gdn2_chunk_bwd_saved_f32", "gdn2_recurrent_bwd_workspace_bytes",
            "gdn2_gated_scan_workspace_bytes", "gdn2_gated_scan_fwd_f32", "gdn2_gated_scan_fwd_bf16",
@@ -187,6 +188,10 @@ def lib():
         L.gdn2_chunk_inter_pass_f32.restype = ctypes.c_int
         vp = ctypes.c_void_p
         L.gdn2_short_conv_f32.argtypes = [vp, vp, vp, vp, vp, _i64, _i64, _i64, vp]
+        L.gdn2_short_conv_bwd_workspace_bytes.argtypes = [_i64, _i64, _i64]
+        L.gdn2_short_conv_bwd_workspace_bytes.restype = ctypes.c_size_t
+        L.gdn2_short_conv_bwd_f32.argtypes = [vp] * 8 + [_i64] * 3 + [vp, ctypes.c_size_t, vp]
+        L.gdn2_short_conv_bwd_f32.restype = ctypes.c_int
         L.gdn2_l2_normalize_f32.argtypes = [vp, vp, _i64, _i64, _dbl, vp]
         L.gdn2_rms_norm_gate_f32.argtypes = [vp, vp, vp, vp, _i64, _i64, _dbl, vp]
         for n in ("gdn2_short_conv_f32", "gdn2_l2_normalize_f32", "gdn2_rms_norm_gate_f32"):

@@ -9,6 +9,7 @@ libgdn2_amd.so.
                            src/kernel/chunk_cube.rs:781-952)
   decode_fused             forward() at T == 1, src/module.rs:224-316
   short_conv_1d            src/short_conv.rs:22-65
+  short_conv_1d_backward   its gradients (burn's autodiff in the reference)
   l2_normalize(_4d)        src/l2norm.rs:4-16
   rms_norm_gate_per_head   src/module.rs:501-517
 
@@ -381,6 +382,35 @@ def short_conv_1d(x, weight, cache=None):
     new_cache = torch.empty((B, 3, Cn), device=x.device, dtype=torch.float32)
     C.check(C.lib().gdn2_short_conv_f32(_p(x), _p(weight), _p(cache), _p(out), _p(new_cache), B, T, Cn, _stream()))
     return out, new_cache
+
+
+def short_conv_1d_backward(x, weight, d_out, cache=None, d_cache=None, workspace=None) -> dict:
+    """The gradients of L = <d_out, out> + <d_cache, new cache> for short_conv_1d's
+    arguments: dict dx [B, T, C] (without a cache the padding's share is in the
+    first token's), dweight [C, 4] and dcache [B, 3, C] (None without a cache)."""
+    if x.dim() != 3 or tuple(weight.shape) != (x.shape[2], 4):
+        raise ValueError("short_conv_1d_backward: x must be [B, T, C] and weight [C, 4]")
+    B, T, Cn = x.shape
+    if d_out.shape != x.shape or any(t is not None and tuple(t.shape) != (B, 3, Cn) for t in (cache, d_cache)):
+        raise ValueError("short_conv_1d_backward: d_out must have x's shape, cache and d_cache be [B, 3, C]")
+    _check_f32_cuda(x, weight, d_out, cache, d_cache)
+    if any(t is not None and t.device != x.device for t in (weight, d_out, cache, d_cache)):
+        raise ValueError("short_conv_1d_backward: the operands are on several devices")
+    x, weight, d_out = x.contiguous(), weight.contiguous(), d_out.contiguous()
+    cache = None if cache is None else cache.contiguous()
+    d_cache = None if d_cache is None else d_cache.contiguous()
+    dx, dweight = torch.empty_like(x), torch.empty_like(weight)
+    dcache = None if cache is None else torch.empty_like(cache)
+    L = C.lib()
+    need = L.gdn2_short_conv_bwd_workspace_bytes(B, T, Cn)
+    if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
+        workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+    with torch.cuda.device(x.device):
+        C.check(L.gdn2_short_conv_bwd_f32(_p(x), _p(weight), _p(cache), _p(d_out), _p(d_cache), _p(dx), _p(dweight),
+                                          _p(dcache), B, T, Cn, _p(workspace),
+                                          0 if workspace is None else workspace.numel() * workspace.element_size(),
+                                          _stream()))
+    return {"dx": dx, "dweight": dweight, "dcache": dcache}
 
 
 def l2_normalize(x, eps: float = 1e-6):

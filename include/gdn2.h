@@ -250,6 +250,24 @@ GDN2_API gdn2_status gdn2_l2_normalize_f32(const float *x, float *y, int64_t row
 GDN2_API gdn2_status gdn2_rms_norm_gate_f32(const float *x, const float *gate, const float *weight, float *y,
                                             int64_t rows, int64_t V, double eps, gdn2_stream_t stream);
 
+/* The gradients of L = <d_out, out> + <d_cache_out, cache_out> for
+ * gdn2_short_conv_f32 (burn's autodiff of short_conv_1d in the reference):
+ *   x, weight, cache_in  the forward's
+ *   d_out        [B, T, C]
+ *   d_cache_out  [B, 3, C], or NULL (zero)
+ *   dx           [B, T, C], not overlapping x or d_out; without a cache the
+ *                padding's gradient is in dx of the first token
+ *   dweight      [C, 4], overwritten: summed over B and T in a fixed order
+ *   d_cache_in   [B, 3, C], or NULL (not wanted; NULL without cache_in)
+ * workspace: gdn2_short_conv_bwd_workspace_bytes(B, T, C) bytes, 256-byte
+ * aligned (0 without tokens).  Limits (else GDN2_NOT_APPLICABLE): C < 2^22 and
+ * B (T / 32 + 1) < 2^24. */
+GDN2_API size_t gdn2_short_conv_bwd_workspace_bytes(int64_t B, int64_t T, int64_t C);
+GDN2_API gdn2_status gdn2_short_conv_bwd_f32(const float *x, const float *weight, const float *cache_in,
+                                             const float *d_out, const float *d_cache_out, float *dx, float *dweight,
+                                             float *d_cache_in, int64_t B, int64_t T, int64_t C, void *workspace,
+                                             size_t workspace_bytes, gdn2_stream_t stream);
+
 /* A streaming copy of n floats (dst, src 16-byte aligned, not overlapping)
  * over `workgroups` workgroups of 256 threads (0 = 8 per compute unit), each
  * looping over the array with 16-byte non-temporal loads and stores.  No

@@ -158,3 +158,42 @@ def norm_bwd64(x, groups, weight, bias, act, gate, stats, dy, sum_terms=200):
         out["dgate"] = dy * f["z"] * f["d"]
         err["dgate"] = np.abs(dy) * (f["z_err"] * np.abs(f["d"]) + np.abs(f["z"]) * f["d_err"]) + 2 * EPS * np.abs(out["dgate"])
     return out, err
+
+
+# -- short conv -------------------------------------------------------------------
+
+def conv64(x, w, cache):
+    """x [B, T, C], w [C, 4], cache [B, 3, C] or None: out, new cache."""
+    B, T, C = x.shape
+    xp = np.concatenate([cache if cache is not None else np.repeat(x[:, :1], 3, 1), x], 1)
+    z = sum(xp[:, i:i + T] * w[:, i] for i in range(4))
+    return act64(z, "silu")[0], xp[:, T:], xp, z
+
+
+def conv_bwd64(x, w, cache, dy, dc, sum_terms=120):
+    """The gradients and the bounds on their f32 errors.  sum_terms: roundings of a
+    sum over tokens (32 of a thread, its workgroup's waves, 16 threads over the
+    workgroups' sums and these)."""
+    B, T, C = x.shape
+    _, _, xp, z = conv64(x, w, cache)
+    d = act64(z, "silu")[1]
+    z_err = 5 * EPS * sum(np.abs(xp[:, i:i + T] * w[:, i]) for i in range(4))
+    dz = dy * d
+    dz_err = np.abs(dy) * _act_err(z, z_err, z)[1] + EPS * np.abs(dz)
+    dp, dp_err = np.zeros_like(xp), np.zeros_like(xp)
+    for i in range(4):
+        dp[:, i:i + T] += dz * w[:, i]
+        dp_err[:, i:i + T] += (dz_err + 6 * EPS * np.abs(dz)) * np.abs(w[:, i])
+    if dc is not None:
+        dp[:, T:] += dc
+        dp_err[:, T:] += 3 * EPS * np.abs(dc)
+    out = {"dweight": np.stack([(dz * xp[:, i:i + T]).sum((0, 1)) for i in range(4)], 1), "dx": dp[:, 3:].copy(), "dcache": None}
+    err = {"dweight": np.stack([((dz_err + sum_terms * EPS * np.abs(dz)) * np.abs(xp[:, i:i + T])).sum((0, 1))
+                                for i in range(4)], 1), "dx": dp_err[:, 3:] + 4 * EPS * np.abs(dp[:, 3:]), "dcache": None}
+    if cache is None:
+        if T:
+            out["dx"][:, 0] += dp[:, :3].sum(1)
+            err["dx"][:, 0] += (dp_err[:, :3] + 4 * EPS * np.abs(dp[:, :3])).sum(1)
+    else:
+        out["dcache"], err["dcache"] = dp[:, :3], dp_err[:, :3]
+    return out, err

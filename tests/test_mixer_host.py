@@ -207,3 +207,49 @@ def test_norm_refusals_in_python():
                       (ValueError, (x, 2, st, x[:1])), (TypeError, (x, 2, st, x.bfloat16()))]:
         with pytest.raises(err):
             G.group_norm_act_backward(*args)
+
+
+@pytest.mark.parametrize("T,cache", [(1, False), (2, True), (5, False), (6, True)])
+def test_conv_gradients_against_differences(T, cache):
+    r = np.random.default_rng(5)
+    B, C = 2, 3
+    x = {"x": r.standard_normal((B, T, C)), "weight": r.uniform(-0.5, 0.5, (C, 4)), "cache": r.standard_normal((B, 3, C))}
+    dy, dc = r.standard_normal((B, T, C)), r.standard_normal((B, 3, C))
+
+    def loss(y):
+        out, new, _, _ = M.conv64(y["x"], y["weight"], y["cache"] if cache else None)
+        return (out * dy).sum() + (new * dc).sum()
+
+    got, _ = M.conv_bwd64(x["x"], x["weight"], x["cache"] if cache else None, dy, dc)
+    for name in ("x", "weight") + (("cache",) if cache else ()):
+        for i in np.ndindex(x[name].shape):
+            up, down = dict(x, **{name: x[name].copy()}), dict(x, **{name: x[name].copy()})
+            up[name][i] += 1e-6
+            down[name][i] -= 1e-6
+            d = (loss(up) - loss(down)) / 2e-6
+            assert abs(d - got["d" + name][i]) <= 1e-7 * (1 + abs(d)), (name, i)
+
+
+def test_conv_refusals():
+    torch = pytest.importorskip("torch")
+    import gdn2_amd as G
+    from gdn2_amd import _capi as C
+
+    L = C.lib()
+    ok = dict(x=256, w=256, cache=None, dy=256, dc=None, dx=1 << 20, dw=256, dci=None, B=2, T=5, C=8, ws=256, n=1 << 40)
+    call = lambda **kw: L.gdn2_short_conv_bwd_f32(*{**ok, **kw}.values(), None)  # noqa: E731
+    for bad in (dict(B=-1), dict(T=-1), dict(C=-1), dict(x=None), dict(w=None), dict(dy=None), dict(dx=None), dict(dw=None),
+                dict(dci=256), dict(ws=None), dict(n=8), dict(ws=264), dict(dx=256), dict(dx=260)):
+        assert call(**bad) == C.GDN2_EINVAL, bad
+        assert b"gdn2_short_conv_bwd_f32" in L.gdn2_last_error()
+    for big in (dict(C=1 << 22), dict(B=1 << 24), dict(T=1 << 30)):
+        assert call(**big) == C.GDN2_NOT_APPLICABLE, big
+    assert call(C=0) == C.GDN2_OK
+    size = L.gdn2_short_conv_bwd_workspace_bytes
+    assert size(0, 5, 8) == size(2, 0, 8) == size(2, 5, 0) == size(-1, 5, 8) == 0 and size(2, 5, 8) > 0
+    x, w, c = torch.zeros(2, 5, 8), torch.zeros(8, 4), torch.zeros(2, 3, 8)
+    for err, args, kw in [(TypeError, (x, w, x), {}), (ValueError, (x, w[:4], x), {}), (ValueError, (x, w, x[:1]), {}),
+                          (ValueError, (x, w, x, c[:1]), {}), (ValueError, (x[0], w, x), {}),
+                          (ValueError, (x, w, x), {"d_cache": c[:, :2]})]:
+        with pytest.raises(err):
+            G.short_conv_1d_backward(*args, **kw)
