@@ -13,13 +13,13 @@
 // recurrence from the last token to the first,
 //   D_t = dy_t + E_{t+1},  E_t = e^{g_t} D_t,  dv = w D, dw = v D, dg_t = E_t h_{t-1}.
 //
-// Decays above e^-0.34 are kept as expm1(g) and the state is advanced as
+// Decays above e^-1/8 are kept as expm1(g) and the state is advanced as
 // h + (expm1(g) h + u): the error of a rounded e^g, the same at every token, would
 // otherwise add up over the tokens that a slowly decaying state lives through.
 //
 // Tiles of one (row, CH channels) form a chain.  A tile publishes (G, X) once it
-// is loaded, and its final state once it knows what enters it.  It looks at the
-// TL tiles before it at once, takes the nearest final state among them and
+// is loaded, and its final state once it knows what enters it.  It looks at
+// several tiles before it at once, takes the nearest final state among them and
 // applies the (G, X) after it in order, which gives the same bits whichever of
 // them that was.  Words carry their own readiness (all ones: not yet), so that no
 // other memory has to be ordered with them.  A workgroup draws its tile's number
@@ -29,7 +29,9 @@
 // Bound: HBM, 16 bytes an element forward and 32 backward in f32.
 #include <algorithm>
 #include <exception>
+#include <initializer_list>
 #include <string>
+#include <type_traits>
 
 #include "common.hpp"
 #include "gdn2_mixer.h"
@@ -46,50 +48,47 @@ struct GatedScanParams {
     const float *state_in;
     float *state_out; // forward: final states; backward: d_state0
     void *out;        // forward: written; backward: h, read
-    const int *info;  // packed: the sequence of every token (-1: none), with a -1 before and after; else NULL
+    const int *cu, *info; // packed: the N + 1 offsets; the sequence of every token (-1: none), a -1 before and after
     const void *dy;
     const float *ds;
     float *dg;
     void *dv, *dw;
     float *dgp; // partial sums of dg over a unit's channel tiles, or NULL
     int64_t sgb, sgh, sgt, svb, svh, svt, sob, soh, sot;
-    int T, H, V;
+    int T, H, V, N;
     int unit, units; // channels are tiled within runs of `unit`: the whole row, or a head
     unsigned tiles_c, chains;
     unsigned tiles_t;
-    unsigned *tickets;
+    unsigned *ticket; // the next tile
     unsigned *pre;           // [chain][tile][CH] final states
     unsigned long long *agg; // [chain][tile][CH] (G, X)
 };
 
-// A token's decay in a register.  Sign bit set: expm1(g), for -0.34 < g <= 0, by
-// seven terms of its series (the rest is below 2^-26 of it).  Clear: e^g.
+// A token's decay in a register.  Sign bit set: expm1(g), for -1/8 < g <= -0, by
+// four terms of its series (the rest is below 2^-24 of it).  Clear: e^g.
 __device__ __forceinline__ float decay(float g) {
-    float p = __builtin_fmaf(g, 1.f / 5040, 1.f / 720);
-    p = __builtin_fmaf(p, g, 1.f / 120);
-    p = __builtin_fmaf(p, g, 1.f / 24);
-    p = __builtin_fmaf(p, g, 1.f / 6);
-    p = __builtin_fmaf(p, g, 0.5f);
-    p = __builtin_fmaf(p * g, g, g);
-    return g > -0.34f && g <= 0.f ? -__builtin_fabsf(p) : fast_exp2(g * kLog2e);
+    const float p = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(g, 1.f / 120, 1.f / 24), g, 1.f / 6), g, 0.5f);
+    return __builtin_bit_cast(unsigned, g) - 0x80000000u < 0x3E000000u ? __builtin_fmaf(p * g, g, g) : fast_exp2(g * kLog2e);
 }
-// e^g s + u.  Nothing of s, an infinity or NaN either, passes an e^g of zero; an
-// infinity passes any other.
+// e^g s + u for finite s
 __device__ __forceinline__ float advance(float c, float s, float u) {
+    const int mask = __builtin_bit_cast(int, c) >> 31;
+    return __builtin_fmaf(c, s, u) + __builtin_bit_cast(float, __builtin_bit_cast(int, s) & mask);
+}
+// ... for any s.  Nothing of s, an infinity or NaN either, passes an e^g of zero;
+// an infinity passes any other.
+__device__ __forceinline__ float advance_any(float c, float s, float u) {
     const int bits = __builtin_bit_cast(int, c);
     const float t = __builtin_fmaf(c, s, u);
     return bits == 0 ? u : bits < 0 ? s + (__builtin_isinf(s) ? u : t) : t;
 }
 
-// e^G h + X of a joined run.  e^G of a growing run can overflow where e^G h does not.
-__device__ __forceinline__ float join(float G, float X, float h) {
-    if (G > 80.f) {
-        const float e = fast_exp2(G * (0.5f * kLog2e));
-        return h == 0.f ? X : __builtin_fmaf(e * h, e, X);
-    }
-    const float e = fast_exp2(G * kLog2e);
-    return e == 0.f ? X : __builtin_fmaf(e, h, X);
-}
+// A run's G is kept as G log2(e) / 2, so that e^G h can be formed in two steps
+// where e^G alone overflows.
+constexpr float kHalf = 0.5f * kLog2e;
+// e^G h + X of a joined run, e = growth(G).  Nothing of h passes e = 0.
+__device__ __forceinline__ float growth(float G) { return fast_exp2(fminf(G, 127.f)); }
+__device__ __forceinline__ float join(float e, float X, float h) { return e == 0.f ? X : __builtin_fmaf(e * h, e, X); }
 
 // A published word is never all ones.
 __device__ __forceinline__ unsigned word(float x) { return x != x ? kNaN : __builtin_bit_cast(unsigned, x); }
@@ -119,300 +118,423 @@ __global__ __launch_bounds__(256) void scan_prepare_kernel(uint4 *words, int64_t
     }
 }
 
-// States of sequences without tokens.
-__global__ __launch_bounds__(256) void empty_states_kernel(const int *cu, int64_t N, int64_t n, const float *in, float *out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= N * n) return;
-    const int64_t s = i / n;
-    if (cu[s + 1] <= cu[s]) out[i] = in ? in[i] : 0.f;
-}
+// A tile: NW waves of LC lanes along the channels, VEC each, and 64 / LC along
+// the tokens, R each.
+template <int VEC_, int LC_, int R_, int NW_> struct Form {
+    static constexpr int VEC = VEC_, LC = LC_, R = R_, NW = NW_, TL = 64 / LC, CH = LC * VEC, TT = TL * R * NW;
+};
+// (how much each takes of the registers goes by the types and by what is loaded)
+template <typename T, bool BWD, bool HEAD> struct FormOf;
+template <> struct FormOf<float, false, false> : Form<4, 32, 4, 8> {};
+template <> struct FormOf<float, false, true> : Form<4, 32, 4, 8> {};
+template <> struct FormOf<bf16, false, false> : Form<8, 16, 4, 8> {};
+template <> struct FormOf<bf16, false, true> : Form<8, 16, 8, 8> {};
+template <> struct FormOf<float, true, false> : Form<4, 32, 4, 8> {};
+template <> struct FormOf<float, true, true> : Form<4, 32, 4, 8> {};
+template <> struct FormOf<bf16, true, false> : Form<8, 16, 2, 8> {};
+template <> struct FormOf<bf16, true, true> : Form<8, 16, 4, 8> {};
+// Rows that are no multiple of 16 bytes, or not aligned to them.
+typedef Form<4, 16, 4, 8> HalfForm;
+typedef Form<1, 32, 8, 4> OddForm;
 
-template <typename T, int VEC, int LC, int R, int NW, bool BWD, bool HEAD, bool HASW>
-__global__ __launch_bounds__(64 * NW) void gated_scan_kernel(GatedScanParams p) {
-    constexpr int TL = 64 / LC, CH = LC * VEC, TT = TL * R * NW;
+// A workgroup takes tile after tile: the number of the next one is drawn while
+// this one's run is computed, and its loads are in flight from there on.
+template <typename T, typename F, bool BWD, bool HEAD, bool HASW>
+__global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams p) {
+    constexpr int VEC = F::VEC, LC = F::LC, R = F::R, NW = F::NW, TL = F::TL, CH = F::CH, TT = F::TT;
+    constexpr int GV = HEAD ? 1 : VEC; // decays a token
+    constexpr int LOOK = (CH + 63) / 64; // waves that join the tiles, a lane a channel
+    static_assert(LOOK <= NW && R <= 32, "a bit a token of the run");
     __shared__ float tot[2][NW][CH]; // the waves' runs (G, X)
-    __shared__ float enter[CH];
-    __shared__ unsigned drawn;
+    __shared__ float enter[NW][CH];  // the states entering them
+    __shared__ unsigned first_drawn, drawn;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int cl = lane % LC, tl = lane / LC;
+    const bool chained = p.tiles_t > 1;
+    const unsigned tiles = p.chains * p.tiles_t;
 
-    const unsigned chain = blockIdx.x % p.chains;
-    unsigned tile = 0;
-    if (p.tiles_t > 1) {
-        if (tid == 0) drawn = atomicAdd(p.tickets + chain, 1u) + 1u; // from all ones
-        __syncthreads();
-        tile = __builtin_amdgcn_readfirstlane(drawn);
-    }
-    const unsigned ct = chain % p.tiles_c;
-    const unsigned bu = chain / p.tiles_c, b = bu / (unsigned)p.units, un = bu % (unsigned)p.units;
-    const int in_unit = (int)ct * CH + cl * VEC; // (VEC divides V where it is not 1)
-    const bool ok = in_unit < p.unit;
-    const int ch = (int)un * p.unit + (ok ? in_unit : 0), h = ch / p.V, c = ch % p.V;
-
-    const float *g = p.g + b * p.sgb + h * p.sgh + (HEAD ? 0 : c);
-    const T *v = static_cast<const T *>(p.v) + b * p.svb + h * p.svh + c;
-    const T *w = static_cast<const T *>(p.w) + b * p.svb + h * p.svh + c;
-    const int64_t oo = b * p.sob + h * p.soh + c;
-
-    // p0: the run's first token in the direction of the recurrence; token(i) its i-th
-    const int p0 = (int)tile * TT + (wave * TL + tl) * R;
-    auto token = [&](int i) { return BWD ? p.T - 1 - (p0 + i) : p0 + i; };
-
-    // masks of the run's tokens: present, first of a sequence, last of one
-    unsigned have = 0, first = 0, last = 0;
-    int seq[R];
-    if (p.info) {
-        int near[R + 2]; // the tokens around and in the run, in its direction
-#pragma unroll
-        for (int i = 0; i < R + 2; ++i) {
-            const int t = token(i - 1);
-            near[i] = t >= -1 && t <= p.T ? p.info[t + 1] : -1;
+    struct Place {
+        unsigned number, chain, tile, ct; // tile number; its chain, place along the tokens and the channels
+        int b, un, c, h;
+        bool ok;    // the lane's channels are there
+        bool plain; // see below
+        int p0;     // the run's first token in the direction of the recurrence
+        unsigned have, first, last; // masks of the run's tokens: there, first of a sequence, last of one
+    };
+    auto token = [&](const Place &q, int i) { return BWD ? p.T - 1 - (q.p0 + i) : q.p0 + i; };
+    auto place = [&](unsigned number) {
+        Place q;
+        q.number = number;
+        q.tile = number / p.chains;
+        q.chain = number % p.chains;
+        q.ct = q.chain % p.tiles_c;
+        const unsigned bu = q.chain / p.tiles_c;
+        q.b = (int)(bu / (unsigned)p.units);
+        q.un = (int)(bu % (unsigned)p.units);
+        const int in_unit = (int)q.ct * CH + cl * VEC; // (VEC divides the unit)
+        q.ok = in_unit < p.unit;
+        const int ch0 = q.un * p.unit + (int)q.ct * CH; // (uniform)
+        q.h = ch0 / p.V;
+        q.c = ch0 % p.V + (q.ok ? cl * VEC : 0);
+        while (q.c >= p.V) { // (once at most where a head fills a tile)
+            q.c -= p.V;
+            ++q.h;
         }
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            seq[i] = near[i + 1];
-            const bool in = near[i + 1] >= 0;
-            have |= (unsigned)in << i;
-            first |= (unsigned)(in && near[BWD ? i + 2 : i] != near[i + 1]) << i;
-            last |= (unsigned)(in && near[BWD ? i : i + 2] != near[i + 1]) << i;
+        const int w0 = (int)q.tile * TT + wave * TL * R;
+        q.p0 = w0 + tl * R;
+        // Whether the wave's tokens are all there and of one sequence that neither
+        // starts nor ends among them (for any offsets: all reads stay in bounds).
+        bool plain = (int)(q.ct + 1) * CH <= p.unit && w0 + TL * R <= p.T;
+        if (p.info) {
+            if (plain) {
+                const int lo = BWD ? p.T - w0 - TL * R : w0; // first token of the wave
+                const int n = p.info[lo + 1];
+                plain = n >= 0 && n == p.info[lo] && n == p.info[lo + TL * R + 1] && n == p.info[lo + TL * R];
+            }
+        } else {
+            plain = plain && w0 > 0 && w0 + TL * R < p.T;
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-            seq[i] = (int)b;
-            have |= (unsigned)(p0 + i < p.T) << i;
-            first |= (unsigned)(token(i) == 0) << i;
-            last |= (unsigned)(token(i) == p.T - 1) << i;
+        q.plain = __builtin_amdgcn_readfirstlane((int)plain);
+        q.have = q.first = q.last = 0;
+        if (!q.plain && q.ok) {
+#pragma unroll 1
+            for (int i = 0; i < R; ++i) {
+                const int t = token(q, i);
+                bool in = t >= 0 && t < p.T, f = t == 0, l = t == p.T - 1;
+                if (p.info && in) {
+                    const int n = p.info[t + 1];
+                    in = n >= 0;
+                    f = in && p.info[t] != n;
+                    l = in && p.info[t + 2] != n;
+                }
+                q.have |= (unsigned)in << i;
+                q.first |= (unsigned)(in && f) << i;
+                q.last |= (unsigned)(in && l) << i;
+            }
         }
-    }
-    if (!ok) have = first = last = 0;
-    auto state_at = [&](int n) { return ((int64_t)n * p.H + h) * p.V + c; };
+        return q;
+    };
 
-    // All loads of the run, from a row of the tensor in any case (what an absent
-    // token's row holds is dropped), so that they are in flight together.
-    // Backward: u is dy, hb the state before the token.
-    constexpr int GV = HEAD ? 1 : VEC;
+    // All loads of a run, so that they are in flight together.  What is not there
+    // reads some row of the tensor and is dropped.
     Raw<float, GV> rg[R];
     Raw<T, VEC> ru[R], rw[HASW ? R : 1], rv[BWD && HASW ? R : 1], rh[BWD ? R : 1];
+    auto load = [&](const Place &q) {
+        const float *g = p.g + (q.b * p.sgb + q.h * p.sgh + (HEAD ? 0 : q.c));
+        const int64_t ov = q.b * p.svb + q.h * p.svh + q.c, oo = q.b * p.sob + q.h * p.soh + q.c;
+        const T *v = static_cast<const T *>(p.v) + ov, *w = static_cast<const T *>(p.w) + ov;
+        const T *out = static_cast<const T *>(p.out) + oo, *dy = static_cast<const T *>(p.dy) + oo;
+        auto one = [&](int i, const float *gi, const T *vi, const T *wi, const T *yi, const T *hi) {
+            rg[i] = raw_n<float, GV>(gi);
+            ru[i] = raw_n<T, VEC>(BWD ? yi : vi); // backward: dy
+            if constexpr (BWD) rh[i] = raw_n<T, VEC>(hi); // the state before the token
+            if constexpr (BWD && HASW) rv[i] = raw_n<T, VEC>(vi);
+            if constexpr (HASW) rw[i] = raw_n<T, VEC>(wi);
+        };
+        if (q.plain) {
+            const int64_t t0 = token(q, 0);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const int64_t t = min(max(token(i), 0), p.T - 1);
-        rg[i] = raw_n<float, GV>(g + t * p.sgt);
-        if constexpr (!BWD) {
-            ru[i] = raw_n<T, VEC>(v + t * p.svt);
+            for (int i = 0; i < R; ++i) {
+                const int64_t d = BWD ? -i : i;
+                one(i, g + t0 * p.sgt + d * p.sgt, v + t0 * p.svt + d * p.svt, w + t0 * p.svt + d * p.svt,
+                    dy + t0 * p.sot + d * p.sot, out + (t0 - 1) * p.sot + d * p.sot);
+            }
         } else {
-            ru[i] = raw_n<T, VEC>(static_cast<const T *>(p.dy) + oo + t * p.sot);
-            rh[i] = raw_n<T, VEC>(static_cast<const T *>(p.out) + oo + max(t - 1, (int64_t)0) * p.sot);
-            if constexpr (HASW) rv[i] = raw_n<T, VEC>(v + t * p.svt);
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int64_t t = min(max(token(q, i), 0), p.T - 1);
+                one(i, g + t * p.sgt, v + t * p.svt, w + t * p.svt, dy + t * p.sot, out + max(t - 1, (int64_t)0) * p.sot);
+            }
         }
-        if constexpr (HASW) rw[i] = raw_n<T, VEC>(w + t * p.svt);
-    }
-    float em[R][GV], u[R][VEC];
+    };
 
-    // the run
-    float G[VEC], X[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) G[j] = X[j] = 0.f;
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const bool in = have >> i & 1;
-        float g0 = 0.f;
-        if constexpr (HEAD) em[i][0] = decay(g0 = in ? rg[i][0] : 0.f);
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            u[i][j] = (float)ru[i][j];
-            if constexpr (HASW && !BWD) u[i][j] *= (float)rw[i][j];
-            u[i][j] = in ? u[i][j] : 0.f;
-        }
-        const bool cut = (BWD ? last : first) >> i & 1; // nothing comes from the token before in this direction
-        float s0[VEC]; // forward: the state before a sequence; backward: the gradient of the one after it
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s0[j] = 0.f;
-        if (cut) {
-            const float *s = BWD ? p.ds : p.state_in;
-            if (s) load_n<float, VEC>(s + state_at(seq[i]), s0);
-        }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float gj = HEAD ? g0 : in ? rg[i][HEAD ? 0 : j] : 0.f;
-            if constexpr (!HEAD) em[i][j] = decay(gj);
-            const float dec = em[i][HEAD ? 0 : j];
-            if constexpr (!BWD) {
-                if (cut) u[i][j] = advance(dec, s0[j], u[i][j]);
-                X[j] = cut ? u[i][j] : advance(dec, X[j], u[i][j]);
-            } else {
-                if (cut) u[i][j] += s0[j];
-                X[j] = advance(dec, cut ? u[i][j] : u[i][j] + X[j], 0.f);
-            }
-            G[j] = cut ? -INFINITY : G[j] + gj;
-        }
+    unsigned number = blockIdx.x;
+    if (chained) {
+        if (tid == 0) first_drawn = atomicAdd(p.ticket, 1u) + 1u; // from all ones
+        __syncthreads();
+        number = __builtin_amdgcn_readfirstlane(first_drawn);
     }
+    if (number >= tiles) return; // (the same for the whole workgroup)
+    Place q = place(number);
+    load(q);
+    for (;;) {
+        unsigned after = q.number + gridDim.x;
+        if (chained && tid == 0) after = atomicAdd(p.ticket, 1u) + 1u;
+        auto state_at = [&](int i) {
+            return ((int64_t)(p.info ? p.info[token(q, i) + 1] : q.b) * p.H + q.h) * p.V + q.c;
+        };
+        const unsigned cut = BWD ? q.last : q.first; // nothing comes from the token before in this direction
 
-    // runs before this one: in the wave ...
-    float Gw[VEC], Xw[VEC];
+        // decays, u (backward: dy), G
+        float em[R][GV], u[R][VEC], G[GV], X[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) Gw[j] = G[j], Xw[j] = X[j];
+        for (int j = 0; j < GV; ++j) G[j] = 0.f;
+        if (q.plain) {
 #pragma unroll
-    for (int o = 1; o < TL; o <<= 1) {
+            for (int i = 0; i < R; ++i) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float Gp = __shfl_up(Gw[j], o * LC, 64), Xp = __shfl_up(Xw[j], o * LC, 64);
-            if (tl >= o) {
-                Xw[j] = join(Gw[j], Xw[j], Xp);
-                Gw[j] = Gw[j] == -INFINITY ? -INFINITY : Gw[j] + Gp;
-            }
-        }
-    }
-    if (tl == TL - 1) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            tot[0][wave][cl * VEC + j] = Gw[j];
-            tot[1][wave][cl * VEC + j] = Xw[j];
-        }
-    }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        const float Gp = __shfl_up(Gw[j], LC, 64), Xp = __shfl_up(Xw[j], LC, 64);
-        Gw[j] = tl ? Gp : 0.f;
-        Xw[j] = tl ? Xp : 0.f;
-    }
-    __syncthreads();
-
-    // ... and before the tile
-    if (p.tiles_t > 1) {
-        if (wave == 0) {
-            const int64_t at = ((int64_t)chain * p.tiles_t + tile) * CH;
-            float Gt[VEC], Xt[VEC], hin[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                Gt[j] = 0.f;
-                Xt[j] = 0.f;
-#pragma unroll
-                for (int k = 0; k < NW; ++k) {
-                    const float Gk = tot[0][k][cl * VEC + j], Xk = tot[1][k][cl * VEC + j];
-                    Xt[j] = join(Gk, Xk, Xt[j]);
-                    Gt[j] = Gk == -INFINITY ? -INFINITY : Gt[j] + Gk;
+                for (int j = 0; j < GV; ++j) {
+                    em[i][j] = decay(rg[i][j]);
+                    G[j] = __builtin_fmaf(rg[i][j], kHalf, G[j]);
                 }
-                hin[j] = 0.f;
-            }
-            if (tl == 0 && tile + 1 < p.tiles_t) {
-#pragma unroll
-                for (int j = 0; j < VEC; ++j)
-                    publish(p.agg + at + cl * VEC + j, (unsigned long long)word(Gt[j]) | (unsigned long long)word(Xt[j]) << 32);
-            }
-            if (tile > 0) {
-                const bool there = (int)tile - 1 - tl >= 0;
-                const int64_t from = at - (int64_t)(there ? tl + 1 : 0) * CH + cl * VEC;
-                unsigned P[VEC];
-                unsigned long long A[VEC];
-                int nearest;
-                for (;;) {
-                    bool hasP = there, hasA = there;
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        P[j] = peek(p.pre + from + j);
-                        A[j] = peek(p.agg + from + j);
-                    }
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        hasP = hasP && P[j] != ~0u;
-                        hasA = hasA && A[j] != ~0ull;
-                    }
-                    const unsigned long long mp = __ballot(hasP) >> cl, ma = __ballot(hasA || hasP) >> cl;
-                    nearest = -1;
-                    bool all = true;
-#pragma unroll
-                    for (int k = 0; k < TL; ++k) {
-                        if (nearest < 0 && all && (mp >> (k * LC) & 1)) nearest = k;
-                        all = all && (ma >> (k * LC) & 1);
-                    }
-                    if (__all(nearest >= 0)) break;
-                    __builtin_amdgcn_s_sleep(1);
-                }
-#pragma unroll
-                for (int k = TL - 1; k >= 0; --k) {
-#pragma unroll
-                    for (int j = 0; j < VEC; ++j) {
-                        const int src = k * LC + cl;
-                        const float Pk = __builtin_bit_cast(float, (unsigned)__shfl((int)P[j], src, 64));
-                        const float Gk = __builtin_bit_cast(float, (unsigned)__shfl((int)(unsigned)A[j], src, 64));
-                        const float Xk = __builtin_bit_cast(float, (unsigned)__shfl((int)(unsigned)(A[j] >> 32), src, 64));
-                        hin[j] = k > nearest ? 0.f : k == nearest ? Pk : join(Gk, Xk, hin[j]);
-                    }
-                }
-            }
-            if (tl == 0) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    if (tile + 1 < p.tiles_t) publish(p.pre + at + cl * VEC + j, word(join(Gt[j], Xt[j], hin[j])));
-                    enter[cl * VEC + j] = hin[j];
+                    u[i][j] = (float)ru[i][j];
+                    if constexpr (HASW && !BWD) u[i][j] *= (float)rw[i][j];
                 }
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const bool in = q.have >> i & 1, ct_i = cut >> i & 1;
+#pragma unroll
+                for (int j = 0; j < GV; ++j) {
+                    const float gj = in ? rg[i][j] : 0.f;
+                    em[i][j] = decay(gj);
+                    G[j] = ct_i ? -INFINITY : __builtin_fmaf(gj, kHalf, G[j]);
+                }
+                float s0[VEC]; // forward: the state before a sequence; backward: the gradient of the one after it
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) s0[j] = 0.f;
+                const float *s = BWD ? p.ds : p.state_in;
+                if (ct_i && s) load_n<float, VEC>(s + state_at(i), s0);
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    u[i][j] = (float)ru[i][j];
+                    if constexpr (HASW && !BWD) u[i][j] *= (float)rw[i][j];
+                    u[i][j] = in ? u[i][j] : 0.f;
+                    if (ct_i) u[i][j] = BWD ? u[i][j] + s0[j] : advance_any(em[i][HEAD ? 0 : j], s0[j], u[i][j]);
+                }
+            }
+        }
+
+        // the run, from a zero state
+        bool finite = q.plain;
+        if (q.plain) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) X[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float e = em[i][HEAD ? 0 : j];
+                    X[j] = BWD ? advance(e, u[i][j] + X[j], 0.f) : advance(e, X[j], u[i][j]);
+                }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) finite = finite && __builtin_isfinite(X[j]);
+        }
+        if (!__all(finite)) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) X[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < R; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float e = em[i][HEAD ? 0 : j];
+                    const bool fresh = cut >> i & 1;
+                    X[j] = BWD ? advance_any(e, fresh ? u[i][j] : u[i][j] + X[j], 0.f)
+                               : fresh ? u[i][j] : advance_any(e, X[j], u[i][j]);
+                }
+        }
+
+        // runs before this one: in the wave ...
+        float Gw[GV], Xw[VEC];
+#pragma unroll
+        for (int j = 0; j < GV; ++j) Gw[j] = G[j];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) Xw[j] = X[j];
+#pragma unroll
+        for (int o = 1; o < TL; o <<= 1) {
+            float e[GV];
+#pragma unroll
+            for (int j = 0; j < GV; ++j) {
+                e[j] = growth(Gw[j]);
+                const float Gp = __shfl_up(Gw[j], o * LC, 64);
+                Gw[j] = tl >= o && Gw[j] != -INFINITY ? Gw[j] + Gp : Gw[j];
+            }
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float Xp = __shfl_up(Xw[j], o * LC, 64);
+                Xw[j] = tl >= o ? join(e[HEAD ? 0 : j], Xw[j], Xp) : Xw[j];
+            }
+        }
+        if (tl == TL - 1) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                tot[0][wave][cl * VEC + j] = Gw[HEAD ? 0 : j];
+                tot[1][wave][cl * VEC + j] = Xw[j];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < GV; ++j) {
+            const float Gp = __shfl_up(Gw[j], LC, 64);
+            Gw[j] = tl ? Gp : 0.f;
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float Xp = __shfl_up(Xw[j], LC, 64);
+            Xw[j] = tl ? Xp : 0.f;
+        }
+        if (tid == 0) drawn = after;
+        __syncthreads();
+        const unsigned next_number = __builtin_amdgcn_readfirstlane(drawn);
+        const bool more = next_number < tiles;
+        Place next = q;
+
+        // what the backward still needs of this tile's rows
+        Raw<T, VEC> kw[BWD && HASW ? R : 1], kv[BWD && HASW ? R : 1], kh[BWD ? R : 1];
+        if constexpr (BWD) {
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                kh[i] = rh[i];
+                if constexpr (HASW) kw[i] = rw[i], kv[i] = rv[i];
+            }
+        }
+
+        // ... and before the tile
+        if (wave < LOOK) {
+            const int me = LOOK == 1 ? lane % CH : wave * 64 + lane;
+            float hin = 0.f;
+            if (chained) {
+                const int tile = (int)q.tile;
+                const int64_t at = (int64_t)q.chain * p.tiles_t * CH + me;
+                float Gt = 0.f, Xt = 0.f;
+#pragma unroll
+                for (int k = 0; k < NW; ++k) {
+                    const float Gk = tot[0][k][me];
+                    Xt = join(growth(Gk), tot[1][k][me], Xt);
+                    Gt = Gk == -INFINITY ? Gk : Gt + Gk;
+                }
+                const bool follows = q.tile + 1 < p.tiles_t && (LOOK > 1 || lane < CH);
+                if (follows) publish(p.agg + at + (int64_t)tile * CH, (unsigned long long)word(Gt) | (unsigned long long)word(Xt) << 32);
+                if (tile > 0) {
+                    // Looks at the W tiles before this one (tile 0 stands in for any before it).
+                    constexpr int W = 4;
+                    for (;;) {
+                        unsigned P[W];
+                        unsigned long long A[W];
+#pragma unroll
+                        for (int j = 0; j < W; ++j) {
+                            const int64_t from = at + (int64_t)max(tile - 1 - j, 0) * CH;
+                            P[j] = peek(p.pre + from);
+                            A[j] = peek(p.agg + from);
+                        }
+                        int nearest = W; // the nearest with its final state
+                        bool gap = false;
+#pragma unroll
+                        for (int j = 0; j < W; ++j) {
+                            nearest = nearest == W && !gap && P[j] != ~0u ? j : nearest;
+                            gap = gap || A[j] == ~0ull;
+                        }
+                        if (__all(nearest < W)) {
+#pragma unroll
+                            for (int j = W - 1; j >= 0; --j) {
+                                if (!__any(nearest >= j)) continue;
+                                const float Gj = __builtin_bit_cast(float, (unsigned)A[j]), Xj = __builtin_bit_cast(float, (unsigned)(A[j] >> 32));
+                                hin = j == nearest ? __builtin_bit_cast(float, P[j]) : j < nearest ? join(growth(Gj), Xj, hin) : hin;
+                            }
+                            break;
+                        }
+                        __builtin_amdgcn_s_sleep(1);
+                    }
+                }
+                if (follows) publish(p.pre + at + (int64_t)tile * CH, word(join(growth(Gt), Xt, hin)));
+            }
+#pragma unroll
+            for (int k = 0; k < NW; ++k) {
+                if (LOOK > 1 || lane < CH) enter[k][me] = hin;
+                hin = join(growth(tot[0][k][me]), tot[1][k][me], hin);
+            }
+        }
+        // (the waves above only now: their looks would wait for these loads)
+        if (more) {
+            next = place(next_number);
+            load(next);
         }
         __syncthreads();
-    }
 
-    float s[VEC]; // the state (or gradient) entering this thread's run
+        float s[VEC]; // the state (or gradient) entering this thread's run
+        float eg[GV];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        float x = p.tiles_t > 1 ? enter[cl * VEC + j] : 0.f;
-        for (int k = 0; k < wave; ++k) x = join(tot[0][k][cl * VEC + j], tot[1][k][cl * VEC + j], x);
-        s[j] = join(Gw[j], Xw[j], x);
-    }
+        for (int j = 0; j < GV; ++j) eg[j] = growth(Gw[j]);
+        finite = q.plain;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            s[j] = join(eg[HEAD ? 0 : j], Xw[j], enter[wave][cl * VEC + j]);
+            finite = finite && __builtin_isfinite(s[j]);
+        }
 
+        // The results.  Each token's go out as soon as they are known.
+        auto results = [&](auto quick) {
+            constexpr bool QUICK = decltype(quick)::value;
+            const int64_t og = q.b * p.sgb + q.h * p.sgh + (HEAD ? 0 : q.c), ov = q.b * p.svb + q.h * p.svh + q.c;
+            T *const yo = static_cast<T *>(p.out) + (q.b * p.sob + q.h * p.soh + q.c);
+            T *const dv = static_cast<T *>(p.dv) + ov, *const dw = static_cast<T *>(p.dw) + ov;
+            float *const dg = p.dg + og;
+            const int64_t t0 = token(q, 0);
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-        const bool in = have >> i & 1, cut = (BWD ? last : first) >> i & 1;
-        const int64_t t = token(i);
-        if constexpr (!BWD) {
+            for (int i = 0; i < R; ++i) {
+                const bool in = QUICK || (q.have >> i & 1), fresh = !QUICK && (cut >> i & 1);
+                const bool row = QUICK || (q.ok && q.p0 + i < p.T);
+                const int64_t t = t0 + (BWD ? -i : i);
+                if constexpr (!BWD) {
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                s[j] = cut ? u[i][j] : advance(em[i][HEAD ? 0 : j], s[j], u[i][j]);
-            }
-            if (in) store_n<T, VEC>(static_cast<T *>(p.out) + oo + t * p.sot, s);
-            if ((last >> i & 1) && p.state_out) store_n<float, VEC>(p.state_out + state_at(seq[i]), s);
-        } else {
-            float dg[VEC], dv[VEC], dw[VEC], hb[VEC]; // hb: the state before the token
+                    for (int j = 0; j < VEC; ++j) {
+                        const float e = em[i][HEAD ? 0 : j];
+                        s[j] = QUICK ? advance(e, s[j], u[i][j]) : fresh ? u[i][j] : advance_any(e, s[j], u[i][j]);
+                    }
+                    if (in) store_n<T, VEC>(yo + t * p.sot, s);
+                    if (!QUICK && (q.last >> i & 1) && p.state_out) store_n<float, VEC>(p.state_out + state_at(i), s);
+                } else {
+                    float xg[VEC], xv[VEC], xw[VEC], hb[VEC]; // hb: the state before the token
+                    const bool start = !QUICK && (q.first >> i & 1);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) hb[j] = first >> i & 1 ? 0.f : (float)rh[i][j];
-            if ((first >> i & 1) && p.state_in) load_n<float, VEC>(p.state_in + state_at(seq[i]), hb);
+                    for (int j = 0; j < VEC; ++j) hb[j] = start ? 0.f : (float)kh[i][j];
+                    if (start && p.state_in) load_n<float, VEC>(p.state_in + state_at(i), hb);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                const float d = cut ? u[i][j] : u[i][j] + s[j];
-                s[j] = advance(em[i][HEAD ? 0 : j], d, 0.f);
-                dg[j] = s[j] * hb[j];
-                dv[j] = d;
-                if constexpr (HASW) {
-                    dv[j] *= (float)rw[i][j];
-                    dw[j] = (float)rv[i][j] * d;
+                    for (int j = 0; j < VEC; ++j) {
+                        const float e = em[i][HEAD ? 0 : j], d = fresh ? u[i][j] : u[i][j] + s[j];
+                        s[j] = QUICK ? advance(e, d, 0.f) : advance_any(e, d, 0.f);
+                        xg[j] = in ? s[j] * hb[j] : 0.f; // (rows outside every sequence have no part in L)
+                        xv[j] = in ? (HASW ? (float)kw[HASW ? i : 0][j] * d : d) : 0.f;
+                        if constexpr (HASW) xw[j] = in ? (float)kv[i][j] * d : 0.f;
+                    }
+                    if (row) {
+                        store_n<T, VEC>(dv + t * p.svt, xv);
+                        if constexpr (HASW) store_n<T, VEC>(dw + t * p.svt, xw);
+                        if constexpr (!HEAD) store_n<float, VEC>(dg + t * p.sgt, xg);
+                    }
+                    if (start && p.state_out) store_n<float, VEC>(p.state_out + state_at(i), s);
+                    if constexpr (HEAD) { // the tile's channels are of one head
+                        float sum = 0.f;
+#pragma unroll
+                        for (int j = 0; j < VEC; ++j) sum += xg[j];
+#pragma unroll
+                        for (int o = 1; o < LC; o <<= 1) sum += __shfl_xor(sum, o, 64);
+                        if (cl == 0 && row) {
+                            if (p.dgp) p.dgp[(((int64_t)q.b * p.units + q.un) * p.T + t) * p.tiles_c + q.ct] = sum;
+                            else dg[t * p.sgt] = sum;
+                        }
+                    }
                 }
             }
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) { // rows outside every sequence have no part in L
-                dg[j] = in ? dg[j] : 0.f;
-                dv[j] = in ? dv[j] : 0.f;
-                if constexpr (HASW) dw[j] = in ? dw[j] : 0.f;
-            }
-            const bool row = ok && p0 + i < p.T;
-            if (row) {
-                store_n<T, VEC>(static_cast<T *>(p.dv) + (v - static_cast<const T *>(p.v)) + t * p.svt, dv);
-                if constexpr (HASW)
-                    store_n<T, VEC>(static_cast<T *>(p.dw) + (v - static_cast<const T *>(p.v)) + t * p.svt, dw);
-                if constexpr (!HEAD) store_n<float, VEC>(p.dg + (g - p.g) + t * p.sgt, dg);
-            }
-            if ((first >> i & 1) && p.state_out) store_n<float, VEC>(p.state_out + state_at(seq[i]), s);
-            if constexpr (HEAD) { // the tile's channels are of one head
-                float sum = 0.f;
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) sum += dg[j];
-#pragma unroll
-                for (int o = 1; o < LC; o <<= 1) sum += __shfl_xor(sum, o, 64);
-                if (cl == 0 && row) {
-                    if (p.dgp) p.dgp[(((int64_t)b * p.units + un) * p.T + t) * p.tiles_c + ct] = sum;
-                    else p.dg[b * p.sgb + h * p.sgh + t * p.sgt] = sum;
+        };
+        if (__all(finite)) results(std::true_type());
+        else results(std::false_type());
+
+        // the states of sequences without tokens, some a tile
+        if (p.cu && p.state_out) {
+            const float *in = BWD ? p.ds : p.state_in;
+            for (int n = (int)q.tile * (64 * NW / CH) + tid / CH; n < p.N; n += (int)p.tiles_t * (64 * NW / CH)) {
+                const int at = (int)q.ct * CH + tid % CH;
+                if (at < p.unit && p.cu[n + 1] <= p.cu[n]) {
+                    const int64_t e = (int64_t)n * p.H * p.V + (int64_t)q.un * p.unit + at;
+                    p.state_out[e] = in ? in[e] : 0.f;
                 }
             }
         }
+        if (!more) break;
+        q = next;
     }
 }
 
@@ -450,7 +572,7 @@ __global__ __launch_bounds__(256) void gated_step_kernel(GatedScanParams p, int6
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             if constexpr (!HEAD) dec = decay(gg[j]);
-            s[j] = advance(dec, s[j], HASW ? x[j] * y[j] : x[j]);
+            s[j] = advance_any(dec, s[j], HASW ? x[j] * y[j] : x[j]);
         }
         store_n<T, VEC>(out + t * p.sot, s);
     }
@@ -461,33 +583,48 @@ __global__ __launch_bounds__(256) void gated_step_kernel(GatedScanParams p, int6
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
-constexpr int kWalk = 8; // tokens that gated_step_kernel takes
+constexpr int kWalk = 8;        // tokens that gated_step_kernel takes
+constexpr int kResident = 1024; // workgroups, four a compute unit
 
 struct Plan {
-    bool vec, walk;
+    int vec;
+    bool walk;
     int ch, tt;
     int unit, units;
     int64_t tiles_c, tiles_t, chains;
-    size_t o_pre, o_agg, words, o_info, o_dgp, bytes; // workspace: tickets, pre, agg; the tokens' sequences; dg sums
+    size_t o_pre, o_agg, words, o_info, o_dgp, bytes; // workspace: the ticket, pre, agg; the tokens' sequences; dg sums
 };
 
-Plan plan_of(const gdn2_gated_scan_args &a, bool bwd, bool vec) {
+// f(form) for the form that `vec` values a lane stand for
+template <typename T, bool BWD, bool HEAD, typename Fn> auto with_form(int vec, Fn f) {
+    if (vec == FormOf<T, BWD, HEAD>::VEC) return f(FormOf<T, BWD, HEAD>());
+    if constexpr (FormOf<T, BWD, HEAD>::VEC == 8)
+        if (vec == 4) return f(HalfForm());
+    return f(OddForm());
+}
+
+template <typename T, bool BWD> Plan plan_of(const gdn2_gated_scan_args &a, int vec) {
+    constexpr bool bwd = BWD;
     Plan q{};
     q.vec = vec;
-    const int64_t T = a.seq_len, HV = a.num_heads * a.head_v_dim;
-    q.walk = !bwd && !a.cu_seqlens && T <= kWalk;
+    const int64_t len = a.seq_len, HV = a.num_heads * a.head_v_dim;
+    q.walk = !bwd && !a.cu_seqlens && len <= kWalk;
     if (q.walk) return q;
-    q.ch = 32;
-    q.tt = vec ? (bwd ? 128 : 256) : 64;
+    auto size = [&](auto form) {
+        q.ch = form.CH;
+        q.tt = form.TT;
+    };
+    if (a.g_per_head) with_form<T, BWD, true>(vec, size);
+    else with_form<T, BWD, false>(vec, size);
     const bool heads = bwd && a.g_per_head;
     q.unit = (int)(heads ? a.head_v_dim : HV);
     q.units = (int)(heads ? a.num_heads : 1);
     q.tiles_c = (q.unit + q.ch - 1) / q.ch;
-    q.tiles_t = (T + q.tt - 1) / q.tt;
+    q.tiles_t = (len + q.tt - 1) / q.tt;
     q.chains = a.batch * q.units * q.tiles_c;
     size_t at = 0;
     if (q.tiles_t > 1) {
-        at = up256(4 * (size_t)q.chains);
+        at = 256;
         q.o_pre = at;
         at += up256(4 * (size_t)(q.chains * q.tiles_t * q.ch));
         q.o_agg = at;
@@ -495,9 +632,9 @@ Plan plan_of(const gdn2_gated_scan_args &a, bool bwd, bool vec) {
         q.words = at;
     }
     q.o_info = at;
-    if (a.cu_seqlens) at += up256(4 * (size_t)(T + 2));
+    if (a.cu_seqlens) at += up256(4 * (size_t)(len + 2));
     q.o_dgp = at;
-    if (heads && q.tiles_c > 1) at += up256(4 * (size_t)(a.batch * a.num_heads * T * q.tiles_c));
+    if (heads && q.tiles_c > 1) at += up256(4 * (size_t)(a.batch * a.num_heads * len * q.tiles_c));
     q.bytes = at;
     return q;
 }
@@ -526,18 +663,24 @@ const char *check(const gdn2_gated_scan_args &a, bool *nothing, bool *limits) {
     return nullptr;
 }
 
-bool mult(int64_t s, int64_t m) { return s % m == 0; }
-bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
-
-template <typename T> bool can_vec(const gdn2_gated_scan_args &a) {
-    const size_t e = 4 * sizeof(T);
-    bool ok = a.head_v_dim % 4 == 0 && mult(a.stride_vw_b, 4) && mult(a.stride_vw_h, 4) && mult(a.stride_vw_t, 4) &&
-              mult(a.stride_o_b, 4) && mult(a.stride_o_h, 4) && mult(a.stride_o_t, 4) && aligned(a.v, e) &&
-              aligned(a.w, e) && aligned(a.out, e) && aligned(a.state_in, 16) && aligned(a.state_out, 16);
-    if (!a.g_per_head)
-        ok = ok && mult(a.stride_g_b, 4) && mult(a.stride_g_h, 4) && mult(a.stride_g_t, 4) && aligned(a.g, 16);
-    return ok;
+// Values a lane: 16 bytes of T, half of them, or one, as the rows' lengths,
+// strides and addresses allow; `more`: f32 and T pointers beside those of a.
+template <typename T>
+int vec_of(const gdn2_gated_scan_args &a, std::initializer_list<const void *> more_t, std::initializer_list<const void *> more_f) {
+    int64_t s = a.head_v_dim | a.stride_vw_b | a.stride_vw_h | a.stride_vw_t | a.stride_o_b | a.stride_o_h | a.stride_o_t;
+    uintptr_t t = reinterpret_cast<uintptr_t>(a.v) | reinterpret_cast<uintptr_t>(a.w) | reinterpret_cast<uintptr_t>(a.out);
+    uintptr_t f = reinterpret_cast<uintptr_t>(a.state_in) | reinterpret_cast<uintptr_t>(a.state_out);
+    for (const void *q : more_t) t |= reinterpret_cast<uintptr_t>(q);
+    for (const void *q : more_f) f |= reinterpret_cast<uintptr_t>(q);
+    if (!a.g_per_head) {
+        s |= a.stride_g_b | a.stride_g_h | a.stride_g_t;
+        f |= reinterpret_cast<uintptr_t>(a.g);
+    }
+    for (int n = 16 / (int)sizeof(T); n >= 4; n /= 2)
+        if (s % n == 0 && t % (n * sizeof(T)) == 0 && f % (4 * n) == 0) return n;
+    return 1;
 }
+bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
 void fill(const gdn2_gated_scan_args &a, const Plan &q, void *workspace, GatedScanParams *p) {
     p->g = a.g; p->v = a.v; p->w = a.w; p->state_in = a.state_in; p->state_out = a.state_out; p->out = a.out;
@@ -550,25 +693,31 @@ void fill(const gdn2_gated_scan_args &a, const Plan &q, void *workspace, GatedSc
     p->tiles_c = (unsigned)q.tiles_c; p->chains = (unsigned)q.chains; p->tiles_t = (unsigned)q.tiles_t;
     char *ws = static_cast<char *>(workspace);
     if (q.tiles_t > 1) {
-        p->tickets = reinterpret_cast<unsigned *>(ws);
+        p->ticket = reinterpret_cast<unsigned *>(ws);
         p->pre = reinterpret_cast<unsigned *>(ws + q.o_pre);
         p->agg = reinterpret_cast<unsigned long long *>(ws + q.o_agg);
     }
-    if (a.cu_seqlens) p->info = reinterpret_cast<const int *>(ws + q.o_info);
+    if (a.cu_seqlens) {
+        p->cu = a.cu_seqlens;
+        p->N = (int)a.num_seqs;
+        p->info = reinterpret_cast<const int *>(ws + q.o_info);
+    }
 }
 
 template <typename T, bool BWD, bool HEAD, bool HASW>
 hipError_t launch_tiles(const Plan &q, const GatedScanParams &p, hipStream_t s) {
-    const dim3 grid((unsigned)(q.chains * q.tiles_t));
-    if (q.vec) hipLaunchKernelGGL((gated_scan_kernel<T, 4, 8, BWD ? 4 : 8, 4, BWD, HEAD, HASW>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((gated_scan_kernel<T, 1, 32, 8, 4, BWD, HEAD, HASW>), grid, dim3(256), 0, s, p);
+    // as many workgroups as run at once
+    const dim3 grid((unsigned)std::min<int64_t>(q.chains * q.tiles_t, kResident));
+    with_form<T, BWD, HEAD>(q.vec, [&](auto form) {
+        hipLaunchKernelGGL((gated_scan_kernel<T, decltype(form), BWD, HEAD, HASW>), grid, dim3(64 * form.NW), 0, s, p);
+    });
     return hipGetLastError();
 }
 template <typename T, bool HEAD, bool HASW>
 hipError_t launch_walk(const gdn2_gated_scan_args &a, const Plan &q, const GatedScanParams &p, hipStream_t s) {
-    const int64_t n = a.batch * a.num_heads * a.head_v_dim / (q.vec ? 4 : 1);
+    const int64_t n = a.batch * a.num_heads * a.head_v_dim / (q.vec > 1 ? 4 : 1);
     const dim3 grid((unsigned)((n + 255) / 256));
-    if (q.vec) hipLaunchKernelGGL((gated_step_kernel<T, 4, HEAD, HASW>), grid, dim3(256), 0, s, p, n);
+    if (q.vec > 1) hipLaunchKernelGGL((gated_step_kernel<T, 4, HEAD, HASW>), grid, dim3(256), 0, s, p, n);
     else hipLaunchKernelGGL((gated_step_kernel<T, 1, HEAD, HASW>), grid, dim3(256), 0, s, p, n);
     return hipGetLastError();
 }
@@ -579,14 +728,6 @@ hipError_t prepare(const gdn2_gated_scan_args &a, const Plan &q, void *ws, hipSt
     const unsigned blocks = (unsigned)std::min<int64_t>((n + 255) / 256, 2048);
     hipLaunchKernelGGL(scan_prepare_kernel, dim3(blocks), dim3(256), 0, s, reinterpret_cast<uint4 *>(ws), n16, a.cu_seqlens,
                        (int)a.num_seqs, (int)a.seq_len, reinterpret_cast<int *>(static_cast<char *>(ws) + q.o_info));
-    return hipGetLastError();
-}
-
-hipError_t empty_states(const gdn2_gated_scan_args &a, const float *in, float *out, hipStream_t s) {
-    if (!a.cu_seqlens || !out) return hipSuccess;
-    const int64_t n = a.num_heads * a.head_v_dim;
-    hipLaunchKernelGGL(empty_states_kernel, dim3((unsigned)((a.num_seqs * n + 255) / 256)), dim3(256), 0, s, a.cu_seqlens,
-                       a.num_seqs, n, in, out);
     return hipGetLastError();
 }
 
@@ -616,7 +757,7 @@ template <typename T> gdn2_status forward(const char *who, const gdn2_gated_scan
     if (nothing) return GDN2_OK;
     if (a->seq_len == 0) return no_tokens(*a, a->state_in, a->state_out, s);
     if (!a->g || !a->v || !a->out) return fail(GDN2_EINVAL, std::string(who) + ": null tensor pointer");
-    const Plan q = plan_of(*a, false, can_vec<T>(*a));
+    const Plan q = plan_of<T, false>(*a, vec_of<T>(*a, {}, {}));
     if (q.bytes > 0 && (!a->workspace || a->workspace_bytes < q.bytes || !aligned(a->workspace, 256))) return bad_workspace(who);
     GatedScanParams p{};
     fill(*a, q, a->workspace, &p);
@@ -629,7 +770,6 @@ template <typename T> gdn2_status forward(const char *who, const gdn2_gated_scan
     GDN2_HIP_CHECK(a->g_per_head
                        ? (a->w ? launch_tiles<T, false, true, true>(q, p, s) : launch_tiles<T, false, true, false>(q, p, s))
                        : (a->w ? launch_tiles<T, false, false, true>(q, p, s) : launch_tiles<T, false, false, false>(q, p, s)));
-    GDN2_HIP_CHECK(empty_states(*a, a->state_in, a->state_out, s));
     return GDN2_OK;
 }
 
@@ -644,10 +784,8 @@ template <typename T> gdn2_status backward(const char *who, const gdn2_gated_sca
     if (!f.g || !f.out || !a->d_out || !a->dg || !a->dv || (f.w && !f.v))
         return fail(GDN2_EINVAL, std::string(who) + ": null tensor pointer");
     if (!f.w != !a->dw) return fail(GDN2_EINVAL, std::string(who) + ": dw must be given exactly where w is");
-    const size_t e = 4 * sizeof(T);
-    const bool vec = can_vec<T>(f) && aligned(a->d_out, e) && aligned(a->dv, e) && aligned(a->dw, e) &&
-                     aligned(a->d_state_out, 16) && aligned(a->d_state0, 16) && (f.g_per_head || aligned(a->dg, 16));
-    const Plan q = plan_of(f, true, vec);
+    const int vec = vec_of<T>(f, {a->d_out, a->dv, a->dw}, {a->d_state_out, a->d_state0, f.g_per_head ? nullptr : a->dg});
+    const Plan q = plan_of<T, true>(f, vec);
     if (q.bytes > 0 && (!a->workspace || a->workspace_bytes < q.bytes || !aligned(a->workspace, 256))) return bad_workspace(who);
     GatedScanParams p{};
     fill(f, q, a->workspace, &p);
@@ -663,14 +801,17 @@ template <typename T> gdn2_status backward(const char *who, const gdn2_gated_sca
         hipLaunchKernelGGL(dg_sum_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, n);
         GDN2_HIP_CHECK(hipGetLastError());
     }
-    GDN2_HIP_CHECK(empty_states(f, a->d_state_out, a->d_state0, s));
     return GDN2_OK;
 }
 
-size_t workspace_of(const gdn2_gated_scan_args *a, bool bwd) {
+// (of either type and alignment: the call knows them, the size does not)
+template <bool BWD> size_t workspace_of(const gdn2_gated_scan_args *a) {
     bool nothing, limits;
     if (!a || check(*a, &nothing, &limits) || nothing || a->seq_len == 0) return 0;
-    return std::max(plan_of(*a, bwd, true).bytes, plan_of(*a, bwd, false).bytes);
+    size_t n = 0;
+    for (const int vec : {8, 4, 1})
+        n = std::max({n, plan_of<float, BWD>(*a, vec).bytes, plan_of<bf16, BWD>(*a, vec).bytes});
+    return n;
 }
 
 // No exception leaves a C entry.
@@ -687,9 +828,9 @@ template <typename F> gdn2_status guarded(F f) {
 
 using namespace gdn2;
 
-extern "C" size_t gdn2_gated_scan_workspace_bytes(const gdn2_gated_scan_args *a) { return workspace_of(a, false); }
+extern "C" size_t gdn2_gated_scan_workspace_bytes(const gdn2_gated_scan_args *a) { return workspace_of<false>(a); }
 extern "C" size_t gdn2_gated_scan_bwd_workspace_bytes(const gdn2_gated_scan_bwd_args *a) {
-    return a ? workspace_of(&a->fwd, true) : 0;
+    return a ? workspace_of<true>(&a->fwd) : 0;
 }
 extern "C" gdn2_status gdn2_gated_scan_fwd_f32(const gdn2_gated_scan_args *a, gdn2_stream_t s) {
     return guarded([&] { return forward<float>("gdn2_gated_scan_fwd_f32", a, (hipStream_t)s); });
