@@ -121,6 +121,7 @@ __global__ __launch_bounds__(256) void scan_prepare_kernel(uint4 *words, int64_t
 // A tile: NW waves of LC lanes along the channels, VEC each, and 64 / LC along
 // the tokens, R each.
 template <int VEC_, int LC_, int R_, int NW_> struct Form {
+    static constexpr bool NEAR = VEC_ > 1; // 32-bit offsets within a wave, see near_rows
     static constexpr int VEC = VEC_, LC = LC_, R = R_, NW = NW_, TL = 64 / LC, CH = LC * VEC, TT = TL * R * NW;
 };
 // (how much each takes of the registers goes by the types and by what is loaded)
@@ -155,10 +156,11 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
 
     struct Place {
         unsigned number, chain, tile, ct; // tile number; its chain, place along the tokens and the channels
-        int b, un, c, h;
+        int b, un, hu, h, c; // batch row, unit; the tile's first head, the lane's, its channel there
+        int w0;              // the wave's first token in the direction of the recurrence
         bool ok;    // the lane's channels are there
         bool plain; // see below
-        int p0;     // the run's first token in the direction of the recurrence
+        int p0;     // the run's first token
         unsigned have, first, last; // masks of the run's tokens: there, first of a sequence, last of one
     };
     auto token = [&](const Place &q, int i) { return BWD ? p.T - 1 - (q.p0 + i) : q.p0 + i; };
@@ -174,13 +176,13 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
         const int in_unit = (int)q.ct * CH + cl * VEC; // (VEC divides the unit)
         q.ok = in_unit < p.unit;
         const int ch0 = q.un * p.unit + (int)q.ct * CH; // (uniform)
-        q.h = ch0 / p.V;
+        q.h = q.hu = ch0 / p.V;
         q.c = ch0 % p.V + (q.ok ? cl * VEC : 0);
         while (q.c >= p.V) { // (once at most where a head fills a tile)
             q.c -= p.V;
             ++q.h;
         }
-        const int w0 = (int)q.tile * TT + wave * TL * R;
+        const int w0 = q.w0 = (int)q.tile * TT + wave * TL * R;
         q.p0 = w0 + tl * R;
         // Whether the wave's tokens are all there and of one sequence that neither
         // starts nor ends among them (for any offsets: all reads stay in bounds).
@@ -215,37 +217,49 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
         return q;
     };
 
+    // Channel `chan` of the lane's head at token(i) - shift of a tensor (the nearest
+    // row where that is outside it): an address that the wave shares and 32 bits a
+    // lane beside it, the same for every i of a plain run (`quick`).  Only rows too
+    // far apart for that take 64 bits a lane.
+    auto at = [&](const Place &q, auto quick, int i, const void *base, int size, int64_t sb, int64_t sh, int64_t st, int chan,
+                  int shift) {
+        const int t = min(max(token(q, i) - shift, 0), p.T - 1);
+        const char *x = static_cast<const char *>(base);
+        if constexpr (!F::NEAR) return x + size * (q.b * sb + q.h * sh + chan + t * st);
+        constexpr bool Q = decltype(quick)::value;
+        const int low = BWD ? max(p.T - q.w0 - TL * R, 0) : min(q.w0, p.T - 1); // the wave's lowest token
+        const int row = Q ? low - shift + (BWD ? R - 1 - i : i) : max(low - shift, 0);
+        const int lane_row = Q ? (BWD ? TL - 1 - tl : tl) * R : t - row;
+        return x + size * (q.b * sb + q.hu * sh + row * st) +
+               (unsigned)size * ((unsigned)(q.h - q.hu) * (unsigned)sh + (unsigned)chan + (unsigned)lane_row * (unsigned)st);
+    };
+    auto at_g = [&](const Place &q, auto quick, int i, const float *g) {
+        return (float *)at(q, quick, i, g, 4, p.sgb, p.sgh, p.sgt, HEAD ? 0 : q.c, 0);
+    };
+    auto at_v = [&](const Place &q, auto quick, int i, const void *v) {
+        return (T *)at(q, quick, i, v, sizeof(T), p.svb, p.svh, p.svt, q.c, 0);
+    };
+    auto at_o = [&](const Place &q, auto quick, int i, const void *o, int shift) {
+        return (T *)at(q, quick, i, o, sizeof(T), p.sob, p.soh, p.sot, q.c, shift);
+    };
+
     // All loads of a run, so that they are in flight together.  What is not there
     // reads some row of the tensor and is dropped.
     Raw<float, GV> rg[R];
     Raw<T, VEC> ru[R], rw[HASW ? R : 1], rv[BWD && HASW ? R : 1], rh[BWD ? R : 1];
-    auto load = [&](const Place &q) {
-        const float *g = p.g + (q.b * p.sgb + q.h * p.sgh + (HEAD ? 0 : q.c));
-        const int64_t ov = q.b * p.svb + q.h * p.svh + q.c, oo = q.b * p.sob + q.h * p.soh + q.c;
-        const T *v = static_cast<const T *>(p.v) + ov, *w = static_cast<const T *>(p.w) + ov;
-        const T *out = static_cast<const T *>(p.out) + oo, *dy = static_cast<const T *>(p.dy) + oo;
-        auto one = [&](int i, const float *gi, const T *vi, const T *wi, const T *yi, const T *hi) {
-            rg[i] = raw_n<float, GV>(gi);
-            ru[i] = raw_n<T, VEC>(BWD ? yi : vi); // backward: dy
-            if constexpr (BWD) rh[i] = raw_n<T, VEC>(hi); // the state before the token
-            if constexpr (BWD && HASW) rv[i] = raw_n<T, VEC>(vi);
-            if constexpr (HASW) rw[i] = raw_n<T, VEC>(wi);
-        };
-        if (q.plain) {
-            const int64_t t0 = token(q, 0);
+    auto load_run = [&](const Place &q, auto quick) {
 #pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const int64_t d = BWD ? -i : i;
-                one(i, g + t0 * p.sgt + d * p.sgt, v + t0 * p.svt + d * p.svt, w + t0 * p.svt + d * p.svt,
-                    dy + t0 * p.sot + d * p.sot, out + (t0 - 1) * p.sot + d * p.sot);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-                const int64_t t = min(max(token(q, i), 0), p.T - 1);
-                one(i, g + t * p.sgt, v + t * p.svt, w + t * p.svt, dy + t * p.sot, out + max(t - 1, (int64_t)0) * p.sot);
-            }
+        for (int i = 0; i < R; ++i) {
+            rg[i] = raw_n<float, GV>(at_g(q, quick, i, p.g));
+            ru[i] = raw_n<T, VEC>(BWD ? at_o(q, quick, i, p.dy, 0) : at_v(q, quick, i, p.v)); // backward: dy
+            if constexpr (BWD) rh[i] = raw_n<T, VEC>(at_o(q, quick, i, p.out, 1)); // the state before the token
+            if constexpr (BWD && HASW) rv[i] = raw_n<T, VEC>(at_v(q, quick, i, p.v));
+            if constexpr (HASW) rw[i] = raw_n<T, VEC>(at_v(q, quick, i, p.w));
         }
+    };
+    auto load = [&](const Place &q) {
+        if (q.plain) load_run(q, std::true_type());
+        else load_run(q, std::false_type());
     };
 
     unsigned number = blockIdx.x;
@@ -467,23 +481,17 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
         // The results.  Each token's go out as soon as they are known.
         auto results = [&](auto quick) {
             constexpr bool QUICK = decltype(quick)::value;
-            const int64_t og = q.b * p.sgb + q.h * p.sgh + (HEAD ? 0 : q.c), ov = q.b * p.svb + q.h * p.svh + q.c;
-            T *const yo = static_cast<T *>(p.out) + (q.b * p.sob + q.h * p.soh + q.c);
-            T *const dv = static_cast<T *>(p.dv) + ov, *const dw = static_cast<T *>(p.dw) + ov;
-            float *const dg = p.dg + og;
-            const int64_t t0 = token(q, 0);
 #pragma unroll
             for (int i = 0; i < R; ++i) {
                 const bool in = QUICK || (q.have >> i & 1), fresh = !QUICK && (cut >> i & 1);
                 const bool row = QUICK || (q.ok && q.p0 + i < p.T);
-                const int64_t t = t0 + (BWD ? -i : i);
                 if constexpr (!BWD) {
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) {
                         const float e = em[i][HEAD ? 0 : j];
                         s[j] = QUICK ? advance(e, s[j], u[i][j]) : fresh ? u[i][j] : advance_any(e, s[j], u[i][j]);
                     }
-                    if (in) store_n<T, VEC>(yo + t * p.sot, s);
+                    if (in) store_n<T, VEC>(at_o(q, quick, i, p.out, 0), s);
                     if (!QUICK && (q.last >> i & 1) && p.state_out) store_n<float, VEC>(p.state_out + state_at(i), s);
                 } else {
                     float xg[VEC], xv[VEC], xw[VEC], hb[VEC]; // hb: the state before the token
@@ -500,9 +508,9 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
                         if constexpr (HASW) xw[j] = in ? (float)kv[i][j] * d : 0.f;
                     }
                     if (row) {
-                        store_n<T, VEC>(dv + t * p.svt, xv);
-                        if constexpr (HASW) store_n<T, VEC>(dw + t * p.svt, xw);
-                        if constexpr (!HEAD) store_n<float, VEC>(dg + t * p.sgt, xg);
+                        store_n<T, VEC>(at_v(q, quick, i, p.dv), xv);
+                        if constexpr (HASW) store_n<T, VEC>(at_v(q, quick, i, p.dw), xw);
+                        if constexpr (!HEAD) store_n<float, VEC>(at_g(q, quick, i, p.dg), xg);
                     }
                     if (start && p.state_out) store_n<float, VEC>(p.state_out + state_at(i), s);
                     if constexpr (HEAD) { // the tile's channels are of one head
@@ -512,8 +520,8 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
 #pragma unroll
                         for (int o = 1; o < LC; o <<= 1) sum += __shfl_xor(sum, o, 64);
                         if (cl == 0 && row) {
-                            if (p.dgp) p.dgp[(((int64_t)q.b * p.units + q.un) * p.T + t) * p.tiles_c + q.ct] = sum;
-                            else dg[t * p.sgt] = sum;
+                            if (p.dgp) p.dgp[(((int64_t)q.b * p.units + q.un) * p.T + token(q, i)) * p.tiles_c + q.ct] = sum;
+                            else *at_g(q, quick, i, p.dg) = sum;
                         }
                     }
                 }
@@ -585,6 +593,7 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 constexpr int kWalk = 8;        // tokens that gated_step_kernel takes
 constexpr int kResident = 1024; // workgroups, four a compute unit
+constexpr int kMostTokens = 64, kMostChannels = 128; // of a wave, of a tile
 
 struct Plan {
     int vec;
@@ -611,6 +620,7 @@ template <typename T, bool BWD> Plan plan_of(const gdn2_gated_scan_args &a, int 
     q.walk = !bwd && !a.cu_seqlens && len <= kWalk;
     if (q.walk) return q;
     auto size = [&](auto form) {
+        static_assert(form.TL * form.R <= kMostTokens && form.CH <= kMostChannels, "near_rows");
         q.ch = form.CH;
         q.tt = form.TT;
     };
@@ -663,6 +673,21 @@ const char *check(const gdn2_gated_scan_args &a, bool *nothing, bool *limits) {
     return nullptr;
 }
 
+// A dimension of one has no stride to speak of.
+gdn2_gated_scan_args tidy(gdn2_gated_scan_args a) {
+    if (a.batch == 1) a.stride_g_b = a.stride_vw_b = a.stride_o_b = 0;
+    if (a.num_heads == 1) a.stride_g_h = a.stride_vw_h = a.stride_o_h = 0;
+    if (a.seq_len == 1) a.stride_g_t = a.stride_vw_t = a.stride_o_t = 0;
+    return a;
+}
+// Whether the offsets within a wave's tokens and a tile's heads fit 31 bits.
+bool near_rows(const gdn2_gated_scan_args &a) {
+    const int64_t heads = std::min<int64_t>(a.num_heads, kMostChannels / a.head_v_dim + 2), most = (int64_t(1) << 29) - kMostChannels;
+    auto fits = [&](int64_t sh, int64_t st) { // (each below 2^29 first, so that the sum is exact)
+        return sh >= 0 && st >= 0 && sh < most && st < most && heads * sh + kMostTokens * st < most;
+    };
+    return fits(a.stride_g_h, a.stride_g_t) && fits(a.stride_vw_h, a.stride_vw_t) && fits(a.stride_o_h, a.stride_o_t);
+}
 // Values a lane: 16 bytes of T, half of them, or one, as the rows' lengths,
 // strides and addresses allow; `more`: f32 and T pointers beside those of a.
 template <typename T>
@@ -676,6 +701,7 @@ int vec_of(const gdn2_gated_scan_args &a, std::initializer_list<const void *> mo
         s |= a.stride_g_b | a.stride_g_h | a.stride_g_t;
         f |= reinterpret_cast<uintptr_t>(a.g);
     }
+    if (!near_rows(a)) return 1;
     for (int n = 16 / (int)sizeof(T); n >= 4; n /= 2)
         if (s % n == 0 && t % (n * sizeof(T)) == 0 && f % (4 * n) == 0) return n;
     return 1;
@@ -749,8 +775,9 @@ gdn2_status no_tokens(const gdn2_gated_scan_args &a, const float *in, float *out
     return GDN2_OK;
 }
 
-template <typename T> gdn2_status forward(const char *who, const gdn2_gated_scan_args *a, hipStream_t s) {
-    if (!a) return fail(GDN2_EINVAL, std::string(who) + ": null args");
+template <typename T> gdn2_status forward(const char *who, const gdn2_gated_scan_args *args, hipStream_t s) {
+    if (!args) return fail(GDN2_EINVAL, std::string(who) + ": null args");
+    const gdn2_gated_scan_args tidied = tidy(*args), *const a = &tidied;
     bool nothing, limits;
     if (const char *e = check(*a, &nothing, &limits))
         return fail(limits ? GDN2_NOT_APPLICABLE : GDN2_EINVAL, std::string(who) + ": " + e);
@@ -775,7 +802,7 @@ template <typename T> gdn2_status forward(const char *who, const gdn2_gated_scan
 
 template <typename T> gdn2_status backward(const char *who, const gdn2_gated_scan_bwd_args *a, hipStream_t s) {
     if (!a) return fail(GDN2_EINVAL, std::string(who) + ": null args");
-    const gdn2_gated_scan_args &f = a->fwd;
+    const gdn2_gated_scan_args f = tidy(a->fwd);
     bool nothing, limits;
     if (const char *e = check(f, &nothing, &limits))
         return fail(limits ? GDN2_NOT_APPLICABLE : GDN2_EINVAL, std::string(who) + ": " + e);
