@@ -669,6 +669,13 @@ const char *check(const gdn2_group_norm_args &a, bool *nothing, bool *limits) {
 bool mult4(int64_t s) { return s % 4 == 0; }
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// A dimension of one has no stride to speak of.
+gdn2_group_norm_args tidy(gdn2_group_norm_args a) {
+    if (a.samples == 1) a.stride_x_n = a.stride_gate_n = 0;
+    if (a.rows == 1) a.stride_x_s = a.stride_gate_s = 0;
+    return a;
+}
+
 template <typename T> bool can_vec(const gdn2_group_norm_args &a) {
     const size_t e = 4 * sizeof(T);
     return aligned(a.x, e) && aligned(a.gate, e) && aligned(a.y, e) && aligned(a.weight, 16) && aligned(a.bias, 16) &&
@@ -738,8 +745,9 @@ bool grid_fits(const gdn2_group_norm_args &a, const Plan &q) {
     return (double)a.samples * q.chunks < 16777216.0 && q.tiles < 65536;
 }
 
-template <typename T> gdn2_status forward(const char *who, const gdn2_group_norm_args *a, hipStream_t s) {
-    if (!a) return refuse(who, "null args");
+template <typename T> gdn2_status forward(const char *who, const gdn2_group_norm_args *args, hipStream_t s) {
+    if (!args) return refuse(who, "null args");
+    const gdn2_group_norm_args tidied = tidy(*args), *const a = &tidied;
     bool nothing, limits;
     if (const char *e = check(*a, &nothing, &limits)) return refuse(who, e, limits ? GDN2_NOT_APPLICABLE : GDN2_EINVAL);
     if (nothing) return GDN2_OK;
@@ -756,7 +764,7 @@ template <typename T> gdn2_status forward(const char *who, const gdn2_group_norm
 
 template <typename T> gdn2_status backward(const char *who, const gdn2_group_norm_bwd_args *a, hipStream_t s) {
     if (!a) return refuse(who, "null args");
-    const gdn2_group_norm_args &f = a->fwd;
+    const gdn2_group_norm_args f = tidy(a->fwd);
     bool nothing, limits;
     if (const char *e = check(f, &nothing, &limits)) return refuse(who, e, limits ? GDN2_NOT_APPLICABLE : GDN2_EINVAL);
     if (!nothing) {

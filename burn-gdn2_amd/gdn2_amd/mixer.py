@@ -12,7 +12,6 @@ workspaces come from torch's allocator, so a call may be captured into a graph.
 """
 from __future__ import annotations
 
-import ctypes
 from typing import Optional, Tuple
 
 import torch
@@ -26,46 +25,53 @@ def _p(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-def _device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> torch.device:
-    """The device of every operand; TypeError off the GPU, ValueError for several devices."""
-    for t in (first, *others):
-        if t is not None:
+def _device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The index of every operand's device; TypeError off the GPU, ValueError for
+    several devices."""
+    if not first.is_cuda:
+        raise TypeError("gdn2_amd operators take device tensors")
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
             if not t.is_cuda:
                 raise TypeError("gdn2_amd operators take device tensors")
-            if t.device != first.device:
-                raise ValueError("the operands are on several devices")
-    return first.device
+            raise ValueError("the operands are on several devices")
+    return index
 
 
-def _f32(name: str, t: Optional[torch.Tensor]) -> None:
-    if t is not None and t.dtype != torch.float32:
-        raise TypeError(f"{name} must be float32")
+# torch.cuda.current_stream(i).cuda_stream without building the stream object
+# (0.1 against 2.9 us of a call's 10)
+_stream_of = torch._C._cuda_getCurrentRawStream
 
 
-def _call(fn, args, device: torch.device) -> None:
-    if torch.cuda.current_device() == device.index:
-        status = fn(ctypes.byref(args), torch.cuda.current_stream().cuda_stream)
+def _call(fn, args, index: int) -> None:
+    if torch.cuda.current_device() == index:
+        status = fn(args, _stream_of(index))
     else:
-        with torch.cuda.device(device):
-            status = fn(ctypes.byref(args), torch.cuda.current_stream().cuda_stream)
-    C.check(status)
+        with torch.cuda.device(index):
+            status = fn(args, _stream_of(index))
+    if status:
+        C.check(status)
 
 
-def _workspace(workspace: Optional[torch.Tensor], need: int, device: torch.device) -> Optional[torch.Tensor]:
+def _workspace(args, workspace: Optional[torch.Tensor], need: int, like: torch.Tensor):
+    """Sets the workspace of `args`, a new one where none or too small a one is
+    given; returns the tensor, to be kept until the call is made."""
     if need == 0:
-        return workspace
+        return None
     if workspace is None or workspace.numel() * workspace.element_size() < need:
-        return torch.empty(need, dtype=torch.uint8, device=device)
+        workspace = torch.empty(need, dtype=torch.uint8, device=like.device)
+    args.workspace, args.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     return workspace
 
 
 def _dense_rows(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy of it, with contiguous channels and no element of memory in
     two places (what the gradients are laid out like)."""
-    if t.shape[-1] != 1 and t.stride(-1) != 1:
-        return t.contiguous()
     if t.is_contiguous():
         return t
+    if t.shape[-1] != 1 and t.stride(-1) != 1:
+        return t.contiguous()
     span = 1
     for n, s in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1), key=lambda x: x[1]):
         if s < span:
@@ -86,45 +92,51 @@ def _in_layout(t: torch.Tensor, ref: torch.Tensor) -> torch.Tensor:
 
 # -- gated scan -----------------------------------------------------------------
 
-def _scan_check(g, v, w, state, cu_seqlens, more=()):
-    """The checks of both directions; the number of states."""
-    if v.dim() != 4:
+def _scan_check(g, v, w, state, cu_seqlens, others=(), states=()):
+    """The checks of both directions; the shape of the states.  others: (name,
+    tensor) of v's shape and type; states: (name, tensor) beside `state`."""
+    ty, shape = v.dtype, v.shape
+    if len(shape) != 4:
         raise ValueError("v must be [B, H, T, V]")
-    if v.dtype not in _SUFFIX:
+    if ty not in _SUFFIX:
         raise TypeError("v must be float32 or bfloat16")
-    _f32("g", g)
-    if g.dim() != 4 or g.shape[:3] != v.shape[:3] or g.shape[3] not in (1, v.shape[3]):
+    if g.dtype is not torch.float32:
+        raise TypeError("g must be float32")
+    gs = g.shape
+    if gs != shape and (len(gs) != 4 or gs[:3] != shape[:3] or gs[3] != 1):
         raise ValueError("g must be [B, H, T, V] or [B, H, T, 1]")
-    for name, t in (("w", w), *more):
-        if t is not None and t.dtype != v.dtype:
-            raise TypeError(f"{name} must have v's type")
-        if t is not None and t.shape != v.shape:
-            raise ValueError(f"{name} must have v's shape")
-    n = v.shape[0]
+    for name, t in (("w", w), *others):
+        if t is not None:
+            if t.dtype is not ty:
+                raise TypeError(f"{name} must have v's type")
+            if t.shape != shape:
+                raise ValueError(f"{name} must have v's shape")
+    n = shape[0]
     if cu_seqlens is not None:
         if cu_seqlens.dtype != torch.int32 or cu_seqlens.dim() != 1 or not cu_seqlens.is_contiguous():
             raise TypeError("cu_seqlens must be a contiguous int32 vector")
-        if v.shape[0] != 1:
+        if n != 1:
             raise ValueError("packed sequences need a batch of 1")
         n = cu_seqlens.shape[0] - 1
         if n < 0:
             raise ValueError("cu_seqlens needs at least one offset")
-    _state_check("state", state, n, v)
-    return n
-
-
-def _state_check(name, state, n, v):
-    _f32(name, state)
-    if state is not None and tuple(state.shape) != (n, v.shape[1], v.shape[3]):
-        raise ValueError(f"{name} must be [{n}, H, V]")
+    of_states = (n, shape[1], shape[3])
+    for name, t in (("state", state), *states):
+        if t is not None:
+            if t.dtype is not torch.float32:
+                raise TypeError(f"{name} must be float32")
+            if t.shape != of_states:
+                raise ValueError(f"{name} must be [{n}, H, V]")
+    return of_states
 
 
 def _scan_args(g, v, w, state, new_state, out, cu_seqlens, n):
     B, H, T, V = v.shape
-    sg, sv, so = g.stride(), v.stride(), out.stride()
-    return C.GatedScanArgs(_p(g), _p(v), _p(w), _p(state), _p(new_state), _p(out), _p(cu_seqlens), B, H, T, V, n,
-                           int(g.shape[3] != V or V == 1), sg[0], sg[1], sg[2], sv[0], sv[1], sv[2], so[0], so[1], so[2],
-                           None, 0)
+    gb, gh, gt, _ = g.stride()
+    vb, vh, vt, _ = v.stride()
+    ob, oh, ot, _ = out.stride()
+    return C.GatedScanArgs(g.data_ptr(), v.data_ptr(), _p(w), _p(state), _p(new_state), out.data_ptr(), _p(cu_seqlens), B,
+                           H, T, V, n, g.shape[3] == 1, gb, gh, gt, vb, vh, vt, ob, oh, ot, None, 0)
 
 
 def _channels(t: torch.Tensor) -> torch.Tensor:
@@ -142,9 +154,9 @@ def gated_scan(g, v, w=None, state=None, cu_seqlens=None, out=None, new_state=No
     rows of out outside all of them are left as they were.  Otherwise N = B.
     T = 1 is the serving step.  `out` and `new_state` (which may be `state`) take
     the results where given."""
-    n = _scan_check(g, v, w, state, cu_seqlens, (("out", out),))
-    _state_check("new_state", new_state, n, v)
-    dev = _device(v, g, w, state, cu_seqlens, out, new_state)
+    of_states = _scan_check(g, v, w, state, cu_seqlens, (("out", out),) if out is not None else (),
+                            (("new_state", new_state),) if new_state is not None else ())
+    index = _device(v, g, w, state, cu_seqlens, out, new_state)
     v, g = _channels(v), _channels(g)
     if w is not None:
         w = _in_layout(w, v)
@@ -152,17 +164,19 @@ def gated_scan(g, v, w=None, state=None, cu_seqlens=None, out=None, new_state=No
         state = state.contiguous()
     if out is None:
         out = torch.empty_like(v)
+    elif out.shape[3] != 1 and out.stride(3) != 1:
+        raise ValueError("out's channels must be contiguous")
     if new_state is None:
-        new_state = torch.empty((n, v.shape[1], v.shape[3]), dtype=torch.float32, device=dev)
-    elif not new_state.is_contiguous() or (out.shape[3] != 1 and out.stride(3) != 1):
-        raise ValueError("new_state must be contiguous, and out's channels")
-    a = _scan_args(g, v, w, state, new_state, out, cu_seqlens, n)
+        new_state = torch.empty(of_states, dtype=torch.float32, device=v.device) if state is None else torch.empty_like(state)
+    elif not new_state.is_contiguous():
+        raise ValueError("new_state must be contiguous")
+    a = _scan_args(g, v, w, state, new_state, out, cu_seqlens, of_states[0])
     L = C.lib()
-    if v.shape[2] > 8 or cu_seqlens is not None:  # (up to 8 tokens never need one)
-        workspace = _workspace(workspace, L.gdn2_gated_scan_workspace_bytes(ctypes.byref(a)), dev)
-        if workspace is not None:
-            a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _call(L.gdn2_gated_scan_fwd_f32 if v.dtype == torch.float32 else L.gdn2_gated_scan_fwd_bf16, a, dev)
+    keep = None
+    if v.shape[2] > 8 or cu_seqlens is not None:  # (up to 8 tokens never need a workspace)
+        keep = _workspace(a, workspace, L.gdn2_gated_scan_workspace_bytes(a), v)
+    _call(L.gdn2_gated_scan_fwd_f32 if v.dtype is torch.float32 else L.gdn2_gated_scan_fwd_bf16, a, index)
+    del keep
     return out, new_state
 
 
@@ -171,9 +185,8 @@ def gated_scan_backward(g, v, w, out, d_out, state=None, d_state=None, cu_seqlen
     arguments and its `out`: dict dg (g's shape), dv, dw (v's; dw None without w)
     and dS0 (the state's gradient, also for state None).  Rows outside every
     sequence of cu_seqlens have no gradient: dg, dv and dw are zero there."""
-    n = _scan_check(g, v, w, state, cu_seqlens, (("out", out), ("d_out", d_out)))
-    _state_check("d_state", d_state, n, v)
-    dev = _device(v, g, w, state, cu_seqlens, out, d_out, d_state)
+    of_states = _scan_check(g, v, w, state, cu_seqlens, (("out", out), ("d_out", d_out)), (("d_state", d_state),))
+    index = _device(v, g, w, state, cu_seqlens, out, d_out, d_state)
     v, g = _dense_rows(v), _dense_rows(g)
     if w is not None:
         w = _in_layout(w, v)
@@ -182,14 +195,13 @@ def gated_scan_backward(g, v, w, out, d_out, state=None, d_state=None, cu_seqlen
     state = None if state is None else state.contiguous()
     d_state = None if d_state is None else d_state.contiguous()
     dg, dv, dw = _empty_like(g), _empty_like(v), None if w is None else _empty_like(v)
-    dS0 = torch.empty((n, v.shape[1], v.shape[3]), dtype=torch.float32, device=dev)
-    a = C.GatedScanBwdArgs(_scan_args(g, v, w, state, None, out, cu_seqlens, n), _p(d_out), _p(d_state), _p(dg), _p(dv),
-                           _p(dw), _p(dS0), None, 0)
+    dS0 = torch.empty(of_states, dtype=torch.float32, device=v.device)
+    a = C.GatedScanBwdArgs(_scan_args(g, v, w, state, None, out, cu_seqlens, of_states[0]), d_out.data_ptr(), _p(d_state),
+                           dg.data_ptr(), dv.data_ptr(), _p(dw), dS0.data_ptr(), None, 0)
     L = C.lib()
-    workspace = _workspace(workspace, L.gdn2_gated_scan_bwd_workspace_bytes(ctypes.byref(a)), dev)
-    if workspace is not None:
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _call(L.gdn2_gated_scan_bwd_f32 if v.dtype == torch.float32 else L.gdn2_gated_scan_bwd_bf16, a, dev)
+    keep = _workspace(a, workspace, L.gdn2_gated_scan_bwd_workspace_bytes(a), v)
+    _call(L.gdn2_gated_scan_bwd_f32 if v.dtype is torch.float32 else L.gdn2_gated_scan_bwd_bf16, a, index)
+    del keep
     return {"dg": dg, "dv": dv, "dw": dw, "dS0": dS0}
 
 
@@ -203,24 +215,28 @@ def _rows3(t: torch.Tensor) -> torch.Tensor:
     return t if t.dim() == 3 else t.unsqueeze(1) if t.dim() == 2 else t.reshape(t.shape[0], -1, t.shape[-1])
 
 
-def _norm_check(x, groups, weight, bias, activation, gate, more=()):
-    if x.dim() < 2:
+def _norm_check(x, groups, weight, bias, activation, gate, others=()):
+    ty, shape = x.dtype, x.shape
+    if len(shape) < 2:
         raise ValueError("x must be [N, C] or [N, ..., C]")
-    if x.dtype not in _SUFFIX:
+    if ty not in _SUFFIX:
         raise TypeError("x must be float32 or bfloat16")
     if activation not in _ACTS:
         raise ValueError(f"activation must be one of {sorted(_ACTS)}, got {activation!r}")
-    if groups < 1 or x.shape[-1] % groups:
+    if groups < 1 or shape[-1] % groups:
         raise ValueError("the channels must be a multiple of groups")
-    for name, t in (("gate", gate), *more):
-        if t is not None and t.dtype != x.dtype:
-            raise TypeError(f"{name} must have x's type")
-        if t is not None and t.shape != x.shape:
-            raise ValueError(f"{name} must have x's shape")
+    for name, t in (("gate", gate), *others):
+        if t is not None:
+            if t.dtype is not ty:
+                raise TypeError(f"{name} must have x's type")
+            if t.shape != shape:
+                raise ValueError(f"{name} must have x's shape")
     for name, t in (("weight", weight), ("bias", bias)):
-        _f32(name, t)
-        if t is not None and tuple(t.shape) != (x.shape[-1],):
-            raise ValueError(f"{name} must be [C]")
+        if t is not None:
+            if t.dtype is not torch.float32:
+                raise TypeError(f"{name} must be float32")
+            if t.shape != shape[-1:]:
+                raise ValueError(f"{name} must be [C]")
 
 
 def _contig(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -229,10 +245,9 @@ def _contig(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 def _norm_args(x, groups, weight, bias, eps, activation, gate, y, stats):
     N, S, Ch = x.shape
-    sx, sg = x.stride(), (0, 0) if gate is None else gate.stride()
-    one_n, one_s = N == 1, S == 1  # (a dimension of one has no stride to speak of)
-    return C.GroupNormArgs(_p(x), _p(gate), _p(weight), _p(bias), _p(y), _p(stats), N, S, Ch, groups,
-                           0 if one_n else sx[0], 0 if one_s else sx[1], 0 if one_n else sg[0], 0 if one_s else sg[1],
+    xn, xs, _ = x.stride()
+    gn, gs, _ = (0, 0, 0) if gate is None else gate.stride()
+    return C.GroupNormArgs(x.data_ptr(), _p(gate), _p(weight), _p(bias), _p(y), _p(stats), N, S, Ch, groups, xn, xs, gn, gs,
                            eps, _ACTS[activation], None, 0)
 
 
@@ -246,21 +261,20 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-5, ac
     activation: "silu", "gelu" (with erf) or "none".  weight, bias [C].
     With return_stats also stats [N, groups, 2] (mean, 1 / sqrt(variance + eps)),
     which the backward takes.  `out` takes the result where given (it may be x)."""
-    _norm_check(x, groups, weight, bias, activation, gate, (("out", out),))
-    dev = _device(x, weight, bias, gate, out)
+    _norm_check(x, groups, weight, bias, activation, gate, (("out", out),) if out is not None else ())
+    index = _device(x, weight, bias, gate, out)
     shape, x = x.shape, _dense_rows(_rows3(x))
     gate = None if gate is None else _dense_rows(_rows3(gate))
     weight, bias = _contig(weight), _contig(bias)
-    y = _empty_like(x) if out is None else _rows3(out)
+    y = torch.empty_like(x) if out is None else _rows3(out)
     if out is not None and (y.data_ptr() != out.data_ptr() or y.stride() != x.stride()):
         raise ValueError("out must have x's layout")
-    stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=dev) if return_stats else None
+    stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device) if return_stats else None
     a = _norm_args(x, groups, weight, bias, eps, activation, gate, y, stats)
     L = C.lib()
-    workspace = _workspace(workspace, L.gdn2_group_norm_act_workspace_bytes(ctypes.byref(a)), dev)
-    if workspace is not None:
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _call(L.gdn2_group_norm_act_f32 if x.dtype == torch.float32 else L.gdn2_group_norm_act_bf16, a, dev)
+    keep = _workspace(a, workspace, L.gdn2_group_norm_act_workspace_bytes(a), x)
+    _call(L.gdn2_group_norm_act_f32 if x.dtype is torch.float32 else L.gdn2_group_norm_act_bf16, a, index)
+    del keep
     y = out if out is not None else y.view(shape) if len(shape) != 3 else y
     return (y, stats) if return_stats else y
 
@@ -271,22 +285,24 @@ def group_norm_act_backward(x, groups: int, stats, d_out, weight=None, bias=None
     returned: dict dx, dgate (None without a gate), dweight and dbias [C] (also for
     weight or bias None: of ones and zeros)."""
     _norm_check(x, groups, weight, bias, activation, gate, (("d_out", d_out),))
-    _f32("stats", stats)
-    if tuple(stats.shape) != (x.shape[0], groups, 2):
+    if stats.dtype is not torch.float32:
+        raise TypeError("stats must be float32")
+    if stats.shape != (x.shape[0], groups, 2):
         raise ValueError("stats must be [N, groups, 2]")
-    dev = _device(x, weight, bias, gate, d_out, stats)
+    index = _device(x, weight, bias, gate, d_out, stats)
     shape, x = x.shape, _dense_rows(_rows3(x))
     gate = None if gate is None else _dense_rows(_rows3(gate))
     d_out = _in_layout(_rows3(d_out), x)
     weight, bias, stats = _contig(weight), _contig(bias), stats.contiguous()
     dx, dgate = _empty_like(x), None if gate is None else _empty_like(gate)
-    dweight, dbias = torch.empty((2, shape[-1]), dtype=torch.float32, device=dev).unbind(0)
-    a = C.GroupNormBwdArgs(_norm_args(x, groups, weight, bias, 0.0, activation, gate, None, stats), _p(d_out), _p(dx),
-                           _p(dgate), _p(dweight), _p(dbias), None, 0)
+    dweight = torch.empty(shape[-1], dtype=torch.float32, device=x.device) if weight is None else torch.empty_like(weight)
+    dbias = torch.empty_like(dweight)
+    a = C.GroupNormBwdArgs(_norm_args(x, groups, weight, bias, 0.0, activation, gate, None, stats), d_out.data_ptr(),
+                           dx.data_ptr(), _p(dgate), dweight.data_ptr(), dbias.data_ptr(), None, 0)
     L = C.lib()
-    workspace = _workspace(workspace, L.gdn2_group_norm_act_bwd_workspace_bytes(ctypes.byref(a)), dev)
-    if workspace is not None:
-        a.workspace, a.workspace_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-    _call(L.gdn2_group_norm_act_bwd_f32 if x.dtype == torch.float32 else L.gdn2_group_norm_act_bwd_bf16, a, dev)
-    return {"dx": dx.view(shape), "dgate": None if dgate is None else dgate.view(shape), "dweight": dweight,
-            "dbias": dbias}
+    keep = _workspace(a, workspace, L.gdn2_group_norm_act_bwd_workspace_bytes(a), x)
+    _call(L.gdn2_group_norm_act_bwd_f32 if x.dtype is torch.float32 else L.gdn2_group_norm_act_bwd_bf16, a, index)
+    del keep
+    if len(shape) != 3:
+        dx, dgate = dx.view(shape), None if dgate is None else dgate.view(shape)
+    return {"dx": dx, "dgate": dgate, "dweight": dweight, "dbias": dbias}

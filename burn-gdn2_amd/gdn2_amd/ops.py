@@ -405,11 +405,15 @@ def short_conv_1d_backward(x, weight, d_out, cache=None, d_cache=None, workspace
     need = L.gdn2_short_conv_bwd_workspace_bytes(B, T, Cn)
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-    with torch.cuda.device(x.device):
-        C.check(L.gdn2_short_conv_bwd_f32(_p(x), _p(weight), _p(cache), _p(d_out), _p(d_cache), _p(dx), _p(dweight),
-                                          _p(dcache), B, T, Cn, _p(workspace),
-                                          0 if workspace is None else workspace.numel() * workspace.element_size(),
-                                          _stream()))
+    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
+    args = (x.data_ptr(), weight.data_ptr(), ptr(cache), d_out.data_ptr(), ptr(d_cache), dx.data_ptr(), dweight.data_ptr(),
+            ptr(dcache), B, T, Cn, ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size())
+    index = x.get_device()
+    if torch.cuda.current_device() == index:
+        C.check(L.gdn2_short_conv_bwd_f32(*args, torch._C._cuda_getCurrentRawStream(index)))
+    else:
+        with torch.cuda.device(index):
+            C.check(L.gdn2_short_conv_bwd_f32(*args, torch._C._cuda_getCurrentRawStream(index)))
     return {"dx": dx, "dweight": dweight, "dcache": dcache}
 
 
