@@ -81,6 +81,9 @@ def _dense_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _empty_like(t: torch.Tensor) -> torch.Tensor:
+    """A tensor of t's shape, type and strides."""
+    if t.is_contiguous():
+        return torch.empty_like(t)
     return torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=t.device)
 
 
@@ -266,7 +269,7 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-5, ac
     shape, x = x.shape, _dense_rows(_rows3(x))
     gate = None if gate is None else _dense_rows(_rows3(gate))
     weight, bias = _contig(weight), _contig(bias)
-    y = torch.empty_like(x) if out is None else _rows3(out)
+    y = _empty_like(x) if out is None else _rows3(out)
     if out is not None and (y.data_ptr() != out.data_ptr() or y.stride() != x.stride()):
         raise ValueError("out must have x's layout")
     stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device) if return_stats else None
