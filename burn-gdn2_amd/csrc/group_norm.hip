@@ -5,10 +5,12 @@
 //   dx = rstd (dn - mean(dn) - n mean(dn n)),  dweight = sum dz n,  dbias = sum dz
 //
 // S = 1 (a token's heads): L lanes hold a group in registers, so that everything
-// is read once; the variance is taken about the mean.  Other groups are too large
-// for one wave: a first pass leaves sums for every channel and chunk of rows, a
-// second joins them, a third reads x again and writes.  Every sum runs in a
-// fixed order.
+// is read once; the variance is taken about the mean.  A larger group is held by
+// up to kMostParts workgroups: each publishes its part's sums, reads those of
+// the others, and goes on with its registers, so that again everything is read
+// once.  Groups larger than that take three passes: sums for every channel and
+// chunk of rows, a join, and one that reads x again.  Every sum runs in a fixed
+// order.
 //
 // Bound: HBM.
 #include <algorithm>
@@ -38,11 +40,16 @@ struct GroupNormParams {
     float eps;
     int log_l;         // rows kernels: lanes a group, as a power of two
     int row_blocks;    // backward rows kernel
-    int lc;            // tile kernels: lanes along the channels (a power of two)
+    int lc;            // tile kernels: lanes along the channels (a power of two); held groups: any number
     int chunks, chunk; // row chunks of a sample, rows in one
+    // held groups: channels a tile, tiles a set of groups, sets; a part: a chunk of rows by a tile
+    int tile, tiles, sets, set_groups;
+    unsigned *ticket;           // the next part
+    unsigned long long *words;  // [sample][set][part][set_groups] what the parts publish
 };
 
-__device__ __forceinline__ float sigmoid_f(float z) { return 1.f / (1.f + fast_exp2(-kLog2e * z)); }
+// (v_rcp_f32 is within one unit in the last place)
+__device__ __forceinline__ float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * z)); }
 
 template <int N> __device__ __forceinline__ void act_n(int act, const float *z, float *a) {
     if (act == GDN2_ACT_SILU) {
@@ -580,12 +587,349 @@ template <typename T, int VEC, bool GATE> __global__ __launch_bounds__(256) void
     }
 }
 
+// -- groups that several workgroups hold ----------------------------------------
+
+// All ones over the words that parts publish and the ticket before them.
+__global__ __launch_bounds__(256) void norm_prepare_kernel(uint4 *words, int64_t n16) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n16; i += (int64_t)gridDim.x * 256)
+        words[i] = uint4{~0u, ~0u, ~0u, ~0u};
+}
+
+// A part of a set of groups: E rows a thread of VEC channels, lc lanes along the
+// tile's channels.  Parts are numbered by a ticket, a set's next to each other: at
+// most one set of a running kernel is not drawn completely, so that at most
+// kMostParts - 1 of its workgroups wait for one that has not started.  They are
+// few enough to leave room on the chip (256 workgroups at least) for it to start,
+// with as many kernels at once.
+constexpr int kMostParts = 16;
+template <int VEC, int E, int NT> struct Held {
+    int c, in_tile, rl, rows; // the lane's first channel, that in its tile; its row and the rows at a time
+    int set, part, parts, count; // rows of this chunk
+    bool ok;
+    int64_t n, s0;
+    __device__ Held(const GroupNormParams &p, unsigned number) {
+        parts = p.chunks * p.tiles;
+        part = (int)(number % (unsigned)parts);
+        const unsigned ns = number / (unsigned)parts;
+        set = (int)(ns % (unsigned)p.sets);
+        n = ns / (unsigned)p.sets;
+        const int tl = part % p.tiles;
+        rows = NT / p.lc;
+        rl = (int)threadIdx.x / p.lc;
+        const int cl = (int)threadIdx.x % p.lc;
+        const int set_c = set * p.set_groups * p.D, most = min(p.set_groups * p.D, p.C - set_c);
+        in_tile = cl * VEC;
+        c = set_c + tl * p.tile + in_tile;
+        ok = rl < rows && in_tile < p.tile && tl * p.tile + in_tile < most; // (VEC divides all of these)
+        c = ok ? c : set_c;
+        s0 = (int64_t)(part / p.tiles) * p.chunk;
+        count = (int)min((int64_t)p.chunk, p.S - s0);
+    }
+    __device__ int64_t row(int i) const { return s0 + min(rl + i * rows, count - 1); }
+    __device__ bool has(int i) const { return ok && rl + i * rows < count; }
+    // rows that thread row r has
+    __device__ int of(int r) const { return r < count ? (count - r + rows - 1) / rows : 0; }
+    // channels of the tile, and groups of the set that are there
+    __device__ int channels(const GroupNormParams &p) const {
+        const int set_c = set * p.set_groups * p.D;
+        return min(p.tile, min(p.set_groups * p.D, p.C - set_c) - (part % p.tiles) * p.tile);
+    }
+    __device__ int groups(const GroupNormParams &p) const { return min(p.set_groups, p.G - set * p.set_groups); }
+};
+
+__device__ __forceinline__ unsigned draw_part(const GroupNormParams &p, unsigned *lds, unsigned parts) {
+    if (parts == 1) return blockIdx.x;
+    if (threadIdx.x == 0) *lds = atomicAdd(p.ticket, 1u) + 1u; // from all ones
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(*lds);
+}
+
+// A published pair is never all ones.
+__device__ __forceinline__ unsigned long long pair(float a, float b) {
+    const unsigned lo = __builtin_bit_cast(unsigned, a), hi = b != b ? 0x7FC00000u : __builtin_bit_cast(unsigned, b);
+    return (unsigned long long)hi << 32 | lo;
+}
+__device__ __forceinline__ unsigned long long wait_for(const unsigned long long *w) {
+    for (;;) {
+        const unsigned long long v = __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (v != ~0ull) return v;
+        __builtin_amdgcn_s_sleep(1);
+    }
+}
+
+// Publishes the part's pair of every group and returns all parts' pairs in all_a,
+// all_b [parts][groups] (this part's alone where it is the only one).
+__device__ __forceinline__ void exchange(const GroupNormParams &p, int64_t at, int part, int parts, int ng, int nt, const float *own_a,
+                                         const float *own_b, float *all_a, float *all_b) {
+    unsigned long long *w = p.words + at;
+    if (parts > 1)
+        for (int g = threadIdx.x; g < ng; g += nt)
+            __hip_atomic_store(w + (int64_t)part * p.set_groups + g, pair(own_a[g], own_b[g]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = threadIdx.x; i < parts * ng; i += nt) {
+        const int k = i / ng, g = i % ng;
+        if (k == part) { // (also all there is where nothing is published)
+            all_a[i] = own_a[g];
+            all_b[i] = own_b[g];
+        } else {
+            const unsigned long long v = wait_for(w + (int64_t)k * p.set_groups + g);
+            all_a[i] = __builtin_bit_cast(float, (unsigned)v);
+            all_b[i] = __builtin_bit_cast(float, (unsigned)(v >> 32));
+        }
+    }
+}
+
+constexpr int kTile = 256;       // channels a tile at most
+constexpr int kMostWords = kMostParts * 128; // pairs of a set: parts x groups
+
+template <typename T, int VEC, int E, int NT, bool GATE>
+__global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
+    __shared__ float lds[VEC * NT + 2 * kTile + 2 * kTile + 2 * kMostWords];
+    __shared__ unsigned drawn;
+    float *const red = lds, *const chan = red + VEC * NT, *const own = chan + 2 * kTile, *const all = own + 2 * kTile;
+    const int tid = threadIdx.x;
+    const Held<VEC, E, NT> at(p, draw_part(p, &drawn, (unsigned)(p.chunks * p.tiles)));
+    const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c;
+    const T *gate = static_cast<const T *>(p.gate) + at.n * p.sgn + at.c;
+    Raw<T, VEC> rx[E], rg[GATE ? E : 1];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        rx[i] = raw_n<T, VEC>(x + at.row(i) * p.sxs);
+        if constexpr (GATE) rg[i] = raw_n<T, VEC>(gate + at.row(i) * p.sgs);
+    }
+    const int nc = at.channels(p), ng = at.groups(p), gc = min(p.D, nc); // the tile's channels of a group
+    float wt[VEC], bs[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) wt[j] = 1.f, bs[j] = 0.f;
+    if (p.weight) load_n<float, VEC>(p.weight + at.c, wt);
+    if (p.bias) load_n<float, VEC>(p.bias + at.c, bs);
+
+    // the mean of every channel over the chunk, a thread's about its first row
+    const int mine = at.ok ? at.of(at.rl) : 0;
+    {
+        const float inv = mine ? 1.f / mine : 0.f;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float first = (float)rx[0][j];
+            float s = 0.f;
+#pragma unroll
+            for (int i = 1; i < E; ++i) s += at.has(i) ? (float)rx[i][j] - first : 0.f;
+            red[j * NT + tid] = __builtin_fmaf(s, inv, first);
+        }
+    }
+    __syncthreads();
+    // a channel's over the rows of threads; element c of the tile is in red[c % VEC] of lane c / VEC
+    auto column = [&](int c, int r) { return red[(c % VEC) * NT + r * p.lc + c / VEC]; };
+    for (int c = tid; c < nc; c += NT) {
+        const float base = column(c, 0);
+        float s = 0.f;
+        for (int r = 1; r < at.rows; ++r) {
+            const int k = at.of(r);
+            if (k > 0) s = __builtin_fmaf((float)k, column(c, r) - base, s);
+        }
+        chan[c] = base + s / (float)at.count;
+    }
+    __syncthreads();
+    for (int g = tid; g < ng; g += NT) { // a group's over its channels in the tile
+        const float base = chan[g * p.D];
+        float s = 0.f;
+        for (int c = 1; c < gc; ++c) s += chan[g * p.D + c] - base;
+        own[g] = base + s / (float)gc;
+    }
+    __syncthreads();
+    // squares about it
+    float m[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        m[j] = own[at.ok ? min(at.in_tile + j, nc - 1) / p.D : 0];
+        float q = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) {
+            const float d = at.has(i) ? (float)rx[i][j] - m[j] : 0.f;
+            q = __builtin_fmaf(d, d, q);
+        }
+        red[j * NT + tid] = q;
+    }
+    __syncthreads();
+    for (int c = tid; c < nc; c += NT) {
+        float s = 0.f;
+        for (int r = 0; r < at.rows; ++r) s += column(c, r);
+        chan[c] = s;
+    }
+    __syncthreads();
+    for (int g = tid; g < ng; g += NT) {
+        float s = 0.f;
+        for (int c = 0; c < gc; ++c) s += chan[g * p.D + c];
+        own[kTile + g] = s;
+    }
+    __syncthreads();
+    exchange(p, (at.n * p.sets + at.set) * at.parts * p.set_groups, at.part, at.parts, ng, NT, own, own + kTile, all, all + kMostWords);
+    __syncthreads();
+    // the groups' statistics, in chan
+    for (int g = tid; g < ng; g += NT) {
+        auto size = [&](int k) { // elements of part k
+            const int64_t rows = min((int64_t)p.chunk, p.S - (int64_t)(k / p.tiles) * p.chunk);
+            const int cols = p.tiles == 1 ? p.D : min(p.tile, p.D - (k % p.tiles) * p.tile);
+            return (float)rows * (float)cols;
+        };
+        const float base = all[g], total = (float)p.S * (float)p.D;
+        float s = 0.f, q = 0.f;
+        for (int k = 1; k < at.parts; ++k) s = __builtin_fmaf(size(k), all[k * ng + g] - base, s);
+        const float mean = base + s / total;
+        for (int k = 0; k < at.parts; ++k) {
+            const float d = all[k * ng + g] - mean;
+            q += __builtin_fmaf(size(k) * d, d, all[kMostWords + k * ng + g]);
+        }
+        const float rstd = 1.f / sqrtf(q / total + p.eps);
+        chan[g] = mean;
+        chan[kTile + g] = rstd;
+        if (p.stats && at.part == 0) {
+            float *st = p.stats + (at.n * p.G + at.set * p.set_groups + g) * 2;
+            st[0] = mean;
+            st[1] = rstd;
+        }
+    }
+    __syncthreads();
+    if (!at.ok) return;
+    float mean[VEC], rstd[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const int g = p.tiles == 1 ? (at.in_tile + j) / p.D : 0;
+        mean[j] = chan[g];
+        rstd[j] = chan[kTile + g];
+    }
+    T *y = static_cast<T *>(p.y) + at.n * p.sxn + at.c;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        if (!at.has(i)) break;
+        float z[VEC], a[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) z[j] = __builtin_fmaf(((float)rx[i][j] - mean[j]) * rstd[j], wt[j], bs[j]);
+        if constexpr (GATE) {
+            float gt[VEC];
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) gt[j] = (float)rg[i][j];
+            act_n<VEC>(p.act, gt, a);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) a[j] *= z[j];
+        } else {
+            act_n<VEC>(p.act, z, a);
+        }
+        store_n<T, VEC>(y + at.row(i) * p.sxs, a);
+    }
+}
+
+template <typename T, int VEC, int E, int NT, bool GATE>
+__global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
+    __shared__ float lds[2 * VEC * NT + 2 * kTile + 2 * kTile + 2 * kMostWords];
+    __shared__ unsigned drawn;
+    float *const red = lds, *const chan = red + 2 * VEC * NT, *const own = chan + 2 * kTile, *const all = own + 2 * kTile;
+    const int tid = threadIdx.x;
+    const Held<VEC, E, NT> at(p, draw_part(p, &drawn, (unsigned)(p.chunks * p.tiles)));
+    const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c, *dy = static_cast<const T *>(p.dy) + at.n * p.sxn + at.c;
+    const T *gate = static_cast<const T *>(p.gate) + at.n * p.sgn + at.c;
+    Raw<T, VEC> rx[E], ry[E], rg[GATE ? E : 1];
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        rx[i] = raw_n<T, VEC>(x + at.row(i) * p.sxs);
+        ry[i] = raw_n<T, VEC>(dy + at.row(i) * p.sxs);
+        if constexpr (GATE) rg[i] = raw_n<T, VEC>(gate + at.row(i) * p.sgs);
+    }
+    const int nc = at.channels(p), ng = at.groups(p), gc = min(p.D, nc);
+    const Channels<VEC> ch(p, at.n, at.c);
+    T *dgate = static_cast<T *>(p.dgate) + at.n * p.sgn + at.c;
+    // n and dz (and the gate's gradient) of row i
+    auto element = [&](int i, float *n, float *dz, float *dg) {
+        float vx[VEC], vy[VEC], vg[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            vx[j] = (float)rx[i][j];
+            vy[j] = (float)ry[i][j];
+            if constexpr (GATE) vg[j] = (float)rg[GATE ? i : 0][j];
+        }
+        dz_n<T, VEC, GATE>(p, ch, vx, vy, vg, n, dz, dg);
+    };
+    float a[VEC], b[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) a[j] = b[j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        if (!at.has(i)) break;
+        float n[VEC], dz[VEC], dg[VEC];
+        element(i, n, dz, dg);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            a[j] = __builtin_fmaf(dz[j], n[j], a[j]);
+            b[j] += dz[j];
+        }
+        if constexpr (GATE) store_n<T, VEC>(dgate + at.row(i) * p.sgs, dg);
+    }
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        red[j * NT + tid] = a[j];
+        red[(VEC + j) * NT + tid] = b[j];
+    }
+    __syncthreads();
+    {
+        // a part's sums of a channel go to part [sample][chunk][2][C] for the weights' gradients
+        const int tl = at.part % p.tiles, c0 = at.set * p.set_groups * p.D + tl * p.tile;
+        float *out = p.part ? p.part + (at.n * p.chunks + at.part / p.tiles) * 2 * p.C + c0 : nullptr;
+        for (int i = tid; i < 2 * nc; i += NT) {
+            const int c = i < nc ? i : i - nc;
+            const float *u = red + (i < nc ? 0 : VEC * NT) + (c % VEC) * NT + c / VEC;
+            float s = 0.f;
+            for (int r = 0; r < at.rows; ++r) s += u[r * p.lc];
+            if (out) out[i < nc ? c : p.C + c] = s;
+            chan[(i < nc ? 0 : kTile) + c] = p.weight ? s * p.weight[c0 + c] : s;
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < 2 * ng; i += NT) {
+        const int g = i < ng ? i : i - ng, o = i < ng ? 0 : kTile;
+        float s = 0.f;
+        for (int c = 0; c < gc; ++c) s += chan[o + g * p.D + c];
+        own[o + g] = s;
+    }
+    __syncthreads();
+    exchange(p, (at.n * p.sets + at.set) * at.parts * p.set_groups, at.part, at.parts, ng, NT, own, own + kTile, all, all + kMostWords);
+    __syncthreads();
+    for (int i = tid; i < 2 * ng; i += NT) {
+        const int g = i < ng ? i : i - ng;
+        const float *u = all + (i < ng ? 0 : kMostWords) + g;
+        float s = 0.f;
+        for (int k = 0; k < at.parts; ++k) s += u[k * ng];
+        chan[(i < ng ? 0 : kTile) + g] = s / ((float)p.S * (float)p.D);
+    }
+    __syncthreads();
+    if (!at.ok) return;
+    float s2[VEC], s1[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const int g = p.tiles == 1 ? (at.in_tile + j) / p.D : 0;
+        s2[j] = chan[g];
+        s1[j] = chan[kTile + g];
+    }
+    T *dx = static_cast<T *>(p.y) + at.n * p.sxn + at.c;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        if (!at.has(i)) break;
+        float n[VEC], dz[VEC], dg[VEC], o[VEC];
+        element(i, n, dz, dg);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) o[j] = ch.rstd[j] * (dz[j] * ch.wt[j] - s1[j] - n[j] * s2[j]);
+        store_n<T, VEC>(dx + at.row(i) * p.sxs, o);
+    }
+}
+
 // -- host ---------------------------------------------------------------------
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 struct Plan {
     bool rows; // S = 1 with groups that a wave holds
+    bool held; // groups that up to kMostParts workgroups hold
+    int e, nt; // rows a thread, threads
+    int tile, set_groups;
+    int64_t o_words, words; // bytes: the ticket and the words that parts publish
     int vec, nv, u, log_l, sets;
     int row_blocks;
     int lc, tiles, chunks, chunk;
@@ -596,6 +940,38 @@ int up_log2(int64_t n) {
     int k = 0;
     while ((int64_t(1) << k) < n) ++k;
     return k;
+}
+
+// The plan of a held group; false where it takes too many parts.
+constexpr int kRows3 = 16, kRows3Bwd = 12; // rows a thread of 512 (as many as leave no register in memory)
+bool hold(const gdn2_group_norm_args &a, bool bwd, int vec, Plan *q) {
+    const int G = (int)a.groups, D = (int)a.channels / G;
+    int unit = 1; // groups that make a multiple of vec channels
+    while ((int64_t)unit * D % vec) unit *= 2;
+    for (const int width : {128, 64}) { // channels of a set of whole groups
+        const int sg = std::max(unit, width / D / unit * unit);
+        if (width == 64 && sg == std::max(unit, 128 / D / unit * unit)) break;
+        q->set_groups = std::min(sg, G);
+        q->sets = (G + q->set_groups - 1) / q->set_groups;
+        const int64_t set_c = (int64_t)q->set_groups * D;
+        if (q->set_groups > 1 && set_c > kTile) return false;
+        q->tile = (int)std::min<int64_t>(set_c, kTile);
+        q->tiles = (int)((set_c + q->tile - 1) / q->tile);
+        q->lc = q->tile / vec;
+        const int forms[][2] = {{4, 256}, {8, 256}, {bwd ? kRows3Bwd : kRows3, 512}};
+        for (const auto &f : forms) { // the least that a thread holds
+            const int64_t chunk = (int64_t)(f[1] / q->lc) * f[0], chunks = (a.rows + chunk - 1) / chunk;
+            if (chunks * q->tiles > kMostParts) continue;
+            q->held = true;
+            q->vec = vec;
+            q->e = f[0];
+            q->nt = f[1];
+            q->chunk = (int)std::min<int64_t>(chunk, a.rows);
+            q->chunks = (int)chunks;
+            return true;
+        }
+    }
+    return false;
 }
 
 Plan plan_of(const gdn2_group_norm_args &a, bool bwd, bool vec4, bool sums_wanted) {
@@ -619,6 +995,13 @@ Plan plan_of(const gdn2_group_norm_args &a, bool bwd, bool vec4, bool sums_wante
         return q;
     }
     q.vec = vec4 && C % 4 == 0 ? 4 : 1;
+    if (hold(a, bwd, q.vec, &q) || (q.vec > 1 && hold(a, bwd, 1, &q))) {
+        size_t at = bwd && sums_wanted ? up256(8 * (size_t)(N * q.chunks) * C) : 0;
+        q.o_words = (int64_t)at;
+        q.words = q.chunks * q.tiles > 1 ? 256 + (int64_t)up256(8 * (size_t)(N * q.sets * q.chunks * q.tiles * q.set_groups)) : 0;
+        q.bytes = at + (size_t)q.words;
+        return q;
+    }
     // the widest tile that wastes at most an eighth of its lanes, or the one that wastes least
     const int64_t need = (C + q.vec - 1) / q.vec;
     int64_t best = 0;
@@ -691,6 +1074,14 @@ GroupNormParams fill(const gdn2_group_norm_args &a, const Plan &q, void *ws) {
     p.log_l = q.log_l; p.row_blocks = q.row_blocks; p.lc = q.lc; p.chunks = q.chunks; p.chunk = q.chunk;
     char *w = static_cast<char *>(ws);
     if (q.bytes) p.part = reinterpret_cast<float *>(w);
+    if (q.held) {
+        p.tile = q.tile; p.tiles = q.tiles; p.sets = q.sets; p.set_groups = q.set_groups;
+        if (q.words) {
+            p.ticket = reinterpret_cast<unsigned *>(w + q.o_words);
+            p.words = reinterpret_cast<unsigned long long *>(w + q.o_words + 256);
+        }
+        if (q.o_words == 0) p.part = nullptr;
+    }
     return p;
 }
 
@@ -709,12 +1100,30 @@ template <typename T, int VEC, bool GATE> hipError_t run_rows_bwd(const Plan &q,
     return hipGetLastError();
 }
 
+template <typename T, int VEC, int E, int NT, bool GATE, bool BWD> void launch_held(const Plan &q, const GroupNormParams &p, hipStream_t s) {
+    const dim3 grid((unsigned)(p.N * q.sets * q.chunks * q.tiles));
+    if constexpr (BWD) hipLaunchKernelGGL((norm_held_bwd_kernel<T, VEC, E, NT, GATE>), grid, dim3(NT), 0, s, p);
+    else hipLaunchKernelGGL((norm_held_kernel<T, VEC, E, NT, GATE>), grid, dim3(NT), 0, s, p);
+}
+template <typename T, int VEC, bool GATE, bool BWD> hipError_t run_held(const Plan &q, const GroupNormParams &p, hipStream_t s) {
+    if (q.words) {
+        const int64_t n16 = q.words / 16;
+        hipLaunchKernelGGL(norm_prepare_kernel, dim3((unsigned)std::min<int64_t>((n16 + 255) / 256, 1024)), dim3(256), 0, s,
+                           reinterpret_cast<uint4 *>(p.ticket), n16);
+    }
+    if (q.e == 4) launch_held<T, VEC, 4, 256, GATE, BWD>(q, p, s);
+    else if (q.e == 8) launch_held<T, VEC, 8, 256, GATE, BWD>(q, p, s);
+    else launch_held<T, VEC, BWD ? kRows3Bwd : kRows3, 512, GATE, BWD>(q, p, s);
+    return hipGetLastError();
+}
+
 gdn2_status refuse(const char *who, const char *what, gdn2_status st = GDN2_EINVAL) {
     return fail(st, std::string(who) + ": " + what);
 }
 
 template <typename T, int VEC> hipError_t run_forward(const Plan &q, const GroupNormParams &p, hipStream_t s) {
     if (q.rows) return p.gate ? run_rows<T, VEC, true>(q, p, s) : run_rows<T, VEC, false>(q, p, s);
+    if (q.held) return p.gate ? run_held<T, VEC, true, false>(q, p, s) : run_held<T, VEC, false, false>(q, p, s);
     const dim3 grid((unsigned)(p.N * q.chunks), (unsigned)q.tiles);
     hipLaunchKernelGGL((norm_moments_kernel<T, VEC>), grid, dim3(256), 0, s, p);
     hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)(p.N * p.G)), dim3(256), 0, s, p);
@@ -727,6 +1136,9 @@ template <typename T, int VEC, bool GATE> hipError_t run_backward(const Plan &q,
     int64_t blocks = q.row_blocks;
     if (q.rows) {
         if (const hipError_t e = run_rows_bwd<T, VEC, GATE>(q, p, s); e != hipSuccess) return e;
+    } else if (q.held) {
+        if (const hipError_t e = run_held<T, VEC, GATE, true>(q, p, s); e != hipSuccess) return e;
+        blocks = p.N * q.chunks;
     } else {
         const dim3 grid((unsigned)(p.N * q.chunks), (unsigned)q.tiles);
         hipLaunchKernelGGL((norm_bwd_sums_kernel<T, VEC, GATE>), grid, dim3(256), 0, s, p);
@@ -742,6 +1154,7 @@ template <typename T, int VEC, bool GATE> hipError_t run_backward(const Plan &q,
 
 bool grid_fits(const gdn2_group_norm_args &a, const Plan &q) {
     if (q.rows) return q.sets < 65536;
+    if (q.held) return (double)a.samples * q.sets * q.chunks * q.tiles * (q.nt / 256) < 16777216.0;
     return (double)a.samples * q.chunks < 16777216.0 && q.tiles < 65536;
 }
 
@@ -757,7 +1170,7 @@ template <typename T> gdn2_status forward(const char *who, const gdn2_group_norm
     if (q.bytes > 0 && (!a->workspace || a->workspace_bytes < q.bytes || !aligned(a->workspace, 256)))
         return refuse(who, "workspace missing, too small or not 256-byte aligned");
     GroupNormParams p = fill(*a, q, a->workspace);
-    if (!q.rows && !p.stats) p.stats = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + q.o_stats);
+    if (!q.rows && !q.held && !p.stats) p.stats = reinterpret_cast<float *>(static_cast<char *>(a->workspace) + q.o_stats);
     GDN2_HIP_CHECK((q.vec == 4 ? run_forward<T, 4>(q, p, s) : run_forward<T, 1>(q, p, s)));
     return GDN2_OK;
 }

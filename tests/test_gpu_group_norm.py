@@ -63,6 +63,9 @@ CASES = [  # N, S, C, groups
     (70, 1, 320, 32), (5, 1, 500, 2), (3, 1, 2048, 1), (4, 1, 4096, 1), (3, 1, 5000, 2), (2, 1, 8192, 1), (3, 1, 1001, 1),
     (2, 1, 1500, 1), (600, 1, 64, 4), (3, 2, 64, 4), (2, 5, 10, 2), (1, 9, 33, 3), (2, 100, 320, 32), (1, 257, 1024, 32),
     (3, 64, 7, 1), (4, 1000, 64, 8), (1, 5000, 12, 3), (2, 33, 1100, 4), (300, 3, 40, 4),
+    # a group held by several workgroups: by rows, by channels, by both; too many for that; odd widths
+    (2, 513, 128, 4), (1, 4096, 128, 1), (2, 4097, 64, 2), (1, 2100, 512, 1), (2, 40, 4100, 1), (1, 700, 1500, 3),
+    (2, 600, 264, 8), (2, 90, 500, 2), (3, 37, 65, 5), (1, 3100, 96, 32), (1, 9000, 24, 2), (2, 17, 130, 2), (5, 8, 9, 9),
 ]
 
 
