@@ -598,11 +598,15 @@ __global__ __launch_bounds__(256) void norm_prepare_kernel(uint4 *words, int64_t
 // A part of a set of groups: E rows a thread of VEC channels, lc lanes along the
 // tile's channels.  Parts are numbered by a ticket, a set's next to each other: at
 // most one set of a running kernel is not drawn completely, so that at most
-// kMostParts - 1 of its workgroups wait for one that has not started.  They are
-// few enough to leave room on the chip (256 workgroups at least) for it to start,
-// with as many kernels at once.
-constexpr int kMostParts = 16;
-template <int VEC, int E, int NT> struct Held {
+// kMostParts - 1 of its workgroups wait for one that has not started.  They leave
+// room on the chip for it to start: two workgroups a compute unit fit at least
+// (256 threads of 256 registers), 512, more than 16 such kernels at once can
+// have waiting.
+constexpr int kMostParts = 32;
+constexpr int NT = 256;     // threads
+constexpr int kTile = 256;  // channels a tile at most
+constexpr int kSet = 128;   // groups a set at most
+template <int VEC, int E> struct Held {
     int c, in_tile, rl, rows; // the lane's first channel, that in its tile; its row and the rows at a time
     int set, part, parts, count; // rows of this chunk
     bool ok;
@@ -657,37 +661,51 @@ __device__ __forceinline__ unsigned long long wait_for(const unsigned long long 
     }
 }
 
-// Publishes the part's pair of every group and returns all parts' pairs in all_a,
-// all_b [parts][groups] (this part's alone where it is the only one).
-__device__ __forceinline__ void exchange(const GroupNormParams &p, int64_t at, int part, int parts, int ng, int nt, const float *own_a,
-                                         const float *own_b, float *all_a, float *all_b) {
-    unsigned long long *w = p.words + at;
-    if (parts > 1)
-        for (int g = threadIdx.x; g < ng; g += nt)
-            __hip_atomic_store(w + (int64_t)part * p.set_groups + g, pair(own_a[g], own_b[g]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int i = threadIdx.x; i < parts * ng; i += nt) {
-        const int k = i / ng, g = i % ng;
-        if (k == part) { // (also all there is where nothing is published)
-            all_a[i] = own_a[g];
-            all_b[i] = own_b[g];
+// The threads that work on a group: `share` neighbouring lanes of a wave, a power
+// of two.
+struct GroupLanes {
+    int share, g, t;
+    bool ok;
+    __device__ explicit GroupLanes(int ng) {
+        share = 64;
+        while (share * ng > NT) share /= 2; // (at most kSet groups)
+        g = (int)threadIdx.x / share;
+        t = (int)threadIdx.x % share;
+        ok = g < ng;
+        g = ok ? g : 0;
+    }
+    __device__ float sum(float v) const { // to all of them
+        for (int o = 1; o < share; o <<= 1) v += __shfl_xor(v, o, kWave);
+        return v;
+    }
+};
+
+// Publishes the part's pair of the group and calls f(k, pair of part k) for the
+// parts k that fall to this lane, in order.
+template <typename F> __device__ __forceinline__ void each_part(const GroupNormParams &p, const GroupLanes &gl, int64_t set, int part, int parts,
+                                                                float a, float b, F f) {
+    if (!gl.ok) return;
+    unsigned long long *w = p.words + set * parts * p.set_groups + gl.g;
+    if (parts > 1 && gl.t == 0)
+        __hip_atomic_store(w + (int64_t)part * p.set_groups, pair(a, b), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int k = gl.t; k < parts; k += gl.share) {
+        if (k == part) {
+            f(k, a, b);
         } else {
-            const unsigned long long v = wait_for(w + (int64_t)k * p.set_groups + g);
-            all_a[i] = __builtin_bit_cast(float, (unsigned)v);
-            all_b[i] = __builtin_bit_cast(float, (unsigned)(v >> 32));
+            const unsigned long long v = wait_for(w + (int64_t)k * p.set_groups);
+            f(k, __builtin_bit_cast(float, (unsigned)v), __builtin_bit_cast(float, (unsigned)(v >> 32)));
         }
     }
 }
 
-constexpr int kTile = 256;       // channels a tile at most
-constexpr int kMostWords = kMostParts * 128; // pairs of a set: parts x groups
-
-template <typename T, int VEC, int E, int NT, bool GATE>
+template <typename T, int VEC, int E, bool GATE>
 __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
-    __shared__ float lds[VEC * NT + 2 * kTile + 2 * kTile + 2 * kMostWords];
+    // sums and squares of a thread's channels; afterwards the parts' means and squares
+    __shared__ float red[2][VEC * NT > kMostParts * kSet ? VEC * NT : kMostParts * kSet];
+    __shared__ float first[kSet], stat[2][kSet];
     __shared__ unsigned drawn;
-    float *const red = lds, *const chan = red + VEC * NT, *const own = chan + 2 * kTile, *const all = own + 2 * kTile;
     const int tid = threadIdx.x;
-    const Held<VEC, E, NT> at(p, draw_part(p, &drawn, (unsigned)(p.chunks * p.tiles)));
+    const Held<VEC, E> at(p, draw_part(p, &drawn, (unsigned)(p.chunks * p.tiles)));
     const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c;
     const T *gate = static_cast<const T *>(p.gate) + at.n * p.sgn + at.c;
     Raw<T, VEC> rx[E], rg[GATE ? E : 1];
@@ -697,105 +715,87 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
         if constexpr (GATE) rg[i] = raw_n<T, VEC>(gate + at.row(i) * p.sgs);
     }
     const int nc = at.channels(p), ng = at.groups(p), gc = min(p.D, nc); // the tile's channels of a group
+    const GroupLanes gl(ng);
     float wt[VEC], bs[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) wt[j] = 1.f, bs[j] = 0.f;
     if (p.weight) load_n<float, VEC>(p.weight + at.c, wt);
     if (p.bias) load_n<float, VEC>(p.bias + at.c, bs);
+    int group[VEC]; // of the set
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) group[j] = p.tiles == 1 && at.ok ? (at.in_tile + j) / p.D : 0;
 
-    // the mean of every channel over the chunk, a thread's about its first row
-    const int mine = at.ok ? at.of(at.rl) : 0;
-    {
-        const float inv = mine ? 1.f / mine : 0.f;
+    // Sums about a value of the group's, so that a large mean costs no digits.
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float first = (float)rx[0][j];
-            float s = 0.f;
-#pragma unroll
-            for (int i = 1; i < E; ++i) s += at.has(i) ? (float)rx[i][j] - first : 0.f;
-            red[j * NT + tid] = __builtin_fmaf(s, inv, first);
-        }
-    }
+    for (int j = 0; j < VEC; ++j)
+        if (at.ok && at.rl == 0 && (at.in_tile + j) % p.D == 0) first[group[j]] = (float)rx[0][j];
     __syncthreads();
-    // a channel's over the rows of threads; element c of the tile is in red[c % VEC] of lane c / VEC
-    auto column = [&](int c, int r) { return red[(c % VEC) * NT + r * p.lc + c / VEC]; };
-    for (int c = tid; c < nc; c += NT) {
-        const float base = column(c, 0);
-        float s = 0.f;
-        for (int r = 1; r < at.rows; ++r) {
-            const int k = at.of(r);
-            if (k > 0) s = __builtin_fmaf((float)k, column(c, r) - base, s);
-        }
-        chan[c] = base + s / (float)at.count;
-    }
-    __syncthreads();
-    for (int g = tid; g < ng; g += NT) { // a group's over its channels in the tile
-        const float base = chan[g * p.D];
-        float s = 0.f;
-        for (int c = 1; c < gc; ++c) s += chan[g * p.D + c] - base;
-        own[g] = base + s / (float)gc;
-    }
-    __syncthreads();
-    // squares about it
-    float m[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-        m[j] = own[at.ok ? min(at.in_tile + j, nc - 1) / p.D : 0];
-        float q = 0.f;
+        const float base = first[group[j]];
+        float s = 0.f, q = 0.f;
 #pragma unroll
         for (int i = 0; i < E; ++i) {
-            const float d = at.has(i) ? (float)rx[i][j] - m[j] : 0.f;
+            const float d = at.has(i) ? (float)rx[i][j] - base : 0.f;
+            s += d;
             q = __builtin_fmaf(d, d, q);
         }
-        red[j * NT + tid] = q;
+        red[0][j * NT + tid] = s;
+        red[1][j * NT + tid] = q;
     }
     __syncthreads();
-    for (int c = tid; c < nc; c += NT) {
-        float s = 0.f;
-        for (int r = 0; r < at.rows; ++r) s += column(c, r);
-        chan[c] = s;
-    }
-    __syncthreads();
-    for (int g = tid; g < ng; g += NT) {
-        float s = 0.f;
-        for (int c = 0; c < gc; ++c) s += chan[g * p.D + c];
-        own[kTile + g] = s;
-    }
-    __syncthreads();
-    exchange(p, (at.n * p.sets + at.set) * at.parts * p.set_groups, at.part, at.parts, ng, NT, own, own + kTile, all, all + kMostWords);
-    __syncthreads();
-    // the groups' statistics, in chan
-    for (int g = tid; g < ng; g += NT) {
-        auto size = [&](int k) { // elements of part k
-            const int64_t rows = min((int64_t)p.chunk, p.S - (int64_t)(k / p.tiles) * p.chunk);
-            const int cols = p.tiles == 1 ? p.D : min(p.tile, p.D - (k % p.tiles) * p.tile);
-            return (float)rows * (float)cols;
-        };
-        const float base = all[g], total = (float)p.S * (float)p.D;
-        float s = 0.f, q = 0.f;
-        for (int k = 1; k < at.parts; ++k) s = __builtin_fmaf(size(k), all[k * ng + g] - base, s);
-        const float mean = base + s / total;
-        for (int k = 0; k < at.parts; ++k) {
-            const float d = all[k * ng + g] - mean;
-            q += __builtin_fmaf(size(k) * d, d, all[kMostWords + k * ng + g]);
+    // channel c of the tile is at c % VEC of lane c / VEC, for every row of threads
+    float s = 0.f, q = 0.f;
+    if (gl.ok)
+        for (int c = gl.g * p.D + gl.t; c < gl.g * p.D + gc; c += gl.share) {
+            const int o = (c % VEC) * NT + c / VEC;
+#pragma unroll 4
+            for (int r = 0; r < at.rows; ++r) {
+                s += red[0][o + r * p.lc];
+                q += red[1][o + r * p.lc];
+            }
         }
-        const float rstd = 1.f / sqrtf(q / total + p.eps);
-        chan[g] = mean;
-        chan[kTile + g] = rstd;
+    s = gl.sum(s);
+    q = gl.sum(q);
+    const float base = first[gl.g], elements = (float)at.count * (float)gc;
+    __syncthreads(); // red is read
+    const float shift = s / elements, own = base + shift, own2 = fmaxf(__builtin_fmaf(-shift, s, q), q - q); // (a NaN stays)
+    float *const means = red[0], *const squares = red[1];
+    each_part(p, gl, at.n * p.sets + at.set, at.part, at.parts, own, own2, [&](int k, float a, float b) {
+        means[k * ng + gl.g] = a;
+        squares[k * ng + gl.g] = b;
+    });
+    auto size = [&](int k) { // elements of part k
+        const int64_t rows = min((int64_t)p.chunk, p.S - (int64_t)(k / p.tiles) * p.chunk);
+        return (float)rows * (float)(p.tiles == 1 ? p.D : min(p.tile, p.D - (k % p.tiles) * p.tile));
+    };
+    // (a lane reads what it wrote itself; sums about part 0's mean, the same in every part)
+    const float base0 = __shfl(gl.t == 0 ? means[gl.g] : 0.f, 0, gl.share);
+    s = 0.f;
+    for (int k = gl.t; gl.ok && k < at.parts; k += gl.share) s = __builtin_fmaf(size(k), means[k * ng + gl.g] - base0, s);
+    const float total = (float)p.S * (float)p.D, mean = base0 + gl.sum(s) / total;
+    q = 0.f;
+    for (int k = gl.t; gl.ok && k < at.parts; k += gl.share) {
+        const float d = means[k * ng + gl.g] - mean;
+        q += __builtin_fmaf(size(k) * d, d, squares[k * ng + gl.g]);
+    }
+    const float rstd = 1.f / sqrtf(gl.sum(q) / total + p.eps);
+    if (gl.ok && gl.t == 0) {
+        stat[0][gl.g] = mean;
+        stat[1][gl.g] = rstd;
         if (p.stats && at.part == 0) {
-            float *st = p.stats + (at.n * p.G + at.set * p.set_groups + g) * 2;
+            float *st = p.stats + (at.n * p.G + at.set * p.set_groups + gl.g) * 2;
             st[0] = mean;
             st[1] = rstd;
         }
     }
     __syncthreads();
     if (!at.ok) return;
-    float mean[VEC], rstd[VEC];
+    float m[VEC], rs[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-        const int g = p.tiles == 1 ? (at.in_tile + j) / p.D : 0;
-        mean[j] = chan[g];
-        rstd[j] = chan[kTile + g];
+        m[j] = stat[0][group[j]];
+        rs[j] = stat[1][group[j]];
     }
     T *y = static_cast<T *>(p.y) + at.n * p.sxn + at.c;
 #pragma unroll
@@ -803,7 +803,7 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
         if (!at.has(i)) break;
         float z[VEC], a[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) z[j] = __builtin_fmaf(((float)rx[i][j] - mean[j]) * rstd[j], wt[j], bs[j]);
+        for (int j = 0; j < VEC; ++j) z[j] = __builtin_fmaf(((float)rx[i][j] - m[j]) * rs[j], wt[j], bs[j]);
         if constexpr (GATE) {
             float gt[VEC];
 #pragma unroll
@@ -818,13 +818,13 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
     }
 }
 
-template <typename T, int VEC, int E, int NT, bool GATE>
+template <typename T, int VEC, int E, bool GATE>
 __global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
-    __shared__ float lds[2 * VEC * NT + 2 * kTile + 2 * kTile + 2 * kMostWords];
+    __shared__ float red[2][VEC * NT]; // sums of dz n and dz of a thread's channels
+    __shared__ float stat[2][kSet];
     __shared__ unsigned drawn;
-    float *const red = lds, *const chan = red + 2 * VEC * NT, *const own = chan + 2 * kTile, *const all = own + 2 * kTile;
     const int tid = threadIdx.x;
-    const Held<VEC, E, NT> at(p, draw_part(p, &drawn, (unsigned)(p.chunks * p.tiles)));
+    const Held<VEC, E> at(p, draw_part(p, &drawn, (unsigned)(p.chunks * p.tiles)));
     const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c, *dy = static_cast<const T *>(p.dy) + at.n * p.sxn + at.c;
     const T *gate = static_cast<const T *>(p.gate) + at.n * p.sgn + at.c;
     Raw<T, VEC> rx[E], ry[E], rg[GATE ? E : 1];
@@ -835,6 +835,7 @@ __global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
         if constexpr (GATE) rg[i] = raw_n<T, VEC>(gate + at.row(i) * p.sgs);
     }
     const int nc = at.channels(p), ng = at.groups(p), gc = min(p.D, nc);
+    const GroupLanes gl(ng);
     const Channels<VEC> ch(p, at.n, at.c);
     T *dgate = static_cast<T *>(p.dgate) + at.n * p.sgn + at.c;
     // n and dz (and the gate's gradient) of row i
@@ -865,48 +866,54 @@ __global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
     }
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
-        red[j * NT + tid] = a[j];
-        red[(VEC + j) * NT + tid] = b[j];
+        red[0][j * NT + tid] = a[j];
+        red[1][j * NT + tid] = b[j];
     }
     __syncthreads();
-    {
-        // a part's sums of a channel go to part [sample][chunk][2][C] for the weights' gradients
-        const int tl = at.part % p.tiles, c0 = at.set * p.set_groups * p.D + tl * p.tile;
-        float *out = p.part ? p.part + (at.n * p.chunks + at.part / p.tiles) * 2 * p.C + c0 : nullptr;
-        for (int i = tid; i < 2 * nc; i += NT) {
-            const int c = i < nc ? i : i - nc;
-            const float *u = red + (i < nc ? 0 : VEC * NT) + (c % VEC) * NT + c / VEC;
-            float s = 0.f;
-            for (int r = 0; r < at.rows; ++r) s += u[r * p.lc];
-            if (out) out[i < nc ? c : p.C + c] = s;
-            chan[(i < nc ? 0 : kTile) + c] = p.weight ? s * p.weight[c0 + c] : s;
+    // A channel's sums over the part go to part [sample][chunk][2][C] for the weights'
+    // gradients, times its weight into the group's.
+    const int c0 = at.set * p.set_groups * p.D + at.part % p.tiles * p.tile;
+    float *out = p.part ? p.part + (at.n * p.chunks + at.part / p.tiles) * 2 * p.C + c0 : nullptr;
+    float s2 = 0.f, s1 = 0.f;
+    if (gl.ok)
+        for (int c = gl.g * p.D + gl.t; c < gl.g * p.D + gc; c += gl.share) {
+            const int o = (c % VEC) * NT + c / VEC;
+            const float w = p.weight ? p.weight[c0 + c] : 1.f;
+            float u = 0.f, v = 0.f;
+#pragma unroll 4
+            for (int r = 0; r < at.rows; ++r) {
+                u += red[0][o + r * p.lc];
+                v += red[1][o + r * p.lc];
+            }
+            if (out) {
+                out[c] = u;
+                out[p.C + c] = v;
+            }
+            s2 = __builtin_fmaf(u, w, s2);
+            s1 = __builtin_fmaf(v, w, s1);
         }
-    }
-    __syncthreads();
-    for (int i = tid; i < 2 * ng; i += NT) {
-        const int g = i < ng ? i : i - ng, o = i < ng ? 0 : kTile;
-        float s = 0.f;
-        for (int c = 0; c < gc; ++c) s += chan[o + g * p.D + c];
-        own[o + g] = s;
-    }
-    __syncthreads();
-    exchange(p, (at.n * p.sets + at.set) * at.parts * p.set_groups, at.part, at.parts, ng, NT, own, own + kTile, all, all + kMostWords);
-    __syncthreads();
-    for (int i = tid; i < 2 * ng; i += NT) {
-        const int g = i < ng ? i : i - ng;
-        const float *u = all + (i < ng ? 0 : kMostWords) + g;
-        float s = 0.f;
-        for (int k = 0; k < at.parts; ++k) s += u[k * ng];
-        chan[(i < ng ? 0 : kTile) + g] = s / ((float)p.S * (float)p.D);
+    s2 = gl.sum(s2);
+    s1 = gl.sum(s1);
+    float t2 = 0.f, t1 = 0.f;
+    each_part(p, gl, at.n * p.sets + at.set, at.part, at.parts, s2, s1, [&](int, float u, float v) {
+        t2 += u;
+        t1 += v;
+    });
+    t2 = gl.sum(t2);
+    t1 = gl.sum(t1);
+    if (gl.ok && gl.t == 0) {
+        const float size = (float)p.S * (float)p.D;
+        stat[0][gl.g] = t2 / size;
+        stat[1][gl.g] = t1 / size;
     }
     __syncthreads();
     if (!at.ok) return;
-    float s2[VEC], s1[VEC];
+    float m2[VEC], m1[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         const int g = p.tiles == 1 ? (at.in_tile + j) / p.D : 0;
-        s2[j] = chan[g];
-        s1[j] = chan[kTile + g];
+        m2[j] = stat[0][g];
+        m1[j] = stat[1][g];
     }
     T *dx = static_cast<T *>(p.y) + at.n * p.sxn + at.c;
 #pragma unroll
@@ -915,7 +922,7 @@ __global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
         float n[VEC], dz[VEC], dg[VEC], o[VEC];
         element(i, n, dz, dg);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) o[j] = ch.rstd[j] * (dz[j] * ch.wt[j] - s1[j] - n[j] * s2[j]);
+        for (int j = 0; j < VEC; ++j) o[j] = ch.rstd[j] * (dz[j] * ch.wt[j] - m1[j] - n[j] * m2[j]);
         store_n<T, VEC>(dx + at.row(i) * p.sxs, o);
     }
 }
@@ -927,7 +934,7 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 struct Plan {
     bool rows; // S = 1 with groups that a wave holds
     bool held; // groups that up to kMostParts workgroups hold
-    int e, nt; // rows a thread, threads
+    int e; // rows a thread
     int tile, set_groups;
     int64_t o_words, words; // bytes: the ticket and the words that parts publish
     int vec, nv, u, log_l, sets;
@@ -943,7 +950,7 @@ int up_log2(int64_t n) {
 }
 
 // The plan of a held group; false where it takes too many parts.
-constexpr int kRows3 = 16, kRows3Bwd = 12; // rows a thread of 512 (as many as leave no register in memory)
+constexpr int kRows3 = 16, kRows3Bwd = 12; // rows a thread at most (as many as leave no register in memory)
 bool hold(const gdn2_group_norm_args &a, bool bwd, int vec, Plan *q) {
     const int G = (int)a.groups, D = (int)a.channels / G;
     int unit = 1; // groups that make a multiple of vec channels
@@ -958,14 +965,12 @@ bool hold(const gdn2_group_norm_args &a, bool bwd, int vec, Plan *q) {
         q->tile = (int)std::min<int64_t>(set_c, kTile);
         q->tiles = (int)((set_c + q->tile - 1) / q->tile);
         q->lc = q->tile / vec;
-        const int forms[][2] = {{4, 256}, {8, 256}, {bwd ? kRows3Bwd : kRows3, 512}};
-        for (const auto &f : forms) { // the least that a thread holds
-            const int64_t chunk = (int64_t)(f[1] / q->lc) * f[0], chunks = (a.rows + chunk - 1) / chunk;
+        for (const int e : {4, 8, bwd ? kRows3Bwd : kRows3}) { // the least that a thread holds
+            const int64_t chunk = (int64_t)(NT / q->lc) * e, chunks = (a.rows + chunk - 1) / chunk;
             if (chunks * q->tiles > kMostParts) continue;
             q->held = true;
             q->vec = vec;
-            q->e = f[0];
-            q->nt = f[1];
+            q->e = e;
             q->chunk = (int)std::min<int64_t>(chunk, a.rows);
             q->chunks = (int)chunks;
             return true;
@@ -1100,10 +1105,10 @@ template <typename T, int VEC, bool GATE> hipError_t run_rows_bwd(const Plan &q,
     return hipGetLastError();
 }
 
-template <typename T, int VEC, int E, int NT, bool GATE, bool BWD> void launch_held(const Plan &q, const GroupNormParams &p, hipStream_t s) {
+template <typename T, int VEC, int E, bool GATE, bool BWD> void launch_held(const Plan &q, const GroupNormParams &p, hipStream_t s) {
     const dim3 grid((unsigned)(p.N * q.sets * q.chunks * q.tiles));
-    if constexpr (BWD) hipLaunchKernelGGL((norm_held_bwd_kernel<T, VEC, E, NT, GATE>), grid, dim3(NT), 0, s, p);
-    else hipLaunchKernelGGL((norm_held_kernel<T, VEC, E, NT, GATE>), grid, dim3(NT), 0, s, p);
+    if constexpr (BWD) hipLaunchKernelGGL((norm_held_bwd_kernel<T, VEC, E, GATE>), grid, dim3(NT), 0, s, p);
+    else hipLaunchKernelGGL((norm_held_kernel<T, VEC, E, GATE>), grid, dim3(NT), 0, s, p);
 }
 template <typename T, int VEC, bool GATE, bool BWD> hipError_t run_held(const Plan &q, const GroupNormParams &p, hipStream_t s) {
     if (q.words) {
@@ -1111,9 +1116,9 @@ template <typename T, int VEC, bool GATE, bool BWD> hipError_t run_held(const Pl
         hipLaunchKernelGGL(norm_prepare_kernel, dim3((unsigned)std::min<int64_t>((n16 + 255) / 256, 1024)), dim3(256), 0, s,
                            reinterpret_cast<uint4 *>(p.ticket), n16);
     }
-    if (q.e == 4) launch_held<T, VEC, 4, 256, GATE, BWD>(q, p, s);
-    else if (q.e == 8) launch_held<T, VEC, 8, 256, GATE, BWD>(q, p, s);
-    else launch_held<T, VEC, BWD ? kRows3Bwd : kRows3, 512, GATE, BWD>(q, p, s);
+    if (q.e == 4) launch_held<T, VEC, 4, GATE, BWD>(q, p, s);
+    else if (q.e == 8) launch_held<T, VEC, 8, GATE, BWD>(q, p, s);
+    else launch_held<T, VEC, BWD ? kRows3Bwd : kRows3, GATE, BWD>(q, p, s);
     return hipGetLastError();
 }
 
@@ -1154,7 +1159,7 @@ template <typename T, int VEC, bool GATE> hipError_t run_backward(const Plan &q,
 
 bool grid_fits(const gdn2_group_norm_args &a, const Plan &q) {
     if (q.rows) return q.sets < 65536;
-    if (q.held) return (double)a.samples * q.sets * q.chunks * q.tiles * (q.nt / 256) < 16777216.0;
+    if (q.held) return (double)a.samples * q.sets * q.chunks * q.tiles < 16777216.0;
     return (double)a.samples * q.chunks < 16777216.0 && q.tiles < 65536;
 }
 
