@@ -517,8 +517,7 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
                         float sum = 0.f;
 #pragma unroll
                         for (int j = 0; j < VEC; ++j) sum += xg[j];
-#pragma unroll
-                        for (int o = 1; o < LC; o <<= 1) sum += __shfl_xor(sum, o, 64);
+                        sum = lanes_sum(sum, __builtin_ctz(LC));
                         if (cl == 0 && row) {
                             if (p.dgp) p.dgp[(((int64_t)q.b * p.units + q.un) * p.T + token(q, i)) * p.tiles_c + q.ct] = sum;
                             else *at_g(q, quick, i, p.dg) = sum;

@@ -85,12 +85,6 @@ template <int N> __device__ __forceinline__ void act_grad_n(int act, const float
     }
 }
 
-// Sum over the 2^log_l lanes of a group, to all of them.
-__device__ __forceinline__ float lanes_sum(float v, int log_l) {
-    for (int o = 1; o < 1 << log_l; o <<= 1) v += __shfl_xor(v, o, kWave);
-    return v;
-}
-
 // The place of a lane: VEC channels from c of the wave's groups, chunk k of NV.
 template <int VEC, int NV> struct Lanes {
     int g, c[NV];
@@ -134,33 +128,42 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(GroupNormParams p) {
         if (p.bias) load_n<float, VEC>(p.bias + at.c[k], bs[k]);
     }
     const float inv_d = 1.f / p.D;
+    float x[U][NV][VEC], mean[U], rstd[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-        float x[NV][VEC], sum = 0.f;
+        mean[u] = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                x[k][j] = at.ok[k] ? (float)rx[u][k][j] : 0.f;
-                sum += x[k][j];
+                x[u][k][j] = at.ok[k] ? (float)rx[u][k][j] : 0.f;
+                mean[u] += x[u][k][j];
             }
-        const float mean = lanes_sum(sum, p.log_l) * inv_d;
-        float sq = 0.f;
+    }
+    lanes_sum<U>(mean, p.log_l);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        mean[u] *= inv_d;
+        rstd[u] = 0.f;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                x[k][j] -= mean;
-                sq = at.ok[k] ? __builtin_fmaf(x[k][j], x[k][j], sq) : sq;
+                x[u][k][j] = at.ok[k] ? x[u][k][j] - mean[u] : 0.f;
+                rstd[u] = __builtin_fmaf(x[u][k][j], x[u][k][j], rstd[u]);
             }
-        const float rstd = 1.f / sqrtf(__builtin_fmaf(lanes_sum(sq, p.log_l), inv_d, p.eps));
+    }
+    lanes_sum<U>(rstd, p.log_l);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        rstd[u] = 1.f / sqrtf(__builtin_fmaf(rstd[u], inv_d, p.eps));
         const int64_t n = n0 + u;
         if (n >= p.N) break;
 #pragma unroll
         for (int k = 0; k < NV; ++k) {
             float z[VEC], a[VEC];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) z[j] = __builtin_fmaf(x[k][j] * rstd, wt[k][j], bs[k][j]);
+            for (int j = 0; j < VEC; ++j) z[j] = __builtin_fmaf(x[u][k][j] * rstd[u], wt[k][j], bs[k][j]);
             if constexpr (GATE) {
                 float gt[VEC];
 #pragma unroll
@@ -174,16 +177,16 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(GroupNormParams p) {
             if (at.ok[k]) store_n<T, VEC>(static_cast<T *>(p.y) + n * p.sxn + at.c[k], a);
         }
         if (p.stats && at.g < p.G && (lane & ((1 << p.log_l) - 1)) == 0) {
-            p.stats[(n * p.G + at.g) * 2] = mean;
-            p.stats[(n * p.G + at.g) * 2 + 1] = rstd;
+            p.stats[(n * p.G + at.g) * 2] = mean[u];
+            p.stats[(n * p.G + at.g) * 2 + 1] = rstd[u];
         }
     }
 }
 
-// S = 1, adjoint.  A wave walks rows wave, wave + 4, ... of its workgroup's
-// block of them and keeps dweight and dbias of its channels in registers; the
+// S = 1, adjoint.  A workgroup's waves walk its block of rows, U at a time each,
+// the next ones' loads in flight, and keep dweight and dbias of its channels in registers; the
 // workgroup's go to part [row_blocks][2][C].
-template <typename T, int VEC, int NV, bool GATE>
+template <typename T, int VEC, int NV, int U, bool GATE>
 __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(GroupNormParams p) {
     __shared__ float red[2][4][kWave * VEC * NV];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -199,67 +202,81 @@ __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(GroupNormParams p) {
     }
     const float inv_d = 1.f / p.D;
     const int gs = min(at.g, p.G - 1);
-    struct Row {
-        Raw<T, VEC> x[NV], dy[NV], gate[GATE ? NV : 1];
-        float mean, rstd;
+    struct Rows {
+        Raw<T, VEC> x[U][NV], dy[U][NV], gate[U][GATE ? NV : 1];
+        float mean[U], rstd[U];
     };
-    auto load = [&](int64_t n, Row &r) {
+    auto load = [&](int64_t first, Rows &r) {
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            r.x[k] = raw_n<T, VEC>(static_cast<const T *>(p.x) + n * p.sxn + at.c[k]);
-            r.dy[k] = raw_n<T, VEC>(static_cast<const T *>(p.dy) + n * p.sxn + at.c[k]);
-            if constexpr (GATE) r.gate[k] = raw_n<T, VEC>(static_cast<const T *>(p.gate) + n * p.sgn + at.c[k]);
-        }
-        r.mean = p.stats[(n * p.G + gs) * 2];
-        r.rstd = p.stats[(n * p.G + gs) * 2 + 1];
-    };
-    Row next;
-    if (n0 + wave < n1) load(n0 + wave, next);
-    for (int64_t n = n0 + wave; n < n1; n += 4) {
-        const Row r = next;
-        load(min(n + 4, n1 - 1), next);
-        float nn[NV][VEC], dn[NV][VEC], s1 = 0.f, s2 = 0.f;
+        for (int u = 0; u < U; ++u) {
+            const int64_t n = min(first + u, n1 - 1);
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            float z[VEC], a[VEC], d[VEC], dz[VEC];
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                nn[k][j] = ((float)r.x[k][j] - r.mean) * r.rstd;
-                z[j] = __builtin_fmaf(nn[k][j], wt[k][j], bs[k][j]);
+            for (int k = 0; k < NV; ++k) {
+                r.x[u][k] = raw_n<T, VEC>(static_cast<const T *>(p.x) + n * p.sxn + at.c[k]);
+                r.dy[u][k] = raw_n<T, VEC>(static_cast<const T *>(p.dy) + n * p.sxn + at.c[k]);
+                if constexpr (GATE) r.gate[u][k] = raw_n<T, VEC>(static_cast<const T *>(p.gate) + n * p.sgn + at.c[k]);
             }
-            if constexpr (GATE) {
-                float gt[VEC], dg[VEC];
+            r.mean[u] = p.stats[(n * p.G + gs) * 2];
+            r.rstd[u] = p.stats[(n * p.G + gs) * 2 + 1];
+        }
+    };
+    Rows next;
+    if (n0 + wave * U < n1) load(n0 + wave * U, next);
+    for (int64_t first = n0 + wave * U; first < n1; first += 4 * U) {
+        const Rows r = next;
+        load(min(first + 4 * U, n1 - 1), next);
+        float nn[U][NV][VEC], dn[U][NV][VEC], s[2 * U]; // sums of dn, of dn n
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) gt[j] = (float)r.gate[k][j];
-                act_grad_n<VEC>(p.act, gt, a, d);
+        for (int u = 0; u < U; ++u) {
+            const int64_t n = first + u;
+            const bool in = n < n1;
+            s[2 * u] = s[2 * u + 1] = 0.f;
+#pragma unroll
+            for (int k = 0; k < NV; ++k) {
+                float z[VEC], a[VEC], d[VEC], dz[VEC];
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    dg[j] = (float)r.dy[k][j] * z[j] * d[j];
-                    dz[j] = (float)r.dy[k][j] * a[j];
+                    nn[u][k][j] = ((float)r.x[u][k][j] - r.mean[u]) * r.rstd[u];
+                    z[j] = __builtin_fmaf(nn[u][k][j], wt[k][j], bs[k][j]);
                 }
-                if (at.ok[k]) store_n<T, VEC>(static_cast<T *>(p.dgate) + n * p.sgn + at.c[k], dg);
-            } else {
-                act_grad_n<VEC>(p.act, z, a, d);
+                if constexpr (GATE) {
+                    float gt[VEC], dg[VEC];
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) dz[j] = (float)r.dy[k][j] * d[j];
-            }
+                    for (int j = 0; j < VEC; ++j) gt[j] = (float)r.gate[u][k][j];
+                    act_grad_n<VEC>(p.act, gt, a, d);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                dwt[k][j] = __builtin_fmaf(dz[j], nn[k][j], dwt[k][j]);
-                dbs[k][j] += dz[j];
-                dn[k][j] = dz[j] * wt[k][j];
-                s1 += at.ok[k] ? dn[k][j] : 0.f;
-                s2 = at.ok[k] ? __builtin_fmaf(dn[k][j], nn[k][j], s2) : s2;
+                    for (int j = 0; j < VEC; ++j) {
+                        dg[j] = (float)r.dy[u][k][j] * z[j] * d[j];
+                        dz[j] = (float)r.dy[u][k][j] * a[j];
+                    }
+                    if (in && at.ok[k]) store_n<T, VEC>(static_cast<T *>(p.dgate) + n * p.sgn + at.c[k], dg);
+                } else {
+                    act_grad_n<VEC>(p.act, z, a, d);
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) dz[j] = (float)r.dy[u][k][j] * d[j];
+                }
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    dz[j] = in ? dz[j] : 0.f;
+                    dwt[k][j] = in ? __builtin_fmaf(dz[j], nn[u][k][j], dwt[k][j]) : dwt[k][j];
+                    dbs[k][j] += dz[j];
+                    dn[u][k][j] = dz[j] * wt[k][j];
+                    s[2 * u] += at.ok[k] ? dn[u][k][j] : 0.f;
+                    s[2 * u + 1] = at.ok[k] ? __builtin_fmaf(dn[u][k][j], nn[u][k][j], s[2 * u + 1]) : s[2 * u + 1];
+                }
             }
         }
-        s1 = lanes_sum(s1, p.log_l) * inv_d;
-        s2 = lanes_sum(s2, p.log_l) * inv_d;
+        lanes_sum<2 * U>(s, p.log_l);
 #pragma unroll
-        for (int k = 0; k < NV; ++k) {
-            float dx[VEC];
+        for (int u = 0; u < U; ++u) {
+            if (first + u >= n1) break;
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) dx[j] = r.rstd * (dn[k][j] - s1 - nn[k][j] * s2);
-            if (at.ok[k]) store_n<T, VEC>(static_cast<T *>(p.y) + n * p.sxn + at.c[k], dx);
+            for (int k = 0; k < NV; ++k) {
+                float dx[VEC];
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) dx[j] = r.rstd[u] * (dn[u][k][j] - s[2 * u] * inv_d - nn[u][k][j] * (s[2 * u + 1] * inv_d));
+                if (at.ok[k]) store_n<T, VEC>(static_cast<T *>(p.y) + (first + u) * p.sxn + at.c[k], dx);
+            }
         }
     }
     if (!p.part) return;
@@ -606,6 +623,7 @@ constexpr int kMostParts = 32;
 constexpr int NT = 256;     // threads
 constexpr int kTile = 256;  // channels a tile at most
 constexpr int kSet = 128;   // groups a set at most
+constexpr int kMostWords = 1024; // parts by groups of a set at most
 template <int VEC, int E> struct Held {
     int c, in_tile, rl, rows; // the lane's first channel, that in its tile; its row and the rows at a time
     int set, part, parts, count; // rows of this chunk
@@ -668,16 +686,14 @@ struct GroupLanes {
     bool ok;
     __device__ explicit GroupLanes(int ng) {
         share = 64;
-        while (share * ng > NT) share /= 2; // (at most kSet groups)
+        while (share * ng > NT) share /= 2; // (ng is the same in the workgroup, and at most kSet)
+        share = __builtin_amdgcn_readfirstlane(share);
         g = (int)threadIdx.x / share;
         t = (int)threadIdx.x % share;
         ok = g < ng;
         g = ok ? g : 0;
     }
-    __device__ float sum(float v) const { // to all of them
-        for (int o = 1; o < share; o <<= 1) v += __shfl_xor(v, o, kWave);
-        return v;
-    }
+    __device__ float sum(float v) const { return lanes_sum(v, __builtin_ctz(share)); } // to all of them
 };
 
 // Publishes the part's pair of the group and calls f(k, pair of part k) for the
@@ -701,7 +717,7 @@ template <typename F> __device__ __forceinline__ void each_part(const GroupNormP
 template <typename T, int VEC, int E, bool GATE>
 __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
     // sums and squares of a thread's channels; afterwards the parts' means and squares
-    __shared__ float red[2][VEC * NT > kMostParts * kSet ? VEC * NT : kMostParts * kSet];
+    __shared__ float red[2][VEC * NT > kMostWords ? VEC * NT : kMostWords];
     __shared__ float first[kSet], stat[2][kSet];
     __shared__ unsigned drawn;
     const int tid = threadIdx.x;
@@ -827,6 +843,7 @@ __global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
     const Held<VEC, E> at(p, draw_part(p, &drawn, (unsigned)(p.chunks * p.tiles)));
     const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c, *dy = static_cast<const T *>(p.dy) + at.n * p.sxn + at.c;
     const T *gate = static_cast<const T *>(p.gate) + at.n * p.sgn + at.c;
+    const Channels<VEC> ch(p, at.n, at.c);
     Raw<T, VEC> rx[E], ry[E], rg[GATE ? E : 1];
 #pragma unroll
     for (int i = 0; i < E; ++i) {
@@ -836,7 +853,6 @@ __global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
     }
     const int nc = at.channels(p), ng = at.groups(p), gc = min(p.D, nc);
     const GroupLanes gl(ng);
-    const Channels<VEC> ch(p, at.n, at.c);
     T *dgate = static_cast<T *>(p.dgate) + at.n * p.sgn + at.c;
     // n and dz (and the gate's gradient) of row i
     auto element = [&](int i, float *n, float *dz, float *dg) {
@@ -955,19 +971,18 @@ bool hold(const gdn2_group_norm_args &a, bool bwd, int vec, Plan *q) {
     const int G = (int)a.groups, D = (int)a.channels / G;
     int unit = 1; // groups that make a multiple of vec channels
     while ((int64_t)unit * D % vec) unit *= 2;
-    for (const int width : {128, 64}) { // channels of a set of whole groups
-        const int sg = std::max(unit, width / D / unit * unit);
-        if (width == 64 && sg == std::max(unit, 128 / D / unit * unit)) break;
-        q->set_groups = std::min(sg, G);
-        q->sets = (G + q->set_groups - 1) / q->set_groups;
-        const int64_t set_c = (int64_t)q->set_groups * D;
-        if (q->set_groups > 1 && set_c > kTile) return false;
-        q->tile = (int)std::min<int64_t>(set_c, kTile);
-        q->tiles = (int)((set_c + q->tile - 1) / q->tile);
-        q->lc = q->tile / vec;
-        for (const int e : {4, 8, bwd ? kRows3Bwd : kRows3}) { // the least that a thread holds
+    for (const int e : {4, 8, bwd ? kRows3Bwd : kRows3}) // the least that a thread holds
+        for (const int width : {128, 64}) {              // channels of a set of whole groups
+            const int sg = std::max(unit, width / D / unit * unit);
+            q->set_groups = std::min(sg, G);
+            q->sets = (G + q->set_groups - 1) / q->set_groups;
+            const int64_t set_c = (int64_t)q->set_groups * D;
+            if (q->set_groups > 1 && set_c > kTile) return false;
+            q->tile = (int)std::min<int64_t>(set_c, kTile);
+            q->tiles = (int)((set_c + q->tile - 1) / q->tile);
+            q->lc = q->tile / vec;
             const int64_t chunk = (int64_t)(NT / q->lc) * e, chunks = (a.rows + chunk - 1) / chunk;
-            if (chunks * q->tiles > kMostParts) continue;
+            if (chunks * q->tiles > kMostParts || chunks * q->tiles * q->set_groups > kMostWords) continue;
             q->held = true;
             q->vec = vec;
             q->e = e;
@@ -975,7 +990,6 @@ bool hold(const gdn2_group_norm_args &a, bool bwd, int vec, Plan *q) {
             q->chunks = (int)chunks;
             return true;
         }
-    }
     return false;
 }
 
@@ -1099,9 +1113,9 @@ template <typename T, int VEC, bool GATE> hipError_t run_rows(const Plan &q, con
 }
 template <typename T, int VEC, bool GATE> hipError_t run_rows_bwd(const Plan &q, const GroupNormParams &p, hipStream_t s) {
     const dim3 grid((unsigned)q.row_blocks, (unsigned)q.sets);
-    if (q.nv == 1) hipLaunchKernelGGL((norm_rows_bwd_kernel<T, VEC, 1, GATE>), grid, dim3(256), 0, s, p);
-    else if (q.nv == 4) hipLaunchKernelGGL((norm_rows_bwd_kernel<T, VEC, 4, GATE>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((norm_rows_bwd_kernel<T, VEC, VEC == 4 ? 8 : 16, GATE>), grid, dim3(256), 0, s, p);
+    if (q.nv == 1) hipLaunchKernelGGL((norm_rows_bwd_kernel<T, VEC, 1, 2, GATE>), grid, dim3(256), 0, s, p);
+    else if (q.nv == 4) hipLaunchKernelGGL((norm_rows_bwd_kernel<T, VEC, 4, 1, GATE>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((norm_rows_bwd_kernel<T, VEC, VEC == 4 ? 8 : 16, 1, GATE>), grid, dim3(256), 0, s, p);
     return hipGetLastError();
 }
 

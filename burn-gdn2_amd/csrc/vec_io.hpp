@@ -28,4 +28,30 @@ template <typename T, int N> __device__ __forceinline__ void store_n(T *p, const
     *reinterpret_cast<Raw<T, N> *>(p) = v;
 }
 
+// Sums of n values over the 2^log_l neighbouring lanes of each group of lanes, to
+// all of them (log_l the same in the wave).  Up to 16 lanes by the adder's own lane
+// moves: the other lane of a pair, the other pair, and, the sums being the same in
+// a quad by then, the mirrored half and the mirrored row.
+template <int N> __device__ __forceinline__ void lanes_sum(float (&v)[N], int log_l) {
+#define GDN2_STEP(least, other)                              \
+    if (log_l >= least) {                                    \
+        _Pragma("unroll") for (int i = 0; i < N; ++i) {      \
+            const int x = __builtin_bit_cast(int, v[i]);     \
+            v[i] += __builtin_bit_cast(float, (other));      \
+        }                                                    \
+    }
+    GDN2_STEP(1, __builtin_amdgcn_mov_dpp(x, 0xB1, 0xF, 0xF, true))  // quad_perm [1, 0, 3, 2]
+    GDN2_STEP(2, __builtin_amdgcn_mov_dpp(x, 0x4E, 0xF, 0xF, true))  // quad_perm [2, 3, 0, 1]
+    GDN2_STEP(3, __builtin_amdgcn_mov_dpp(x, 0x141, 0xF, 0xF, true)) // row_half_mirror
+    GDN2_STEP(4, __builtin_amdgcn_mov_dpp(x, 0x140, 0xF, 0xF, true)) // row_mirror
+    GDN2_STEP(5, __builtin_amdgcn_ds_swizzle(x, 0x401F))             // lane ^ 16
+    GDN2_STEP(6, __shfl_xor(x, 32, kWave))
+#undef GDN2_STEP
+}
+__device__ __forceinline__ float lanes_sum(float x, int log_l) {
+    float v[1] = {x};
+    lanes_sum<1>(v, log_l);
+    return v[0];
+}
+
 }  // namespace gdn2
