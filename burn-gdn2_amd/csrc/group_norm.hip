@@ -6,17 +6,20 @@
 //
 // S = 1 (a token's heads): L lanes hold a group in registers, so that everything
 // is read once; the variance is taken about the mean.  A larger group is held by
-// up to kMostParts workgroups: each publishes its part's sums, reads those of
-// the others, and goes on with its registers, so that again everything is read
-// once.  Groups larger than that take three passes: sums for every channel and
+// up to kMostParts workgroups: each publishes its part's sums, takes those of the
+// others, and goes on with its registers, so that again everything is read
+// once.  Sums that do not come in time it forms itself, so that no workgroup
+// depends on another's being started.  Groups larger than that take three passes: sums for every channel and
 // chunk of rows, a join, and one that reads x again.  Every sum runs in a fixed
 // order.
 //
 // Bound: HBM.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <exception>
 #include <string>
+#include <type_traits>
 
 #include "common.hpp"
 #include "gdn2_mixer.h"
@@ -44,8 +47,8 @@ struct GroupNormParams {
     int chunks, chunk; // row chunks of a sample, rows in one
     // held groups: channels a tile, tiles a set of groups, sets; a part: a chunk of rows by a tile
     int tile, tiles, sets, set_groups;
-    unsigned *ticket;           // the next part
-    unsigned long long *words;  // [sample][set][part][set_groups] what the parts publish
+    unsigned long long *words; // [sample][set][part][set_groups] what the parts publish
+    int patience;              // looks at a word before its part's sums are formed here
 };
 
 // (v_rcp_f32 is within one unit in the last place)
@@ -606,26 +609,22 @@ template <typename T, int VEC, bool GATE> __global__ __launch_bounds__(256) void
 
 // -- groups that several workgroups hold ----------------------------------------
 
-// All ones over the words that parts publish and the ticket before them.
+// All ones over the words that parts publish.
 __global__ __launch_bounds__(256) void norm_prepare_kernel(uint4 *words, int64_t n16) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n16; i += (int64_t)gridDim.x * 256)
         words[i] = uint4{~0u, ~0u, ~0u, ~0u};
 }
 
 // A part of a set of groups: E rows a thread of VEC channels, lc lanes along the
-// tile's channels.  Parts are numbered by a ticket, a set's next to each other: at
-// most one set of a running kernel is not drawn completely, so that at most
-// kMostParts - 1 of its workgroups wait for one that has not started.  They leave
-// room on the chip for it to start: two workgroups a compute unit fit at least
-// (256 threads of 256 registers), 512, more than 16 such kernels at once can
-// have waiting.
-constexpr int kMostParts = 32;
+// tile's channels.
+constexpr int kMostParts = 64;
 constexpr int NT = 256;     // threads
 constexpr int kTile = 256;  // channels a tile at most
 constexpr int kSet = 128;   // groups a set at most
 constexpr int kMostWords = 1024; // parts by groups of a set at most
 template <int VEC, int E> struct Held {
     int c, in_tile, rl, rows; // the lane's first channel, that in its tile; its row and the rows at a time
+    unsigned number;
     int set, part, parts, count; // rows of this chunk
     bool ok;
     int64_t n, s0;
@@ -636,6 +635,7 @@ template <int VEC, int E> struct Held {
         set = (int)(ns % (unsigned)p.sets);
         n = ns / (unsigned)p.sets;
         const int tl = part % p.tiles;
+        this->number = number;
         rows = NT / p.lc;
         rl = (int)threadIdx.x / p.lc;
         const int cl = (int)threadIdx.x % p.lc;
@@ -649,8 +649,6 @@ template <int VEC, int E> struct Held {
     }
     __device__ int64_t row(int i) const { return s0 + min(rl + i * rows, count - 1); }
     __device__ bool has(int i) const { return ok && rl + i * rows < count; }
-    // rows that thread row r has
-    __device__ int of(int r) const { return r < count ? (count - r + rows - 1) / rows : 0; }
     // channels of the tile, and groups of the set that are there
     __device__ int channels(const GroupNormParams &p) const {
         const int set_c = set * p.set_groups * p.D;
@@ -659,26 +657,11 @@ template <int VEC, int E> struct Held {
     __device__ int groups(const GroupNormParams &p) const { return min(p.set_groups, p.G - set * p.set_groups); }
 };
 
-__device__ __forceinline__ unsigned draw_part(const GroupNormParams &p, unsigned *lds, unsigned parts) {
-    if (parts == 1) return blockIdx.x;
-    if (threadIdx.x == 0) *lds = atomicAdd(p.ticket, 1u) + 1u; // from all ones
-    __syncthreads();
-    return __builtin_amdgcn_readfirstlane(*lds);
-}
-
 // A published pair is never all ones.
 __device__ __forceinline__ unsigned long long pair(float a, float b) {
     const unsigned lo = __builtin_bit_cast(unsigned, a), hi = b != b ? 0x7FC00000u : __builtin_bit_cast(unsigned, b);
     return (unsigned long long)hi << 32 | lo;
 }
-__device__ __forceinline__ unsigned long long wait_for(const unsigned long long *w) {
-    for (;;) {
-        const unsigned long long v = __hip_atomic_load(w, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        if (v != ~0ull) return v;
-        __builtin_amdgcn_s_sleep(1);
-    }
-}
-
 // The threads that work on a group: `share` neighbouring lanes of a wave, a power
 // of two.
 struct GroupLanes {
@@ -696,32 +679,66 @@ struct GroupLanes {
     __device__ float sum(float v) const { return lanes_sum(v, __builtin_ctz(share)); } // to all of them
 };
 
-// Publishes the part's pair of the group and calls f(k, pair of part k) for the
-// parts k that fall to this lane, in order.
-template <typename F> __device__ __forceinline__ void each_part(const GroupNormParams &p, const GroupLanes &gl, int64_t set, int part, int parts,
-                                                                float a, float b, F f) {
-    if (!gl.ok) return;
-    unsigned long long *w = p.words + set * parts * p.set_groups + gl.g;
-    if (parts > 1 && gl.t == 0)
-        __hip_atomic_store(w + (int64_t)part * p.set_groups, pair(a, b), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    for (int k = gl.t; k < parts; k += gl.share) {
-        if (k == part) {
-            f(k, a, b);
-        } else {
-            const unsigned long long v = wait_for(w + (int64_t)k * p.set_groups);
-            f(k, __builtin_bit_cast(float, (unsigned)v), __builtin_bit_cast(float, (unsigned)(v >> 32)));
+// f(i) for E rows, unrolled where they are in registers
+template <int E, bool ONCE, typename F> __device__ __forceinline__ void each_row(std::integral_constant<bool, ONCE>, F f) {
+    if constexpr (ONCE) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) f(i);
+    } else {
+#pragma unroll 1
+        for (int i = 0; i < E; ++i) f(i);
+    }
+}
+
+// Publishes the part's pair of every group and collects those of all parts in
+// all[2][parts][groups] (each entry by the lane that reads it).  `form`(k) makes
+// every thread of a group return the pair of part k, by the operations of its own
+// workgroup.
+template <typename Form>
+__device__ __forceinline__ void collect(const GroupNormParams &p, const GroupLanes &gl, int64_t set, int part, int parts, int ng, float2 own,
+                                        float *all, unsigned long long *missing, Form form) {
+    unsigned long long *const w = p.words + set * parts * p.set_groups + gl.g;
+    float *const a = all, *const b = all + kMostWords;
+    auto look = [&](int k) { return __hip_atomic_load(w + (int64_t)k * p.set_groups, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+    auto take = [&](int k, unsigned long long v) {
+        a[k * ng + gl.g] = __builtin_bit_cast(float, (unsigned)v);
+        b[k * ng + gl.g] = __builtin_bit_cast(float, (unsigned)(v >> 32));
+    };
+    if (gl.ok && parts > 1 && gl.t == 0)
+        __hip_atomic_store(w + (int64_t)part * p.set_groups, pair(own.x, own.y), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    bool late = false;
+    if (gl.ok)
+        for (int k = gl.t; k < parts; k += gl.share) {
+            unsigned long long v = pair(own.x, own.y);
+            if (k != part) {
+                v = look(k);
+                for (int i = 0; i < p.patience && v == ~0ull; ++i) {
+                    __builtin_amdgcn_s_sleep(1);
+                    v = look(k);
+                }
+                if (v == ~0ull) {
+                    late = true;
+                    atomicOr(missing, 1ull << k);
+                }
+            }
+            take(k, v);
         }
+    if (parts == 1 || !__syncthreads_or(late)) return;
+    const unsigned long long these = *missing;
+    for (int k = 0; k < parts; ++k) {
+        if (!(these >> k & 1)) continue;
+        const float2 f = form(k);
+        if (gl.ok && k % gl.share == gl.t) take(k, pair(f.x, f.y));
     }
 }
 
 template <typename T, int VEC, int E, bool GATE>
 __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
-    // sums and squares of a thread's channels; afterwards the parts' means and squares
-    __shared__ float red[2][VEC * NT > kMostWords ? VEC * NT : kMostWords];
-    __shared__ float first[kSet], stat[2][kSet];
-    __shared__ unsigned drawn;
+    __shared__ float red[2][VEC * NT]; // sums and squares of a thread's channels
+    __shared__ float all[2][kMostWords], first[kSet], stat[2][kSet];
+    __shared__ unsigned long long missing;
     const int tid = threadIdx.x;
-    const Held<VEC, E> at(p, draw_part(p, &drawn, (unsigned)(p.chunks * p.tiles)));
+    const Held<VEC, E> at(p, blockIdx.x);
     const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c;
     const T *gate = static_cast<const T *>(p.gate) + at.n * p.sgn + at.c;
     Raw<T, VEC> rx[E], rg[GATE ? E : 1];
@@ -730,57 +747,72 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
         rx[i] = raw_n<T, VEC>(x + at.row(i) * p.sxs);
         if constexpr (GATE) rg[i] = raw_n<T, VEC>(gate + at.row(i) * p.sgs);
     }
-    const int nc = at.channels(p), ng = at.groups(p), gc = min(p.D, nc); // the tile's channels of a group
+    if (tid == 0) missing = 0;
+    const int ng = at.groups(p);
     const GroupLanes gl(ng);
     float wt[VEC], bs[VEC];
 #pragma unroll
     for (int j = 0; j < VEC; ++j) wt[j] = 1.f, bs[j] = 0.f;
     if (p.weight) load_n<float, VEC>(p.weight + at.c, wt);
     if (p.bias) load_n<float, VEC>(p.bias + at.c, bs);
-    int group[VEC]; // of the set
+    int group[VEC]; // of the set (the same in every part of it)
 #pragma unroll
     for (int j = 0; j < VEC; ++j) group[j] = p.tiles == 1 && at.ok ? (at.in_tile + j) / p.D : 0;
 
-    // Sums about a value of the group's, so that a large mean costs no digits.
+    // The mean of a part and the squares about it, from sums about one value of the
+    // group's, so that a large mean costs no digits.
+    auto moments = [&](const Held<VEC, E> &h, auto at_once, auto value) { // value(i): the i-th row's; at_once: rows unrolled
+        const int gc = min(p.D, h.channels(p)); // the tile's channels of a group
 #pragma unroll
-    for (int j = 0; j < VEC; ++j)
-        if (at.ok && at.rl == 0 && (at.in_tile + j) % p.D == 0) first[group[j]] = (float)rx[0][j];
-    __syncthreads();
+        for (int j = 0; j < VEC; ++j)
+            if (h.ok && h.rl == 0 && (h.in_tile + j) % p.D == 0) first[group[j]] = (float)value(0)[j];
+        __syncthreads();
+        float base[VEC], s[VEC], q[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        const float base = first[group[j]];
-        float s = 0.f, q = 0.f;
-#pragma unroll
-        for (int i = 0; i < E; ++i) {
-            const float d = at.has(i) ? (float)rx[i][j] - base : 0.f;
-            s += d;
-            q = __builtin_fmaf(d, d, q);
+        for (int j = 0; j < VEC; ++j) {
+            base[j] = first[group[j]];
+            s[j] = q[j] = 0.f;
         }
-        red[0][j * NT + tid] = s;
-        red[1][j * NT + tid] = q;
-    }
-    __syncthreads();
-    // channel c of the tile is at c % VEC of lane c / VEC, for every row of threads
-    float s = 0.f, q = 0.f;
-    if (gl.ok)
-        for (int c = gl.g * p.D + gl.t; c < gl.g * p.D + gc; c += gl.share) {
-            const int o = (c % VEC) * NT + c / VEC;
-#pragma unroll 4
-            for (int r = 0; r < at.rows; ++r) {
-                s += red[0][o + r * p.lc];
-                q += red[1][o + r * p.lc];
+        each_row<E>(at_once, [&](int i) {
+            const Raw<T, VEC> v = value(i);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                const float d = h.has(i) ? (float)v[j] - base[j] : 0.f;
+                s[j] += d;
+                q[j] = __builtin_fmaf(d, d, q[j]);
             }
+        });
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            red[0][j * NT + tid] = s[j];
+            red[1][j * NT + tid] = q[j];
         }
-    s = gl.sum(s);
-    q = gl.sum(q);
-    const float base = first[gl.g], elements = (float)at.count * (float)gc;
-    __syncthreads(); // red is read
-    const float shift = s / elements, own = base + shift, own2 = fmaxf(__builtin_fmaf(-shift, s, q), q - q); // (a NaN stays)
-    float *const means = red[0], *const squares = red[1];
-    each_part(p, gl, at.n * p.sets + at.set, at.part, at.parts, own, own2, [&](int k, float a, float b) {
-        means[k * ng + gl.g] = a;
-        squares[k * ng + gl.g] = b;
+        __syncthreads();
+        // channel c of the tile is at c % VEC of lane c / VEC, for every row of threads
+        float t[2] = {0.f, 0.f};
+        if (gl.ok)
+            for (int c = gl.g * p.D + gl.t; c < gl.g * p.D + gc; c += gl.share) {
+                const int o = (c % VEC) * NT + c / VEC;
+#pragma unroll 4
+                for (int r = 0; r < h.rows; ++r) {
+                    t[0] += red[0][o + r * p.lc];
+                    t[1] += red[1][o + r * p.lc];
+                }
+            }
+        lanes_sum<2>(t, __builtin_ctz(gl.share));
+        const float shift = t[0] / ((float)h.count * (float)gc);
+        const float2 m = {first[gl.g] + shift, fmaxf(__builtin_fmaf(-shift, t[0], t[1]), t[1] - t[1])}; // (a NaN stays)
+        __syncthreads(); // (first and red may be written again)
+        return m;
+    };
+    const float2 own = moments(at, std::true_type(), [&](int i) { return rx[i]; });
+    collect(p, gl, at.n * p.sets + at.set, at.part, at.parts, ng, own, all[0], &missing, [&](int k) {
+        const Held<VEC, E> other(p, at.number - at.part + k);
+        const T *const y = static_cast<const T *>(p.x) + other.n * p.sxn + other.c;
+        return moments(other, std::false_type(), [&](int i) { return raw_n<T, VEC>(y + other.row(i) * p.sxs); });
     });
+    const float *const means = all[0], *const squares = all[1];
+    float s, q;
     auto size = [&](int k) { // elements of part k
         const int64_t rows = min((int64_t)p.chunk, p.S - (int64_t)(k / p.tiles) * p.chunk);
         return (float)rows * (float)(p.tiles == 1 ? p.D : min(p.tile, p.D - (k % p.tiles) * p.tile));
@@ -837,10 +869,10 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
 template <typename T, int VEC, int E, bool GATE>
 __global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
     __shared__ float red[2][VEC * NT]; // sums of dz n and dz of a thread's channels
-    __shared__ float stat[2][kSet];
-    __shared__ unsigned drawn;
+    __shared__ float all[2][kMostWords], stat[2][kSet];
+    __shared__ unsigned long long missing;
     const int tid = threadIdx.x;
-    const Held<VEC, E> at(p, draw_part(p, &drawn, (unsigned)(p.chunks * p.tiles)));
+    const Held<VEC, E> at(p, blockIdx.x);
     const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c, *dy = static_cast<const T *>(p.dy) + at.n * p.sxn + at.c;
     const T *gate = static_cast<const T *>(p.gate) + at.n * p.sgn + at.c;
     const Channels<VEC> ch(p, at.n, at.c);
@@ -851,76 +883,90 @@ __global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
         ry[i] = raw_n<T, VEC>(dy + at.row(i) * p.sxs);
         if constexpr (GATE) rg[i] = raw_n<T, VEC>(gate + at.row(i) * p.sgs);
     }
-    const int nc = at.channels(p), ng = at.groups(p), gc = min(p.D, nc);
+    if (tid == 0) missing = 0;
+    const int ng = at.groups(p);
     const GroupLanes gl(ng);
     T *dgate = static_cast<T *>(p.dgate) + at.n * p.sgn + at.c;
-    // n and dz (and the gate's gradient) of row i
-    auto element = [&](int i, float *n, float *dz, float *dg) {
+    // n and dz (and the gate's gradient) of a row
+    auto element = [&](const Channels<VEC> &ch, const Raw<T, VEC> &x, const Raw<T, VEC> &y, const Raw<T, VEC> &g, float *n, float *dz, float *dg) {
         float vx[VEC], vy[VEC], vg[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            vx[j] = (float)rx[i][j];
-            vy[j] = (float)ry[i][j];
-            if constexpr (GATE) vg[j] = (float)rg[GATE ? i : 0][j];
+            vx[j] = (float)x[j];
+            vy[j] = (float)y[j];
+            if constexpr (GATE) vg[j] = (float)g[j];
         }
         dz_n<T, VEC, GATE>(p, ch, vx, vy, vg, n, dz, dg);
     };
-    float a[VEC], b[VEC];
+    // The sums of a part: a group's of dn n and dn; a channel's of dz n and dz go to
+    // part [sample][chunk][2][C] for the weights' gradients.
+    auto sums = [&](const Held<VEC, E> &h, const Channels<VEC> &ch, auto at_once, auto value_x, auto value_y, auto value_g) {
+        constexpr bool keep = decltype(at_once)::value; // this workgroup's own
+        float a[VEC], b[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) a[j] = b[j] = 0.f;
+        for (int j = 0; j < VEC; ++j) a[j] = b[j] = 0.f;
+        each_row<E>(at_once, [&](int i) {
+            if (!h.has(i)) return;
+            float n[VEC], dz[VEC], dg[VEC];
+            element(ch, value_x(i), value_y(i), value_g(i), n, dz, dg);
 #pragma unroll
-    for (int i = 0; i < E; ++i) {
-        if (!at.has(i)) break;
-        float n[VEC], dz[VEC], dg[VEC];
-        element(i, n, dz, dg);
+            for (int j = 0; j < VEC; ++j) {
+                a[j] = __builtin_fmaf(dz[j], n[j], a[j]);
+                b[j] += dz[j];
+            }
+            if constexpr (GATE && keep) store_n<T, VEC>(dgate + h.row(i) * p.sgs, dg);
+        });
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            a[j] = __builtin_fmaf(dz[j], n[j], a[j]);
-            b[j] += dz[j];
+            red[0][j * NT + tid] = a[j];
+            red[1][j * NT + tid] = b[j];
         }
-        if constexpr (GATE) store_n<T, VEC>(dgate + at.row(i) * p.sgs, dg);
-    }
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        red[0][j * NT + tid] = a[j];
-        red[1][j * NT + tid] = b[j];
-    }
-    __syncthreads();
-    // A channel's sums over the part go to part [sample][chunk][2][C] for the weights'
-    // gradients, times its weight into the group's.
-    const int c0 = at.set * p.set_groups * p.D + at.part % p.tiles * p.tile;
-    float *out = p.part ? p.part + (at.n * p.chunks + at.part / p.tiles) * 2 * p.C + c0 : nullptr;
-    float s2 = 0.f, s1 = 0.f;
-    if (gl.ok)
-        for (int c = gl.g * p.D + gl.t; c < gl.g * p.D + gc; c += gl.share) {
-            const int o = (c % VEC) * NT + c / VEC;
-            const float w = p.weight ? p.weight[c0 + c] : 1.f;
-            float u = 0.f, v = 0.f;
+        __syncthreads();
+        const int c0 = h.set * p.set_groups * p.D + h.part % p.tiles * p.tile, gc = min(p.D, h.channels(p));
+        float *out = p.part && keep ? p.part + (h.n * p.chunks + h.part / p.tiles) * 2 * p.C + c0 : nullptr;
+        float t[2] = {0.f, 0.f};
+        if (gl.ok)
+            for (int c = gl.g * p.D + gl.t; c < gl.g * p.D + gc; c += gl.share) {
+                const int o = (c % VEC) * NT + c / VEC;
+                const float w = p.weight ? p.weight[c0 + c] : 1.f;
+                float u = 0.f, v = 0.f;
 #pragma unroll 4
-            for (int r = 0; r < at.rows; ++r) {
-                u += red[0][o + r * p.lc];
-                v += red[1][o + r * p.lc];
+                for (int r = 0; r < h.rows; ++r) {
+                    u += red[0][o + r * p.lc];
+                    v += red[1][o + r * p.lc];
+                }
+                if (out) {
+                    out[c] = u;
+                    out[p.C + c] = v;
+                }
+                t[0] = __builtin_fmaf(u, w, t[0]);
+                t[1] = __builtin_fmaf(v, w, t[1]);
             }
-            if (out) {
-                out[c] = u;
-                out[p.C + c] = v;
-            }
-            s2 = __builtin_fmaf(u, w, s2);
-            s1 = __builtin_fmaf(v, w, s1);
-        }
-    s2 = gl.sum(s2);
-    s1 = gl.sum(s1);
-    float t2 = 0.f, t1 = 0.f;
-    each_part(p, gl, at.n * p.sets + at.set, at.part, at.parts, s2, s1, [&](int, float u, float v) {
-        t2 += u;
-        t1 += v;
+        lanes_sum<2>(t, __builtin_ctz(gl.share));
+        __syncthreads(); // (red may be written again)
+        return float2{t[0], t[1]};
+    };
+    const float2 own = sums(at, ch, std::true_type(), [&](int i) { return rx[i]; }, [&](int i) { return ry[i]; },
+                           [&](int i) { return rg[GATE ? i : 0]; });
+    collect(p, gl, at.n * p.sets + at.set, at.part, at.parts, ng, own, all[0], &missing, [&](int k) {
+        const Held<VEC, E> o(p, at.number - at.part + k);
+        auto from = [&](const void *base, int64_t sn, int64_t ss, int i) {
+            return raw_n<T, VEC>(static_cast<const T *>(base) + o.n * sn + o.row(i) * ss + o.c);
+        };
+        return sums(o, Channels<VEC>(p, o.n, o.c), std::false_type(), [&](int i) { return from(p.x, p.sxn, p.sxs, i); },
+                    [&](int i) { return from(p.dy, p.sxn, p.sxs, i); },
+                    [&](int i) { return GATE ? from(p.gate, p.sgn, p.sgs, i) : Raw<T, VEC>{}; });
     });
-    t2 = gl.sum(t2);
-    t1 = gl.sum(t1);
+    float t[2] = {0.f, 0.f};
+    for (int k = gl.t; gl.ok && k < at.parts; k += gl.share) { // (a lane reads what it wrote itself)
+        t[0] += all[0][k * ng + gl.g];
+        t[1] += all[1][k * ng + gl.g];
+    }
+    lanes_sum<2>(t, __builtin_ctz(gl.share));
     if (gl.ok && gl.t == 0) {
         const float size = (float)p.S * (float)p.D;
-        stat[0][gl.g] = t2 / size;
-        stat[1][gl.g] = t1 / size;
+        stat[0][gl.g] = t[0] / size;
+        stat[1][gl.g] = t[1] / size;
     }
     __syncthreads();
     if (!at.ok) return;
@@ -936,7 +982,7 @@ __global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
     for (int i = 0; i < E; ++i) {
         if (!at.has(i)) break;
         float n[VEC], dz[VEC], dg[VEC], o[VEC];
-        element(i, n, dz, dg);
+        element(ch, rx[i], ry[i], rg[GATE ? i : 0], n, dz, dg);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) o[j] = ch.rstd[j] * (dz[j] * ch.wt[j] - m1[j] - n[j] * m2[j]);
         store_n<T, VEC>(dx + at.row(i) * p.sxs, o);
@@ -952,7 +998,7 @@ struct Plan {
     bool held; // groups that up to kMostParts workgroups hold
     int e; // rows a thread
     int tile, set_groups;
-    int64_t o_words, words; // bytes: the ticket and the words that parts publish
+    int64_t o_words, words; // bytes of the words that parts publish
     int vec, nv, u, log_l, sets;
     int row_blocks;
     int lc, tiles, chunks, chunk;
@@ -965,35 +1011,43 @@ int up_log2(int64_t n) {
     return k;
 }
 
+// see gdn2_group_norm_patience; 512 looks are about half a millisecond
+std::atomic<int> g_patience{512};
+
 // The plan of a held group; false where it takes too many parts.
 constexpr int kRows3 = 16, kRows3Bwd = 12; // rows a thread at most (as many as leave no register in memory)
 bool hold(const gdn2_group_norm_args &a, bool bwd, int vec, Plan *q) {
     const int G = (int)a.groups, D = (int)a.channels / G;
     int unit = 1; // groups that make a multiple of vec channels
     while ((int64_t)unit * D % vec) unit *= 2;
-    for (const int e : {4, 8, bwd ? kRows3Bwd : kRows3}) // the least that a thread holds
-        for (const int width : {128, 64}) {              // channels of a set of whole groups
-            const int sg = std::max(unit, width / D / unit * unit);
-            q->set_groups = std::min(sg, G);
-            q->sets = (G + q->set_groups - 1) / q->set_groups;
-            const int64_t set_c = (int64_t)q->set_groups * D;
-            if (q->set_groups > 1 && set_c > kTile) return false;
-            q->tile = (int)std::min<int64_t>(set_c, kTile);
-            q->tiles = (int)((set_c + q->tile - 1) / q->tile);
-            q->lc = q->tile / vec;
-            const int64_t chunk = (int64_t)(NT / q->lc) * e, chunks = (a.rows + chunk - 1) / chunk;
-            if (chunks * q->tiles > kMostParts || chunks * q->tiles * q->set_groups > kMostWords) continue;
-            q->held = true;
-            q->vec = vec;
-            q->e = e;
-            q->chunk = (int)std::min<int64_t>(chunk, a.rows);
-            q->chunks = (int)chunks;
-            return true;
-        }
+    // Rows a thread, channels of a set of whole groups, parts at most.  Eight rows run
+    // faster than four (8 x 4096 x 1024 f32 in 64 channels: 70 against 96 us) and than
+    // sixteen (4 x 2000 x 2048 bf16 gated: 33 against 36 us); 128 channels faster
+    // than 64 but for more than 32 parts (84 against 70 us).
+    const int most = bwd ? kRows3Bwd : kRows3;
+    const int forms[][3] = {{4, 128, 1}, {8, 128, 32}, {8, 64, 32}, {most, 64, 32}, {most, 128, kMostParts}, {most, 64, kMostParts}};
+    for (const auto &f : forms) {
+        const int sg = std::max(unit, f[1] / D / unit * unit);
+        q->set_groups = std::min(sg, G);
+        q->sets = (G + q->set_groups - 1) / q->set_groups;
+        const int64_t set_c = (int64_t)q->set_groups * D;
+        if (q->set_groups > 1 && set_c > kTile) return false;
+        q->tile = (int)std::min<int64_t>(set_c, kTile);
+        q->tiles = (int)((set_c + q->tile - 1) / q->tile);
+        q->lc = q->tile / vec;
+        const int64_t chunk = (int64_t)(NT / q->lc) * f[0], chunks = (a.rows + chunk - 1) / chunk, parts = chunks * q->tiles;
+        if (parts > f[2] || parts * q->set_groups > kMostWords) continue;
+        q->held = true;
+        q->vec = vec;
+        q->e = f[0];
+        q->chunk = (int)std::min<int64_t>(chunk, a.rows);
+        q->chunks = (int)chunks;
+        return true;
+    }
     return false;
 }
 
-Plan plan_of(const gdn2_group_norm_args &a, bool bwd, bool vec4, bool sums_wanted) {
+Plan plan_of(const gdn2_group_norm_args &a, bool bwd, bool vec4, bool sums_wanted, bool in_place) {
     Plan q{};
     const int64_t C = a.channels, D = C / a.groups, N = a.samples, S = a.rows;
     q.vec = vec4 && D % 4 == 0 ? 4 : 1;
@@ -1014,10 +1068,10 @@ Plan plan_of(const gdn2_group_norm_args &a, bool bwd, bool vec4, bool sums_wante
         return q;
     }
     q.vec = vec4 && C % 4 == 0 ? 4 : 1;
-    if (hold(a, bwd, q.vec, &q) || (q.vec > 1 && hold(a, bwd, 1, &q))) {
+    if (!in_place && (hold(a, bwd, q.vec, &q) || (q.vec > 1 && hold(a, bwd, 1, &q)))) {
         size_t at = bwd && sums_wanted ? up256(8 * (size_t)(N * q.chunks) * C) : 0;
         q.o_words = (int64_t)at;
-        q.words = q.chunks * q.tiles > 1 ? 256 + (int64_t)up256(8 * (size_t)(N * q.sets * q.chunks * q.tiles * q.set_groups)) : 0;
+        q.words = q.chunks * q.tiles > 1 ? (int64_t)up256(8 * (size_t)(N * q.sets * q.chunks * q.tiles * q.set_groups)) : 0;
         q.bytes = at + (size_t)q.words;
         return q;
     }
@@ -1096,8 +1150,8 @@ GroupNormParams fill(const gdn2_group_norm_args &a, const Plan &q, void *ws) {
     if (q.held) {
         p.tile = q.tile; p.tiles = q.tiles; p.sets = q.sets; p.set_groups = q.set_groups;
         if (q.words) {
-            p.ticket = reinterpret_cast<unsigned *>(w + q.o_words);
-            p.words = reinterpret_cast<unsigned long long *>(w + q.o_words + 256);
+            p.words = reinterpret_cast<unsigned long long *>(w + q.o_words);
+            p.patience = g_patience.load(std::memory_order_relaxed);
         }
         if (q.o_words == 0) p.part = nullptr;
     }
@@ -1128,7 +1182,7 @@ template <typename T, int VEC, bool GATE, bool BWD> hipError_t run_held(const Pl
     if (q.words) {
         const int64_t n16 = q.words / 16;
         hipLaunchKernelGGL(norm_prepare_kernel, dim3((unsigned)std::min<int64_t>((n16 + 255) / 256, 1024)), dim3(256), 0, s,
-                           reinterpret_cast<uint4 *>(p.ticket), n16);
+                           reinterpret_cast<uint4 *>(p.words), n16);
     }
     if (q.e == 4) launch_held<T, VEC, 4, GATE, BWD>(q, p, s);
     else if (q.e == 8) launch_held<T, VEC, 8, GATE, BWD>(q, p, s);
@@ -1184,7 +1238,7 @@ template <typename T> gdn2_status forward(const char *who, const gdn2_group_norm
     if (const char *e = check(*a, &nothing, &limits)) return refuse(who, e, limits ? GDN2_NOT_APPLICABLE : GDN2_EINVAL);
     if (nothing) return GDN2_OK;
     if (!a->x || !a->y) return refuse(who, "null tensor pointer");
-    const Plan q = plan_of(*a, false, can_vec<T>(*a), false);
+    const Plan q = plan_of(*a, false, can_vec<T>(*a), false, a->y == a->x || a->y == a->gate);
     if (!grid_fits(*a, q)) return refuse(who, "sizes above the kernels' limits", GDN2_NOT_APPLICABLE);
     if (q.bytes > 0 && (!a->workspace || a->workspace_bytes < q.bytes || !aligned(a->workspace, 256)))
         return refuse(who, "workspace missing, too small or not 256-byte aligned");
@@ -1215,7 +1269,7 @@ template <typename T> gdn2_status backward(const char *who, const gdn2_group_nor
     }
     const size_t e = 4 * sizeof(T);
     const bool vec4 = can_vec<T>(f) && aligned(a->d_y, e) && aligned(a->dx, e) && aligned(a->dgate, e);
-    const Plan q = plan_of(f, true, vec4, sums);
+    const Plan q = plan_of(f, true, vec4, sums, a->dx == a->d_y);
     if (!grid_fits(f, q)) return refuse(who, "sizes above the kernels' limits", GDN2_NOT_APPLICABLE);
     if (q.bytes > 0 && (!a->workspace || a->workspace_bytes < q.bytes || !aligned(a->workspace, 256)))
         return refuse(who, "workspace missing, too small or not 256-byte aligned");
@@ -1229,10 +1283,14 @@ template <typename T> gdn2_status backward(const char *who, const gdn2_group_nor
     return GDN2_OK;
 }
 
+// (of either alignment, in place or not: the call knows them, the size does not)
 size_t workspace_of(const gdn2_group_norm_args *a, bool bwd) {
     bool nothing, limits;
     if (!a || check(*a, &nothing, &limits) || nothing) return 0;
-    return std::max(plan_of(*a, bwd, true, true).bytes, plan_of(*a, bwd, false, true).bytes);
+    size_t n = 0;
+    for (const bool vec4 : {true, false})
+        for (const bool in_place : {true, false}) n = std::max(n, plan_of(*a, bwd, vec4, true, in_place).bytes);
+    return n;
 }
 
 // No exception leaves a C entry.
@@ -1265,3 +1323,4 @@ extern "C" gdn2_status gdn2_group_norm_act_bwd_f32(const gdn2_group_norm_bwd_arg
 extern "C" gdn2_status gdn2_group_norm_act_bwd_bf16(const gdn2_group_norm_bwd_args *a, gdn2_stream_t s) {
     return guarded([&] { return backward<bf16>("gdn2_group_norm_act_bwd_bf16", a, (hipStream_t)s); });
 }
+extern "C" int gdn2_group_norm_patience(int looks) { return g_patience.exchange(std::max(looks, 0), std::memory_order_relaxed); }

@@ -20,7 +20,7 @@ namespace gdn2 {
 namespace {
 
 constexpr int kCache = 3;
-constexpr int kStep = 8; // tokens whose rows are loaded together
+constexpr int kStep = 4; // tokens whose rows are loaded together
 
 struct ConvGradParams {
     const float *x, *w, *cache, *dy, *dcache;
@@ -69,7 +69,7 @@ template <int VEC> __global__ __launch_bounds__(256) void short_conv_bwd_kernel(
         for (int j = 0; j < VEC; ++j) {
             const float z = __builtin_fmaf(xw[0][j], w[j][0], __builtin_fmaf(xw[1][j], w[j][1],
                             __builtin_fmaf(xw[2][j], w[j][2], xt[j] * w[j][3])));
-            const float s = 1.f / (1.f + fast_exp2(-kLog2e * z));
+            const float s = __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * z)); // (within one unit in the last place)
             const float d = t < p.T ? dyt[j] * (s * __builtin_fmaf(z, 1.f - s, 1.f)) : 0.f;
             out[j] = __builtin_fmaf(d, w[j][0], __builtin_fmaf(dz[0][j], w[j][1],
                      __builtin_fmaf(dz[1][j], w[j][2], dz[2][j] * w[j][3])));
@@ -114,13 +114,22 @@ template <int VEC> __global__ __launch_bounds__(256) void short_conv_bwd_kernel(
                 }
             }
         }
-        for (int64_t s0 = t0; s0 < t1; s0 += kStep) { // tokens s0 + 3 .. s0 + 3 + kStep: outputs s0 ..
-            float xs[kStep][VEC], gs[kStep][VEC];
+        float xn[kStep][VEC], gn[kStep][VEC]; // the rows of tokens s0 + 3 .. s0 + 3 + kStep: outputs s0 ..
+        auto load = [&](int64_t s0) {
 #pragma unroll
             for (int i = 0; i < kStep; ++i) {
-                row(x, s0 + 3 + i, xs[i]);
-                row(dy, s0 + 3 + i, gs[i]);
+                row(x, s0 + 3 + i, xn[i]);
+                row(dy, s0 + 3 + i, gn[i]);
             }
+        };
+        load(t0);
+        for (int64_t s0 = t0; s0 < t1; s0 += kStep) {
+            float xs[kStep][VEC], gs[kStep][VEC];
+#pragma unroll
+            for (int i = 0; i < kStep; ++i)
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) xs[i][j] = xn[i][j], gs[i][j] = gn[i][j];
+            load(s0 + kStep); // in flight beside this step
 #pragma unroll
             for (int i = 0; i < kStep; ++i) {
                 const int64_t s = s0 + i;
@@ -186,7 +195,7 @@ ConvPlan plan_of(int64_t B, int64_t T, int64_t C, bool vec4) {
     // a wave's run: up to 32 tokens (3 of 35 computed twice) while 2048 waves, eight a
     // compute unit, remain
     q.run = 32;
-    while (q.run > kStep && B * q.tiles * ((T + q.run - 1) / q.run) < 2048) q.run -= kStep;
+    while (q.run > 8 && B * q.tiles * ((T + q.run - 1) / q.run) < 2048) q.run -= 8;
     q.blocks = (T + 4 * q.run - 1) / (4 * q.run);
     q.bytes = (sizeof(float) * 4 * (size_t)(B * q.blocks) * C + 255) & ~(size_t)255;
     return q;

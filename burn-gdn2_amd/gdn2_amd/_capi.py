@@ -140,6 +140,7 @@ EXPORTS = ("gdn2_last_error", "gdn2_hip_available", "gdn2_recurrent_step_f32", "
            "gdn2_gated_scan_bwd_workspace_bytes", "gdn2_gated_scan_bwd_f32", "gdn2_gated_scan_bwd_bf16",
            "gdn2_group_norm_act_workspace_bytes", "gdn2_group_norm_act_f32", "gdn2_group_norm_act_bf16",
            "gdn2_group_norm_act_bwd_workspace_bytes", "gdn2_group_norm_act_bwd_f32", "gdn2_group_norm_act_bwd_bf16",
+           "gdn2_group_norm_patience",
            "gdn2_recurrent_bwd_f32", "gdn2_decode_fused_f32",
            "gdn2_config_default", "gdn2_config_validate", "gdn2_config_dims", "gdn2_param_count",
            "gdn2_param_name", "gdn2_param_shape", "gdn2_param_init", "gdn2_layer_create", "gdn2_layer_destroy",
@@ -222,6 +223,7 @@ def _declare_mixer(L):
         for ty in ("_f32", "_bf16"):
             fn = getattr(L, entry + ty)
             fn.argtypes, fn.restype = [ctypes.POINTER(st), ctypes.c_void_p], ctypes.c_int
+    L.gdn2_group_norm_patience.argtypes, L.gdn2_group_norm_patience.restype = [ctypes.c_int], ctypes.c_int
 
 
 def _declare_layer(L):

@@ -144,6 +144,12 @@ GDN2_API size_t gdn2_group_norm_act_workspace_bytes(const gdn2_group_norm_args *
 GDN2_API gdn2_status gdn2_group_norm_act_f32(const gdn2_group_norm_args *args, gdn2_stream_t stream);
 GDN2_API gdn2_status gdn2_group_norm_act_bf16(const gdn2_group_norm_args *args, gdn2_stream_t stream);
 
+/* A group that several workgroups hold is normalised once each has the others'
+ * sums.  One that has looked `looks` times for another's forms them itself: the
+ * results are the same bits.  Sets that number for calls that follow (512 in the
+ * beginning; 0: hardly ever waits) and returns the one before; for tests. */
+GDN2_API int gdn2_group_norm_patience(int looks);
+
 /* The gradients of L = <d_y, y> of that call.  fwd: its arguments with the
  * stats it wrote (y unused).  d_y and dx strided like x, dgate like gate (NULL
  * iff gate is); dweight, dbias [C], either NULL (not wanted).  Every output is

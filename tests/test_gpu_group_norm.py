@@ -107,6 +107,35 @@ def test_many_rows_and_samples(gpu):
         _check_backward(d, groups, "silu", stats, dy, r, "f32")
 
 
+@pytest.mark.parametrize("looks", [0, 3])
+def test_parts_formed_by_those_who_wait(gpu, looks):
+    """A workgroup that stops waiting for another's sums forms them itself: the same
+    bits, whichever parts that were."""
+    import torch
+
+    import gdn2_amd as G
+    from gdn2_amd import _capi as C
+
+    for N, S, C_, groups, ty in ((3, 700, 128, 4, "f32"), (2, 333, 320, 32, "bf16"), (1, 40, 2048, 1, "f32"), (2, 900, 33, 11, "f32")):
+        for gate in (False, True):
+            d, dy = _make(gpu, S, N, S, C_, ty, gate)
+
+            def both():
+                y, st = G.group_norm_act(d["x"], groups, d["weight"], d["bias"], EPS, "silu", gate=d["gate"], return_stats=True)
+                r = G.group_norm_act_backward(d["x"], groups, st, dy, d["weight"], d["bias"], "silu", gate=d["gate"])
+                return [y, st] + [t for t in r.values() if t is not None]
+
+            want = both()
+            torch.cuda.synchronize()
+            before = C.lib().gdn2_group_norm_patience(looks)
+            try:
+                got = both()
+                torch.cuda.synchronize()
+            finally:
+                assert C.lib().gdn2_group_norm_patience(before) == looks
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), (N, S, C_, groups, gate)
+
+
 @pytest.mark.parametrize("N,S", [(8, 1), (2, 300)])
 def test_large_mean(gpu, N, S):
     """A mean of 1000 standard deviations: sums of raw squares would leave nothing
