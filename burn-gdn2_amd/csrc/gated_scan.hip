@@ -491,7 +491,7 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
                         const float e = em[i][HEAD ? 0 : j];
                         s[j] = QUICK ? advance(e, s[j], u[i][j]) : fresh ? u[i][j] : advance_any(e, s[j], u[i][j]);
                     }
-                    if (in) store_n<T, VEC>(at_o(q, quick, i, p.out, 0), s);
+                    if (in) stream_n<T, VEC>(at_o(q, quick, i, p.out, 0), s);
                     if (!QUICK && (q.last >> i & 1) && p.state_out) store_n<float, VEC>(p.state_out + state_at(i), s);
                 } else {
                     float xg[VEC], xv[VEC], xw[VEC], hb[VEC]; // hb: the state before the token
@@ -508,9 +508,9 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
                         if constexpr (HASW) xw[j] = in ? (float)kv[i][j] * d : 0.f;
                     }
                     if (row) {
-                        store_n<T, VEC>(at_v(q, quick, i, p.dv), xv);
-                        if constexpr (HASW) store_n<T, VEC>(at_v(q, quick, i, p.dw), xw);
-                        if constexpr (!HEAD) store_n<float, VEC>(at_g(q, quick, i, p.dg), xg);
+                        stream_n<T, VEC>(at_v(q, quick, i, p.dv), xv);
+                        if constexpr (HASW) stream_n<T, VEC>(at_v(q, quick, i, p.dw), xw);
+                        if constexpr (!HEAD) stream_n<float, VEC>(at_g(q, quick, i, p.dg), xg);
                     }
                     if (start && p.state_out) store_n<float, VEC>(p.state_out + state_at(i), s);
                     if constexpr (HEAD) { // the tile's channels are of one head

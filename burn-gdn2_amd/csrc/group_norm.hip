@@ -46,7 +46,7 @@ struct GroupNormParams {
     int lc;            // tile kernels: lanes along the channels (a power of two); held groups: any number
     int chunks, chunk; // row chunks of a sample, rows in one
     // held groups: channels a tile, tiles a set of groups, sets; a part: a chunk of rows by a tile
-    int tile, tiles, sets, set_groups;
+    int tile, tiles, sets, set_groups; // (sets: rows kernels, too)
     unsigned long long *words; // [sample][set][part][set_groups] what the parts publish
     int patience;              // looks at a word before its part's sums are formed here
 };
@@ -109,8 +109,8 @@ template <int VEC, int NV> struct Lanes {
 template <typename T, int VEC, int NV, int U, bool GATE>
 __global__ __launch_bounds__(256) void norm_rows_kernel(GroupNormParams p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Lanes<VEC, NV> at(p, blockIdx.y, lane);
-    const int64_t n0 = ((int64_t)blockIdx.x * 4 + wave) * U;
+    const Lanes<VEC, NV> at(p, blockIdx.x % p.sets, lane); // (neighbours read neighbouring channels)
+    const int64_t n0 = ((int64_t)(blockIdx.x / p.sets) * 4 + wave) * U;
     if (n0 >= p.N) return;
     Raw<T, VEC> rx[U][NV], rg[U][GATE ? NV : 1];
 #pragma unroll
@@ -177,7 +177,7 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(GroupNormParams p) {
             } else {
                 act_n<VEC>(p.act, z, a);
             }
-            if (at.ok[k]) store_n<T, VEC>(static_cast<T *>(p.y) + n * p.sxn + at.c[k], a);
+            if (at.ok[k]) stream_n<T, VEC>(static_cast<T *>(p.y) + n * p.sxn + at.c[k], a);
         }
         if (p.stats && at.g < p.G && (lane & ((1 << p.log_l) - 1)) == 0) {
             p.stats[(n * p.G + at.g) * 2] = mean[u];
@@ -186,15 +186,16 @@ __global__ __launch_bounds__(256) void norm_rows_kernel(GroupNormParams p) {
     }
 }
 
-// S = 1, adjoint.  A workgroup's waves walk its block of rows, U at a time each,
-// the next ones' loads in flight, and keep dweight and dbias of its channels in registers; the
+// S = 1, adjoint.  The waves of all workgroups walk the rows together, U at a time
+// each (blocks of rows of their own, a power of two apart, meet in few memory
+// channels: 94 against 66 us), the next ones' loads in flight, and keep dweight and dbias of its channels in registers; the
 // workgroup's go to part [row_blocks][2][C].
 template <typename T, int VEC, int NV, int U, bool GATE>
 __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(GroupNormParams p) {
     __shared__ float red[2][4][kWave * VEC * NV];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const Lanes<VEC, NV> at(p, blockIdx.y, lane);
-    const int64_t n0 = p.N * blockIdx.x / p.row_blocks, n1 = p.N * (blockIdx.x + 1) / p.row_blocks;
+    const Lanes<VEC, NV> at(p, blockIdx.x % p.sets, lane);
+    const int64_t block = blockIdx.x / p.sets, n0 = block * 4 * U, step = (int64_t)p.row_blocks * 4 * U, n1 = p.N;
     float wt[NV][VEC], bs[NV][VEC], dwt[NV][VEC], dbs[NV][VEC];
 #pragma unroll
     for (int k = 0; k < NV; ++k) {
@@ -225,9 +226,9 @@ __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(GroupNormParams p) {
     };
     Rows next;
     if (n0 + wave * U < n1) load(n0 + wave * U, next);
-    for (int64_t first = n0 + wave * U; first < n1; first += 4 * U) {
+    for (int64_t first = n0 + wave * U; first < n1; first += step) {
         const Rows r = next;
-        load(min(first + 4 * U, n1 - 1), next);
+        load(min(first + step, n1 - 1), next);
         float nn[U][NV][VEC], dn[U][NV][VEC], s[2 * U]; // sums of dn, of dn n
 #pragma unroll
         for (int u = 0; u < U; ++u) {
@@ -252,7 +253,7 @@ __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(GroupNormParams p) {
                         dg[j] = (float)r.dy[u][k][j] * z[j] * d[j];
                         dz[j] = (float)r.dy[u][k][j] * a[j];
                     }
-                    if (in && at.ok[k]) store_n<T, VEC>(static_cast<T *>(p.dgate) + n * p.sgn + at.c[k], dg);
+                    if (in && at.ok[k]) stream_n<T, VEC>(static_cast<T *>(p.dgate) + n * p.sgn + at.c[k], dg);
                 } else {
                     act_grad_n<VEC>(p.act, z, a, d);
 #pragma unroll
@@ -278,7 +279,7 @@ __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(GroupNormParams p) {
                 float dx[VEC];
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) dx[j] = r.rstd[u] * (dn[u][k][j] - s[2 * u] * inv_d - nn[u][k][j] * (s[2 * u + 1] * inv_d));
-                if (at.ok[k]) store_n<T, VEC>(static_cast<T *>(p.y) + (first + u) * p.sxn + at.c[k], dx);
+                if (at.ok[k]) stream_n<T, VEC>(static_cast<T *>(p.y) + (first + u) * p.sxn + at.c[k], dx);
             }
         }
     }
@@ -292,7 +293,7 @@ __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(GroupNormParams p) {
         }
     __syncthreads();
     if (wave == 0) {
-        float *out = p.part + (int64_t)blockIdx.x * 2 * p.C;
+        float *out = p.part + block * 2 * p.C;
 #pragma unroll
         for (int k = 0; k < NV; ++k)
             if (at.ok[k]) {
@@ -630,7 +631,7 @@ template <int VEC, int E> struct Held {
     int64_t n, s0;
     __device__ Held(const GroupNormParams &p, unsigned number) {
         parts = p.chunks * p.tiles;
-        part = (int)(number % (unsigned)parts);
+        part = (int)(number % (unsigned)parts); // (a set's parts start together: the waits are shorter)
         const unsigned ns = number / (unsigned)parts;
         set = (int)(ns % (unsigned)p.sets);
         n = ns / (unsigned)p.sets;
@@ -862,7 +863,7 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
         } else {
             act_n<VEC>(p.act, z, a);
         }
-        store_n<T, VEC>(y + at.row(i) * p.sxs, a);
+        stream_n<T, VEC>(y + at.row(i) * p.sxs, a);
     }
 }
 
@@ -914,7 +915,7 @@ __global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
                 a[j] = __builtin_fmaf(dz[j], n[j], a[j]);
                 b[j] += dz[j];
             }
-            if constexpr (GATE && keep) store_n<T, VEC>(dgate + h.row(i) * p.sgs, dg);
+            if constexpr (GATE && keep) stream_n<T, VEC>(dgate + h.row(i) * p.sgs, dg);
         });
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
@@ -985,7 +986,7 @@ __global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
         element(ch, rx[i], ry[i], rg[GATE ? i : 0], n, dz, dg);
 #pragma unroll
         for (int j = 0; j < VEC; ++j) o[j] = ch.rstd[j] * (dz[j] * ch.wt[j] - m1[j] - n[j] * m2[j]);
-        store_n<T, VEC>(dx + at.row(i) * p.sxs, o);
+        stream_n<T, VEC>(dx + at.row(i) * p.sxs, o);
     }
 }
 
@@ -1061,8 +1062,9 @@ Plan plan_of(const gdn2_group_norm_args &a, bool bwd, bool vec4, bool sums_wante
         const int gpw = 64 >> q.log_l;
         q.sets = (int)((a.groups + gpw - 1) / gpw);
         if (bwd) {
-            // 2048 workgroups, eight a compute unit, of at least two rows a wave
-            q.row_blocks = (int)std::max<int64_t>(1, std::min<int64_t>((2048 + q.sets - 1) / q.sets, (N + 7) / 8));
+            // 512 workgroups, two a compute unit (1024: 67 against 62.5 us at 8192 x 2048
+            // gated f32), of at least two rows a wave
+            q.row_blocks = (int)std::max<int64_t>(1, std::min<int64_t>((512 + q.sets - 1) / q.sets, (N + 7) / 8));
             q.bytes = sums_wanted ? up256(8 * (size_t)q.row_blocks * C) : 0;
         }
         return q;
@@ -1144,11 +1146,11 @@ GroupNormParams fill(const gdn2_group_norm_args &a, const Plan &q, void *ws) {
     p.sxn = a.stride_x_n; p.sxs = a.stride_x_s; p.sgn = a.stride_gate_n; p.sgs = a.stride_gate_s;
     p.N = a.samples; p.S = a.rows; p.C = (int)a.channels; p.G = (int)a.groups; p.D = p.C / p.G;
     p.act = a.activation; p.eps = (float)a.eps;
-    p.log_l = q.log_l; p.row_blocks = q.row_blocks; p.lc = q.lc; p.chunks = q.chunks; p.chunk = q.chunk;
+    p.sets = q.sets; p.log_l = q.log_l; p.row_blocks = q.row_blocks; p.lc = q.lc; p.chunks = q.chunks; p.chunk = q.chunk;
     char *w = static_cast<char *>(ws);
     if (q.bytes) p.part = reinterpret_cast<float *>(w);
     if (q.held) {
-        p.tile = q.tile; p.tiles = q.tiles; p.sets = q.sets; p.set_groups = q.set_groups;
+        p.tile = q.tile; p.tiles = q.tiles; p.set_groups = q.set_groups;
         if (q.words) {
             p.words = reinterpret_cast<unsigned long long *>(w + q.o_words);
             p.patience = g_patience.load(std::memory_order_relaxed);
@@ -1159,14 +1161,14 @@ GroupNormParams fill(const gdn2_group_norm_args &a, const Plan &q, void *ws) {
 }
 
 template <typename T, int VEC, bool GATE> hipError_t run_rows(const Plan &q, const GroupNormParams &p, hipStream_t s) {
-    const dim3 grid((unsigned)((p.N + 4 * q.u - 1) / (4 * q.u)), (unsigned)q.sets);
+    const dim3 grid((unsigned)((p.N + 4 * q.u - 1) / (4 * q.u) * q.sets));
     if (q.nv == 1) hipLaunchKernelGGL((norm_rows_kernel<T, VEC, 1, 4, GATE>), grid, dim3(256), 0, s, p);
     else if (q.nv == 4) hipLaunchKernelGGL((norm_rows_kernel<T, VEC, 4, 1, GATE>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((norm_rows_kernel<T, VEC, 16, 1, GATE>), grid, dim3(256), 0, s, p);
     return hipGetLastError();
 }
 template <typename T, int VEC, bool GATE> hipError_t run_rows_bwd(const Plan &q, const GroupNormParams &p, hipStream_t s) {
-    const dim3 grid((unsigned)q.row_blocks, (unsigned)q.sets);
+    const dim3 grid((unsigned)(q.row_blocks * q.sets));
     if (q.nv == 1) hipLaunchKernelGGL((norm_rows_bwd_kernel<T, VEC, 1, 2, GATE>), grid, dim3(256), 0, s, p);
     else if (q.nv == 4) hipLaunchKernelGGL((norm_rows_bwd_kernel<T, VEC, 4, 1, GATE>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((norm_rows_bwd_kernel<T, VEC, VEC == 4 ? 8 : 16, 1, GATE>), grid, dim3(256), 0, s, p);
@@ -1226,7 +1228,7 @@ template <typename T, int VEC, bool GATE> hipError_t run_backward(const Plan &q,
 }
 
 bool grid_fits(const gdn2_group_norm_args &a, const Plan &q) {
-    if (q.rows) return q.sets < 65536;
+    if (q.rows) return (double)((a.samples + 3) / 4) * q.sets < 16777216.0;
     if (q.held) return (double)a.samples * q.sets * q.chunks * q.tiles < 16777216.0;
     return (double)a.samples * q.chunks < 16777216.0 && q.tiles < 65536;
 }

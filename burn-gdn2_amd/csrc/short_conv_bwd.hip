@@ -20,7 +20,7 @@ namespace gdn2 {
 namespace {
 
 constexpr int kCache = 3;
-constexpr int kStep = 4; // tokens whose rows are loaded together
+constexpr int kStep = 2; // tokens whose rows are loaded together
 
 struct ConvGradParams {
     const float *x, *w, *cache, *dy, *dcache;
@@ -87,18 +87,27 @@ template <int VEC> __global__ __launch_bounds__(256) void short_conv_bwd_kernel(
         }
     };
     if (t0 < t1) {
-        float a[VEC], g[VEC], out[VEC];
+        float xp[3][VEC], gp[3][VEC], xn[kStep][VEC], gn[kStep][VEC], out[VEC];
+        auto load = [&](int64_t s0) { // the rows of tokens s0 + 3 .. s0 + 3 + kStep: outputs s0 ..
 #pragma unroll
-        for (int i = 0; i < 3; ++i) pad(t0 + i, xw[i]);
+            for (int i = 0; i < kStep; ++i) {
+                row(x, s0 + 3 + i, xn[i]);
+                row(dy, s0 + 3 + i, gn[i]);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            pad(t0 + i, xw[i]);
+            row(x, t0 + i, xp[i]);
+            row(dy, t0 + i, gp[i]);
+        }
+        load(t0);
         float first[VEC]; // dxpad[0 .. 2] where the run starts the sequence
 #pragma unroll
         for (int j = 0; j < VEC; ++j) first[j] = 0.f;
 #pragma unroll
         for (int i = 0; i < 3; ++i) {
-            const int64_t t = t0 + i;
-            row(x, t, a);
-            row(dy, t, g);
-            token(t, t < t1, a, g, out);
+            token(t0 + i, t0 + i < t1, xp[i], gp[i], out);
             if (t0 == 0) {
                 if (dc && i >= p.T) {
                     float e[VEC];
@@ -114,15 +123,6 @@ template <int VEC> __global__ __launch_bounds__(256) void short_conv_bwd_kernel(
                 }
             }
         }
-        float xn[kStep][VEC], gn[kStep][VEC]; // the rows of tokens s0 + 3 .. s0 + 3 + kStep: outputs s0 ..
-        auto load = [&](int64_t s0) {
-#pragma unroll
-            for (int i = 0; i < kStep; ++i) {
-                row(x, s0 + 3 + i, xn[i]);
-                row(dy, s0 + 3 + i, gn[i]);
-            }
-        };
-        load(t0);
         for (int64_t s0 = t0; s0 < t1; s0 += kStep) {
             float xs[kStep][VEC], gs[kStep][VEC];
 #pragma unroll
@@ -145,7 +145,7 @@ template <int VEC> __global__ __launch_bounds__(256) void short_conv_bwd_kernel(
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) out[j] += first[j];
                 }
-                if (ok) store_n<float, VEC>(dx + s * p.C, out);
+                if (ok) stream_n<float, VEC>(dx + s * p.C, out);
             }
         }
     }

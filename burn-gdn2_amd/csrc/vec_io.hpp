@@ -28,6 +28,15 @@ template <typename T, int N> __device__ __forceinline__ void store_n(T *p, const
     *reinterpret_cast<Raw<T, N> *>(p) = v;
 }
 
+// ... for results that are larger than the caches and not read again here: a hint
+// that leaves the caches to what is (up to a tenth of a kernel's time)
+template <typename T, int N> __device__ __forceinline__ void stream_n(T *p, const float *x) {
+    Raw<T, N> v;
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = (T)x[j];
+    __builtin_nontemporal_store(v, reinterpret_cast<Raw<T, N> *>(p));
+}
+
 // Sums of n values over the 2^log_l neighbouring lanes of each group of lanes, to
 // all of them (log_l the same in the wave).  Up to 16 lanes by the adder's own lane
 // moves: the other lane of a pair, the other pair, and, the sums being the same in

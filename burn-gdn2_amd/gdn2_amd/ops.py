@@ -388,14 +388,19 @@ def short_conv_1d_backward(x, weight, d_out, cache=None, d_cache=None, workspace
     """The gradients of L = <d_out, out> + <d_cache, new cache> for short_conv_1d's
     arguments: dict dx [B, T, C] (without a cache the padding's share is in the
     first token's), dweight [C, 4] and dcache [B, 3, C] (None without a cache)."""
-    if x.dim() != 3 or tuple(weight.shape) != (x.shape[2], 4):
+    if x.dim() != 3 or weight.shape != (x.shape[2], 4):
         raise ValueError("short_conv_1d_backward: x must be [B, T, C] and weight [C, 4]")
     B, T, Cn = x.shape
-    if d_out.shape != x.shape or any(t is not None and tuple(t.shape) != (B, 3, Cn) for t in (cache, d_cache)):
-        raise ValueError("short_conv_1d_backward: d_out must have x's shape, cache and d_cache be [B, 3, C]")
+    if d_out.shape != x.shape:
+        raise ValueError("short_conv_1d_backward: d_out must have x's shape")
+    for t in (cache, d_cache):
+        if t is not None and t.shape != (B, 3, Cn):
+            raise ValueError("short_conv_1d_backward: cache and d_cache must be [B, 3, C]")
     _check_f32_cuda(x, weight, d_out, cache, d_cache)
-    if any(t is not None and t.device != x.device for t in (weight, d_out, cache, d_cache)):
-        raise ValueError("short_conv_1d_backward: the operands are on several devices")
+    index = x.get_device()
+    for t in (weight, d_out, cache, d_cache):
+        if t is not None and t.get_device() != index:
+            raise ValueError("short_conv_1d_backward: the operands are on several devices")
     x, weight, d_out = x.contiguous(), weight.contiguous(), d_out.contiguous()
     cache = None if cache is None else cache.contiguous()
     d_cache = None if d_cache is None else d_cache.contiguous()
@@ -405,15 +410,17 @@ def short_conv_1d_backward(x, weight, d_out, cache=None, d_cache=None, workspace
     need = L.gdn2_short_conv_bwd_workspace_bytes(B, T, Cn)
     if need and (workspace is None or workspace.numel() * workspace.element_size() < need):
         workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
-    ptr = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-    args = (x.data_ptr(), weight.data_ptr(), ptr(cache), d_out.data_ptr(), ptr(d_cache), dx.data_ptr(), dweight.data_ptr(),
-            ptr(dcache), B, T, Cn, ptr(workspace), 0 if workspace is None else workspace.numel() * workspace.element_size())
-    index = x.get_device()
+    args = (x.data_ptr(), weight.data_ptr(), None if cache is None else cache.data_ptr(), d_out.data_ptr(),
+            None if d_cache is None else d_cache.data_ptr(), dx.data_ptr(), dweight.data_ptr(),
+            None if dcache is None else dcache.data_ptr(), B, T, Cn, None if workspace is None else workspace.data_ptr(),
+            0 if workspace is None else workspace.numel() * workspace.element_size())
     if torch.cuda.current_device() == index:
-        C.check(L.gdn2_short_conv_bwd_f32(*args, torch._C._cuda_getCurrentRawStream(index)))
+        status = L.gdn2_short_conv_bwd_f32(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(index):
-            C.check(L.gdn2_short_conv_bwd_f32(*args, torch._C._cuda_getCurrentRawStream(index)))
+            status = L.gdn2_short_conv_bwd_f32(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        C.check(status)
     return {"dx": dx, "dweight": dweight, "dcache": dcache}
 
 

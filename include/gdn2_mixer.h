@@ -117,8 +117,7 @@ GDN2_API gdn2_status gdn2_gated_scan_bwd_bf16(const gdn2_gated_scan_bwd_args *ar
  * what the backward takes.
  * workspace: gdn2_group_norm_act_workspace_bytes(args) bytes (0 for S = 1 and
  * ordinary groups), 256-byte aligned.
- * Limits (else GDN2_NOT_APPLICABLE): C < 2^24, S < 2^30, N groups < 2^24, and at
- * most 2^16 groups where a wave holds fewer than two of them.
+ * Limits (else GDN2_NOT_APPLICABLE): C < 2^24, S < 2^30, N and N groups < 2^24.
  * ---------------------------------------------------------------------- */
 typedef enum gdn2_activation {
     GDN2_ACT_NONE = 0,
