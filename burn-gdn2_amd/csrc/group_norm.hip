@@ -439,6 +439,7 @@ __global__ __launch_bounds__(256) void norm_join_kernel(GroupNormParams p) {
     auto rows = [&](int k) { return (float)min((int64_t)p.chunk, p.S - (int64_t)k * p.chunk); };
     const float base = part[0]; // a mean to sum about
     float s = 0.f;
+#pragma unroll 8
     for (int i = threadIdx.x; i < entries; i += 256) {
         const int k = i / p.D;
         s += rows(k) * (part[(int64_t)k * 2 * p.C + i % p.D] - base);
@@ -446,6 +447,7 @@ __global__ __launch_bounds__(256) void norm_join_kernel(GroupNormParams p) {
     const float size = (float)p.S * (float)p.D;
     const float mean = base + block_sum(s, red) / size;
     float t = 0.f;
+#pragma unroll 8
     for (int i = threadIdx.x; i < entries; i += 256) {
         const int k = i / p.D;
         const float *e = part + (int64_t)k * 2 * p.C + i % p.D;
@@ -562,6 +564,7 @@ __global__ __launch_bounds__(256) void norm_bwd_join_kernel(GroupNormParams p) {
     const int g = (int)(blockIdx.x % p.G), entries = p.chunks * p.D;
     const float *part = p.part + n * p.chunks * 2 * p.C + g * p.D;
     float s = 0.f, t = 0.f;
+#pragma unroll 8
     for (int i = threadIdx.x; i < entries; i += 256) {
         const float *e = part + (int64_t)(i / p.D) * 2 * p.C + i % p.D;
         const float w = p.weight ? p.weight[g * p.D + i % p.D] : 1.f;
@@ -1092,7 +1095,8 @@ Plan plan_of(const gdn2_group_norm_args &a, bool bwd, bool vec4, bool sums_wante
     // about 2048 workgroups, of at least four rows a thread
     const int64_t rows = 256 / q.lc;
     const int64_t most = std::max<int64_t>(1, S / (4 * rows)), want = std::max<int64_t>(1, 2048 / (N * q.tiles));
-    const int64_t chunks = std::min(most, want);
+    // and few enough for the join, one workgroup a group, to read them quickly
+    const int64_t chunks = std::min({most, want, std::max<int64_t>(1, 16384 / (C / a.groups))});
     q.chunk = (int)((S + chunks - 1) / chunks);
     q.chunks = (int)((S + q.chunk - 1) / q.chunk);
     size_t at = up256(8 * (size_t)(N * q.chunks) * C);

@@ -68,7 +68,7 @@ def _workspace(args, workspace: Optional[torch.Tensor], need: int, like: torch.T
 def _dense_rows(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy of it, with contiguous channels and no element of memory in
     two places (what the gradients are laid out like)."""
-    if t.is_contiguous():
+    if t.is_contiguous() or (t.dim() == 4 and t.transpose(1, 2).is_contiguous()):
         return t
     if t.shape[-1] != 1 and t.stride(-1) != 1:
         return t.contiguous()
@@ -82,8 +82,9 @@ def _dense_rows(t: torch.Tensor) -> torch.Tensor:
 
 def _empty_like(t: torch.Tensor) -> torch.Tensor:
     """A tensor of t's shape, type and strides."""
-    if t.is_contiguous():
-        return torch.empty_like(t)
+    r = torch.empty_like(t)  # (t's strides where no memory is left out between its rows)
+    if r.stride() == t.stride():
+        return r
     return torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=t.device)
 
 
