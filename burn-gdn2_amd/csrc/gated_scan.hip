@@ -422,8 +422,11 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
                 const bool follows = q.tile + 1 < p.tiles_t && (LOOK > 1 || lane < CH);
                 if (follows) publish(p.agg + at + (int64_t)tile * CH, (unsigned long long)word(Gt) | (unsigned long long)word(Xt) << 32);
                 if (tile > 0) {
-                    // Looks at the W tiles before this one (tile 0 stands in for any before it).
-                    constexpr int W = 4;
+                    // Looks at the W tiles before this one (tile 0 stands in for any before it):
+                    // a state passes W tiles a look.  4 take 1 % less where the chip is full
+                    // (65536 x 2048 bf16) and 20 to 40 % more for a few channels (32318 x 128: 65
+                    // against 52 us); looks by all waves, 16 tiles at a time, crowd the memory (87).
+                    constexpr int W = VEC == 8 && !HEAD ? 6 : 8; // (as many as the registers hold)
                     for (;;) {
                         unsigned P[W];
                         unsigned long long A[W];
