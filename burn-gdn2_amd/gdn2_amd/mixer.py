@@ -177,7 +177,7 @@ def gated_scan(g, v, w=None, state=None, cu_seqlens=None, out=None, new_state=No
     a = _scan_args(g, v, w, state, new_state, out, cu_seqlens, of_states[0])
     L = C.lib()
     keep = None
-    if v.shape[2] > 8 or cu_seqlens is not None:  # (up to 8 tokens never need a workspace)
+    if v.shape[2] > 12 or cu_seqlens is not None:  # (up to 12 tokens never need a workspace)
         keep = _workspace(a, workspace, L.gdn2_gated_scan_workspace_bytes(a), v)
     _call(L.gdn2_gated_scan_fwd_f32 if v.dtype is torch.float32 else L.gdn2_gated_scan_fwd_bf16, a, index)
     del keep

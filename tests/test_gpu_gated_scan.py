@@ -82,6 +82,22 @@ def test_forward(gpu, B, T, H, V, ty):
 
 
 @pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("B,T", [(1, 12), (1, 13), (80, 13), (80, 32), (80, 33)])
+def test_few_tokens(gpu, B, T, ty):
+    """Lengths at which the walk over the tokens gives way to tiles, with few rows
+    and with more than run at once."""
+    import torch
+
+    import gdn2_amd as G
+
+    for per_head, V in ((False, 128), (True, 128), (False, 127)):
+        d = _make(gpu, T + B, B, T, 16, V, ty, per_head, True, True)
+        out, new = G.gated_scan(**d)
+        torch.cuda.synchronize()
+        assert _check_forward(d, out, new, B, ty).all()
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
 @pytest.mark.parametrize("B,T,H,V", CASES)
 def test_backward(gpu, B, T, H, V, ty):
     import torch
