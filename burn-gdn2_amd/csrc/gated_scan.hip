@@ -23,8 +23,8 @@
 // applies the (G, X) after it in order, which gives the same bits whichever of
 // them that was.  Words carry their own readiness (all ones: not yet), so that no
 // other memory has to be ordered with them.  A workgroup draws its tile's number
-// when it starts: the tiles it waits for have then started too, and a tile
-// publishes (G, X) without waiting for anything, so every wait ends.
+// when it is about to start on it: of the tiles that were drawn and are not
+// finished, the one of the lowest number waits for none, so every wait ends.
 //
 // Bound: HBM, 16 bytes an element forward and 32 backward in f32.
 #include <algorithm>
@@ -660,7 +660,7 @@ const char *check(const gdn2_gated_scan_args &a, bool *nothing, bool *limits) {
     *nothing = *limits = false;
     if (a.batch < 0 || a.num_heads < 0 || a.seq_len < 0 || a.head_v_dim < 0 || a.num_seqs < 0) return "negative dimension";
     if (a.cu_seqlens && a.batch != 1) return "packed sequences need batch 1";
-    if (a.batch == 0 || a.num_heads == 0 || a.head_v_dim == 0 || (a.cu_seqlens && a.num_seqs == 0)) {
+    if (a.batch == 0 || a.num_heads == 0 || a.head_v_dim == 0) {
         *nothing = true;
         return nullptr;
     }
@@ -788,9 +788,10 @@ template <typename T> gdn2_status forward(const char *who, const gdn2_gated_scan
     bool nothing, limits;
     if (const char *e = check(*a, &nothing, &limits))
         return fail(limits ? GDN2_NOT_APPLICABLE : GDN2_EINVAL, std::string(who) + ": " + e);
-    if (nothing) return GDN2_OK;
+    if (nothing || (a->cu_seqlens && a->num_seqs == 0)) return GDN2_OK;
     if (a->seq_len == 0) return no_tokens(*a, a->state_in, a->state_out, s);
     if (!a->g || !a->v || !a->out) return fail(GDN2_EINVAL, std::string(who) + ": null tensor pointer");
+    if (a->out == a->v || a->out == a->w || a->out == a->g) return fail(GDN2_EINVAL, std::string(who) + ": out must not be an input");
     const Plan q = plan_of<T, false>(*a, vec_of<T>(*a, {}, {}));
     if (q.bytes > 0 && (!a->workspace || a->workspace_bytes < q.bytes || !aligned(a->workspace, 256))) return bad_workspace(who);
     GatedScanParams p{};
@@ -813,11 +814,28 @@ template <typename T> gdn2_status backward(const char *who, const gdn2_gated_sca
     bool nothing, limits;
     if (const char *e = check(f, &nothing, &limits))
         return fail(limits ? GDN2_NOT_APPLICABLE : GDN2_EINVAL, std::string(who) + ": " + e);
-    if (nothing) return GDN2_OK;
-    if (f.seq_len == 0) return no_tokens(f, a->d_state_out, a->d_state0, s);
+    if (nothing) { // (heads of no channels still have a log decay)
+        const double all = f.g_per_head ? (double)f.batch * f.num_heads * f.seq_len : 0;
+        if (all == 0) return GDN2_OK;
+        if (f.num_heads >= (1 << 30) || f.seq_len >= (1 << 30) || all >= 4294967040.0)
+            return fail(GDN2_NOT_APPLICABLE, std::string(who) + ": sizes above the kernels' limits");
+        const int64_t n = f.batch * f.num_heads * f.seq_len;
+        if (!a->dg) return fail(GDN2_EINVAL, std::string(who) + ": null tensor pointer");
+        GatedScanParams p{};
+        p.dg = a->dg;
+        p.sgb = f.stride_g_b; p.sgh = f.stride_g_h; p.sgt = f.stride_g_t;
+        p.T = (int)f.seq_len; p.H = (int)f.num_heads;
+        hipLaunchKernelGGL(dg_sum_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, p, n);
+        GDN2_HIP_CHECK(hipGetLastError());
+        return GDN2_OK;
+    }
+    if (f.seq_len == 0) return f.cu_seqlens && f.num_seqs == 0 ? GDN2_OK : no_tokens(f, a->d_state_out, a->d_state0, s);
     if (!f.g || !f.out || !a->d_out || !a->dg || !a->dv || (f.w && !f.v))
         return fail(GDN2_EINVAL, std::string(who) + ": null tensor pointer");
     if (!f.w != !a->dw) return fail(GDN2_EINVAL, std::string(who) + ": dw must be given exactly where w is");
+    for (const void *r : {(const void *)a->dg, (const void *)a->dv, (const void *)a->dw})
+        for (const void *q : {(const void *)f.g, f.v, f.w, (const void *)f.out, a->d_out})
+            if (r && r == q) return fail(GDN2_EINVAL, std::string(who) + ": dg, dv and dw must not be inputs");
     const int vec = vec_of<T>(f, {a->d_out, a->dv, a->dw}, {a->d_state_out, a->d_state0, f.g_per_head ? nullptr : a->dg});
     const Plan q = plan_of<T, true>(f, vec);
     if (q.bytes > 0 && (!a->workspace || a->workspace_bytes < q.bytes || !aligned(a->workspace, 256))) return bad_workspace(who);
@@ -842,6 +860,7 @@ template <typename T> gdn2_status backward(const char *who, const gdn2_gated_sca
 template <bool BWD> size_t workspace_of(const gdn2_gated_scan_args *a) {
     bool nothing, limits;
     if (!a || check(*a, &nothing, &limits) || nothing || a->seq_len == 0) return 0;
+    if (!BWD && a->cu_seqlens && a->num_seqs == 0) return 0;
     size_t n = 0;
     for (const int vec : {8, 4, 1})
         n = std::max({n, plan_of<float, BWD>(*a, vec).bytes, plan_of<bf16, BWD>(*a, vec).bytes});

@@ -1244,6 +1244,8 @@ template <typename T> gdn2_status forward(const char *who, const gdn2_group_norm
     if (const char *e = check(*a, &nothing, &limits)) return refuse(who, e, limits ? GDN2_NOT_APPLICABLE : GDN2_EINVAL);
     if (nothing) return GDN2_OK;
     if (!a->x || !a->y) return refuse(who, "null tensor pointer");
+    if (a->y == a->gate && (a->stride_gate_n != a->stride_x_n || a->stride_gate_s != a->stride_x_s))
+        return refuse(who, "y may be gate only with x's strides");
     const Plan q = plan_of(*a, false, can_vec<T>(*a), false, a->y == a->x || a->y == a->gate);
     if (!grid_fits(*a, q)) return refuse(who, "sizes above the kernels' limits", GDN2_NOT_APPLICABLE);
     if (q.bytes > 0 && (!a->workspace || a->workspace_bytes < q.bytes || !aligned(a->workspace, 256)))
@@ -1262,6 +1264,9 @@ template <typename T> gdn2_status backward(const char *who, const gdn2_group_nor
     if (!nothing) {
         if (!f.x || !f.stats || !a->d_y || !a->dx) return refuse(who, "null tensor pointer");
         if (!f.gate != !a->dgate) return refuse(who, "dgate must be given exactly where gate is");
+        for (const void *in : {f.x, f.gate})
+            if (in && (a->dx == in || a->dgate == in)) return refuse(who, "dx and dgate must not be inputs");
+        if (a->dgate && (a->dgate == a->d_y || a->dgate == a->dx)) return refuse(who, "dgate must not be another operand");
     }
     const bool sums = a->dweight || a->dbias;
     if (nothing) { // no rows: zero gradients of the weights

@@ -230,6 +230,9 @@ gdn2_status run(const float *x, const float *weight, const float *cache_in, cons
     }
     const size_t nx = sizeof(float) * (size_t)(B * T) * C;
     if (overlaps(dx, x, nx) || overlaps(dx, d_out, nx)) return fail(GDN2_EINVAL, who + "dx must not overlap x or d_out");
+    const size_t nc = sizeof(float) * (size_t)(B * kCache) * C;
+    if (d_cache_in && (overlaps(d_cache_in, cache_in, nc) || (d_cache_out && overlaps(d_cache_in, d_cache_out, nc))))
+        return fail(GDN2_EINVAL, who + "d_cache_in must not overlap cache_in or d_cache_out");
     uintptr_t bits = 0;
     for (const void *q : {(const void *)x, (const void *)cache_in, (const void *)d_out, (const void *)d_cache_out,
                           (const void *)dx, (const void *)d_cache_in})

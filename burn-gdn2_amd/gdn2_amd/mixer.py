@@ -12,6 +12,7 @@ workspaces come from torch's allocator, so a call may be captured into a graph.
 """
 from __future__ import annotations
 
+import math
 from typing import Optional, Tuple
 
 import torch
@@ -57,6 +58,8 @@ def _call(fn, args, index: int) -> None:
 def _workspace(args, workspace: Optional[torch.Tensor], need: int, like: torch.Tensor):
     """Sets the workspace of `args`, a new one where none or too small a one is
     given; returns the tensor, to be kept until the call is made."""
+    if workspace is not None and (workspace.get_device() != like.get_device() or not workspace.is_contiguous()):
+        raise ValueError("workspace must be a contiguous tensor on the operands' device")
     if need == 0:
         return None
     if workspace is None or workspace.numel() * workspace.element_size() < need:
@@ -162,14 +165,15 @@ def gated_scan(g, v, w=None, state=None, cu_seqlens=None, out=None, new_state=No
                             (("new_state", new_state),) if new_state is not None else ())
     index = _device(v, g, w, state, cu_seqlens, out, new_state)
     v, g = _channels(v), _channels(g)
-    if w is not None:
+    if w is not None and w.stride() != v.stride():
+        v = _dense_rows(v)
         w = _in_layout(w, v)
     if state is not None:
         state = state.contiguous()
     if out is None:
         out = torch.empty_like(v)
-    elif out.shape[3] != 1 and out.stride(3) != 1:
-        raise ValueError("out's channels must be contiguous")
+    elif _dense_rows(out) is not out:
+        raise ValueError("out's channels must be contiguous and its rows apart")
     if new_state is None:
         new_state = torch.empty(of_states, dtype=torch.float32, device=v.device) if state is None else torch.empty_like(state)
     elif not new_state.is_contiguous():
@@ -194,7 +198,7 @@ def gated_scan_backward(g, v, w, out, d_out, state=None, d_state=None, cu_seqlen
     v, g = _dense_rows(v), _dense_rows(g)
     if w is not None:
         w = _in_layout(w, v)
-    out = _channels(out)
+    out = _dense_rows(out)
     d_out = _in_layout(d_out, out)
     state = None if state is None else state.contiguous()
     d_state = None if d_state is None else d_state.contiguous()
@@ -216,7 +220,7 @@ _ACTS = {"none": C.ACT_NONE, "silu": C.ACT_SILU, "gelu": C.ACT_GELU}
 
 def _rows3(t: torch.Tensor) -> torch.Tensor:
     """[N, ..., C] as [N, S, C]."""
-    return t if t.dim() == 3 else t.unsqueeze(1) if t.dim() == 2 else t.reshape(t.shape[0], -1, t.shape[-1])
+    return t if t.dim() == 3 else t.unsqueeze(1) if t.dim() == 2 else t.reshape(t.shape[0], math.prod(t.shape[1:-1]), t.shape[-1])
 
 
 def _norm_check(x, groups, weight, bias, activation, gate, others=()):

@@ -401,6 +401,8 @@ def short_conv_1d_backward(x, weight, d_out, cache=None, d_cache=None, workspace
     for t in (weight, d_out, cache, d_cache):
         if t is not None and t.get_device() != index:
             raise ValueError("short_conv_1d_backward: the operands are on several devices")
+    if workspace is not None and (workspace.get_device() != index or not workspace.is_contiguous()):
+        raise ValueError("short_conv_1d_backward: workspace must be a contiguous tensor on the operands' device")
     x, weight, d_out = x.contiguous(), weight.contiguous(), d_out.contiguous()
     cache = None if cache is None else cache.contiguous()
     d_cache = None if d_cache is None else d_cache.contiguous()

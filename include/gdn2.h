@@ -258,7 +258,8 @@ GDN2_API gdn2_status gdn2_rms_norm_gate_f32(const float *x, const float *gate, c
  *   dx           [B, T, C], not overlapping x or d_out; without a cache the
  *                padding's gradient is in dx of the first token
  *   dweight      [C, 4], overwritten: summed over B and T in a fixed order
- *   d_cache_in   [B, 3, C], or NULL (not wanted; NULL without cache_in)
+ *   d_cache_in   [B, 3, C], or NULL (not wanted; NULL without cache_in), not
+ *                overlapping cache_in or d_cache_out
  * workspace: gdn2_short_conv_bwd_workspace_bytes(B, T, C) bytes, 256-byte
  * aligned (0 without tokens).  Limits (else GDN2_NOT_APPLICABLE): C < 2^22 and
  * B (T / 32 + 1) < 2^24. */

@@ -84,7 +84,8 @@ GDN2_API gdn2_status gdn2_gated_scan_fwd_bf16(const gdn2_gated_scan_args *args, 
  *   dv, dw       strided like v; dw NULL iff w is
  *   d_state0     [N, H, V] contiguous, or NULL (not wanted); d_state_out may be
  *                the same buffer
- * Rows of dg, dv and dw outside every sequence are zero.
+ * Nothing else may overlap.  Rows of dg, dv and dw outside every
+ * sequence are zero.
  * workspace: gdn2_gated_scan_bwd_workspace_bytes(args) bytes, 256-byte aligned.
  * Limits: those of the forward. */
 typedef struct gdn2_gated_scan_bwd_args {
@@ -152,7 +153,7 @@ GDN2_API int gdn2_group_norm_patience(int looks);
 /* The gradients of L = <d_y, y> of that call.  fwd: its arguments with the
  * stats it wrote (y unused).  d_y and dx strided like x, dgate like gate (NULL
  * iff gate is); dweight, dbias [C], either NULL (not wanted).  Every output is
- * overwritten; dx may be d_y (equal strides), nothing else may overlap.  Sums
+ * overwritten; dx may be d_y, nothing else may overlap.  Sums
  * over samples and rows run in a fixed order.
  * workspace: gdn2_group_norm_act_bwd_workspace_bytes(args) bytes. */
 typedef struct gdn2_group_norm_bwd_args {

@@ -390,6 +390,80 @@ def test_no_tokens(gpu):
     assert torch.equal(out, v) and new.shape == (0, 3, 8)
 
 
+@pytest.mark.parametrize("T", [5, 700])
+def test_gradients_of_nothing_are_zero(gpu, T):
+    """No sequence, and heads of no channels: the gradients that there are are zero."""
+    import torch
+
+    import gdn2_amd as G
+
+    for g_channels in (1, 8):
+        v, g = torch.randn(1, 3, T, 8, device=gpu), -torch.rand(1, 3, T, g_channels, device=gpu)
+        torch.empty(1 << 22, device=gpu).fill_(7.0)  # (what the results' memory held before)
+        cu = torch.zeros(1, dtype=torch.int32, device=gpu)
+        r = G.gated_scan_backward(g, v, v, v, v, cu_seqlens=cu)
+        assert all((r[n] == 0).all() for n in ("dg", "dv", "dw")) and r["dS0"].shape == (0, 3, 8)
+    none, g = torch.empty(2, 3, T, 0, device=gpu), -torch.rand(2, T, 3, 1, device=gpu).transpose(1, 2)
+    torch.empty(1 << 22, device=gpu).fill_(7.0)
+    assert G.gated_scan(g, none)[0].shape == none.shape
+    r = G.gated_scan_backward(g, none, None, none, none)
+    assert r["dg"].shape == g.shape and (r["dg"] == 0).all()
+
+
+@pytest.mark.parametrize("T", [5, 200])
+def test_expanded_operands(gpu, T):
+    """Operands that several batches or tokens share in memory."""
+    import torch
+
+    import gdn2_amd as G
+
+    for per_head in (False, True):
+        d = _make(gpu, 17, 3, T, 2, 64, "f32", per_head, True, True)
+        for share in (("v",), ("w",), ("g",), ("v", "w"), ("g", "v", "w")):
+            for dim in (0, 2):
+                e = {n: t.narrow(dim, 0, 1).expand(t.shape) if n in share else t for n, t in d.items()}
+                c = {n: t.contiguous() for n, t in e.items()}
+                got, want = G.gated_scan(**e), G.gated_scan(**c)
+                assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1]), (share, dim)
+                dy = want[0][:1].expand(want[0].shape)
+                got = G.gated_scan_backward(e["g"], e["v"], e["w"], want[0], dy, e["state"])
+                want = G.gated_scan_backward(c["g"], c["v"], c["w"], want[0], dy.contiguous(), c["state"])
+                assert all(torch.equal(got[n], want[n]) for n in want), (share, dim)
+        h = G.gated_scan(**d)[0]
+        dy = torch.randn_like(h)
+        same = h[:1].expand(h.shape)  # (an `out` of equal batches)
+        got = G.gated_scan_backward(d["g"], d["v"], d["w"], same, dy)
+        want = G.gated_scan_backward(d["g"], d["v"], d["w"], same.contiguous(), dy)
+        assert all(torch.equal(got[n], want[n]) for n in want)
+        for out in (h[:1].expand(h.shape), h.transpose(2, 3).contiguous().transpose(2, 3), d["v"]):
+            with pytest.raises((ValueError, RuntimeError)):
+                G.gated_scan(**d, out=out)
+
+
+def test_workspaces_that_do_not_fit(gpu):
+    """Too small: another is taken.  Not of this device, or not contiguous: refused."""
+    import torch
+
+    import gdn2_amd as G
+
+    d = _make(gpu, 18, 1, 3000, 2, 64, "f32", True, True, True)
+    want = G.gated_scan(**d)[0]
+    x = torch.randn(1, 3000, 64, device=gpu)
+    y, stats = G.group_norm_act(x, 2, return_stats=True)
+    w = torch.randn(64, 4, device=gpu)
+    calls = [lambda ws: G.gated_scan(**d, workspace=ws)[0],
+             lambda ws: G.gated_scan_backward(d["g"], d["v"], d["w"], want, want, workspace=ws)["dv"],
+             lambda ws: G.group_norm_act(x, 2, workspace=ws),
+             lambda ws: G.group_norm_act_backward(x, 2, stats, x, workspace=ws)["dx"],
+             lambda ws: G.short_conv_1d_backward(x, w, x, workspace=ws)["dx"]]
+    small, large = torch.empty(8, dtype=torch.uint8, device=gpu), torch.empty(1 << 24, dtype=torch.uint8, device=gpu)
+    for call in calls:
+        assert torch.equal(call(small), call(None)) and torch.equal(call(large), call(None))
+        for bad in (torch.empty(1 << 24, dtype=torch.uint8), small[:1].expand(1 << 24), large[::2]):
+            with pytest.raises(ValueError):
+                call(bad)
+
+
 def test_bad_offsets_stay_in_bounds(gpu):
     """Offsets outside the row or decreasing: unspecified results, the buffers
     around the tensors untouched."""

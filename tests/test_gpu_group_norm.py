@@ -231,7 +231,7 @@ def test_nothing(gpu):
 
     import gdn2_amd as G
 
-    for shape in ((0, 3, 64), (4, 0, 64), (0, 64)):
+    for shape in ((0, 3, 64), (4, 0, 64), (0, 64), (0, 3, 5, 64), (2, 0, 5, 64)):
         x = torch.empty(shape, device=gpu)
         y, stats = G.group_norm_act(x, 4, return_stats=True)
         assert y.shape == shape

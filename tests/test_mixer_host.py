@@ -253,3 +253,49 @@ def test_conv_refusals():
                           (ValueError, (x, w, x), {"d_cache": c[:, :2]})]:
         with pytest.raises(err):
             G.short_conv_1d_backward(*args, **kw)
+
+
+def test_operands_that_are_one_another():
+    """A result that is an input, where that is not allowed, comes back as EINVAL."""
+    from gdn2_amd import _capi as C
+
+    L = C.lib()
+    ptr = dict(g=1 << 20, v=2 << 20, w=3 << 20, out=4 << 20)
+    for fn in (L.gdn2_gated_scan_fwd_f32, L.gdn2_gated_scan_fwd_bf16):
+        for name in "gvw":
+            assert fn(ctypes.byref(_scan_struct(**{**ptr, "out": ptr[name]})), None) == C.GDN2_EINVAL, name
+            assert b"out must not be" in L.gdn2_last_error()
+    for fn in (L.gdn2_gated_scan_bwd_f32, L.gdn2_gated_scan_bwd_bf16):
+        for name in ("dg", "dv", "dw"):
+            for to in (*ptr.values(), 5 << 20):
+                b = C.GatedScanBwdArgs(_scan_struct(**ptr), 5 << 20, None, 6 << 20, 7 << 20, 8 << 20, None, None, 0)
+                setattr(b, name, to)
+                assert fn(ctypes.byref(b), None) == C.GDN2_EINVAL, (name, to)
+                assert b"must not be inputs" in L.gdn2_last_error()
+    for fn in (L.gdn2_group_norm_act_f32, L.gdn2_group_norm_act_bf16):
+        a = _norm_struct(x=1 << 20, y=2 << 20, gate=2 << 20, stride_x_n=72000, stride_x_s=8, stride_gate_n=144000, stride_gate_s=16)
+        assert fn(ctypes.byref(a), None) == C.GDN2_EINVAL and b"strides" in L.gdn2_last_error()
+    norm = dict(x=1 << 20, gate=2 << 20, stats=256)
+    for fn in (L.gdn2_group_norm_act_bwd_f32, L.gdn2_group_norm_act_bwd_bf16):
+        for name, to in (("dx", 1), ("dx", 2), ("dx", 5), ("dgate", 1), ("dgate", 2), ("dgate", 3), ("dgate", 4)):
+            b = C.GroupNormBwdArgs(_norm_struct(**norm), 3 << 20, 4 << 20, 5 << 20, None, None, 256, 1 << 40)
+            setattr(b, name, to << 20)
+            assert fn(ctypes.byref(b), None) == C.GDN2_EINVAL and b"must not be" in L.gdn2_last_error(), (name, to)
+    conv = lambda dci, dc: L.gdn2_short_conv_bwd_f32(1 << 20, 256, 2 << 20, 3 << 20, dc, 4 << 20, 256, dci, 2, 5, 8, 256, 1 << 40, None)  # noqa: E731
+    for dci, dc in ((2 << 20, None), ((2 << 20) + 16, None), (5 << 20, 5 << 20), ((5 << 20) - 16, 5 << 20)):
+        assert conv(dci, dc) == C.GDN2_EINVAL and b"d_cache_in" in L.gdn2_last_error()
+
+
+def test_layouts_of_results():
+    """Results never share memory between elements; no elements have a shape."""
+    torch = pytest.importorskip("torch")
+    from gdn2_amd import mixer
+
+    one = torch.zeros(1, 2, 3, 4)
+    wide = one.expand(5, 2, 3, 4)
+    assert mixer._dense_rows(wide) is not wide and mixer._dense_rows(wide).is_contiguous()
+    gaps = torch.zeros(5, 2, 3, 8)[..., :4]
+    assert mixer._dense_rows(gaps) is gaps and mixer._empty_like(gaps).stride() == gaps.stride()
+    assert mixer._rows3(torch.zeros(0, 3, 5, 8)).shape == (0, 15, 8)
+    assert mixer._rows3(torch.zeros(2, 0, 5, 8)).shape == (2, 0, 8)
+    assert mixer._rows3(torch.zeros(2, 3, 5, 0)).shape == (2, 15, 0)
