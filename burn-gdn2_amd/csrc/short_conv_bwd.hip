@@ -7,7 +7,8 @@
 // computes again (x and dy from cache).  dw goes to a sum a workgroup, then to
 // one over the workgroups in a fixed order.
 //
-// Bound: HBM, 12 bytes an element.
+// Bound: HBM, 12 bytes an element: 4 x 2048 x 2048 0.20 GB in 43.4 us (4.6 TB/s),
+// 40 of them the walk (5.0) and 4 the second sum.
 #include <algorithm>
 #include <exception>
 #include <string>
@@ -20,7 +21,7 @@ namespace gdn2 {
 namespace {
 
 constexpr int kCache = 3;
-constexpr int kStep = 2; // tokens whose rows are loaded together
+constexpr int kStep = 2; // tokens whose rows are loaded together (1 to 4 of 16 bytes, 2 to 4 of 8: all 44 to 45 us)
 
 struct ConvGradParams {
     const float *x, *w, *cache, *dy, *dcache;
@@ -192,8 +193,9 @@ ConvPlan plan_of(int64_t B, int64_t T, int64_t C, bool vec4) {
     ConvPlan q{};
     q.vec = vec4 && C % 4 == 0 ? 4 : 1;
     q.tiles = (C + kWave * q.vec - 1) / (kWave * q.vec);
-    // a wave's run: up to 32 tokens (3 of 35 computed twice) while 2048 waves, eight a
-    // compute unit, remain
+    // a wave's run: up to 32 tokens (3 of 35 computed twice; 16: 47.7 against 44 us)
+    // while 2048 waves, eight a compute unit, remain (64: 30 against 26 us at 2 x 3000
+    // x 1537)
     q.run = 32;
     while (q.run > 8 && B * q.tiles * ((T + q.run - 1) / q.run) < 2048) q.run -= 8;
     q.blocks = (T + 4 * q.run - 1) / (4 * q.run);

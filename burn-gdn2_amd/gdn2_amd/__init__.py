@@ -1,9 +1,8 @@
 """gdn2_amd: MI355X (gfx950) GDN-2 chunked and recurrent forward, the
-chunked backward and the layer's backward.
+chunked backward, the layer's backward, and the operators of a gated mixer.
 
-Python front end of libgdn2_amd.so (C ABI in include/gdn2.h and
-include/gdn2_layer.h).  The
-operators run hand-written HIP kernels only; when the library is missing
+Python front end of libgdn2_amd.so (C ABI in include/gdn2.h,
+include/gdn2_layer.h and include/gdn2_mixer.h).  The operators run hand-written HIP kernels only; when the library is missing
 they raise instead of falling back to a CPU path.
 """
 from . import _capi
