@@ -1,6 +1,10 @@
 """The mixer operators without a GPU: their 64-bit forms against differences,
 and what they refuse."""
 import ctypes
+import os
+import re
+import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -299,3 +303,22 @@ def test_layouts_of_results():
     assert mixer._rows3(torch.zeros(0, 3, 5, 8)).shape == (0, 15, 8)
     assert mixer._rows3(torch.zeros(2, 0, 5, 8)).shape == (2, 0, 8)
     assert mixer._rows3(torch.zeros(2, 3, 5, 0)).shape == (2, 15, 0)
+
+
+@pytest.mark.parametrize("source", ["gated_scan", "group_norm", "short_conv_bwd"])
+def test_no_kernel_keeps_registers_in_memory(source, tmp_path):
+    """What the forms of the kernels were chosen by (see FormOf in gated_scan.hip)."""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    sys.path.insert(0, os.path.join(root, "burn-gdn2_amd"))
+    import build
+
+    if not os.path.exists(build.HIPCC):
+        pytest.skip("no hipcc")
+    flags = [f for f in build.FLAGS if f != "-shared"]
+    r = subprocess.run([build.HIPCC, *flags, "--offload-device-only", "-Rpass-analysis=kernel-resource-usage", "-c",
+                        os.path.join(root, "burn-gdn2_amd", "csrc", source + ".hip"), "-o", str(tmp_path / "device.o")],
+                       capture_output=True, text=True, check=True)
+    names = re.findall(r"Function Name: (\S+)", r.stderr)
+    scratch = [int(n) for n in re.findall(r"ScratchSize \[bytes/lane\]: (\d+)", r.stderr)]
+    assert names and len(names) == len(scratch)
+    assert not [n for n, size in zip(names, scratch) if size]
