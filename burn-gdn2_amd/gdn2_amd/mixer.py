@@ -71,8 +71,12 @@ def _workspace(args, workspace: Optional[torch.Tensor], need: int, like: torch.T
 def _dense_rows(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy of it, with contiguous channels and no element of memory in
     two places (what the gradients are laid out like)."""
-    if t.is_contiguous() or (t.dim() == 4 and t.transpose(1, 2).is_contiguous()):
+    if t.is_contiguous():
         return t
+    if t.dim() == 4:  # [B, T, H, V] seen as [B, H, T, V]
+        (B, H, T, V), st = t.shape, t.stride()
+        if st == (T * H * V, V, H * V, 1):
+            return t
     if t.shape[-1] != 1 and t.stride(-1) != 1:
         return t.contiguous()
     span = 1
@@ -175,7 +179,7 @@ def gated_scan(g, v, w=None, state=None, cu_seqlens=None, out=None, new_state=No
     elif _dense_rows(out) is not out:
         raise ValueError("out's channels must be contiguous and its rows apart")
     if new_state is None:
-        new_state = torch.empty(of_states, dtype=torch.float32, device=v.device) if state is None else torch.empty_like(state)
+        new_state = v.new_empty(of_states, dtype=torch.float32) if state is None else torch.empty_like(state)
     elif not new_state.is_contiguous():
         raise ValueError("new_state must be contiguous")
     a = _scan_args(g, v, w, state, new_state, out, cu_seqlens, of_states[0])
@@ -203,7 +207,8 @@ def gated_scan_backward(g, v, w, out, d_out, state=None, d_state=None, cu_seqlen
     state = None if state is None else state.contiguous()
     d_state = None if d_state is None else d_state.contiguous()
     dg, dv, dw = _empty_like(g), _empty_like(v), None if w is None else _empty_like(v)
-    dS0 = torch.empty(of_states, dtype=torch.float32, device=v.device)
+    like = d_state if state is None else state
+    dS0 = v.new_empty(of_states, dtype=torch.float32) if like is None else torch.empty_like(like)
     a = C.GatedScanBwdArgs(_scan_args(g, v, w, state, None, out, cu_seqlens, of_states[0]), d_out.data_ptr(), _p(d_state),
                            dg.data_ptr(), dv.data_ptr(), _p(dw), dS0.data_ptr(), None, 0)
     L = C.lib()
@@ -218,9 +223,9 @@ def gated_scan_backward(g, v, w, out, d_out, state=None, d_state=None, cu_seqlen
 _ACTS = {"none": C.ACT_NONE, "silu": C.ACT_SILU, "gelu": C.ACT_GELU}
 
 
-def _rows3(t: torch.Tensor) -> torch.Tensor:
-    """[N, ..., C] as [N, S, C]."""
-    return t if t.dim() == 3 else t.unsqueeze(1) if t.dim() == 2 else t.reshape(t.shape[0], math.prod(t.shape[1:-1]), t.shape[-1])
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """[N, C] as it is, [N, ..., C] as [N, S, C]."""
+    return t if t.dim() <= 3 else t.reshape(t.shape[0], math.prod(t.shape[1:-1]), t.shape[-1])
 
 
 def _norm_check(x, groups, weight, bias, activation, gate, others=()):
@@ -252,11 +257,10 @@ def _contig(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
 
 
 def _norm_args(x, groups, weight, bias, eps, activation, gate, y, stats):
-    N, S, Ch = x.shape
-    xn, xs, _ = x.stride()
-    gn, gs, _ = (0, 0, 0) if gate is None else gate.stride()
-    return C.GroupNormArgs(x.data_ptr(), _p(gate), _p(weight), _p(bias), _p(y), _p(stats), N, S, Ch, groups, xn, xs, gn, gs,
-                           eps, _ACTS[activation], None, 0)
+    N, S, Ch = x.shape if x.dim() == 3 else (x.shape[0], 1, x.shape[1])
+    xs, gs = x.stride(), (0, 0) if gate is None else gate.stride()  # ([N, C]: the one row has no stride to speak of)
+    return C.GroupNormArgs(x.data_ptr(), _p(gate), _p(weight), _p(bias), _p(y), _p(stats), N, S, Ch, groups, xs[0], xs[1], gs[0],
+                           gs[1], eps, _ACTS[activation], None, 0)
 
 
 def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-5, activation: str = "silu", gate=None,
@@ -271,19 +275,19 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-5, ac
     which the backward takes.  `out` takes the result where given (it may be x)."""
     _norm_check(x, groups, weight, bias, activation, gate, (("out", out),) if out is not None else ())
     index = _device(x, weight, bias, gate, out)
-    shape, x = x.shape, _dense_rows(_rows3(x))
-    gate = None if gate is None else _dense_rows(_rows3(gate))
+    shape, x = x.shape, _dense_rows(_rows(x))
+    gate = None if gate is None else _dense_rows(_rows(gate))
     weight, bias = _contig(weight), _contig(bias)
-    y = _empty_like(x) if out is None else _rows3(out)
+    y = _empty_like(x) if out is None else _rows(out)
     if out is not None and (y.data_ptr() != out.data_ptr() or y.stride() != x.stride()):
         raise ValueError("out must have x's layout")
-    stats = torch.empty((x.shape[0], groups, 2), dtype=torch.float32, device=x.device) if return_stats else None
+    stats = x.new_empty((x.shape[0], groups, 2), dtype=torch.float32) if return_stats else None
     a = _norm_args(x, groups, weight, bias, eps, activation, gate, y, stats)
     L = C.lib()
     keep = _workspace(a, workspace, L.gdn2_group_norm_act_workspace_bytes(a), x)
     _call(L.gdn2_group_norm_act_f32 if x.dtype is torch.float32 else L.gdn2_group_norm_act_bf16, a, index)
     del keep
-    y = out if out is not None else y.view(shape) if len(shape) != 3 else y
+    y = out if out is not None else y.view(shape) if len(shape) > 3 else y
     return (y, stats) if return_stats else y
 
 
@@ -298,12 +302,12 @@ def group_norm_act_backward(x, groups: int, stats, d_out, weight=None, bias=None
     if stats.shape != (x.shape[0], groups, 2):
         raise ValueError("stats must be [N, groups, 2]")
     index = _device(x, weight, bias, gate, d_out, stats)
-    shape, x = x.shape, _dense_rows(_rows3(x))
-    gate = None if gate is None else _dense_rows(_rows3(gate))
-    d_out = _in_layout(_rows3(d_out), x)
+    shape, x = x.shape, _dense_rows(_rows(x))
+    gate = None if gate is None else _dense_rows(_rows(gate))
+    d_out = _in_layout(_rows(d_out), x)
     weight, bias, stats = _contig(weight), _contig(bias), stats.contiguous()
     dx, dgate = _empty_like(x), None if gate is None else _empty_like(gate)
-    dweight = torch.empty(shape[-1], dtype=torch.float32, device=x.device) if weight is None else torch.empty_like(weight)
+    dweight = x.new_empty(shape[-1], dtype=torch.float32) if weight is None else torch.empty_like(weight)
     dbias = torch.empty_like(dweight)
     a = C.GroupNormBwdArgs(_norm_args(x, groups, weight, bias, 0.0, activation, gate, None, stats), d_out.data_ptr(),
                            dx.data_ptr(), _p(dgate), dweight.data_ptr(), dbias.data_ptr(), None, 0)
@@ -311,6 +315,6 @@ def group_norm_act_backward(x, groups: int, stats, d_out, weight=None, bias=None
     keep = _workspace(a, workspace, L.gdn2_group_norm_act_bwd_workspace_bytes(a), x)
     _call(L.gdn2_group_norm_act_bwd_f32 if x.dtype is torch.float32 else L.gdn2_group_norm_act_bwd_bf16, a, index)
     del keep
-    if len(shape) != 3:
+    if len(shape) > 3:
         dx, dgate = dx.view(shape), None if dgate is None else dgate.view(shape)
     return {"dx": dx, "dgate": dgate, "dweight": dweight, "dbias": dbias}

@@ -300,9 +300,9 @@ def test_layouts_of_results():
     assert mixer._dense_rows(wide) is not wide and mixer._dense_rows(wide).is_contiguous()
     gaps = torch.zeros(5, 2, 3, 8)[..., :4]
     assert mixer._dense_rows(gaps) is gaps and mixer._empty_like(gaps).stride() == gaps.stride()
-    assert mixer._rows3(torch.zeros(0, 3, 5, 8)).shape == (0, 15, 8)
-    assert mixer._rows3(torch.zeros(2, 0, 5, 8)).shape == (2, 0, 8)
-    assert mixer._rows3(torch.zeros(2, 3, 5, 0)).shape == (2, 15, 0)
+    assert mixer._rows(torch.zeros(0, 3, 5, 8)).shape == (0, 15, 8)
+    assert mixer._rows(torch.zeros(2, 0, 5, 8)).shape == (2, 0, 8)
+    assert mixer._rows(torch.zeros(2, 3, 5, 0)).shape == (2, 15, 0)
 
 
 @pytest.mark.parametrize("source", ["gated_scan", "group_norm", "short_conv_bwd"])
