@@ -162,9 +162,9 @@ def gated_scan(g, v, w=None, state=None, cu_seqlens=None, out=None, new_state=No
     g [B, H, T, V], or [B, H, T, 1] for one log decay per head and token; w None
     means 1, state None zeros.  With cu_seqlens (int32 on the device, N + 1 token
     offsets) the one row of the batch holds N sequences, each with its own state;
-    rows of out outside all of them are left as they were.  Otherwise N = B.
-    T = 1 is the serving step.  `out` and `new_state` (which may be `state`) take
-    the results where given."""
+    rows of out outside all of them are left as they were (as allocated, in a new
+    one).  Otherwise N = B.  T = 1 is the serving step.  `out` (no input of the call)
+    and `new_state` (which may be `state`) take the results where given."""
     of_states = _scan_check(g, v, w, state, cu_seqlens, (("out", out),) if out is not None else (),
                             (("new_state", new_state),) if new_state is not None else ())
     index = _device(v, g, w, state, cu_seqlens, out, new_state)

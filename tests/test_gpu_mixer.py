@@ -137,3 +137,73 @@ def test_captured_training_step(gpu):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(out, want[k % 2]))
         step(ins[1 - k % 2])
+
+
+def test_captured_decoding(gpu):
+    """One token through scan and norm in a graph that hands the state on in place,
+    replayed token after token, equals the eager steps."""
+    import torch
+
+    import gdn2_amd as G
+
+    B, H, V, steps = 5, 2, 64, 6
+    C = H * V
+    g, v = -torch.rand(steps, B, H, 1, 1, device=gpu), torch.randn(steps, B, H, 1, V, device=gpu)
+    z, weight = torch.randn(steps, B, C, device=gpu), torch.rand(C, device=gpu)
+    start = torch.randn(B, H, V, device=gpu)
+    cur = {"g": g[0].clone(), "v": v[0].clone(), "z": z[0].clone(), "state": start.clone()}
+
+    def step(i):
+        o, _ = G.gated_scan(i["g"], i["v"], None, i["state"], new_state=i["state"])
+        return G.group_norm_act(o.view(B, C), H, weight, None, EPS, "silu", gate=i["z"])
+
+    step(cur)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = step(cur)
+    cur["state"].copy_(start)
+    eager = {"state": start.clone()}
+    for t in range(steps):
+        for n, x in (("g", g), ("v", v), ("z", z)):
+            cur[n].copy_(x[t])
+            eager[n] = x[t].clone()
+        graph.replay()
+        want = step(eager)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and torch.equal(cur["state"], eager["state"]), t
+
+
+def test_graphs_that_share_a_workspace(gpu):
+    """Two graphs captured with one workspace, replayed in turn, and an eager call
+    with it between them."""
+    import torch
+
+    import gdn2_amd as G
+
+    ws = torch.empty(1 << 24, dtype=torch.uint8, device=gpu)
+    ins = [{"g": -torch.rand(1, 2, T, 64, device=gpu), "v": torch.randn(1, 2, T, 64, device=gpu),
+            "x": torch.randn(1, T, 128, device=gpu), "w": torch.randn(128, 4, device=gpu)} for T in (3000, 1700)]
+
+    def all_of(i, ws):
+        o, s = G.gated_scan(i["g"], i["v"], workspace=ws)
+        r = G.gated_scan_backward(i["g"], i["v"], None, o, o, workspace=ws)
+        y, stats = G.group_norm_act(i["x"], 4, return_stats=True, workspace=ws)
+        n = G.group_norm_act_backward(i["x"], 4, stats, y, workspace=ws)
+        c = G.short_conv_1d_backward(i["x"], i["w"], y, workspace=ws)
+        return [o, s, r["dg"], r["dv"], r["dS0"], y, n["dx"], n["dweight"], n["dbias"], c["dx"], c["dweight"]]
+
+    want = [all_of(i, None) for i in ins]
+    graphs, got = [], []
+    for i in ins:
+        all_of(i, ws)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            got.append(all_of(i, ws))
+    for k in (0, 1, 1, 0, 1, 0):
+        for t in got[k]:
+            t.zero_()
+        graphs[k].replay()
+        eager = all_of(ins[1 - k], ws)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got[k], want[k])), k
+        assert all(torch.equal(a, b) for a, b in zip(eager, want[1 - k])), k
