@@ -70,11 +70,12 @@ struct GatedScanParams {
     unsigned long long *agg; // [chain][tile][CH] (G, X)
 };
 
-// A token's decay in a register.  Sign bit set: expm1(g), for -1/8 < g <= -0, by
-// four terms of its series (the rest is below 2^-24 of it).  Clear: e^g.
+// A token's decay in a register.  Sign bit set: expm1(g), for -1/8 < g < 0, by
+// four terms of its series (the rest is below 2^-24 of it).  Clear: e^g (of -0,
+// too: its series ends in a zero whose sign says e^g).
 __device__ __forceinline__ float decay(float g) {
     const float p = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(g, 1.f / 120, 1.f / 24), g, 1.f / 6), g, 0.5f);
-    return __builtin_bit_cast(unsigned, g) - 0x80000000u < 0x3E000000u ? __builtin_fmaf(p * g, g, g) : fast_exp2(g * kLog2e);
+    return __builtin_bit_cast(unsigned, g) - 0x80000001u < 0x3DFFFFFFu ? __builtin_fmaf(p * g, g, g) : fast_exp2(g * kLog2e);
 }
 // e^g s + u for finite s
 __device__ __forceinline__ float advance(float c, float s, float u) {

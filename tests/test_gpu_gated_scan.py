@@ -290,6 +290,31 @@ def test_special_values(gpu):
     assert np.abs(_np(out)[0, 0, :, 0] / want - 1).max() < 1e-4
 
 
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [3, 40, 700])
+def test_decays_at_the_borders(gpu, T, ty):
+    """Log decays of either zero, the smallest numbers, and both sides of where the
+    decay's form changes, among ordinary ones; values and gradients."""
+    import torch
+
+    import gdn2_amd as G
+
+    edge = torch.tensor([-0.0, 0.0, -1e-45, -1e-38, -2e-30, -1e-9, -0.125, -0.12499999, -0.12500001, -1e-3], device=gpu)
+    for per_head, V in ((False, 64), (True, 64), (False, 5), (True, 36)):
+        d = _make(gpu, 31 + T, 2, T, 3, V, ty, per_head, True, True)
+        g = d["g"].clone()
+        pick = torch.randint(0, 2 * len(edge), g.shape, device=gpu)
+        d["g"] = torch.where(pick < len(edge), edge[pick.clamp(max=len(edge) - 1)], g)
+        out, new = G.gated_scan(**d)
+        assert _check_forward(d, out, new, 2, ty).all()
+        d_out, d_state = torch.randn_like(out), torch.randn_like(new)
+        r = G.gated_scan_backward(d["g"], d["v"], d["w"], out, d_out, d["state"], d_state=d_state)
+        _check_backward(d, out, d_out, d_state, r, 2, ty)
+        keep = {n: t for n, t in d.items() if n != "g"}
+        zeros = G.gated_scan(torch.zeros_like(d["g"]), **keep), G.gated_scan(-torch.zeros_like(d["g"]), **keep)
+        assert all(torch.equal(a, b) for a, b in zip(*zeros))
+
+
 def test_slow_decay_keeps_its_digits(gpu):
     """A constant log decay of -2^-13 over 30000 tokens.  The state's own rounding
     is half a step of it a token, which decays too: after many tokens at most
