@@ -32,7 +32,7 @@ extern "C" {
  *       factor at every token that the state lives through): [B, H, T, V], or
  *       [B, H, T] with g_per_head (one value per head and token).  Ordinary
  *       values are <= 0; where e^g is 0 in f32 (-inf, too) the state is
- *       forgotten, whatever it held.
+ *       forgotten, whatever it held.  (An e^g below 2^-126 may count as 0.)
  * v, w  [B, H, T, V]; w NULL means 1
  * out   [B, H, T, V], not overlapping the inputs
  * state_in [N, H, V] contiguous, or NULL (zeros); state_out likewise, or NULL
