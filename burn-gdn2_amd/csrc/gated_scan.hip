@@ -142,6 +142,10 @@ template <> struct FormOf<float, true, false> : Form<4, 32, 4, 8> {};
 template <> struct FormOf<float, true, true> : Form<4, 32, 4, 8> {};
 template <> struct FormOf<bf16, true, false> : Form<8, 16, 2, 8> {};
 template <> struct FormOf<bf16, true, true> : Form<8, 16, 4, 8> {};
+// The same for few chains: of fewer channels, so that a look reaches over four
+// times the tokens (see plan_of).
+template <typename T, bool BWD, bool HEAD> struct NarrowOf : Form<4, 8, 4, 8> {};
+template <bool BWD, bool HEAD> struct NarrowOf<bf16, BWD, HEAD> : Form<8, 4, BWD && !HEAD ? 2 : 4, 8> {};
 // Rows that are no multiple of 16 bytes, or not aligned to them.
 typedef Form<4, 16, 4, 8> HalfForm;
 typedef Form<1, 32, 8, 4> OddForm;
@@ -608,20 +612,22 @@ size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 // B = 1: 5.4 and 7.5 us at T = 8, 7.1 and 7.6 at 12, 8.7 and 7.6 at 16;
 // B = 64: 6 and 27 us at T = 8, 25 and 31 at 32, 36 and 34 at 48.
 constexpr int kWalk = 12, kWalkMany = 32;
+constexpr int kFewChains = 4;   // see plan_of
 constexpr int kResident = 1024; // workgroups, four a compute unit
 constexpr int kMostTokens = 64, kMostChannels = 128; // of a wave, of a tile
 
 struct Plan {
     int vec;
-    bool walk;
+    bool walk, narrow;
     int ch, tt;
     int unit, units;
     int64_t tiles_c, tiles_t, chains;
     size_t o_pre, o_agg, words, o_info, o_dgp, bytes; // workspace: the ticket, pre, agg; the tokens' sequences; dg sums
 };
 
-// f(form) for the form that `vec` values a lane stand for
-template <typename T, bool BWD, bool HEAD, typename Fn> auto with_form(int vec, Fn f) {
+// f(form) for the form that `vec` values a lane, and a plan's `narrow`, stand for
+template <typename T, bool BWD, bool HEAD, typename Fn> auto with_form(int vec, bool narrow, Fn f) {
+    if (vec == FormOf<T, BWD, HEAD>::VEC && narrow) return f(NarrowOf<T, BWD, HEAD>());
     if (vec == FormOf<T, BWD, HEAD>::VEC) return f(FormOf<T, BWD, HEAD>());
     if constexpr (FormOf<T, BWD, HEAD>::VEC == 8)
         if (vec == 4) return f(HalfForm());
@@ -633,19 +639,28 @@ template <typename T, bool BWD> Plan plan_of(const gdn2_gated_scan_args &a, int 
     Plan q{};
     q.vec = vec;
     const int64_t len = a.seq_len, HV = a.num_heads * a.head_v_dim;
-    auto size = [&](auto form) {
-        static_assert(form.TL * form.R <= kMostTokens && form.CH <= kMostChannels, "near_rows");
-        q.ch = form.CH;
-        q.tt = form.TT;
-    };
-    if (a.g_per_head) with_form<T, BWD, true>(vec, size);
-    else with_form<T, BWD, false>(vec, size);
     const bool heads = bwd && a.g_per_head;
     q.unit = (int)(heads ? a.head_v_dim : HV);
     q.units = (int)(heads ? a.num_heads : 1);
-    q.tiles_c = (q.unit + q.ch - 1) / q.ch;
-    q.tiles_t = (len + q.tt - 1) / q.tt;
-    q.chains = a.batch * q.units * q.tiles_c;
+    auto size = [&](bool narrow) {
+        auto set = [&](auto form) {
+            static_assert(form.TL * form.R <= kMostTokens && form.CH <= kMostChannels, "near_rows");
+            q.ch = form.CH;
+            q.tt = form.TT;
+        };
+        if (a.g_per_head) with_form<T, BWD, true>(vec, narrow, set);
+        else with_form<T, BWD, false>(vec, narrow, set);
+        q.tiles_c = (q.unit + q.ch - 1) / q.ch;
+        q.tiles_t = (len + q.tt - 1) / q.tt;
+        q.chains = a.batch * q.units * q.tiles_c;
+    };
+    size(false);
+    // Up to four chains of more than one look are bound by what passes along them.
+    // 32 channels a tile against 128: one row of 32318 x 128 bf16 30 and 57 us, 39921
+    // x 200 f32 58 and 101, 8192 x 512 25 and 31 (adjoint 30 and 36); but 65536 x 2048
+    // bf16 312 and 218, and equal at 8192 x 1024.
+    q.narrow = q.chains <= kFewChains && q.tiles_t > 8;
+    if (q.narrow) size(true);
     q.walk = !bwd && !a.cu_seqlens && len <= (q.chains > kResident ? kWalkMany : kWalk);
     if (q.walk) return q;
     size_t at = 0;
@@ -750,7 +765,7 @@ template <typename T, bool BWD, bool HEAD, bool HASW>
 hipError_t launch_tiles(const Plan &q, const GatedScanParams &p, hipStream_t s) {
     // as many workgroups as run at once
     const dim3 grid((unsigned)std::min<int64_t>(q.chains * q.tiles_t, kResident));
-    with_form<T, BWD, HEAD>(q.vec, [&](auto form) {
+    with_form<T, BWD, HEAD>(q.vec, q.narrow, [&](auto form) {
         hipLaunchKernelGGL((gated_scan_kernel<T, decltype(form), BWD, HEAD, HASW>), grid, dim3(64 * form.NW), 0, s, p);
     });
     return hipGetLastError();

@@ -61,7 +61,7 @@ def _check_forward(d, out, new, N, ty, bounds=None):
 CASES = [  # B, T, H, V
     (1, 1, 1, 1), (3, 1, 2, 128), (2, 7, 3, 5), (2, 8, 2, 4), (1, 9, 2, 64), (2, 31, 1, 33), (1, 64, 2, 36),
     (2, 65, 3, 12), (1, 127, 1, 100), (1, 128, 2, 32), (1, 129, 4, 96), (2, 256, 1, 128), (1, 257, 2, 40),
-    (1, 1000, 1, 7), (2, 1025, 2, 36), (1, 2500, 1, 64), (5, 300, 2, 1),
+    (1, 1000, 1, 7), (2, 1025, 2, 36), (1, 2500, 1, 64), (5, 300, 2, 1), (1, 3000, 3, 128), (2, 2400, 1, 96), (1, 4500, 1, 40),
 ]
 
 
