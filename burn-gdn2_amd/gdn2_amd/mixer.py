@@ -9,6 +9,8 @@ Tensors as in ops.py, of any strides with contiguous channels, in float32 or
 bfloat16; log decays, states, weights and their gradients are
 float32.  A call runs on its tensors' device, on torch's current stream there;
 workspaces come from torch's allocator, so a call may be captured into a graph.
+No autograd graph is recorded: a torch.autograd.Function calls the backward with
+what it kept of the forward.
 """
 from __future__ import annotations
 
