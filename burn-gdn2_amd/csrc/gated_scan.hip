@@ -209,7 +209,8 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
             plain = plain && w0 > 0 && w0 + TL * R < p.T;
         }
         q.plain = __builtin_amdgcn_readfirstlane((int)plain);
-        q.have = q.first = q.last = 0;
+        q.have = q.plain ? ~0u : 0u;
+        q.first = q.last = 0;
         if (!q.plain && q.ok) {
 #pragma unroll 1
             for (int i = 0; i < R; ++i) {
