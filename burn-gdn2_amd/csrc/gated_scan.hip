@@ -487,11 +487,23 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
         float eg[GV];
 #pragma unroll
         for (int j = 0; j < GV; ++j) eg[j] = growth(Gw[j]);
-        finite = q.plain;
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            s[j] = join(eg[HEAD ? 0 : j], Xw[j], enter[wave][cl * VEC + j]);
-            finite = finite && __builtin_isfinite(s[j]);
+        for (int j = 0; j < VEC; ++j) s[j] = join(eg[HEAD ? 0 : j], Xw[j], enter[wave][cl * VEC + j]);
+        // Whether the run stays finite from there: its recurrence ahead of the results, of
+        // which no step makes a value finite again that is not (c inf + inf with c < 0
+        // and 0 inf are NaN).
+        finite = q.plain;
+        if (q.plain) {
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                float t = s[j];
+#pragma unroll
+                for (int i = 0; i < R; ++i) {
+                    const float e = em[i][HEAD ? 0 : j];
+                    t = BWD ? advance(e, u[i][j] + t, 0.f) : advance(e, t, u[i][j]);
+                }
+                finite = finite && __builtin_isfinite(t);
+            }
         }
 
         // The results.  Each token's go out as soon as they are known.

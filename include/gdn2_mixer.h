@@ -33,6 +33,8 @@ extern "C" {
  *       [B, H, T] with g_per_head (one value per head and token).  Ordinary
  *       values are <= 0; where e^g is 0 in f32 (-inf, too) the state is
  *       forgotten, whatever it held.  (An e^g below 2^-126 may count as 0.)
+ *       A state that leaves f32's range is infinite; the ones after it are
+ *       infinite or what the recurrence gives in a wider range.
  * v, w  [B, H, T, V]; w NULL means 1
  * out   [B, H, T, V], not overlapping the inputs
  * state_in [N, H, V] contiguous, or NULL (zeros); state_out likewise, or NULL

@@ -194,3 +194,76 @@ def test_states_that_are_not_finite(gpu, T, H, V, bounds, ty, per_head, w):
                            x["state"].double().cpu().numpy(), bounds)
     same("dv", _flat(r["dv"]), want["dv"], err["dv"], M.HALF[ty])
     same("dS0", r["dS0"].double().cpu().numpy(), want["dS0"], None, 0)
+
+
+@pytest.mark.parametrize("ty,per_head,w", KINDS)
+@pytest.mark.parametrize("T,H,V,bounds", FORMS)
+def test_values_that_are_not_finite(gpu, T, H, V, bounds, ty, per_head, w):
+    """An infinity or a NaN at another token in every channel, so at every place of a
+    wave's tokens, and a log decay of -inf some tokens later (in the adjoint: before):
+    they reach every token up to there, and none beyond."""
+    for bad, after in itertools.product((float("inf"), float("-inf"), float("nan")), (1, 2, 3, 9, None)):
+        print("values", T, H, V, bounds, ty, per_head, w, bad, after, flush=True)
+        d, N = _operands(gpu, T, H, V, ty, per_head, w, bounds)
+        dy = _gradient(T, H, V)
+        for c in range(V):
+            t = (T // 3 + c) % T
+            d["v"][0, t, :, c] = bad
+            dy[0, t, :, c] = bad
+            if after and not per_head:
+                d["g"][0, (t + after) % T, :, c] = float("-inf")
+                d["g"][0, (t - after) % T, :, c] = float("-inf")
+        if after and per_head:
+            d["g"][0, after::11] = float("-inf")
+        _check(gpu, d, N, ty, bounds, dy)
+
+
+def _overflowing(name, got, wide, step, err, half):
+    """States that leave f32.  wide: the recurrence in 64 bits, whose range holds all of
+    them; step: token by token, infinite from the first that f32 does not hold.  Both
+    are right where they differ: e^G h + X over a run of tokens can be finite again
+    where a state inside the run is not.  So: infinite where `wide` is out of range,
+    else either of the two, and never a NaN."""
+    either = np.isinf(step) & (got == step)
+    same(name, np.where(either, step, got), np.where(either, step, _f32(wide)), err, half)
+
+
+@pytest.mark.parametrize("ty,per_head,w", KINDS)
+def test_states_that_overflow(gpu, ty, per_head, w):
+    """States that leave f32 at some token, another one in every channel, and with them
+    the gradients: infinite, of that sign, and no NaN behind them."""
+    import torch
+
+    import gdn2_amd as G
+
+    T, H, V = 300, 1, 128
+    for reset in (False, True):
+        d, N = _operands(gpu, T, H, V, ty, per_head, w, None)
+        dy = _gradient(T, H, V)
+        big = 1.5 * 2.0 ** 127  # two of them, hardly decayed between, overflow
+        for c in range(V):
+            sign = 1 - 2 * (c % 2)
+            for i in (0, 1):
+                d["v"][0, 70 + c + i, :, c] = sign * big
+                dy[0, 70 + c + i, :, c] = sign * big
+        d["g"][:, 60:210] = -0.01
+        if w:
+            d["w"][...] = 1.0
+        if reset:
+            d["g"][0, 3::17] = float("-inf")
+        x = _on(gpu, d, ty)
+        out, new = G.gated_scan(x["g"], x["v"], x["w"], x["state"])
+        ones = torch.ones_like(x["v"])
+        r = G.gated_scan_backward(x["g"], ones, None, ones, dy.to(gpu, _type(ty)).transpose(1, 2), x["state"])
+        torch.cuda.synchronize()
+        g = np.broadcast_to(_flat(x["g"]), (1, T, H, V))
+        h0, v = x["state"].double().cpu().numpy(), _flat(x["v"])
+        step, _, err = forward64(g, v, h0)
+        with np.errstate(invalid="ignore"):
+            wide = M.scan64(g, v, h0)[0]
+        _overflowing("out", _flat(out), wide, step, err, M.HALF[ty])
+        one, zeros, dy = np.ones((1, T, H, V)), np.zeros((1, H, V)), _flat(dy.to(_type(ty)).transpose(1, 2))
+        step, err = backward64(g, one, one, one, dy, h0, zeros)
+        with np.errstate(invalid="ignore"):
+            wide = M.scan_bwd64(g, one, one, one, dy, h0, zeros)[0]
+        _overflowing("dv", _flat(r["dv"]), wide["dv"], step["dv"], err["dv"], M.HALF[ty])
