@@ -77,6 +77,9 @@ __device__ __forceinline__ float decay(float g) {
     const float p = __builtin_fmaf(__builtin_fmaf(__builtin_fmaf(g, 1.f / 120, 1.f / 24), g, 1.f / 6), g, 0.5f);
     return __builtin_bit_cast(unsigned, g) - 0x80000001u < 0x3DFFFFFFu ? __builtin_fmaf(p * g, g, g) : fast_exp2(g * kLog2e);
 }
+// Whether e^g is zero: nothing passes that token, and of its run, whatever decays lie
+// before it, NaN too, G is -inf.
+__device__ __forceinline__ bool forgets(float c) { return __builtin_bit_cast(int, c) == 0; }
 // e^g s + u for finite s
 __device__ __forceinline__ float advance(float c, float s, float u) {
     const int mask = __builtin_bit_cast(int, c) >> 31;
@@ -87,7 +90,7 @@ __device__ __forceinline__ float advance(float c, float s, float u) {
 __device__ __forceinline__ float advance_any(float c, float s, float u) {
     const int bits = __builtin_bit_cast(int, c);
     const float t = __builtin_fmaf(c, s, u);
-    return bits == 0 ? u : bits < 0 ? s + (__builtin_isinf(s) ? u : t) : t;
+    return forgets(c) ? u : bits < 0 ? s + (__builtin_isinf(s) ? u : t) : t;
 }
 
 // A run's G is kept as G log2(e) / 2, so that e^G h can be formed in two steps
@@ -302,7 +305,7 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
 #pragma unroll
                 for (int j = 0; j < GV; ++j) {
                     em[i][j] = decay(rg[i][j]);
-                    G[j] = __builtin_fmaf(rg[i][j], kHalf, G[j]);
+                    G[j] = forgets(em[i][j]) ? -INFINITY : __builtin_fmaf(rg[i][j], kHalf, G[j]);
                 }
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
@@ -318,7 +321,7 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
                 for (int j = 0; j < GV; ++j) {
                     const float gj = in ? rg[i][j] : 0.f;
                     em[i][j] = decay(gj);
-                    G[j] = ct_i ? -INFINITY : __builtin_fmaf(gj, kHalf, G[j]);
+                    G[j] = ct_i || forgets(em[i][j]) ? -INFINITY : __builtin_fmaf(gj, kHalf, G[j]);
                 }
                 float s0[VEC]; // forward: the state before a sequence; backward: the gradient of the one after it
 #pragma unroll

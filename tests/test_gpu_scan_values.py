@@ -267,3 +267,63 @@ def test_states_that_overflow(gpu, ty, per_head, w):
         with np.errstate(invalid="ignore"):
             wide = M.scan_bwd64(g, one, one, one, dy, h0, zeros)[0]
         _overflowing("dv", _flat(r["dv"]), wide["dv"], step["dv"], err["dv"], M.HALF[ty])
+
+
+@pytest.mark.parametrize("ty,per_head,w", KINDS)
+@pytest.mark.parametrize("T,H,V,bounds", FORMS)
+def test_zero_decays_of_finite_logs(gpu, T, H, V, bounds, ty, per_head, w):
+    """A log decay whose e^g is zero in f32 forgets a state that is not finite as -inf
+    does, wherever the borders of runs, waves and tiles fall; so does one behind a log
+    decay that is NaN itself."""
+    import torch
+
+    for reset, bad in itertools.product((-110.0, -130.0, -170.0, -1e30, float("-inf")), ("state", "nan decay")):
+        print("zero decays", T, H, V, bounds, ty, per_head, w, reset, bad, flush=True)
+        d, N = _operands(gpu, T, H, V, ty, per_head, w, bounds)
+        d["state"][:, :, 1::2] = float("inf")
+        d["state"][:, :, 2::4] = float("nan")
+        for c in range(1 if per_head else V):
+            d["g"][0, (7 + 5 * c) % T::29, :, c] = reset
+            if bad == "nan decay" and c % 2 == 0:
+                d["g"][0, (6 + 5 * c) % T::29, :, c] = float("nan")
+        _check(gpu, d, N, ty, bounds)
+        # the adjoint: the last state's gradient comes from behind
+        import gdn2_amd as G
+
+        x = _on(gpu, d, ty)
+        cu = None if bounds is None else torch.tensor(bounds, dtype=torch.int32, device=gpu)
+        ones, dy = torch.ones_like(x["v"]), torch.ones_like(x["v"])
+        r = G.gated_scan_backward(x["g"], ones, None, ones, dy, None, d_state=x["state"], cu_seqlens=cu)
+        torch.cuda.synchronize()
+        one = np.ones((1, T, H, V))
+        want, err = backward64(np.broadcast_to(_flat(x["g"]), one.shape), one, one, one, one, np.zeros((N, H, V)),
+                               x["state"].double().cpu().numpy(), bounds)
+        same("dv", _flat(r["dv"]), want["dv"], err["dv"], M.HALF[ty])
+        same("dS0", r["dS0"].double().cpu().numpy(), want["dS0"], None, 0)
+
+
+@pytest.mark.parametrize("ty,per_head,w", KINDS)
+def test_the_smallest_decays_count_the_same_in_tiles_and_steps(gpu, ty, per_head, w):
+    """e^g between 2^-150 and 2^-126 may count as zero: then in every form of the call.
+    A prompt in tiles and its tokens one by one are infinite and NaN at the same places."""
+    import torch
+
+    import gdn2_amd as G
+
+    T, V = 200, 128
+    for reset in (-87.2, -87.5, -95.0, -100.0, -103.0):
+        d, N = _operands(gpu, T, 1, V, ty, per_head, w, None)
+        d["state"][:, :, 1::2] = float("inf")
+        d["state"][:, :, 2::4] = float("nan")
+        for c in range(1 if per_head else V):
+            d["g"][0, 20 + c, :, c] = reset
+        x = _on(gpu, d, ty)
+        out, new = G.gated_scan(**x)
+        state, steps = x["state"], []
+        for t in range(T):
+            o, state = G.gated_scan(*(None if x[n] is None else x[n][:, :, t:t + 1] for n in "gvw"), state)
+            steps.append(o)
+        steps = torch.cat(steps, 2)
+        torch.cuda.synchronize()
+        for a, b in ((out, steps), (new, state)):
+            assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.isinf(a), torch.isinf(b)), reset
