@@ -96,8 +96,12 @@ __device__ __forceinline__ float advance_any(float c, float s, float u) {
 // A run's G is kept as G log2(e) / 2, so that e^G h can be formed in two steps
 // where e^G alone overflows.
 constexpr float kHalf = 0.5f * kLog2e;
-// e^G h + X of a joined run, e = growth(G).  Nothing of h passes e = 0.
-__device__ __forceinline__ float growth(float G) { return fast_exp2(fminf(G, 127.f)); }
+// e^G h + X of a joined run, e = growth(G).  Nothing of h passes e = 0, which is that
+// of G = -inf alone: an infinite or NaN h passes any product of decays, as it passes
+// each.  (Of a finite one 2^-252 may be left where it should be less, below 2^-124.)
+__device__ __forceinline__ float growth(float G) {
+    return G == -INFINITY ? 0.f : fast_exp2(__builtin_amdgcn_fmed3f(G, -126.f, 127.f));
+}
 __device__ __forceinline__ float join(float e, float X, float h) { return e == 0.f ? X : __builtin_fmaf(e * h, e, X); }
 
 // A published word is never all ones.

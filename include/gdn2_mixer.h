@@ -32,7 +32,8 @@ extern "C" {
  *       factor at every token that the state lives through): [B, H, T, V], or
  *       [B, H, T] with g_per_head (one value per head and token).  Ordinary
  *       values are <= 0; where e^g is 0 in f32 (-inf, too) the state is
- *       forgotten, whatever it held.  (An e^g below 2^-126 may count as 0.)
+ *       forgotten, whatever it held; an infinity or a NaN lasts until then.  (An e^g
+ *       below 2^-126 may count as 0.)
  *       A state that leaves f32's range is infinite; the ones after it are
  *       infinite or what the recurrence gives in a wider range.
  * v, w  [B, H, T, V]; w NULL means 1

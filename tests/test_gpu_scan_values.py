@@ -39,6 +39,16 @@ def _gone(a):
     return a < 2.0 ** -150
 
 
+# What a log decay's own rounding costs the state that it is of, in half steps of |g|
+# of it (M.scan64 counts it against the state and what is added, of ordinary decays; a
+# state that nothing is added to keeps all of it).  e^g is 2^(g log2 e) with a rounded
+# product and constant: 1.3.  Of a run it is 2^G, G a sum of its tokens' in f32, whose
+# every partial sum is off by half a step of itself, and so of |g| of each token in it:
+# 8 tokens a thread, 2 to 4 steps over lanes and 8 waves, of which no form has more
+# than 18.
+SUMS = 20
+
+
 def forward64(g, u, h0, bounds=None):
     """h_t = e^{g_t} h_{t-1} + u_t, nothing of h passing an e^g that is zero in f32 and
     what leaves f32 infinite; the final states; the bound of f32 arithmetic (the
@@ -52,8 +62,9 @@ def forward64(g, u, h0, bounds=None):
                 a = np.exp(g[row, t])
                 gone, ut = _gone(a), u[row, t]
                 x = _f32(np.where(gone, 0, a * x) + ut)
+                e = np.where(gone, 0, a * e + SUMS * M.EPS * np.abs(g[row, t]) * a * xa)
                 xa = np.where(gone, 0, a * xa) + np.abs(ut)
-                e = np.where(gone, 0, a * e) + 8 * M.EPS * xa
+                e = e + 8 * M.EPS * xa
                 h[row, t], err[row, t] = x, e
             last[n] = x
     return h, last, err
@@ -78,7 +89,7 @@ def backward64(g, v, w, h, dy, h0, ds, bounds=None):
                 err["dv"][row, t] = np.abs(w[row, t]) * (de + 2 * M.EPS * Da)
                 err["dw"][row, t] = np.abs(v[row, t]) * (de + 2 * M.EPS * Da)
                 E, Ea = np.where(gone, 0, a * D), np.where(gone, 0, a * Da)
-                e = np.where(gone, 0, a * de) + 8 * M.EPS * Ea
+                e = np.where(gone, 0, a * de) + (8 + SUMS * np.where(gone, 0, np.abs(g[row, t]))) * M.EPS * Ea
                 before = h0[n] if t == t0 else h[row, t - 1]
                 out["dg"][row, t] = np.where(gone, 0, E * before)
                 err["dg"][row, t] = np.where(gone, 0, np.abs(before) * (e + M.EPS * Ea))
@@ -327,3 +338,32 @@ def test_the_smallest_decays_count_the_same_in_tiles_and_steps(gpu, ty, per_head
         torch.cuda.synchronize()
         for a, b in ((out, steps), (new, state)):
             assert torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(torch.isinf(a), torch.isinf(b)), reset
+
+
+@pytest.mark.parametrize("ty,per_head,w", KINDS)
+@pytest.mark.parametrize("T,H,V,bounds", FORMS)
+def test_long_decays_keep_what_is_not_finite(gpu, T, H, V, bounds, ty, per_head, w):
+    """An infinite state stays infinite and a NaN one NaN through any number of decays
+    that are not zero, also where their product is below f32's range; a finite one
+    of any size leaves nothing there."""
+    import torch
+
+    import gdn2_amd as G
+
+    for pace in (2.0, 60.0):
+        d, N = _operands(gpu, T, H, V, ty, per_head, w, bounds)
+        d["g"] *= pace / 0.1
+        d["g"].clamp_(min=-85.0)
+        d["state"][:, :, 1::4], d["state"][:, :, 2::4], d["state"][:, :, 3::8] = float("inf"), float("nan"), float("-inf")
+        d["state"][:, :, 7::8] = 3e38
+        _check(gpu, d, N, ty, bounds)
+        x = _on(gpu, d, ty)
+        cu = None if bounds is None else torch.tensor(bounds, dtype=torch.int32, device=gpu)
+        ones, dy = torch.ones_like(x["v"]), torch.ones_like(x["v"])
+        r = G.gated_scan_backward(x["g"], ones, None, ones, dy, None, d_state=x["state"], cu_seqlens=cu)
+        torch.cuda.synchronize()
+        one = np.ones((1, T, H, V))
+        want, err = backward64(np.broadcast_to(_flat(x["g"]), one.shape), one, one, one, one, np.zeros((N, H, V)),
+                               x["state"].double().cpu().numpy(), bounds)
+        same("dv", _flat(r["dv"]), want["dv"], err["dv"], M.HALF[ty])
+        same("dS0", r["dS0"].double().cpu().numpy(), want["dS0"], None, 0)
