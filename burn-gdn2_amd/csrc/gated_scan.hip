@@ -538,7 +538,8 @@ __global__ __launch_bounds__(64 * F::NW) void gated_scan_kernel(GatedScanParams 
                     for (int j = 0; j < VEC; ++j) {
                         const float e = em[i][HEAD ? 0 : j], d = fresh ? u[i][j] : u[i][j] + s[j];
                         s[j] = QUICK ? advance(e, d, 0.f) : advance_any(e, d, 0.f);
-                        xg[j] = in ? s[j] * hb[j] : 0.f; // (rows outside every sequence have no part in L)
+                        // (rows outside every sequence have no part in L, nor has a state that is forgotten)
+                        xg[j] = in && !forgets(e) ? s[j] * hb[j] : 0.f;
                         xv[j] = in ? (HASW ? (float)kw[HASW ? i : 0][j] * d : d) : 0.f;
                         if constexpr (HASW) xw[j] = in ? (float)kv[i][j] * d : 0.f;
                     }

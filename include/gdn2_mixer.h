@@ -77,6 +77,7 @@ GDN2_API gdn2_status gdn2_gated_scan_fwd_bf16(const gdn2_gated_scan_args *args, 
 /* The gradients of L = <d_out, out> + <d_state_out, state_out> of that call:
  *   D_t = d_out_t + e^{g_{t+1}} D_{t+1}  (last token of a sequence: + d_state_out)
  *   dv = w D,  dw = v D,  dg_t = e^{g_t} D_t h_{t-1},  d_state0 = e^{g_0} D_0
+ * (where e^{g_t} is 0, nothing of D passes it, and dg_t is 0 for any h_{t-1})
  *   fwd          the forward's arguments: g, v, w, state_in, cu_seqlens, shapes
  *                and strides; out as the forward wrote it (read: h_{t-1});
  *                state_out and workspace unused.  v is read only with w.

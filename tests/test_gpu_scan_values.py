@@ -367,3 +367,43 @@ def test_long_decays_keep_what_is_not_finite(gpu, T, H, V, bounds, ty, per_head,
                                x["state"].double().cpu().numpy(), bounds)
         same("dv", _flat(r["dv"]), want["dv"], err["dv"], M.HALF[ty])
         same("dS0", r["dS0"].double().cpu().numpy(), want["dS0"], None, 0)
+
+
+@pytest.mark.parametrize("ty,per_head,w", KINDS)
+@pytest.mark.parametrize("T,H,V,bounds", FORMS)
+def test_gradient_of_a_zero_decay_is_zero(gpu, T, H, V, bounds, ty, per_head, w):
+    """Padding that holds NaN or infinities, shut off by a log decay of -inf behind it:
+    out does not depend on that decay, and its gradient is zero (the gradients behind
+    it, and those of the tokens before the padding, are those of a clean call)."""
+    import torch
+
+    import gdn2_amd as G
+
+    for bad, reset in itertools.product((float("nan"), float("inf")), (float("-inf"), -150.0)):
+        d, N = _operands(gpu, T, H, V, ty, per_head, w, bounds)
+        dy = _gradient(T, H, V)
+        pads = [(a, a + 5) for a in range(9, T - 8, 14)]
+        inside = np.zeros(T, bool)
+        for a, b in pads:
+            d["v"][0, a:b] = bad
+            d["g"][0, a], d["g"][0, b] = -0.3, reset
+            dy[0, a:b] = 0
+            inside[a:b] = True
+        x = _on(gpu, d, ty)
+        cu = None if bounds is None else torch.tensor(bounds, dtype=torch.int32, device=gpu)
+        out, _ = G.gated_scan(x["g"], x["v"], x["w"], x["state"], cu_seqlens=cu)
+        r = G.gated_scan_backward(x["g"], x["v"], x["w"], out, dy.to(gpu, _type(ty)).transpose(1, 2), x["state"], cu_seqlens=cu)
+        torch.cuda.synchronize()
+        v, w_ = _flat(x["v"]), _flat(x["w"]) if x["w"] is not None else np.ones(d["v"].shape)
+        g = np.broadcast_to(_flat(x["g"]), v.shape)
+        want, err = backward64(g, v, w_, _flat(out), _flat(dy.to(_type(ty)).transpose(1, 2)),
+                               x["state"].double().cpu().numpy(), np.zeros((N, H, V)), bounds)
+        if per_head:
+            with np.errstate(invalid="ignore"):
+                err["dg"] = (err["dg"] + V * M.EPS * np.abs(want["dg"])).sum(3, keepdims=True)
+                want["dg"] = want["dg"].sum(3, keepdims=True)
+        dg = _flat(r["dg"])
+        assert all((dg[0, b] == 0).all() for _, b in pads)
+        for n in ("dg", "dv", "dw"):
+            if r[n] is not None:
+                same(n, _flat(r[n])[:, ~inside], want[n][:, ~inside], err[n][:, ~inside], M.HALF[ty] if n != "dg" else 0)
