@@ -375,40 +375,52 @@ __device__ __forceinline__ void tile_pairs(const GroupNormParams &p, const TileA
 }
 
 // First pass, forward: the mean and the sum of squares about it of every channel
-// over the chunk's rows.  A thread sums about its first row's value, so that a
-// large mean costs no digits.
+// over the chunk's rows.  A thread takes kBatch rows at a time: their sum s and their
+// squares q about their own mean in 32 bits, the batches' sum q, sum s and sum s^2 / n
+// in 64, so that neither a large mean, nor a value far from the others, nor many rows
+// cost digits.
+constexpr int kBatch = 8;
 template <typename T, int VEC> __global__ __launch_bounds__(256) void norm_moments_kernel(GroupNormParams p) {
     const TileAt<VEC> at(p);
-    float first[VEC], sum[VEC], sq[VEC];
+    double sum[VEC], sq[VEC], among[VEC]; // sum s, sum q, sum s^2 / n
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) first[j] = sum[j] = sq[j] = 0.f;
+    for (int j = 0; j < VEC; ++j) sum[j] = sq[j] = among[j] = 0.;
     const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c;
-    int count = 0;
-    if (at.s0 + at.rl < at.s1) {
-        load_n<T, VEC>(x + (at.s0 + at.rl) * p.sxs, first);
-        count = 1;
-#pragma unroll 8
-        for (int64_t s = at.s0 + at.rl + at.rows; s < at.s1; s += at.rows) {
-            float v[VEC];
-            load_n<T, VEC>(x + s * p.sxs, v);
-            ++count;
+    int64_t row = at.s0 + at.rl, count = 0;
+    auto batch = [&](auto rows) {
+        constexpr int B = decltype(rows)::value;
+        Raw<T, VEC> v[B];
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) {
-                v[j] -= first[j];
-                sum[j] += v[j];
-                sq[j] = __builtin_fmaf(v[j], v[j], sq[j]);
+        for (int i = 0; i < B; ++i) v[i] = raw_n<T, VEC>(x + (row + i * at.rows) * p.sxs);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            float s = 0.f, q = 0.f;
+#pragma unroll
+            for (int i = 0; i < B; ++i) s += (float)v[i][j];
+#pragma unroll
+            for (int i = 0; i < B; ++i) {
+                const float d = __builtin_fmaf(-s, 1.f / B, (float)v[i][j]);
+                q = __builtin_fmaf(d, d, q);
             }
+            sum[j] += s;
+            sq[j] += q;
+            among[j] = __builtin_fma((double)s, (double)s * (1. / B), among[j]);
         }
-    }
-    const float inv = count ? 1.f / count : 0.f;
+        row += B * at.rows;
+        count += B;
+    };
+    while (row + (kBatch - 1) * at.rows < at.s1) batch(std::integral_constant<int, kBatch>());
+    while (row < at.s1) batch(std::integral_constant<int, 1>());
+    const double inv = count ? 1. / (double)count : 0.;
+    float mean_of[VEC], sq_of[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) { // mean, and squares about it
-        const float m = sum[j] * inv;
-        sq[j] = fmaxf(__builtin_fmaf(-m, sum[j], sq[j]), 0.f);
-        sum[j] = first[j] + m;
+    for (int j = 0; j < VEC; ++j) {
+        const double m = sum[j] * inv;
+        mean_of[j] = (float)m;
+        sq_of[j] = (float)(sq[j] + fmax(__builtin_fma(-m, sum[j], among[j]), 0.)); // (a NaN is in the mean)
     }
     const int64_t total = at.s1 - at.s0;
-    tile_pairs<VEC>(p, at, sum, sq, [&](const float *m, const float *q, float *mean, float *m2) {
+    tile_pairs<VEC>(p, at, mean_of, sq_of, [&](const float *m, const float *q, float *mean, float *m2) {
         const int cl = threadIdx.x & (p.lc - 1);
         float s = 0.f;
         for (int r = 0; r < at.rows; ++r) {
@@ -441,15 +453,14 @@ __global__ __launch_bounds__(256) void norm_join_kernel(GroupNormParams p) {
     const int g = (int)(blockIdx.x % p.G), entries = p.chunks * p.D;
     const float *part = p.part + n * p.chunks * 2 * p.C + g * p.D;
     auto rows = [&](int k) { return (float)min((int64_t)p.chunk, p.S - (int64_t)k * p.chunk); };
-    const float base = part[0]; // a mean to sum about
     float s = 0.f;
 #pragma unroll 8
     for (int i = threadIdx.x; i < entries; i += 256) {
         const int k = i / p.D;
-        s += rows(k) * (part[(int64_t)k * 2 * p.C + i % p.D] - base);
+        s = __builtin_fmaf(rows(k), part[(int64_t)k * 2 * p.C + i % p.D], s);
     }
     const float size = (float)p.S * (float)p.D;
-    const float mean = base + block_sum(s, red) / size;
+    const float mean = block_sum(s, red) / size;
     float t = 0.f;
 #pragma unroll 8
     for (int i = threadIdx.x; i < entries; i += 256) {
@@ -742,8 +753,8 @@ __device__ __forceinline__ void collect(const GroupNormParams &p, const GroupLan
 
 template <typename T, int VEC, int E, bool GATE>
 __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
-    __shared__ float red[2][VEC * NT]; // sums and squares of a thread's channels
-    __shared__ float all[2][kMostWords], first[kSet], stat[2][kSet];
+    __shared__ float red[2][VEC * NT]; // sums, and squares about their mean, of a thread's channels
+    __shared__ float all[2][kMostWords], stat[2][kSet];
     __shared__ unsigned long long missing;
     const int tid = threadIdx.x;
     const Held<VEC, E> at(p, blockIdx.x);
@@ -767,26 +778,27 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) group[j] = p.tiles == 1 && at.ok ? (at.in_tile + j) / p.D : 0;
 
-    // The mean of a part and the squares about it, from sums about one value of the
-    // group's, so that a large mean costs no digits.
+    // The mean of a part and the squares about it.  A thread's are about its own mean,
+    // and joined about the part's: neither a large mean nor a value far from the others
+    // costs digits.
     auto moments = [&](const Held<VEC, E> &h, auto at_once, auto value) { // value(i): the i-th row's; at_once: rows unrolled
         const int gc = min(p.D, h.channels(p)); // the tile's channels of a group
+        auto rows_of = [&](int r) { return max(0, (h.count - r + h.rows - 1) / h.rows); }; // of a channel's r-th thread
+        const int mine = h.ok ? rows_of(h.rl) : 0;
+        const float inv = mine ? 1.f / mine : 0.f;
+        float s[VEC], q[VEC];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j)
-            if (h.ok && h.rl == 0 && (h.in_tile + j) % p.D == 0) first[group[j]] = (float)value(0)[j];
-        __syncthreads();
-        float base[VEC], s[VEC], q[VEC];
+        for (int j = 0; j < VEC; ++j) s[j] = q[j] = 0.f;
+        each_row<E>(at_once, [&](int i) {
+            const Raw<T, VEC> v = value(i);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            base[j] = first[group[j]];
-            s[j] = q[j] = 0.f;
-        }
+            for (int j = 0; j < VEC; ++j) s[j] += i < mine ? (float)v[j] : 0.f;
+        });
         each_row<E>(at_once, [&](int i) {
             const Raw<T, VEC> v = value(i);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float d = h.has(i) ? (float)v[j] - base[j] : 0.f;
-                s[j] += d;
+                const float d = i < mine ? __builtin_fmaf(-s[j], inv, (float)v[j]) : 0.f;
                 q[j] = __builtin_fmaf(d, d, q[j]);
             }
         });
@@ -796,21 +808,36 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
             red[1][j * NT + tid] = q[j];
         }
         __syncthreads();
-        // channel c of the tile is at c % VEC of lane c / VEC, for every row of threads
-        float t[2] = {0.f, 0.f};
-        if (gl.ok)
-            for (int c = gl.g * p.D + gl.t; c < gl.g * p.D + gc; c += gl.share) {
-                const int o = (c % VEC) * NT + c / VEC;
-#pragma unroll 4
-                for (int r = 0; r < h.rows; ++r) {
-                    t[0] += red[0][o + r * p.lc];
-                    t[1] += red[1][o + r * p.lc];
+        // channel c of the tile is at c % VEC of lane c / VEC, for every row of threads:
+        // f(n, 1 / n, s, q, k) of those of them that hold rows, in four chains
+        const int full = h.count / h.rows, more = h.count % h.rows; // rows of a thread; the first `more` have one more
+        const int there = full ? h.rows : more;
+        const float n0 = (float)full, n1 = (float)(full + 1), inv0 = 1.f / n0, inv1 = 1.f / n1;
+        auto each = [&](auto f) {
+            if (gl.ok)
+                for (int c = gl.g * p.D + gl.t; c < gl.g * p.D + gc; c += gl.share) {
+                    const int o = (c % VEC) * NT + c / VEC;
+                    auto one = [&](int r, int k) {
+                        f(r < more ? n1 : n0, r < more ? inv1 : inv0, red[0][o + r * p.lc], red[1][o + r * p.lc], k);
+                    };
+                    int r = 0;
+                    for (; r + 4 <= there; r += 4)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) one(r + k, k);
+                    for (; r < there; ++r) one(r, 0);
                 }
-            }
-        lanes_sum<2>(t, __builtin_ctz(gl.share));
-        const float shift = t[0] / ((float)h.count * (float)gc);
-        const float2 m = {first[gl.g] + shift, fmaxf(__builtin_fmaf(-shift, t[0], t[1]), t[1] - t[1])}; // (a NaN stays)
-        __syncthreads(); // (first and red may be written again)
+        };
+        float t[4] = {0.f, 0.f, 0.f, 0.f};
+        each([&](float, float, float sum, float, int k) { t[k] += sum; });
+        const float mean = gl.sum((t[0] + t[1]) + (t[2] + t[3])) / ((float)h.count * (float)gc);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) t[k] = 0.f;
+        each([&](float n, float inv_n, float sum, float squares, int k) {
+            const float d = __builtin_fmaf(-mean, n, sum);
+            t[k] += __builtin_fmaf(d * d, inv_n, squares);
+        });
+        const float2 m = {mean, gl.sum((t[0] + t[1]) + (t[2] + t[3]))};
+        __syncthreads(); // (red may be written again)
         return m;
     };
     const float2 own = moments(at, std::true_type(), [&](int i) { return rx[i]; });
@@ -820,17 +847,14 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
         return moments(other, std::false_type(), [&](int i) { return raw_n<T, VEC>(y + other.row(i) * p.sxs); });
     });
     const float *const means = all[0], *const squares = all[1];
-    float s, q;
     auto size = [&](int k) { // elements of part k
         const int64_t rows = min((int64_t)p.chunk, p.S - (int64_t)(k / p.tiles) * p.chunk);
         return (float)rows * (float)(p.tiles == 1 ? p.D : min(p.tile, p.D - (k % p.tiles) * p.tile));
     };
-    // (a lane reads what it wrote itself; sums about part 0's mean, the same in every part)
-    const float base0 = __shfl(gl.t == 0 ? means[gl.g] : 0.f, 0, gl.share);
-    s = 0.f;
-    for (int k = gl.t; gl.ok && k < at.parts; k += gl.share) s = __builtin_fmaf(size(k), means[k * ng + gl.g] - base0, s);
-    const float total = (float)p.S * (float)p.D, mean = base0 + gl.sum(s) / total;
-    q = 0.f;
+    // (a lane reads what it wrote itself)
+    float s = 0.f, q = 0.f;
+    for (int k = gl.t; gl.ok && k < at.parts; k += gl.share) s = __builtin_fmaf(size(k), means[k * ng + gl.g], s);
+    const float total = (float)p.S * (float)p.D, mean = gl.sum(s) / total;
     for (int k = gl.t; gl.ok && k < at.parts; k += gl.share) {
         const float d = means[k * ng + gl.g] - mean;
         q += __builtin_fmaf(size(k) * d, d, squares[k * ng + gl.g]);
