@@ -228,10 +228,30 @@ __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(GroupNormParams p) {
             r.rstd[u] = p.stats[(n * p.G + gs) * 2 + 1];
         }
     };
+    // The sums of kRowsAtOnce rows, those of the rest beside them: in registers all rows'
+    // sums would be one chain of roundings.
+    constexpr int kRowsAtOnce = 128;
+    auto put_by = [&](bool start) {
+#pragma unroll
+        for (int k = 0; k < NV; ++k)
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                float *const a = &red[0][wave][(k * VEC + j) * kWave + lane], *const b = &red[1][wave][(k * VEC + j) * kWave + lane];
+                *a = start ? 0.f : *a + dwt[k][j];
+                *b = start ? 0.f : *b + dbs[k][j];
+                dwt[k][j] = dbs[k][j] = 0.f;
+            }
+    };
+    put_by(true);
+    int taken = 0;
     Rows next;
     if (n0 + wave * U < n1) load(n0 + wave * U, next);
     for (int64_t first = n0 + wave * U; first < n1; first += step) {
         const Rows r = next;
+        if ((taken += U) > kRowsAtOnce) {
+            put_by(false);
+            taken = U;
+        }
         load(min(first + step, n1 - 1), next);
         float nn[U][NV][VEC], dn[U][NV][VEC], s[2 * U]; // sums of dn, of dn n
 #pragma unroll
@@ -288,13 +308,7 @@ __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(GroupNormParams p) {
         }
     }
     if (!p.part) return;
-#pragma unroll
-    for (int k = 0; k < NV; ++k)
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            red[0][wave][(k * VEC + j) * kWave + lane] = dwt[k][j];
-            red[1][wave][(k * VEC + j) * kWave + lane] = dbs[k][j];
-        }
+    put_by(false);
     __syncthreads();
     if (wave == 0) {
         float *out = p.part + block * 2 * p.C;
@@ -312,23 +326,24 @@ __global__ __launch_bounds__(256) void norm_rows_bwd_kernel(GroupNormParams p) {
 }
 
 // dweight and dbias from the blocks' sums: part [blocks][2][C].  A workgroup
-// takes 16 columns (of 2 C), 16 threads a column.
+// takes 16 columns (of 2 C), 16 threads a column, which sum in 64 bits: there may be a
+// million blocks.
 __global__ __launch_bounds__(256) void column_sum_kernel(const float *part, int64_t blocks, int C, float *dweight, float *dbias) {
-    __shared__ float red[16][17];
+    __shared__ double red[16][17];
     const int col = threadIdx.x & 15, r = threadIdx.x >> 4;
     const int64_t i = (int64_t)blockIdx.x * 16 + col;
-    float sum = 0.f;
+    double sum = 0.;
     if (i < 2 * (int64_t)C)
 #pragma unroll 4
         for (int64_t b = r; b < blocks; b += 16) sum += part[b * 2 * C + i];
     red[r][col] = sum;
     __syncthreads();
     if (r == 0 && i < 2 * (int64_t)C) {
-        sum = 0.f;
+        sum = 0.;
 #pragma unroll
         for (int k = 0; k < 16; ++k) sum += red[k][col];
         float *out = i < C ? dweight : dbias;
-        if (out) out[i < C ? i : i - C] = sum;
+        if (out) out[i < C ? i : i - C] = (float)sum;
     }
 }
 
@@ -537,29 +552,52 @@ __device__ __forceinline__ void dz_n(const GroupNormParams &p, const Channels<VE
     }
 }
 
-// First pass, adjoint: sums of dz n and dz of every channel over the chunk's rows.
+// First pass, adjoint: sums of dz n and dz of every channel over the chunk's rows, four
+// at a time in 32 bits and these in 64.
 template <typename T, int VEC, bool GATE> __global__ __launch_bounds__(256) void norm_bwd_sums_kernel(GroupNormParams p) {
     const TileAt<VEC> at(p);
     const Channels<VEC> ch(p, at.n, at.c);
     const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c;
     const T *dy = static_cast<const T *>(p.dy) + at.n * p.sxn + at.c;
     const T *gate = static_cast<const T *>(p.gate) + at.n * p.sgn + at.c;
-    float a[VEC], b[VEC];
+    double sum_a[VEC], sum_b[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) a[j] = b[j] = 0.f;
-#pragma unroll 4
-    for (int64_t s = at.s0 + at.rl; s < at.s1; s += at.rows) {
-        float vx[VEC], vd[VEC], vg[VEC], n[VEC], dz[VEC], dg[VEC];
-        load_n<T, VEC>(x + s * p.sxs, vx);
-        load_n<T, VEC>(dy + s * p.sxs, vd);
-        if constexpr (GATE) load_n<T, VEC>(gate + s * p.sgs, vg);
-        dz_n<T, VEC, GATE>(p, ch, vx, vd, vg, n, dz, dg);
+    for (int j = 0; j < VEC; ++j) sum_a[j] = sum_b[j] = 0.;
+    int64_t row = at.s0 + at.rl;
+    auto batch = [&](auto rows) {
+        constexpr int B = decltype(rows)::value;
+        float vx[B][VEC], vd[B][VEC], vg[B][VEC], a[VEC], b[VEC];
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            const int64_t s = row + i * at.rows;
+            load_n<T, VEC>(x + s * p.sxs, vx[i]);
+            load_n<T, VEC>(dy + s * p.sxs, vd[i]);
+            if constexpr (GATE) load_n<T, VEC>(gate + s * p.sgs, vg[i]);
+        }
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) a[j] = b[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+            float n[VEC], dz[VEC], dg[VEC];
+            dz_n<T, VEC, GATE>(p, ch, vx[i], vd[i], vg[i], n, dz, dg);
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                a[j] = __builtin_fmaf(dz[j], n[j], a[j]);
+                b[j] += dz[j];
+            }
+        }
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            a[j] = __builtin_fmaf(dz[j], n[j], a[j]);
-            b[j] += dz[j];
+            sum_a[j] += a[j];
+            sum_b[j] += b[j];
         }
-    }
+        row += B * at.rows;
+    };
+    while (row + 3 * at.rows < at.s1) batch(std::integral_constant<int, 4>());
+    while (row < at.s1) batch(std::integral_constant<int, 1>());
+    float a[VEC], b[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) a[j] = (float)sum_a[j], b[j] = (float)sum_b[j];
     tile_pairs<VEC>(p, at, a, b, [&](const float *u, const float *v, float *x0, float *x1) {
         const int cl = threadIdx.x & (p.lc - 1);
         float s = 0.f, t = 0.f;
@@ -1094,7 +1132,8 @@ Plan plan_of(const gdn2_group_norm_args &a, bool bwd, bool vec4, bool sums_wante
         q.sets = (int)((a.groups + gpw - 1) / gpw);
         if (bwd) {
             // 512 workgroups, two a compute unit (1024: 67 against 62.5 us at 8192 x 2048
-            // gated f32), of at least two rows a wave
+            // gated f32; more of them for 262144 rows: 1326 against 1195), of at least two rows
+            // a wave
             q.row_blocks = (int)std::max<int64_t>(1, std::min<int64_t>((512 + q.sets - 1) / q.sets, (N + 7) / 8));
             q.bytes = sums_wanted ? up256(8 * (size_t)q.row_blocks * C) : 0;
         }

@@ -160,22 +160,23 @@ template <int VEC> __global__ __launch_bounds__(256) void short_conv_bwd_kernel(
     }
 }
 
-// Sums over `blocks` rows of n columns; a workgroup takes 16 columns, 16 threads each.
+// Sums over `blocks` rows of n columns; a workgroup takes 16 columns, 16 threads each,
+// which sum in 64 bits: there may be tens of thousands of rows.
 __global__ __launch_bounds__(256) void conv_weight_sum_kernel(const float *part, int64_t blocks, int64_t n, float *out) {
-    __shared__ float red[16][17];
+    __shared__ double red[16][17];
     const int col = threadIdx.x & 15, r = threadIdx.x >> 4;
     const int64_t i = (int64_t)blockIdx.x * 16 + col;
-    float sum = 0.f;
+    double sum = 0.;
     if (i < n)
 #pragma unroll 4
         for (int64_t b = r; b < blocks; b += 16) sum += part[b * n + i];
     red[r][col] = sum;
     __syncthreads();
     if (r == 0 && i < n) {
-        sum = 0.f;
+        sum = 0.;
 #pragma unroll
         for (int k = 0; k < 16; ++k) sum += red[k][col];
-        out[i] = sum;
+        out[i] = (float)sum;
     }
 }
 

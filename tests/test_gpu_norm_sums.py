@@ -43,3 +43,55 @@ def test_one_value_far_from_the_others(gpu, N, S, C, groups, ty, at):
     rel = (stats[..., 1].double() * torch.sqrt(var + EPS) - 1).abs().max().item()
     print("rstd off by", rel, flush=True)
     assert rel <= M.SUM * M.EPS, rel
+
+
+# Sums of one sign: a serial f32 sum of n equal terms is off by up to n / 4 half steps
+# (its partial sums' roundings are all the same way within a power of two), one in
+# pieces by its longest chain's.  SUM_TERMS as in M.norm_bwd64; the terms are constants
+# whose sums f32 does not hold.
+SUM_TERMS = 200
+
+
+@pytest.mark.parametrize("N,S,C,groups", [(1 << 22, 1, 64, 1), (1 << 20, 4, 16, 1), (1, 100000, 2048, 1), (1, 1 << 22, 32, 1)])
+def test_gradients_of_weights_over_very_many_rows(gpu, N, S, C, groups):
+    """A loss that is a mean: d_out the same everywhere."""
+    import torch
+
+    import gdn2_amd as G
+
+    r = torch.Generator(device=gpu).manual_seed(3)
+    x = torch.randn(N, S, C, generator=r, device=gpu)
+    y, stats = G.group_norm_act(x, groups, eps=EPS, activation="none", return_stats=True)
+    del y
+    dy = torch.tensor(0.1, device=gpu).expand(C).contiguous().expand(N, S, C)
+    g = G.group_norm_act_backward(x, groups, stats, dy, activation="none")
+    torch.cuda.synchronize()
+    c = float(torch.tensor(0.1))
+    off = (g["dbias"].double() / (N * S * c) - 1).abs().max().item()
+    print("dbias off by", off / M.EPS, "half steps", flush=True)
+    assert off <= SUM_TERMS * M.EPS, off / M.EPS
+    # dn is the same everywhere: what is left of it, dn - mean(dn) - n mean(dn n), are roundings
+    n = C // groups * S
+    mean_n = (SUM_TERMS + 8) * M.EPS  # mean(n) is zero but for the statistics' roundings, of mean |n| < 1
+    left = g["dx"].abs().max().item()
+    bound = stats[..., 1].max().item() * c * ((SUM_TERMS + 8) * M.EPS + 7 * (mean_n + SUM_TERMS * M.EPS))  # (|n| < 7)
+    print("dx", left, "of", bound, n, flush=True)
+    assert left <= bound, (left, bound)
+
+
+def test_gradients_of_conv_weights_over_very_many_tokens(gpu):
+    import torch
+
+    import gdn2_amd as G
+
+    T, C = 1 << 22, 16
+    x, w = torch.full((1, T, C), 0.7, device=gpu), torch.full((C, 4), 0.1, device=gpu)
+    r = G.short_conv_1d_backward(x, w, torch.full_like(x, 0.1))
+    torch.cuda.synchronize()
+    a, d = float(torch.tensor(0.7)), float(torch.tensor(0.1))
+    z = 4 * a * d
+    s = 1 / (1 + 2.718281828459045 ** -z)
+    want = T * d * s * (1 + z * (1 - s)) * a
+    off = (r["dweight"].double() / want - 1).abs().max().item()
+    print("dweight off by", off / M.EPS, "half steps", flush=True)
+    assert off <= 120 * M.EPS, off / M.EPS  # (as M.conv_bwd64; the terms' own few roundings among them)
