@@ -49,6 +49,8 @@ struct GroupNormParams {
     int row_blocks;    // backward rows kernel
     int lc;            // tile kernels: lanes along the channels (a power of two); held groups: any number
     int chunks, chunk; // row chunks of a sample, rows in one
+    int spans, span;   // a group's chunks are joined in spans of `span` chunks
+    float *joined;     // [N][G][spans][2] what they give, where they are several
     // held groups: channels a tile, tiles a set of groups, sets; a part: a chunk of rows by a tile
     int tile, tiles, sets, set_groups; // (sets: rows kernels, too)
     unsigned long long *words; // [sample][set][part][set_groups] what the parts publish
@@ -461,20 +463,22 @@ __device__ __forceinline__ float block_sum(float v, float *red) {
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// Second pass, forward: a group's mean and rstd from its channels' and chunks'.
+// Second pass, forward: a group's mean and rstd from its channels' and chunks', or of
+// a span of chunks the mean and the squares about it.
 __global__ __launch_bounds__(256) void norm_join_kernel(GroupNormParams p) {
     __shared__ float red[4];
     const int64_t n = blockIdx.x / p.G;
-    const int g = (int)(blockIdx.x % p.G), entries = p.chunks * p.D;
-    const float *part = p.part + n * p.chunks * 2 * p.C + g * p.D;
-    auto rows = [&](int k) { return (float)min((int64_t)p.chunk, p.S - (int64_t)k * p.chunk); };
+    const int g = (int)(blockIdx.x % p.G), k0 = (int)blockIdx.y * p.span, k1 = min(k0 + p.span, p.chunks);
+    const int entries = (k1 - k0) * p.D;
+    const float *part = p.part + (n * p.chunks + k0) * 2 * p.C + g * p.D;
+    auto rows = [&](int k) { return (float)min((int64_t)p.chunk, p.S - (int64_t)(k0 + k) * p.chunk); };
     float s = 0.f;
 #pragma unroll 8
     for (int i = threadIdx.x; i < entries; i += 256) {
         const int k = i / p.D;
         s = __builtin_fmaf(rows(k), part[(int64_t)k * 2 * p.C + i % p.D], s);
     }
-    const float size = (float)p.S * (float)p.D;
+    const float size = (float)(min((int64_t)k1 * p.chunk, p.S) - (int64_t)k0 * p.chunk) * (float)p.D;
     const float mean = block_sum(s, red) / size;
     float t = 0.f;
 #pragma unroll 8
@@ -484,10 +488,28 @@ __global__ __launch_bounds__(256) void norm_join_kernel(GroupNormParams p) {
         const float d = e[0] - mean;
         t += e[p.C] + rows(k) * d * d;
     }
-    const float var = block_sum(t, red) / size;
+    const float squares = block_sum(t, red);
     if (threadIdx.x == 0) {
-        p.stats[blockIdx.x * 2] = mean;
-        p.stats[blockIdx.x * 2 + 1] = 1.f / sqrtf(var + p.eps);
+        float *out = p.spans > 1 ? p.joined + ((int64_t)blockIdx.x * p.spans + blockIdx.y) * 2 : p.stats + (int64_t)blockIdx.x * 2;
+        out[0] = mean;
+        out[1] = p.spans > 1 ? squares : 1.f / sqrtf(squares / size + p.eps);
+    }
+}
+// ... the spans of a group: a wave each.
+__global__ __launch_bounds__(64) void norm_join_spans_kernel(GroupNormParams p) {
+    const float *e = p.joined + (int64_t)blockIdx.x * p.spans * 2;
+    auto rows = [&](int k) { return (float)(min((int64_t)(k + 1) * p.span * p.chunk, p.S) - (int64_t)k * p.span * p.chunk); };
+    float s = 0.f, t = 0.f;
+    for (int k = threadIdx.x; k < p.spans; k += kWave) s = __builtin_fmaf(rows(k), e[2 * k], s);
+    const float mean = wave_sum(s) / (float)p.S;
+    for (int k = threadIdx.x; k < p.spans; k += kWave) {
+        const float d = e[2 * k] - mean;
+        t += __builtin_fmaf(rows(k) * (float)p.D * d, d, e[2 * k + 1]);
+    }
+    const float squares = wave_sum(t);
+    if (threadIdx.x == 0) {
+        p.stats[(int64_t)blockIdx.x * 2] = mean;
+        p.stats[(int64_t)blockIdx.x * 2 + 1] = 1.f / sqrtf(squares / ((float)p.S * (float)p.D) + p.eps);
     }
 }
 
@@ -610,12 +632,13 @@ template <typename T, int VEC, bool GATE> __global__ __launch_bounds__(256) void
     });
 }
 
-// Second pass, adjoint: a group's means of dn n and dn.
+// Second pass, adjoint: a group's means of dn n and dn, or a span of chunks' sums.
 __global__ __launch_bounds__(256) void norm_bwd_join_kernel(GroupNormParams p) {
     __shared__ float red[4];
     const int64_t n = blockIdx.x / p.G;
-    const int g = (int)(blockIdx.x % p.G), entries = p.chunks * p.D;
-    const float *part = p.part + n * p.chunks * 2 * p.C + g * p.D;
+    const int g = (int)(blockIdx.x % p.G), k0 = (int)blockIdx.y * p.span, k1 = min(k0 + p.span, p.chunks);
+    const int entries = (k1 - k0) * p.D;
+    const float *part = p.part + (n * p.chunks + k0) * 2 * p.C + g * p.D;
     float s = 0.f, t = 0.f;
 #pragma unroll 8
     for (int i = threadIdx.x; i < entries; i += 256) {
@@ -627,9 +650,26 @@ __global__ __launch_bounds__(256) void norm_bwd_join_kernel(GroupNormParams p) {
     s = block_sum(s, red);
     t = block_sum(t, red);
     if (threadIdx.x == 0) {
+        const float size = p.spans > 1 ? 1.f : (float)p.S * (float)p.D;
+        float *out = p.spans > 1 ? p.joined + ((int64_t)blockIdx.x * p.spans + blockIdx.y) * 2 : p.sums + (int64_t)blockIdx.x * 2;
+        out[0] = s / size;
+        out[1] = t / size;
+    }
+}
+// ... the spans of a group: a wave each.
+__global__ __launch_bounds__(64) void norm_bwd_join_spans_kernel(GroupNormParams p) {
+    const float *e = p.joined + (int64_t)blockIdx.x * p.spans * 2;
+    float s = 0.f, t = 0.f;
+    for (int k = threadIdx.x; k < p.spans; k += kWave) {
+        s += e[2 * k];
+        t += e[2 * k + 1];
+    }
+    s = wave_sum(s);
+    t = wave_sum(t);
+    if (threadIdx.x == 0) {
         const float size = (float)p.S * (float)p.D;
-        p.sums[blockIdx.x * 2] = s / size;
-        p.sums[blockIdx.x * 2 + 1] = t / size;
+        p.sums[(int64_t)blockIdx.x * 2] = s / size;
+        p.sums[(int64_t)blockIdx.x * 2 + 1] = t / size;
     }
 }
 
@@ -1071,8 +1111,8 @@ struct Plan {
     int64_t o_words, words; // bytes of the words that parts publish
     int vec, nv, u, log_l, sets;
     int row_blocks;
-    int lc, tiles, chunks, chunk;
-    size_t o_stats, o_sums, bytes; // workspace: part, then these
+    int lc, tiles, chunks, chunk, spans, span;
+    size_t o_stats, o_sums, o_joined, bytes; // workspace: part, then these
 };
 
 int up_log2(int64_t n) {
@@ -1117,6 +1157,7 @@ bool hold(const gdn2_group_norm_args &a, bool bwd, int vec, Plan *q) {
     return false;
 }
 
+constexpr int kJoin = 16384;
 Plan plan_of(const gdn2_group_norm_args &a, bool bwd, bool vec4, bool sums_wanted, bool in_place) {
     Plan q{};
     const int64_t C = a.channels, D = C / a.groups, N = a.samples, S = a.rows;
@@ -1162,15 +1203,22 @@ Plan plan_of(const gdn2_group_norm_args &a, bool bwd, bool vec4, bool sums_wante
     // about 2048 workgroups, of at least four rows a thread
     const int64_t rows = 256 / q.lc;
     const int64_t most = std::max<int64_t>(1, S / (4 * rows)), want = std::max<int64_t>(1, 2048 / (N * q.tiles));
-    // and few enough for the join, one workgroup a group, to read them quickly
-    const int64_t chunks = std::min({most, want, std::max<int64_t>(1, 16384 / (C / a.groups))});
+    // and as few as one workgroup of the join takes, where 512 or more remain (200000 x 64
+    // f32 in two groups, 512 chunks and 2048: 76 and 89 us; 32768 x 512 in one, 32, 256 and
+    // 1024 chunks: 162, 71 and 73; 50000 x 2048 in one, 8, 64 and 256: 1143, 311 and 282)
+    const int64_t chunks = std::min({most, want, std::max<int64_t>({1, kJoin / D, (512 + N * q.tiles - 1) / (N * q.tiles)})});
     q.chunk = (int)((S + chunks - 1) / chunks);
     q.chunks = (int)((S + q.chunk - 1) / q.chunk);
+    // joined by a workgroup for every kJoin channels of chunks of a group
+    q.span = (int)std::min<int64_t>(q.chunks, std::max<int64_t>(1, kJoin / D));
+    q.spans = (q.chunks + q.span - 1) / q.span;
     size_t at = up256(8 * (size_t)(N * q.chunks) * C);
     q.o_stats = at;
     if (!bwd) at += up256(8 * (size_t)(N * a.groups));
     q.o_sums = at;
     if (bwd) at += up256(8 * (size_t)(N * a.groups));
+    q.o_joined = at;
+    if (q.spans > 1) at += up256(8 * (size_t)(N * a.groups) * q.spans);
     q.bytes = at;
     return q;
 }
@@ -1218,8 +1266,10 @@ GroupNormParams fill(const gdn2_group_norm_args &a, const Plan &q, void *ws) {
     p.N = a.samples; p.S = a.rows; p.C = (int)a.channels; p.G = (int)a.groups; p.D = p.C / p.G;
     p.act = a.activation; p.eps = (float)a.eps;
     p.sets = q.sets; p.log_l = q.log_l; p.row_blocks = q.row_blocks; p.lc = q.lc; p.chunks = q.chunks; p.chunk = q.chunk;
+    p.spans = q.spans; p.span = q.span;
     char *w = static_cast<char *>(ws);
     if (q.bytes) p.part = reinterpret_cast<float *>(w);
+    if (q.spans > 1) p.joined = reinterpret_cast<float *>(w + q.o_joined);
     if (q.held) {
         p.tile = q.tile; p.tiles = q.tiles; p.set_groups = q.set_groups;
         if (q.words) {
@@ -1272,7 +1322,8 @@ template <typename T, int VEC> hipError_t run_forward(const Plan &q, const Group
     if (q.held) return p.gate ? run_held<T, VEC, true, false>(q, p, s) : run_held<T, VEC, false, false>(q, p, s);
     const dim3 grid((unsigned)(p.N * q.chunks), (unsigned)q.tiles);
     hipLaunchKernelGGL((norm_moments_kernel<T, VEC>), grid, dim3(256), 0, s, p);
-    hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)(p.N * p.G)), dim3(256), 0, s, p);
+    hipLaunchKernelGGL(norm_join_kernel, dim3((unsigned)(p.N * p.G), (unsigned)q.spans), dim3(256), 0, s, p);
+    if (q.spans > 1) hipLaunchKernelGGL(norm_join_spans_kernel, dim3((unsigned)(p.N * p.G)), dim3(kWave), 0, s, p);
     if (p.gate) hipLaunchKernelGGL((norm_apply_kernel<T, VEC, true>), grid, dim3(256), 0, s, p);
     else hipLaunchKernelGGL((norm_apply_kernel<T, VEC, false>), grid, dim3(256), 0, s, p);
     return hipGetLastError();
@@ -1288,7 +1339,8 @@ template <typename T, int VEC, bool GATE> hipError_t run_backward(const Plan &q,
     } else {
         const dim3 grid((unsigned)(p.N * q.chunks), (unsigned)q.tiles);
         hipLaunchKernelGGL((norm_bwd_sums_kernel<T, VEC, GATE>), grid, dim3(256), 0, s, p);
-        hipLaunchKernelGGL(norm_bwd_join_kernel, dim3((unsigned)(p.N * p.G)), dim3(256), 0, s, p);
+        hipLaunchKernelGGL(norm_bwd_join_kernel, dim3((unsigned)(p.N * p.G), (unsigned)q.spans), dim3(256), 0, s, p);
+        if (q.spans > 1) hipLaunchKernelGGL(norm_bwd_join_spans_kernel, dim3((unsigned)(p.N * p.G)), dim3(kWave), 0, s, p);
         hipLaunchKernelGGL((norm_bwd_apply_kernel<T, VEC, GATE>), grid, dim3(256), 0, s, p);
         blocks = p.N * q.chunks;
     }

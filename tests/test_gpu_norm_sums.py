@@ -95,3 +95,20 @@ def test_gradients_of_conv_weights_over_very_many_tokens(gpu):
     off = (r["dweight"].double() / want - 1).abs().max().item()
     print("dweight off by", off / M.EPS, "half steps", flush=True)
     assert off <= 120 * M.EPS, off / M.EPS  # (as M.conv_bwd64; the terms' own few roundings among them)
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16"])
+@pytest.mark.parametrize("N,S,C,groups", [(1, 9000, 520, 1), (1, 9000, 521, 1), (2, 5000, 1040, 2), (1, 300, 33000, 1),
+                                          (1, 40000, 64, 1)])
+def test_large_groups(gpu, N, S, C, groups, ty):
+    """Groups whose chunks of rows are joined in several spans, one of them shorter."""
+    import test_gpu_group_norm as B
+
+    import gdn2_amd as G
+
+    for act, gate in (("silu", True), ("gelu", False)):
+        d, dy = B._make(gpu, C + S, N, S, C, ty, gate)
+        y, stats = G.group_norm_act(d["x"], groups, d["weight"], d["bias"], EPS, act, gate=d["gate"], return_stats=True)
+        B._check_forward(d, groups, act, y, stats, ty)
+        r = G.group_norm_act_backward(d["x"], groups, stats, dy, d["weight"], d["bias"], act, gate=d["gate"])
+        B._check_backward(d, groups, act, stats, dy, r, ty)

@@ -1,0 +1,21 @@
+"""What the mixer operators plan for a call, without a GPU."""
+import ctypes
+
+import pytest
+
+
+@pytest.mark.parametrize("S,C,groups,tiles", [(32768, 512, 1, 2), (50000, 2048, 1, 8), (20000, 16384, 1, 64), (20000, 1024, 1, 4)])
+def test_large_groups_are_spread_over_the_device(S, C, groups, tiles):
+    """A group in three passes is read by 512 workgroups or more, two a compute unit,
+    whatever its channels (the workspace holds a pair for each chunk of rows and
+    channel)."""
+    from gdn2_amd import _capi as C_
+
+    a = C_.GroupNormArgs()
+    for k, v in dict(x=256, y=256, samples=1, rows=S, channels=C, groups=groups, eps=1e-5, activation=1, stride_x_n=S * C,
+                     stride_x_s=C).items():
+        setattr(a, k, v)
+    for size in (C_.lib().gdn2_group_norm_act_workspace_bytes(ctypes.byref(a)),
+                 C_.lib().gdn2_group_norm_act_bwd_workspace_bytes(ctypes.byref(C_.GroupNormBwdArgs(a)))):
+        chunks = size // (8 * C)
+        assert 500 <= chunks * tiles <= 4096, chunks
