@@ -70,9 +70,16 @@ def _workspace(args, workspace: Optional[torch.Tensor], need: int, like: torch.T
     return workspace
 
 
-def _dense_rows(t: torch.Tensor) -> torch.Tensor:
-    """t, or a copy of it, with contiguous channels and no element of memory in
-    two places (what the gradients are laid out like)."""
+# A new result is laid out like its operand; where that would take more than so many
+# times the elements' memory (the last token of every sequence of a prompt), like a
+# contiguous copy of the operand, which costs two more passes over few elements.
+_MOST_GAPS = 4
+
+
+def _dense_rows(t: torch.Tensor, most: Optional[int] = None) -> torch.Tensor:
+    """t, or a copy of it, with contiguous channels, no element of memory in two
+    places and, with `most`, elements apart by at most so many times their number
+    (what the gradients are laid out like)."""
     if t.is_contiguous():
         return t
     if t.dim() == 4:  # [B, T, H, V] seen as [B, H, T, V]
@@ -86,7 +93,7 @@ def _dense_rows(t: torch.Tensor) -> torch.Tensor:
         if s < span:
             return t.contiguous()
         span = s * n
-    return t
+    return t if most is None or span <= most * t.numel() else t.contiguous()
 
 
 def _empty_like(t: torch.Tensor) -> torch.Tensor:
@@ -172,7 +179,7 @@ def gated_scan(g, v, w=None, state=None, cu_seqlens=None, out=None, new_state=No
     index = _device(v, g, w, state, cu_seqlens, out, new_state)
     v, g = _channels(v), _channels(g)
     if w is not None and w.stride() != v.stride():
-        v = _dense_rows(v)
+        v = _dense_rows(v, _MOST_GAPS)
         w = _in_layout(w, v)
     if state is not None:
         state = state.contiguous()
@@ -201,10 +208,10 @@ def gated_scan_backward(g, v, w, out, d_out, state=None, d_state=None, cu_seqlen
     sequence of cu_seqlens have no gradient: dg, dv and dw are zero there."""
     of_states = _scan_check(g, v, w, state, cu_seqlens, (("out", out), ("d_out", d_out)), (("d_state", d_state),))
     index = _device(v, g, w, state, cu_seqlens, out, d_out, d_state)
-    v, g = _dense_rows(v), _dense_rows(g)
+    v, g = _dense_rows(v, _MOST_GAPS), _dense_rows(g, _MOST_GAPS)
     if w is not None:
         w = _in_layout(w, v)
-    out = _dense_rows(out)
+    out = _dense_rows(out, _MOST_GAPS)
     d_out = _in_layout(d_out, out)
     state = None if state is None else state.contiguous()
     d_state = None if d_state is None else d_state.contiguous()
@@ -277,7 +284,7 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-5, ac
     which the backward takes.  `out` takes the result where given (it may be x)."""
     _norm_check(x, groups, weight, bias, activation, gate, (("out", out),) if out is not None else ())
     index = _device(x, weight, bias, gate, out)
-    shape, x = x.shape, _dense_rows(_rows(x))
+    shape, x = x.shape, _dense_rows(_rows(x), _MOST_GAPS if out is None else None)
     gate = None if gate is None else _dense_rows(_rows(gate))
     weight, bias = _contig(weight), _contig(bias)
     y = _empty_like(x) if out is None else _rows(out)
@@ -304,8 +311,8 @@ def group_norm_act_backward(x, groups: int, stats, d_out, weight=None, bias=None
     if stats.shape != (x.shape[0], groups, 2):
         raise ValueError("stats must be [N, groups, 2]")
     index = _device(x, weight, bias, gate, d_out, stats)
-    shape, x = x.shape, _dense_rows(_rows(x))
-    gate = None if gate is None else _dense_rows(_rows(gate))
+    shape, x = x.shape, _dense_rows(_rows(x), _MOST_GAPS)
+    gate = None if gate is None else _dense_rows(_rows(gate), _MOST_GAPS)
     d_out = _in_layout(_rows(d_out), x)
     weight, bias, stats = _contig(weight), _contig(bias), stats.contiguous()
     dx, dgate = _empty_like(x), None if gate is None else _empty_like(gate)
