@@ -104,8 +104,14 @@ def _empty_like(t: torch.Tensor) -> torch.Tensor:
     return torch.empty_strided(t.shape, t.stride(), dtype=t.dtype, device=t.device)
 
 
+def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether tensors of one shape have the same strides (a dimension of one has none
+    to speak of)."""
+    return a.stride() == b.stride() or all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
 def _in_layout(t: torch.Tensor, ref: torch.Tensor) -> torch.Tensor:
-    if t.stride() == ref.stride():
+    if _same_layout(t, ref):
         return t
     return _empty_like(ref).copy_(t)
 
@@ -178,7 +184,7 @@ def gated_scan(g, v, w=None, state=None, cu_seqlens=None, out=None, new_state=No
                             (("new_state", new_state),) if new_state is not None else ())
     index = _device(v, g, w, state, cu_seqlens, out, new_state)
     v, g = _channels(v), _channels(g)
-    if w is not None and w.stride() != v.stride():
+    if w is not None and not _same_layout(w, v):
         v = _dense_rows(v, _MOST_GAPS)
         w = _in_layout(w, v)
     if state is not None:
@@ -288,7 +294,7 @@ def group_norm_act(x, groups: int, weight=None, bias=None, eps: float = 1e-5, ac
     gate = None if gate is None else _dense_rows(_rows(gate))
     weight, bias = _contig(weight), _contig(bias)
     y = _empty_like(x) if out is None else _rows(out)
-    if out is not None and (y.data_ptr() != out.data_ptr() or y.stride() != x.stride()):
+    if out is not None and (y.data_ptr() != out.data_ptr() or not _same_layout(y, x)):
         raise ValueError("out must have x's layout")
     stats = x.new_empty((x.shape[0], groups, 2), dtype=torch.float32) if return_stats else None
     a = _norm_args(x, groups, weight, bias, eps, activation, gate, y, stats)

@@ -40,3 +40,26 @@ def test_results_take_little_memory(gpu):
         want_r = G.gated_scan_backward(*c, want, torch.ones_like(want))
         assert torch.equal(out, want) and all(r[n] is None or torch.equal(r[n], want_r[n]) for n in r)
         _small(out, new, *r.values())
+
+
+def test_strides_of_one_element_do_not_count(gpu):
+    """`out` that differs from x in the stride of a dimension of one alone is taken."""
+    import torch
+
+    import gdn2_amd as G
+
+    for shape, strides in (((1, 40, 64), (99999, 64, 1)), ((5, 1, 64), (64, 7, 1)), ((1, 64), (3, 1))):
+        x, out = torch.randn(shape, device=gpu), torch.empty_strided(shape, strides, device=gpu)
+        y = G.group_norm_act(x, 4, out=out)
+        assert y is out and torch.equal(y, G.group_norm_act(x, 4))
+        y, stats = G.group_norm_act(x, 4, return_stats=True)
+        dy = torch.randn(shape, device=gpu)
+        r = G.group_norm_act_backward(x, 4, stats, torch.empty_strided(shape, strides, device=gpu).copy_(dy))
+        want = G.group_norm_act_backward(x, 4, stats, dy)
+        assert all(r[n] is None or torch.equal(r[n], want[n]) for n in r)
+    v, w = torch.randn(2, 1, 16, 128, device=gpu).transpose(1, 2), torch.rand(2, 16, 1, 128, device=gpu)
+    g = -torch.rand(2, 16, 1, 1, device=gpu)
+    out, new = G.gated_scan(g, v, w)
+    want, last = G.gated_scan(g, v.contiguous(), w)
+    r, want_r = (G.gated_scan_backward(g, v, w, out, d) for d in (torch.ones_like(out), torch.ones(2, 16, 1, 128, device=gpu)))
+    assert torch.equal(out, want) and torch.equal(new, last) and all(torch.equal(r[n], want_r[n]) for n in r)

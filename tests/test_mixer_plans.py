@@ -19,3 +19,21 @@ def test_large_groups_are_spread_over_the_device(S, C, groups, tiles):
                  C_.lib().gdn2_group_norm_act_bwd_workspace_bytes(ctypes.byref(C_.GroupNormBwdArgs(a)))):
         chunks = size // (8 * C)
         assert 500 <= chunks * tiles <= 4096, chunks
+
+
+def test_strides_of_one_element_do_not_count():
+    """A dimension of one has no stride to speak of: at T = 1 the v that a projection
+    leaves, [B, 1, H, V] seen as [B, H, 1, V], and a contiguous w are laid out alike, and
+    a decoding step copies neither."""
+    torch = pytest.importorskip("torch")
+    from gdn2_amd import mixer
+
+    v, w = torch.zeros(2, 1, 16, 128).transpose(1, 2), torch.zeros(2, 16, 1, 128)
+    assert v.stride() != w.stride()
+    assert mixer._in_layout(w, v) is w and mixer._in_layout(v, w) is v
+    one = torch.zeros(1, 7, 64)
+    assert mixer._in_layout(torch.zeros(9, 7, 64)[:1], one) is not one  # (equal strides, another tensor)
+    odd = torch.empty_strided((1, 7, 64), (12345, 64, 1))
+    assert mixer._in_layout(odd, one) is odd
+    other = torch.zeros(2, 64, 7).transpose(1, 2)
+    assert mixer._in_layout(other, torch.zeros(2, 7, 64)) is not other
