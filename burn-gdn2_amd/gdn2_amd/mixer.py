@@ -20,6 +20,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _capi as C
+from .ops import _stream_of
 
 _SUFFIX = {torch.float32: "_f32", torch.bfloat16: "_bf16"}
 
@@ -40,11 +41,6 @@ def _device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
                 raise TypeError("gdn2_amd operators take device tensors")
             raise ValueError("the operands are on several devices")
     return index
-
-
-# torch.cuda.current_stream(i).cuda_stream without building the stream object
-# (0.1 against 2.9 us of a call's 10)
-_stream_of = torch._C._cuda_getCurrentRawStream
 
 
 def _call(fn, args, index: int) -> None:

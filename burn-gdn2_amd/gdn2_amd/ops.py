@@ -38,6 +38,13 @@ def _stream(stream=None):
     return ctypes.c_void_p(stream.cuda_stream)
 
 
+def _stream_of(index: int) -> int:
+    """torch.cuda.current_stream(index).cuda_stream, where torch has it without
+    building the stream object (0.1 against 2.9 us of a call's 10)."""
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return raw(index) if raw is not None else torch.cuda.current_stream(index).cuda_stream
+
+
 def _check_f32_cuda(*ts):
     for t in ts:
         if t is None:
@@ -417,10 +424,10 @@ def short_conv_1d_backward(x, weight, d_out, cache=None, d_cache=None, workspace
             None if dcache is None else dcache.data_ptr(), B, T, Cn, None if workspace is None else workspace.data_ptr(),
             0 if workspace is None else workspace.numel() * workspace.element_size())
     if torch.cuda.current_device() == index:
-        status = L.gdn2_short_conv_bwd_f32(*args, torch._C._cuda_getCurrentRawStream(index))
+        status = L.gdn2_short_conv_bwd_f32(*args, _stream_of(index))
     else:
         with torch.cuda.device(index):
-            status = L.gdn2_short_conv_bwd_f32(*args, torch._C._cuda_getCurrentRawStream(index))
+            status = L.gdn2_short_conv_bwd_f32(*args, _stream_of(index))
     if status:
         C.check(status)
     return {"dx": dx, "dweight": dweight, "dcache": dcache}

@@ -37,3 +37,21 @@ def test_strides_of_one_element_do_not_count():
     assert mixer._in_layout(odd, one) is odd
     other = torch.zeros(2, 64, 7).transpose(1, 2)
     assert mixer._in_layout(other, torch.zeros(2, 7, 64)) is not other
+
+
+def test_imports_without_torchs_private_names():
+    """A torch built without a GPU lacks some; the package imports all the same."""
+    import os
+    import subprocess
+    import sys
+
+    pytest.importorskip("torch")
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    code = ("import sys; sys.path.insert(0, 'burn-gdn2_amd')\n"
+            "import torch\n"
+            "for n in [n for n in dir(torch._C) if n.startswith('_cuda_')]:\n"
+            "    delattr(torch._C, n)\n"
+            "import gdn2_amd\n"
+            "assert gdn2_amd.gated_scan")
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
