@@ -161,6 +161,9 @@ def _scan_args(g, v, w, state, new_state, out, cu_seqlens, n):
                            H, T, V, n, g.shape[3] == 1, gb, gh, gt, vb, vh, vt, ob, oh, ot, None, 0)
 
 
+_WALK = 12  # tokens without offsets that never need a workspace (gdn2_mixer.h)
+
+
 def _channels(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
@@ -196,7 +199,7 @@ def gated_scan(g, v, w=None, state=None, cu_seqlens=None, out=None, new_state=No
     a = _scan_args(g, v, w, state, new_state, out, cu_seqlens, of_states[0])
     L = C.lib()
     keep = None
-    if v.shape[2] > 12 or cu_seqlens is not None:  # (up to 12 tokens never need a workspace)
+    if v.shape[2] > _WALK or cu_seqlens is not None:
         keep = _workspace(a, workspace, L.gdn2_gated_scan_workspace_bytes(a), v)
     _call(L.gdn2_gated_scan_fwd_f32 if v.dtype is torch.float32 else L.gdn2_gated_scan_fwd_bf16, a, index)
     del keep

@@ -48,8 +48,8 @@ extern "C" {
  * own state.  An empty sequence hands its state on.  Rows of out outside every
  * sequence are left as they were.  Offsets outside [0, seq_len] or decreasing
  * ones give unspecified results, never an access out of bounds.
- * workspace: gdn2_gated_scan_workspace_bytes(args) bytes (0 for short calls),
- * 256-byte aligned.
+ * workspace: gdn2_gated_scan_workspace_bytes(args) bytes, 256-byte aligned (0
+ * for up to 12 tokens without cu_seqlens).
  * Results do not depend on timing: the same call gives the same bits.
  * Limits (else GDN2_NOT_APPLICABLE): every size < 2^30, H V < 2^30, N H V and
  * B H seq_len < 2^32 - 256, and B H ceil(V / 32) ceil(seq_len / 64) < 2^24.

@@ -55,3 +55,16 @@ def test_imports_without_torchs_private_names():
             "assert gdn2_amd.gated_scan")
     r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_few_tokens_need_no_workspace():
+    """Up to mixer._WALK tokens the Python entry asks for none, at any size."""
+    from gdn2_amd import _capi as C, mixer
+
+    for T in (1, mixer._WALK, mixer._WALK + 1):
+        for B, H, V in ((1, 1, 1), (1, 16, 128), (64, 16, 128), (300, 16, 131)):
+            a = C.GatedScanArgs()
+            for k, v in dict(g=256, v=256, out=256, batch=B, num_heads=H, seq_len=T, head_v_dim=V).items():
+                setattr(a, k, v)
+            n = C.lib().gdn2_gated_scan_workspace_bytes(ctypes.byref(a))
+            assert n == 0 or T > mixer._WALK
