@@ -1099,6 +1099,12 @@ __global__ __launch_bounds__(NT) void norm_held_bwd_kernel(GroupNormParams p) {
     }
 }
 
+// The statistics of groups of nothing.
+__global__ __launch_bounds__(256) void norm_no_stats_kernel(float *stats, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i < n) stats[i] = NAN;
+}
+
 // -- host ---------------------------------------------------------------------
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
@@ -1361,7 +1367,15 @@ template <typename T> gdn2_status forward(const char *who, const gdn2_group_norm
     const gdn2_group_norm_args tidied = tidy(*args), *const a = &tidied;
     bool nothing, limits;
     if (const char *e = check(*a, &nothing, &limits)) return refuse(who, e, limits ? GDN2_NOT_APPLICABLE : GDN2_EINVAL);
-    if (nothing) return GDN2_OK;
+    if (nothing) {
+        if (!a->stats || a->samples == 0 || a->groups == 0) return GDN2_OK;
+        if (a->samples >= (1 << 24) || a->groups >= (1 << 24) || a->samples * a->groups >= (1 << 24))
+            return refuse(who, "sizes above the kernels' limits", GDN2_NOT_APPLICABLE);
+        const int64_t n = 2 * a->samples * a->groups;
+        hipLaunchKernelGGL(norm_no_stats_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, s, a->stats, n);
+        GDN2_HIP_CHECK(hipGetLastError());
+        return GDN2_OK;
+    }
     if (!a->x || !a->y) return refuse(who, "null tensor pointer");
     if (a->y == a->gate && (a->stride_gate_n != a->stride_x_n || a->stride_gate_s != a->stride_x_s))
         return refuse(who, "y may be gate only with x's strides");

@@ -119,7 +119,7 @@ GDN2_API gdn2_status gdn2_gated_scan_bwd_bf16(const gdn2_gated_scan_bwd_args *ar
  * and x share theirs.  y may be x, or gate where their strides are equal, and
  * must not overlap them otherwise.
  * stats [N, groups, 2] f32 contiguous, or NULL: mean and 1 / sqrt(var + eps),
- * what the backward takes.
+ * what the backward takes (NaN for groups of no rows or channels).
  * workspace: gdn2_group_norm_act_workspace_bytes(args) bytes (0 for S = 1 and
  * ordinary groups), 256-byte aligned.
  * Limits (else GDN2_NOT_APPLICABLE): C < 2^24, S < 2^30, N and N groups < 2^24.

@@ -63,3 +63,17 @@ def test_strides_of_one_element_do_not_count(gpu):
     want, last = G.gated_scan(g, v.contiguous(), w)
     r, want_r = (G.gated_scan_backward(g, v, w, out, d) for d in (torch.ones_like(out), torch.ones(2, 16, 1, 128, device=gpu)))
     assert torch.equal(out, want) and torch.equal(new, last) and all(torch.equal(r[n], want_r[n]) for n in r)
+
+
+def test_statistics_of_nothing(gpu):
+    """Groups of no rows have no mean: their statistics are NaN, not what the memory
+    held before."""
+    import torch
+
+    import gdn2_amd as G
+
+    for shape in ((4, 0, 64), (2, 0, 5, 64), (3, 5, 0), (7, 0)):
+        junk = [torch.full((n,), 7.0, device=gpu) for n in (128, 256, 512)]
+        del junk
+        y, stats = G.group_norm_act(torch.empty(shape, device=gpu), 4, return_stats=True)
+        assert y.shape == shape and stats.shape == (shape[0], 4, 2) and torch.isnan(stats).all()
