@@ -17,7 +17,8 @@
 // h + (expm1(g) h + u): the error of a rounded e^g, the same at every token, would
 // otherwise add up over the tokens that a slowly decaying state lives through.
 //
-// Tiles of one (row, CH channels) form a chain.  A tile publishes (G, X) once it
+// Tiles of one (row, CH channels) form a chain (a scan in a single pass, by decoupled
+// look-back).  A tile publishes (G, X) once it
 // is loaded, and its final state once it knows what enters it.  It looks at
 // several tiles before it at once, takes the nearest final state among them and
 // applies the (G, X) after it in order, which gives the same bits whichever of
@@ -27,11 +28,11 @@
 // finished, the one of the lowest number waits for none, so every wait ends.
 //
 // Bound: HBM, 16 bytes an element forward and 32 backward in f32.  (8 x 4096 x
-// 2048 f32, decays per channel: 1.07 GB in 193 us, 5.6 TB/s, where torch's
+// 2048 f32, decays per channel: 1.07 GB in 194 us, 5.5 TB/s, where torch's
 // elementwise kernel of three reads and a write reaches 5.8; backward of 4 x 2048
-// x 2048, 0.54 GB in 102 us, 5.3 TB/s.)  One packed row of bf16, decays
-// per head, has few chains, and long ones: 65536 tokens 218 us (3.7 TB/s), of which
-// waiting for the tiles before is 32; backward of 32767 181 us (4.5 TB/s), 9.
+// x 2048, 0.54 GB in 103 us, 5.2 TB/s.)  One packed row of bf16, decays
+// per head, has few chains, and long ones: 65536 tokens 219 us (3.7 TB/s), of which
+// waiting for the tiles before is 32; backward of 32767 187 us (4.3 TB/s), 9.
 // Prepare beside them is 3 to 6 us.
 #include <algorithm>
 #include <exception>
