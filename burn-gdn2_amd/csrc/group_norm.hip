@@ -349,6 +349,17 @@ __global__ __launch_bounds__(256) void column_sum_kernel(const float *part, int6
     }
 }
 
+// The mean of n values and their squares about it, from sums about a value near the
+// mean: what that one's roundings left (`rest`, sum d) and the squares (sum d^2).
+struct Moments {
+    float mean, squares;
+    __device__ Moments(float about, float rest, float squares_about, float n) {
+        mean = about + rest / n;
+        const float q = __builtin_fmaf(-rest, rest / n, squares_about);
+        squares = fmaxf(q, q - q); // (a NaN stays)
+    }
+};
+
 // A workgroup's tile of the general form: lc lanes of VEC channels, 256 / lc rows
 // at a time of a chunk of rows of sample n.
 template <int VEC> struct TileAt {
@@ -392,10 +403,10 @@ __device__ __forceinline__ void tile_pairs(const GroupNormParams &p, const TileA
 }
 
 // First pass, forward: the mean and the sum of squares about it of every channel
-// over the chunk's rows.  A thread takes kBatch rows at a time: their sum s and their
-// squares q about their own mean in 32 bits, the batches' sum q, sum s and sum s^2 / n
-// in 64, so that neither a large mean, nor a value far from the others, nor many rows
-// cost digits.
+// over the chunk's rows.  A thread takes kBatch rows at a time, less its first one's
+// value: their sum s and their squares q about their own mean in 32 bits, the batches'
+// sum q, sum s and sum s^2 / n in 64, so that neither a large mean, nor a first value
+// far from the others, nor many rows cost digits.
 constexpr int kBatch = 8;
 template <typename T, int VEC> __global__ __launch_bounds__(256) void norm_moments_kernel(GroupNormParams p) {
     const TileAt<VEC> at(p);
@@ -404,6 +415,8 @@ template <typename T, int VEC> __global__ __launch_bounds__(256) void norm_momen
     for (int j = 0; j < VEC; ++j) sum[j] = sq[j] = among[j] = 0.;
     const T *x = static_cast<const T *>(p.x) + at.n * p.sxn + at.c;
     int64_t row = at.s0 + at.rl, count = 0;
+    float first[VEC];
+    load_n<T, VEC>(x + min(row, at.s1 - 1) * p.sxs, first);
     auto batch = [&](auto rows) {
         constexpr int B = decltype(rows)::value;
         Raw<T, VEC> v[B];
@@ -413,10 +426,10 @@ template <typename T, int VEC> __global__ __launch_bounds__(256) void norm_momen
         for (int j = 0; j < VEC; ++j) {
             float s = 0.f, q = 0.f;
 #pragma unroll
-            for (int i = 0; i < B; ++i) s += (float)v[i][j];
+            for (int i = 0; i < B; ++i) s += (float)v[i][j] - first[j];
 #pragma unroll
             for (int i = 0; i < B; ++i) {
-                const float d = __builtin_fmaf(-s, 1.f / B, (float)v[i][j]);
+                const float d = __builtin_fmaf(-s, 1.f / B, (float)v[i][j] - first[j]);
                 q = __builtin_fmaf(d, d, q);
             }
             sum[j] += s;
@@ -433,7 +446,7 @@ template <typename T, int VEC> __global__ __launch_bounds__(256) void norm_momen
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         const double m = sum[j] * inv;
-        mean_of[j] = (float)m;
+        mean_of[j] = (float)(first[j] + m);
         sq_of[j] = (float)(sq[j] + fmax(__builtin_fma(-m, sum[j], among[j]), 0.)); // (a NaN is in the mean)
     }
     const int64_t total = at.s1 - at.s0;
@@ -444,14 +457,19 @@ template <typename T, int VEC> __global__ __launch_bounds__(256) void norm_momen
             const int64_t k = (total - r + at.rows - 1) / at.rows; // rows of thread r
             if (k > 0) s += (float)k * (m[r * p.lc + cl] - m[cl]);
         }
-        *mean = m[cl] + s / (float)total;
-        float t = 0.f;
+        const float about = m[cl] + s / (float)total;
+        float rest = 0.f, t = 0.f; // (see Moments)
         for (int r = 0; r < at.rows; ++r) {
             const int64_t k = (total - r + at.rows - 1) / at.rows;
-            const float d = m[r * p.lc + cl] - *mean;
-            if (k > 0) t += q[r * p.lc + cl] + (float)k * d * d;
+            const float d = m[r * p.lc + cl] - about;
+            if (k > 0) {
+                rest = __builtin_fmaf((float)k, d, rest);
+                t += q[r * p.lc + cl] + (float)k * d * d;
+            }
         }
-        *m2 = t;
+        const Moments of(about, rest, t, (float)total);
+        *mean = of.mean;
+        *m2 = of.squares;
     });
 }
 
@@ -472,44 +490,49 @@ __global__ __launch_bounds__(256) void norm_join_kernel(GroupNormParams p) {
     const int entries = (k1 - k0) * p.D;
     const float *part = p.part + (n * p.chunks + k0) * 2 * p.C + g * p.D;
     auto rows = [&](int k) { return (float)min((int64_t)p.chunk, p.S - (int64_t)(k0 + k) * p.chunk); };
+    const float base = part[0]; // a mean to sum about
     float s = 0.f;
 #pragma unroll 8
     for (int i = threadIdx.x; i < entries; i += 256) {
         const int k = i / p.D;
-        s = __builtin_fmaf(rows(k), part[(int64_t)k * 2 * p.C + i % p.D], s);
+        s = __builtin_fmaf(rows(k), part[(int64_t)k * 2 * p.C + i % p.D] - base, s);
     }
     const float size = (float)(min((int64_t)k1 * p.chunk, p.S) - (int64_t)k0 * p.chunk) * (float)p.D;
-    const float mean = block_sum(s, red) / size;
-    float t = 0.f;
+    const float about = base + block_sum(s, red) / size;
+    float rest = 0.f, t = 0.f;
 #pragma unroll 8
     for (int i = threadIdx.x; i < entries; i += 256) {
         const int k = i / p.D;
         const float *e = part + (int64_t)k * 2 * p.C + i % p.D;
-        const float d = e[0] - mean;
+        const float d = e[0] - about;
+        rest = __builtin_fmaf(rows(k), d, rest);
         t += e[p.C] + rows(k) * d * d;
     }
-    const float squares = block_sum(t, red);
+    rest = block_sum(rest, red);
+    const Moments of(about, rest, block_sum(t, red), size);
     if (threadIdx.x == 0) {
         float *out = p.spans > 1 ? p.joined + ((int64_t)blockIdx.x * p.spans + blockIdx.y) * 2 : p.stats + (int64_t)blockIdx.x * 2;
-        out[0] = mean;
-        out[1] = p.spans > 1 ? squares : 1.f / sqrtf(squares / size + p.eps);
+        out[0] = of.mean;
+        out[1] = p.spans > 1 ? of.squares : 1.f / sqrtf(of.squares / size + p.eps);
     }
 }
 // ... the spans of a group: a wave each.
 __global__ __launch_bounds__(64) void norm_join_spans_kernel(GroupNormParams p) {
     const float *e = p.joined + (int64_t)blockIdx.x * p.spans * 2;
     auto rows = [&](int k) { return (float)(min((int64_t)(k + 1) * p.span * p.chunk, p.S) - (int64_t)k * p.span * p.chunk); };
-    float s = 0.f, t = 0.f;
-    for (int k = threadIdx.x; k < p.spans; k += kWave) s = __builtin_fmaf(rows(k), e[2 * k], s);
-    const float mean = wave_sum(s) / (float)p.S;
+    const float base = e[0], size = (float)p.S * (float)p.D;
+    float s = 0.f, rest = 0.f, t = 0.f;
+    for (int k = threadIdx.x; k < p.spans; k += kWave) s = __builtin_fmaf(rows(k), e[2 * k] - base, s);
+    const float about = base + wave_sum(s) / (float)p.S;
     for (int k = threadIdx.x; k < p.spans; k += kWave) {
-        const float d = e[2 * k] - mean;
-        t += __builtin_fmaf(rows(k) * (float)p.D * d, d, e[2 * k + 1]);
+        const float d = e[2 * k] - about, n = rows(k) * (float)p.D;
+        rest = __builtin_fmaf(n, d, rest);
+        t += __builtin_fmaf(n * d, d, e[2 * k + 1]);
     }
-    const float squares = wave_sum(t);
+    const Moments of(about, wave_sum(rest), wave_sum(t), size);
     if (threadIdx.x == 0) {
-        p.stats[(int64_t)blockIdx.x * 2] = mean;
-        p.stats[(int64_t)blockIdx.x * 2 + 1] = 1.f / sqrtf(squares / ((float)p.S * (float)p.D) + p.eps);
+        p.stats[(int64_t)blockIdx.x * 2] = of.mean;
+        p.stats[(int64_t)blockIdx.x * 2 + 1] = 1.f / sqrtf(of.squares / size + p.eps);
     }
 }
 
@@ -831,7 +854,7 @@ __device__ __forceinline__ void collect(const GroupNormParams &p, const GroupLan
 
 template <typename T, int VEC, int E, bool GATE>
 __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
-    __shared__ float red[2][VEC * NT]; // sums, and squares about their mean, of a thread's channels
+    __shared__ float red[3][VEC * NT]; // a value, sums about it, and squares about their mean, of a thread's channels
     __shared__ float all[2][kMostWords], stat[2][kSet];
     __shared__ unsigned long long missing;
     const int tid = threadIdx.x;
@@ -856,38 +879,40 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) group[j] = p.tiles == 1 && at.ok ? (at.in_tile + j) / p.D : 0;
 
-    // The mean of a part and the squares about it.  A thread's are about its own mean,
-    // and joined about the part's: neither a large mean nor a value far from the others
-    // costs digits.
+    // The mean of a part and the squares about it.  A thread sums less its first value,
+    // its squares are about its own mean, and both are joined about the part's: neither
+    // a large mean nor a value far from the others costs digits.
     auto moments = [&](const Held<VEC, E> &h, auto at_once, auto value) { // value(i): the i-th row's; at_once: rows unrolled
         const int gc = min(p.D, h.channels(p)); // the tile's channels of a group
         auto rows_of = [&](int r) { return max(0, (h.count - r + h.rows - 1) / h.rows); }; // of a channel's r-th thread
         const int mine = h.ok ? rows_of(h.rl) : 0;
         const float inv = mine ? 1.f / mine : 0.f;
-        float s[VEC], q[VEC];
+        float base[VEC], s[VEC], q[VEC];
+        const Raw<T, VEC> v0 = value(0);
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) s[j] = q[j] = 0.f;
+        for (int j = 0; j < VEC; ++j) base[j] = (float)v0[j], s[j] = q[j] = 0.f;
         each_row<E>(at_once, [&](int i) {
             const Raw<T, VEC> v = value(i);
 #pragma unroll
-            for (int j = 0; j < VEC; ++j) s[j] += i < mine ? (float)v[j] : 0.f;
+            for (int j = 0; j < VEC; ++j) s[j] += i < mine ? (float)v[j] - base[j] : 0.f;
         });
         each_row<E>(at_once, [&](int i) {
             const Raw<T, VEC> v = value(i);
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float d = i < mine ? __builtin_fmaf(-s[j], inv, (float)v[j]) : 0.f;
+                const float d = i < mine ? __builtin_fmaf(-s[j], inv, (float)v[j] - base[j]) : 0.f;
                 q[j] = __builtin_fmaf(d, d, q[j]);
             }
         });
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            red[0][j * NT + tid] = s[j];
-            red[1][j * NT + tid] = q[j];
+            red[0][j * NT + tid] = base[j];
+            red[1][j * NT + tid] = s[j];
+            red[2][j * NT + tid] = q[j];
         }
         __syncthreads();
         // channel c of the tile is at c % VEC of lane c / VEC, for every row of threads:
-        // f(n, 1 / n, s, q, k) of those of them that hold rows, in four chains
+        // f(n, 1 / n, place, k) of those of them that hold rows, in four chains
         const int full = h.count / h.rows, more = h.count % h.rows; // rows of a thread; the first `more` have one more
         const int there = full ? h.rows : more;
         const float n0 = (float)full, n1 = (float)(full + 1), inv0 = 1.f / n0, inv1 = 1.f / n1;
@@ -896,7 +921,7 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
                 for (int c = gl.g * p.D + gl.t; c < gl.g * p.D + gc; c += gl.share) {
                     const int o = (c % VEC) * NT + c / VEC;
                     auto one = [&](int r, int k) {
-                        f(r < more ? n1 : n0, r < more ? inv1 : inv0, red[0][o + r * p.lc], red[1][o + r * p.lc], k);
+                        f(r < more ? n1 : n0, r < more ? inv1 : inv0, o + r * p.lc, k);
                     };
                     int r = 0;
                     for (; r + 4 <= there; r += 4)
@@ -905,16 +930,21 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
                     for (; r < there; ++r) one(r, 0);
                 }
         };
-        float t[4] = {0.f, 0.f, 0.f, 0.f};
-        each([&](float, float, float sum, float, int k) { t[k] += sum; });
-        const float mean = gl.sum((t[0] + t[1]) + (t[2] + t[3])) / ((float)h.count * (float)gc);
+        const float one = red[0][gl.g * p.D % VEC * NT + gl.g * p.D / VEC], size = (float)h.count * (float)gc;
+        float t[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+        each([&](float n, float, int at, int k) { t[k] += __builtin_fmaf(n, red[0][at] - one, red[1][at]); });
+        const float about = one + gl.sum((t[0] + t[1]) + (t[2] + t[3])) / size;
 #pragma unroll
         for (int k = 0; k < 4; ++k) t[k] = 0.f;
-        each([&](float n, float inv_n, float sum, float squares, int k) {
-            const float d = __builtin_fmaf(-mean, n, sum);
-            t[k] += __builtin_fmaf(d * d, inv_n, squares);
+        each([&](float n, float inv_n, int at, int k) {
+            const float d = __builtin_fmaf(n, red[0][at] - about, red[1][at]);
+            t[k] += d;
+            t[4 + k] += __builtin_fmaf(d * d, inv_n, red[2][at]);
         });
-        const float2 m = {mean, gl.sum((t[0] + t[1]) + (t[2] + t[3]))};
+        float two[2] = {(t[0] + t[1]) + (t[2] + t[3]), (t[4] + t[5]) + (t[6] + t[7])};
+        lanes_sum<2>(two, __builtin_ctz(gl.share));
+        const Moments of(about, two[0], two[1], size);
+        const float2 m = {of.mean, of.squares};
         __syncthreads(); // (red may be written again)
         return m;
     };
@@ -929,15 +959,19 @@ __global__ __launch_bounds__(NT) void norm_held_kernel(GroupNormParams p) {
         const int64_t rows = min((int64_t)p.chunk, p.S - (int64_t)(k / p.tiles) * p.chunk);
         return (float)rows * (float)(p.tiles == 1 ? p.D : min(p.tile, p.D - (k % p.tiles) * p.tile));
     };
-    // (a lane reads what it wrote itself)
-    float s = 0.f, q = 0.f;
-    for (int k = gl.t; gl.ok && k < at.parts; k += gl.share) s = __builtin_fmaf(size(k), means[k * ng + gl.g], s);
-    const float total = (float)p.S * (float)p.D, mean = gl.sum(s) / total;
+    // (a lane reads what it wrote itself; sums about part 0's mean, the same in every part)
+    const float one = __shfl(gl.t == 0 ? means[gl.g] : 0.f, 0, gl.share);
+    float s = 0.f, about[2] = {0.f, 0.f};
+    for (int k = gl.t; gl.ok && k < at.parts; k += gl.share) s = __builtin_fmaf(size(k), means[k * ng + gl.g] - one, s);
+    const float total = (float)p.S * (float)p.D, near = one + gl.sum(s) / total;
     for (int k = gl.t; gl.ok && k < at.parts; k += gl.share) {
-        const float d = means[k * ng + gl.g] - mean;
-        q += __builtin_fmaf(size(k) * d, d, squares[k * ng + gl.g]);
+        const float d = means[k * ng + gl.g] - near;
+        about[0] = __builtin_fmaf(size(k), d, about[0]);
+        about[1] += __builtin_fmaf(size(k) * d, d, squares[k * ng + gl.g]);
     }
-    const float rstd = 1.f / sqrtf(gl.sum(q) / total + p.eps);
+    lanes_sum<2>(about, __builtin_ctz(gl.share));
+    const Moments of(near, about[0], about[1], total);
+    const float mean = of.mean, rstd = 1.f / sqrtf(of.squares / total + p.eps);
     if (gl.ok && gl.t == 0) {
         stat[0][gl.g] = mean;
         stat[1][gl.g] = rstd;

@@ -45,6 +45,41 @@ def test_one_value_far_from_the_others(gpu, N, S, C, groups, ty, at):
     assert rel <= M.SUM * M.EPS, rel
 
 
+@pytest.mark.parametrize("inplace", [False, True])
+@pytest.mark.parametrize("N,S,C,groups", [(6, 1, 512, 2), (2, 50, 64, 4), (2, 4096, 64, 2), (8, 1000, 1024, 32), (1, 700, 33, 1),
+                                          (1, 600, 1500, 1), (1, 50000, 2048, 1), (1, 200000, 64, 2)])
+def test_large_means(gpu, N, S, C, groups, inplace):
+    """Values around 1000 that differ by 0.01, and constants: the mean is right to the
+    last digit that f32 has for it, and the variance of the values about it too.
+    Tolerance, of the mean: a step of 1000, 2^-14 (half of one is its own rounding).
+    Of the variance: those of the means m_r that are joined, off by d_r of half a step
+    at most, sum n_r (m_r + d_r - m)^2 / n - sum n_r (m_r - m)^2 / n
+    <= 2 (step / 2) sum n_r |m_r - m| / n + step^2 / 4 <= step sd + step^2 / 4 (the mean
+    magnitude of m_r - m is at most its root mean square, and that at most sd); and
+    SUM roundings.  Groups of one row sum the values themselves: their mean is off by
+    SUM roundings of 1000, as in test_gpu_group_norm's test_large_mean, and the variance
+    by the square of that."""
+    import torch
+
+    import gdn2_amd as G
+
+    step = 2.0 ** -14  # of values from 512 to 1024 (x stays below)
+    for spread in (0.0, 0.01):
+        r = torch.Generator(device=gpu).manual_seed(S + C)
+        x = 1000.1 + spread * torch.randn(N, S, C, generator=r, device=gpu).clamp(-5, 5)
+        var, mean = _stats64(x, groups)
+        y, stats = G.group_norm_act(x, groups, eps=EPS, activation="none", return_stats=True, out=x if inplace else None)
+        torch.cuda.synchronize()
+        off = (stats[..., 0] - mean).abs().max().item()
+        rel = (stats[..., 1].double() * torch.sqrt(var + EPS) - 1).abs().max().item()
+        print("mean off by", off / step, "steps, rstd by", rel, flush=True)
+        far = step if S > 1 else M.SUM * M.EPS * 1001
+        assert off <= far
+        extra = step * var.sqrt() + step ** 2 / 4 if S > 1 else far ** 2
+        bound = 0.5 * (extra / (var + EPS)).max().item() + M.SUM * M.EPS
+        assert rel <= bound, (rel, bound)
+
+
 # Sums of one sign: a serial f32 sum of n equal terms is off by up to n / 4 half steps
 # (its partial sums' roundings are all the same way within a power of two), one in
 # pieces by its longest chain's.  SUM_TERMS as in M.norm_bwd64; the terms are constants
