@@ -15,7 +15,7 @@
 //
 // Bound: HBM.  Rows: 32768 x 2048 bf16 gated 0.40 GB in 69.7 us (5.8 TB/s), the
 // adjoint of 8192 x 2048 f32 gated 0.34 GB in 62 (5.4).  Held groups: 8 x 4096 x
-// 1024 f32 in 32 groups 0.27 GB in 67 us (4.0 TB/s, the loads of a part and its
+// 1024 f32 in 32 groups 0.27 GB in 69 us (3.9 TB/s, the loads of a part and its
 // stores do not overlap) where three passes take 76; 4 x 1999 x 320 bf16, adjoint,
 // 15 MB in 22 us: three launches one after the other, the parts' exchange among them.
 #include <algorithm>
