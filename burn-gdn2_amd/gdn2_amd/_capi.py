@@ -82,6 +82,30 @@ class DecodeArgs(ctypes.Structure):
                 ("head_v_dim", _i64), ("scale", _dbl), ("params", ctypes.POINTER(LayerParams))]
 
 
+class Dropout(ctypes.Structure):
+    _fields_ = [("p", _dbl), ("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("rng", _fp)]
+
+
+class ResidualNormArgs(ctypes.Structure):
+    _fields_ = [("x", _fp), ("y", _fp), ("gate", _fp), ("post_weight", _fp), ("pre_weight", _fp),
+                ("out", _fp), ("normed", _fp), ("stats", _fp),
+                ("samples", _i64), ("rows", _i64), ("channels", _i64),
+                ("stride_x_n", _i64), ("stride_x_s", _i64), ("stride_y_n", _i64), ("stride_y_s", _i64),
+                ("stride_gate_n", _i64), ("stride_gate_s", _i64), ("stride_out_n", _i64), ("stride_out_s", _i64),
+                ("stride_normed_n", _i64), ("stride_normed_s", _i64),
+                ("eps", _dbl), ("residual_scale", _dbl), ("branch_scale", _dbl),
+                ("activation", ctypes.c_int32), ("gate_rows", ctypes.c_int32), ("dropout", Dropout)]
+
+
+class ResidualNormBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", ResidualNormArgs), ("d_out", _fp), ("d_normed", _fp), ("dx", _fp), ("dy", _fp), ("dgate", _fp),
+                ("dpost", _fp), ("dpre", _fp),
+                ("stride_d_out_n", _i64), ("stride_d_out_s", _i64), ("stride_d_normed_n", _i64),
+                ("stride_d_normed_s", _i64), ("stride_dx_n", _i64), ("stride_dx_s", _i64),
+                ("stride_dy_n", _i64), ("stride_dy_s", _i64), ("stride_dgate_n", _i64), ("stride_dgate_s", _i64),
+                ("workspace", _fp), ("workspace_bytes", ctypes.c_size_t)]
+
+
 class GatedScanArgs(ctypes.Structure):
     _fields_ = [("g", _fp), ("v", _fp), ("w", _fp), ("state_in", _fp), ("state_out", _fp), ("out", _fp),
                 ("cu_seqlens", _fp),
@@ -111,6 +135,8 @@ class GroupNormBwdArgs(ctypes.Structure):
 
 
 ACT_NONE, ACT_SILU, ACT_GELU = 0, 1, 2
+GATE_NONE, GATE_SILU, GATE_SIGMOID = 0, 1, 2  # gdn2_gate
+GATE_ROW, GATE_SAMPLE, GATE_ALL = 0, 1, 2  # gdn2_gate_rows
 
 
 class Config(ctypes.Structure):
@@ -140,7 +166,10 @@ EXPORTS = ("gdn2_last_error", "gdn2_hip_available", "gdn2_recurrent_step_f32", "
            "gdn2_gated_scan_bwd_workspace_bytes", "gdn2_gated_scan_bwd_f32", "gdn2_gated_scan_bwd_bf16",
            "gdn2_group_norm_act_workspace_bytes", "gdn2_group_norm_act_f32", "gdn2_group_norm_act_bf16",
            "gdn2_group_norm_act_bwd_workspace_bytes", "gdn2_group_norm_act_bwd_f32", "gdn2_group_norm_act_bwd_bf16",
-           "gdn2_group_norm_patience",
+           "gdn2_group_norm_patience", "gdn2_dropout_f32", "gdn2_dropout_bf16",
+           "gdn2_residual_norm_f32", "gdn2_residual_norm_bf16", "gdn2_residual_norm_f32_bf16",
+           "gdn2_residual_norm_bwd_workspace_bytes", "gdn2_residual_norm_bwd_f32", "gdn2_residual_norm_bwd_bf16",
+           "gdn2_residual_norm_bwd_f32_bf16",
            "gdn2_recurrent_bwd_f32", "gdn2_decode_fused_f32",
            "gdn2_config_default", "gdn2_config_validate", "gdn2_config_dims", "gdn2_param_count",
            "gdn2_param_name", "gdn2_param_shape", "gdn2_param_init", "gdn2_layer_create", "gdn2_layer_destroy",
@@ -208,6 +237,7 @@ def lib():
         L.gdn2_recurrent_bwd_workspace_bytes.argtypes = [ctypes.POINTER(RecurrentBwdArgs)]
         L.gdn2_recurrent_bwd_workspace_bytes.restype = ctypes.c_size_t
         _declare_mixer(L)
+        _declare_block(L)
         _declare_layer(L)
         _lib = L
     return _lib
@@ -224,6 +254,19 @@ def _declare_mixer(L):
             fn = getattr(L, entry + ty)
             fn.argtypes, fn.restype = [ctypes.POINTER(st), ctypes.c_void_p], ctypes.c_int
     L.gdn2_group_norm_patience.argtypes, L.gdn2_group_norm_patience.restype = [ctypes.c_int], ctypes.c_int
+
+
+def _declare_block(L):
+    vp = ctypes.c_void_p
+    for ty in ("_f32", "_bf16"):
+        fn = getattr(L, "gdn2_dropout" + ty)
+        fn.argtypes, fn.restype = [vp, vp] + [_i64] * 4 + [ctypes.POINTER(Dropout), vp], ctypes.c_int
+    for entry, st in (("gdn2_residual_norm", ResidualNormArgs), ("gdn2_residual_norm_bwd", ResidualNormBwdArgs)):
+        for ty in ("_f32", "_bf16", "_f32_bf16"):
+            fn = getattr(L, entry + ty)
+            fn.argtypes, fn.restype = [ctypes.POINTER(st), vp], ctypes.c_int
+    fn = L.gdn2_residual_norm_bwd_workspace_bytes
+    fn.argtypes, fn.restype = [ctypes.POINTER(ResidualNormBwdArgs)], ctypes.c_size_t
 
 
 def _declare_layer(L):
