@@ -106,6 +106,24 @@ class ResidualNormBwdArgs(ctypes.Structure):
                 ("workspace", _fp), ("workspace_bytes", ctypes.c_size_t)]
 
 
+class LowRankArgs(ctypes.Structure):
+    _fields_ = [("x", _fp), ("a", _fp), ("b", _fp), ("y", _fp), ("out", _fp), ("adapters", _fp), ("cu_seqlens", _fp),
+                ("scale", _fp), ("hidden", _fp),
+                ("batch", _i64), ("seq_len", _i64), ("in_features", _i64), ("out_features", _i64), ("rank", _i64),
+                ("num_adapters", _i64), ("num_seqs", _i64),
+                ("stride_x_b", _i64), ("stride_x_t", _i64), ("stride_y_b", _i64), ("stride_y_t", _i64),
+                ("stride_out_b", _i64), ("stride_out_t", _i64), ("stride_a_l", _i64), ("stride_a_r", _i64),
+                ("stride_b_l", _i64), ("stride_b_r", _i64),
+                ("workspace", _fp), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class LowRankBwdArgs(ctypes.Structure):
+    _fields_ = [("fwd", LowRankArgs), ("d_out", _fp), ("dx", _fp), ("da", _fp), ("db", _fp),
+                ("accumulate_dx", ctypes.c_int32),
+                ("stride_d_out_b", _i64), ("stride_d_out_t", _i64), ("stride_dx_b", _i64), ("stride_dx_t", _i64),
+                ("workspace", _fp), ("workspace_bytes", ctypes.c_size_t)]
+
+
 class GatedScanArgs(ctypes.Structure):
     _fields_ = [("g", _fp), ("v", _fp), ("w", _fp), ("state_in", _fp), ("state_out", _fp), ("out", _fp),
                 ("cu_seqlens", _fp),
@@ -169,7 +187,9 @@ EXPORTS = ("gdn2_last_error", "gdn2_hip_available", "gdn2_recurrent_step_f32", "
            "gdn2_group_norm_patience", "gdn2_dropout_f32", "gdn2_dropout_bf16",
            "gdn2_residual_norm_f32", "gdn2_residual_norm_bf16", "gdn2_residual_norm_f32_bf16",
            "gdn2_residual_norm_bwd_workspace_bytes", "gdn2_residual_norm_bwd_f32", "gdn2_residual_norm_bwd_bf16",
-           "gdn2_residual_norm_bwd_f32_bf16",
+           "gdn2_residual_norm_bwd_f32_bf16", "gdn2_low_rank_add_workspace_bytes", "gdn2_low_rank_add_f32",
+           "gdn2_low_rank_add_bf16", "gdn2_low_rank_add_bwd_workspace_bytes", "gdn2_low_rank_add_bwd_f32",
+           "gdn2_low_rank_add_bwd_bf16",
            "gdn2_recurrent_bwd_f32", "gdn2_decode_fused_f32",
            "gdn2_config_default", "gdn2_config_validate", "gdn2_config_dims", "gdn2_param_count",
            "gdn2_param_name", "gdn2_param_shape", "gdn2_param_init", "gdn2_layer_create", "gdn2_layer_destroy",
@@ -265,8 +285,14 @@ def _declare_block(L):
         for ty in ("_f32", "_bf16", "_f32_bf16"):
             fn = getattr(L, entry + ty)
             fn.argtypes, fn.restype = [ctypes.POINTER(st), vp], ctypes.c_int
-    fn = L.gdn2_residual_norm_bwd_workspace_bytes
-    fn.argtypes, fn.restype = [ctypes.POINTER(ResidualNormBwdArgs)], ctypes.c_size_t
+    for entry, st in (("gdn2_low_rank_add", LowRankArgs), ("gdn2_low_rank_add_bwd", LowRankBwdArgs)):
+        for ty in ("_f32", "_bf16"):
+            fn = getattr(L, entry + ty)
+            fn.argtypes, fn.restype = [ctypes.POINTER(st), vp], ctypes.c_int
+    for entry, st in (("gdn2_residual_norm_bwd", ResidualNormBwdArgs), ("gdn2_low_rank_add", LowRankArgs),
+                      ("gdn2_low_rank_add_bwd", LowRankBwdArgs)):
+        fn = getattr(L, entry + "_workspace_bytes")
+        fn.argtypes, fn.restype = [ctypes.POINTER(st)], ctypes.c_size_t
 
 
 def _declare_layer(L):

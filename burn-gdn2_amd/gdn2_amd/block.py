@@ -6,6 +6,8 @@ ABI of include/gdn2_block.h (no reference counterpart):
   residual_norm, residual_norm_backward  the norm behind a block, its gate, dropout,
                                          the scaled residual and the norm before the
                                          next block
+  low_rank_add, low_rank_add_backward    every request's own low-rank adapter beside a
+                                         projection that all of them share
 
 Tensors as in mixer.py: any strides with contiguous channels (others are copied),
 float32 or bfloat16; weights, statistics and the weights' gradients are float32.  A
@@ -325,3 +327,117 @@ def residual_norm_backward(out, y, stats, d_out=None, d_normed=None, gate=None, 
             if t is not None:
                 t.zero_()
     return {"dx": _seen(dx, shape), "dy": _seen(dy, shape), "dgate": _seen(dgate, gate_shape), "dpost": dpost, "dpre": dpre}
+
+
+# -- low-rank adapters ----------------------------------------------------------------
+
+def _adapters_check(x, a, b, adapters, scale, cu_seqlens, others) -> None:
+    """The checks of both directions.  others: (name, tensor, channels, type)."""
+    ty, shape = x.dtype, x.shape
+    if len(shape) not in (2, 3):
+        raise ValueError("x must be [N, D] or [B, T, D]")
+    if ty not in _SUFFIX:
+        raise TypeError("x must be float32 or bfloat16")
+    for name, t, ch in (("a", a, shape[-1]), ("b", b, None)):
+        if t.dtype is not ty:
+            raise TypeError(f"{name} must have x's type")
+        if t.dim() != 3 or ch is not None and t.shape[2] != ch:
+            raise ValueError(f"{name} must be [L, R, {'D' if ch is not None else 'O'}]")
+    if a.shape[:2] != b.shape[:2]:
+        raise ValueError("a and b must have the same adapters and ranks")
+    for name, t, ch, dtype in others:
+        if t is not None:
+            if t.dtype is not dtype:
+                raise TypeError(f"{name} must be {dtype}")
+            if t.shape != (*shape[:-1], ch):
+                raise ValueError(f"{name} must be {tuple((*shape[:-1], ch))}")
+    n = shape[0]
+    if cu_seqlens is not None:
+        if cu_seqlens.dtype is not torch.int32 or cu_seqlens.dim() != 1 or not cu_seqlens.is_contiguous():
+            raise TypeError("cu_seqlens must be a contiguous int32 vector")
+        if len(shape) != 3 or n != 1:
+            raise ValueError("packed requests need a batch of 1")
+        n = cu_seqlens.shape[0] - 1
+        if n < 0:
+            raise ValueError("cu_seqlens needs at least one offset")
+    if adapters.dtype is not torch.int32 or not adapters.is_contiguous():
+        raise TypeError("adapters must be a contiguous int32 vector")
+    if adapters.shape != (n,):
+        raise ValueError(f"adapters must be [{n}], one of each request")
+    if scale is not None:
+        if scale.dtype is not torch.float32:
+            raise TypeError("scale must be float32")
+        if scale.shape != a.shape[:1]:
+            raise ValueError("scale must be [L]")
+
+
+def _rowed(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _bt(t: Optional[torch.Tensor]) -> Tuple[int, int]:
+    """The strides of batch and token ([N, D]: a token each)."""
+    if t is None:
+        return 0, 0
+    s = t.stride()
+    return (s[0], s[1]) if len(s) == 3 else (s[0], 0)
+
+
+def _low_rank_args(x, a, b, y, out, adapters, scale, cu_seqlens, hidden):
+    B, T = x.shape[0], x.shape[1] if x.dim() == 3 else 1
+    L, R, D = a.shape
+    return C.LowRankArgs(_p(x), _p(a), _p(b), _p(y), _p(out), _p(adapters), _p(cu_seqlens), _p(scale), _p(hidden), B, T, D,
+                         b.shape[2], R, L, 0 if cu_seqlens is None else cu_seqlens.shape[0] - 1, *_bt(x), *_bt(y), *_bt(out),
+                         a.stride(0), a.stride(1), b.stride(0), b.stride(1), None, 0)
+
+
+def low_rank_add(y, x, a, b, adapters, scale=None, cu_seqlens=None, return_hidden: bool = False, out=None, workspace=None):
+    """y + scale_l (x a_l^T) b_l, with l the adapter of each row's request: what the
+    low-rank adapters of many requests add to the output y of a projection that they
+    share.
+
+    x [B, T, D] (or [N, D], a token each), y [B, T, O]; a [L, R, D], b [L, R, O]: the
+    adapters' vectors, rank by rank (an adapter of fewer ranks is padded with zeros).
+    adapters: int32 on the device, one of each request; outside [0, L) none, and the
+    row is y's.  scale [L] or None (1).  The requests are the batch entries, or with
+    cu_seqlens (int32 on the device, N + 1 token offsets) runs of the one row; rows
+    outside all of them have no adapter.  x a_l^T is not rounded to x's type on its way.
+    With return_hidden also it, [B, T, R] float32 (0 without an adapter), which the
+    backward takes.  `out` takes the result where given (it may be y)."""
+    _adapters_check(x, a, b, adapters, scale, cu_seqlens, (("y", y, b.shape[2], x.dtype),))
+    if out is not None:
+        _takes("out", out, y, x.dtype, y, (x, a, b, adapters, scale, cu_seqlens))
+    index = _device(x, y, a, b, adapters, scale, cu_seqlens, out)
+    x, y, a, b, scale = _rowed(x), _rowed(y), _rowed(a), _rowed(b), _contig(scale)
+    o = _new(y) if out is None else out
+    hidden = x.new_empty((*x.shape[:-1], a.shape[1]), dtype=torch.float32) if return_hidden else None
+    if x.shape[:-1].numel():
+        args = _low_rank_args(x, a, b, y, o, adapters, scale, cu_seqlens, hidden)
+        L = C.lib()
+        keep = _workspace(args, workspace, L.gdn2_low_rank_add_workspace_bytes(args), x)
+        _call(L.gdn2_low_rank_add_f32 if x.dtype is torch.float32 else L.gdn2_low_rank_add_bf16, args, index)
+        del keep
+    return (o, hidden) if return_hidden else o
+
+
+def low_rank_add_backward(x, a, b, adapters, hidden, d_out, scale=None, cu_seqlens=None, dx=None, workspace=None) -> dict:
+    """The gradients of <d_out, low_rank_add(y, x, ...)> for its arguments and the hidden
+    it returned (y's is d_out itself): dict dx (0 in rows without an adapter; where a
+    `dx` is given, the shared projection's gradient of x, it is added to that, in place),
+    da [L, R, D] and db [L, R, O] in float32."""
+    _adapters_check(x, a, b, adapters, scale, cu_seqlens,
+                    (("d_out", d_out, b.shape[2], x.dtype), ("hidden", hidden, a.shape[1], torch.float32)))
+    if dx is not None:
+        _takes("dx", dx, x, x.dtype, None, (x, a, b, adapters, hidden, d_out, scale, cu_seqlens))
+    index = _device(x, a, b, adapters, hidden, d_out, scale, cu_seqlens, dx)
+    x, a, b, d_out, scale, hidden = _rowed(x), _rowed(a), _rowed(b), _rowed(d_out), _contig(scale), hidden.contiguous()
+    into = _new(x) if dx is None else dx
+    da, db = (torch.empty(t.shape, dtype=torch.float32, device=t.device) for t in (a, b))
+    if x.shape[:-1].numel() or da.numel() or db.numel():
+        args = C.LowRankBwdArgs(_low_rank_args(x, a, b, None, None, adapters, scale, cu_seqlens, hidden), _p(d_out), _p(into),
+                                _p(da), _p(db), dx is not None, *_bt(d_out), *_bt(into), None, 0)
+        L = C.lib()
+        keep = _workspace(args, workspace, L.gdn2_low_rank_add_bwd_workspace_bytes(args), x)
+        _call(L.gdn2_low_rank_add_bwd_f32 if x.dtype is torch.float32 else L.gdn2_low_rank_add_bwd_bf16, args, index)
+        del keep
+    return {"dx": into, "da": da, "db": db}

@@ -140,6 +140,72 @@ GDN2_API gdn2_status gdn2_residual_norm_bwd_f32(const gdn2_residual_norm_bwd_arg
 GDN2_API gdn2_status gdn2_residual_norm_bwd_bf16(const gdn2_residual_norm_bwd_args *args, gdn2_stream_t stream);
 GDN2_API gdn2_status gdn2_residual_norm_bwd_f32_bf16(const gdn2_residual_norm_bwd_args *args, gdn2_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside a projection that they share: for
+ * every row x of a request with adapter l
+ *   h = x a_l^T,  out = y + scale_l h b_l
+ * x        [B, T, D];  y, out [B, T, O] (y: the shared projection's output)
+ * a        [L, R, D];  b [L, R, O]: each rank's vectors contiguous
+ * adapters device, int32, one of each request; outside [0, L): none, and out = y
+ * scale    [L], or NULL (1)
+ * hidden   [B, T, R] contiguous f32, or NULL: h (0 without an adapter), which the
+ *          backward takes.  h is not rounded on its way to b.
+ * Without cu_seqlens the requests are the batch entries.  With cu_seqlens (device,
+ * int32, num_seqs + 1 token offsets, not decreasing) batch must be 1, and request n
+ * is tokens cu_seqlens[n] .. cu_seqlens[n + 1] - 1 of the one row; rows outside all
+ * of them have no adapter.  Offsets outside [0, T] or decreasing ones give
+ * unspecified results, never an access out of bounds.
+ * out may be y with the same strides, nothing else may overlap.
+ * workspace: gdn2_low_rank_add_workspace_bytes(args) bytes, 256-byte aligned.
+ * Limits (else GDN2_NOT_APPLICABLE): R <= 512; D, O, L, num_seqs < 2^24; B T < 2^30;
+ * B T O < 2^36 for long requests, less for short ones.
+ * ---------------------------------------------------------------------- */
+typedef struct gdn2_low_rank_args {
+    const void *x, *a, *b, *y;
+    void *out;
+    const int32_t *adapters, *cu_seqlens;
+    const float *scale;
+    float *hidden;
+    int64_t batch, seq_len, in_features, out_features, rank, num_adapters, num_seqs;
+    int64_t stride_x_b, stride_x_t;
+    int64_t stride_y_b, stride_y_t;
+    int64_t stride_out_b, stride_out_t;
+    int64_t stride_a_l, stride_a_r;
+    int64_t stride_b_l, stride_b_r;
+    void *workspace;
+    size_t workspace_bytes;
+} gdn2_low_rank_args;
+
+GDN2_API size_t gdn2_low_rank_add_workspace_bytes(const gdn2_low_rank_args *args);
+GDN2_API gdn2_status gdn2_low_rank_add_f32(const gdn2_low_rank_args *args, gdn2_stream_t stream);
+GDN2_API gdn2_status gdn2_low_rank_add_bf16(const gdn2_low_rank_args *args, gdn2_stream_t stream);
+
+/* The gradients of L = <d_out, out> of that call (y's is d_out itself):
+ *   dh = scale_l d_out b_l^T,  dx = dh a_l,  da_l = sum dh^T x,  db_l = scale_l sum h^T d_out
+ *   fwd    its arguments, with hidden as it wrote it; y, out and workspace unused
+ *   d_out  [B, T, O];  dx [B, T, D], or NULL (not wanted).  Rows without an adapter: 0.
+ *          accumulate_dx: added to what dx holds (the shared projection's gradient)
+ *   da     [L, R, D], db [L, R, O] f32 contiguous, either NULL (not wanted): sums over
+ *          all rows of an adapter's requests, 0 for one without any; in a fixed order,
+ *          in f32 over at most 4096 rows, those in f64
+ * Nothing may overlap.
+ * workspace: gdn2_low_rank_add_bwd_workspace_bytes(args) bytes, 256-byte aligned. */
+typedef struct gdn2_low_rank_bwd_args {
+    gdn2_low_rank_args fwd;
+    const void *d_out;
+    void *dx;
+    float *da, *db;
+    int32_t accumulate_dx;
+    int64_t stride_d_out_b, stride_d_out_t;
+    int64_t stride_dx_b, stride_dx_t;
+    void *workspace;
+    size_t workspace_bytes;
+} gdn2_low_rank_bwd_args;
+
+GDN2_API size_t gdn2_low_rank_add_bwd_workspace_bytes(const gdn2_low_rank_bwd_args *args);
+GDN2_API gdn2_status gdn2_low_rank_add_bwd_f32(const gdn2_low_rank_bwd_args *args, gdn2_stream_t stream);
+GDN2_API gdn2_status gdn2_low_rank_add_bwd_bf16(const gdn2_low_rank_bwd_args *args, gdn2_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -127,3 +127,63 @@ def near(got, want, err, what=""):
     off = (got64 - want).abs()
     bad = ~(off <= bound)
     assert not bad.any(), (what, int(bad.sum()), float(off[bad].max()), float((off / bound.clamp_min(1e-300))[bad].max()))
+
+
+def requests(B, T, cu):
+    """(first row, behind the last) of each request among all rows."""
+    return [(i * T, (i + 1) * T) for i in range(B)] if cu is None else list(zip(cu, cu[1:]))
+
+
+def low_rank64(y, x, a, b, ids, scale, B, T, cu=None):
+    """(out, h), both with the errors of f32 sums: a sum of n products is off by at most n
+    half steps of the terms' magnitudes (however it is arranged, exact products, fewer
+    joins than terms), the product with the scale and the last sum by three."""
+    M, L, R, D = x.shape[0], *a.shape
+    out, h = y.clone(), torch.zeros(M, R, dtype=F64)
+    err, h_err = torch.zeros_like(y), torch.zeros_like(h)
+    for n, (r0, r1) in enumerate(requests(B, T, cu)):
+        l = int(ids[n])
+        if not 0 <= l < L or r1 <= r0:
+            continue
+        s = float(scale[l]) if scale is not None else 1.0
+        at = slice(r0, r1)
+        h[at] = x[at] @ a[l].t()
+        h_err[at] = (D + 8) * U * (x[at].abs() @ a[l].abs().t())
+        e = s * (h[at] @ b[l])
+        out[at] = y[at] + e
+        err[at] = abs(s) * (h_err[at] @ b[l].abs() + (R + 2) * U * (h[at].abs() @ b[l].abs())) + U * out[at].abs()
+    return (out, h), (err, h_err)
+
+
+def low_rank_bwd64(x, a, b, ids, hidden, dy, scale, B, T, cu=None, dx=None):
+    M, L, R, D = x.shape[0], *a.shape
+    O = b.shape[2]
+    g = {"dx": torch.zeros_like(x) if dx is None else dx.clone(), "da": torch.zeros_like(a), "db": torch.zeros_like(b)}
+    e = {k: torch.zeros_like(v) for k, v in g.items()}
+    for n, (r0, r1) in enumerate(requests(B, T, cu)):
+        l = int(ids[n])
+        if not 0 <= l < L or r1 <= r0:
+            continue
+        s = float(scale[l]) if scale is not None else 1.0
+        at, rows = slice(r0, r1), r1 - r0
+        dh = s * (dy[at] @ b[l].t())
+        dh_err = (O + 9) * U * abs(s) * (dy[at].abs() @ b[l].abs().t())
+        g["dx"][at] += dh @ a[l]
+        e["dx"][at] = dh_err @ a[l].abs() + (R + 2) * U * (dh.abs() @ a[l].abs()) + U * g["dx"][at].abs()
+        g["da"][l] += dh.t() @ x[at]
+        e["da"][l] += dh_err.t() @ x[at].abs() + (min(rows, 4096) + 4) * U * (dh.abs().t() @ x[at].abs())
+        g["db"][l] += s * (hidden[at].t() @ dy[at])
+        e["db"][l] += (min(rows, 4096) + 4) * U * abs(s) * (hidden[at].abs().t() @ dy[at].abs())
+    return g, e
+
+
+def alike(got, want, what=""):
+    """All of got as one vector: its error against want's length.  The roundings of sums
+    have either sign, so that n of them come to about the square root of n half steps of
+    sums like the result: 32 of them stand for 1024 terms' sums in two products one after
+    the other; a result's own rounding is at most half a step, and of many results
+    (uniform in it, and half a step at most of each value) 1/sqrt(3) of that."""
+    off = float((got.detach().cpu().double().reshape(want.shape) - want).norm())
+    size = float(want.norm())
+    half = HALF[got.dtype] / (3 ** 0.5 if got.numel() >= 1000 else 1)  # (one result's is half a step, whatever the others')
+    assert off <= (2 * 32 * U + half) * size, (what, off / max(size, 1e-300))

@@ -193,3 +193,106 @@ def test_results_that_share_memory_are_refused():
             G.residual_norm(x, y, gate, **kw)
     with pytest.raises(ValueError):
         G.dropout(x, 0.5, out=buf[:, 1:9])
+
+
+def test_low_rank_gradients_against_differences():
+    g = torch.Generator().manual_seed(8)
+    rnd = lambda *s: torch.randn(*s, generator=g, dtype=K.F64)  # noqa: E731
+    t = {"x": rnd(7, 3), "a": rnd(2, 2, 3), "b": rnd(2, 2, 4)}
+    y, dy, ids, scale, cu = rnd(7, 4), rnd(7, 4), [1, 0, 1, -1], [0.7, 1.3], [1, 3, 3, 5, 6]
+    loss = lambda t: float((K.low_rank64(y, t["x"], t["a"], t["b"], ids, scale, 1, 7, cu)[0][0] * dy).sum())  # noqa: E731
+    h = K.low_rank64(y, t["x"], t["a"], t["b"], ids, scale, 1, 7, cu)[0][1]
+    got = K.low_rank_bwd64(t["x"], t["a"], t["b"], ids, h, dy, scale, 1, 7, cu)[0]
+    for name, v in t.items():
+        for i in np.ndindex(*v.shape):
+            lo, hi = dict(t, **{name: v.clone()}), dict(t, **{name: v.clone()})
+            lo[name][i] -= 1e-6
+            hi[name][i] += 1e-6
+            d = (loss(hi) - loss(lo)) / 2e-6
+            assert abs(d - float(got["d" + name][i])) <= 1e-7 * (1 + abs(d)), (name, i)
+
+
+def _lora(**kw):
+    from gdn2_amd import _capi as C
+
+    a = C.LowRankArgs()
+    for k, v in dict(dict(x=256, a=256, b=256, y=256, out=512, adapters=256, batch=2, seq_len=3, in_features=8, out_features=8,
+                          rank=2, num_adapters=2, workspace=256, workspace_bytes=1 << 30), **kw).items():
+        setattr(a, k, v)
+    return a
+
+
+def test_low_rank_refusals_of_the_c_entry():
+    from gdn2_amd import _capi as C
+
+    L = C.lib()
+    for fn in (L.gdn2_low_rank_add_f32, L.gdn2_low_rank_add_bf16):
+        assert fn(None, None) == C.GDN2_EINVAL
+        for bad in (dict(batch=-1), dict(seq_len=-1), dict(in_features=-1), dict(out_features=-1), dict(rank=-1), dict(num_adapters=-1),
+                    dict(x=None), dict(a=None), dict(b=None), dict(y=None), dict(out=None), dict(adapters=None),
+                    dict(cu_seqlens=256, num_seqs=1), dict(cu_seqlens=256, batch=1, num_seqs=-1), dict(workspace=None),
+                    dict(workspace=264), dict(workspace_bytes=8), dict(out=256, stride_out_t=8)):
+            assert fn(_lora(**bad), None) == C.GDN2_EINVAL, bad
+            assert b"gdn2_low_rank_add" in L.gdn2_last_error()
+        for big in (dict(rank=513), dict(in_features=1 << 24), dict(out_features=1 << 24), dict(batch=1 << 20, seq_len=1 << 20),
+                    dict(num_adapters=1 << 24), dict(batch=1 << 24, seq_len=1), dict(seq_len=1 << 29, out_features=1 << 20)):
+            assert fn(_lora(**big), None) == C.GDN2_NOT_APPLICABLE, big
+        for nothing in (dict(batch=0), dict(seq_len=0), dict(out_features=0)):
+            assert fn(_lora(**nothing), None) == C.GDN2_OK
+    for fn in (L.gdn2_low_rank_add_bwd_f32, L.gdn2_low_rank_add_bwd_bf16):
+        assert fn(None, None) == C.GDN2_EINVAL
+
+        def bwd(fwd={}, **kw):
+            b = C.LowRankBwdArgs()
+            b.fwd = _lora(hidden=256, **fwd)
+            for k, v in dict(dict(d_out=256, dx=256, da=256, db=256, workspace=256, workspace_bytes=1 << 30), **kw).items():
+                setattr(b, k, v)
+            return fn(ctypes.byref(b), None)
+
+        for fwd, kw in ((dict(rank=-1), {}), (dict(x=None), {}), (dict(a=None), {}), (dict(b=None), {}), (dict(adapters=None), {}),
+                        ({}, dict(d_out=None)), ({}, dict(workspace=None)), ({}, dict(workspace=264)), ({}, dict(workspace_bytes=8))):
+            assert bwd(fwd, **kw) == C.GDN2_EINVAL, (fwd, kw)
+        b = C.LowRankBwdArgs(_lora(), 256, 256, 256, 256, 0, 0, 0, 0, 0, 256, 1 << 30)  # hidden missing
+        assert fn(b, None) == C.GDN2_EINVAL
+        assert bwd(dict(rank=513)) == C.GDN2_NOT_APPLICABLE
+
+
+def test_low_rank_workspace_sizes():
+    from gdn2_amd import _capi as C
+
+    L = C.lib()
+    size = lambda **kw: L.gdn2_low_rank_add_workspace_bytes(_lora(**kw))  # noqa: E731
+    assert L.gdn2_low_rank_add_workspace_bytes(None) == L.gdn2_low_rank_add_bwd_workspace_bytes(None) == 0
+    assert size(batch=0) == size(rank=0) == size(rank=513) == size(seq_len=-1) == 0
+    # h alone where the wide dimension is not shared: none, where the caller takes h
+    assert size(batch=8, seq_len=4096, in_features=2048) == 4 * 8 * 4096 * 2 and size(batch=8, seq_len=4096, in_features=2048, hidden=256) == 0
+    assert size(batch=64, seq_len=1, in_features=2048, rank=16) == 8 * 4 * 64 * 16
+
+
+def test_low_rank_refusals_in_python():
+    import gdn2_amd as G
+
+    x, y, a, b = torch.zeros(2, 3, 8), torch.zeros(2, 3, 6), torch.zeros(4, 2, 8), torch.zeros(4, 2, 6)
+    ids, sc, cu = torch.zeros(2, dtype=torch.int32), torch.zeros(4), torch.tensor([0, 2, 3], dtype=torch.int32)
+    h, w = torch.zeros(2, 3, 2), torch.zeros(2, 3, 14)
+    for err, args, kw in [
+        (TypeError, (y, x, a, b, ids), {}),  # not on a device
+        (TypeError, (y.half(), x.half(), a.half(), b.half(), ids), {}), (TypeError, (y, x, a.bfloat16(), b, ids), {}),
+        (TypeError, (y.bfloat16(), x, a, b, ids), {}), (ValueError, (y, x[0, 0], a, b, ids), {}), (ValueError, (y, x, a[0], b, ids), {}),
+        (ValueError, (y, x, a[..., :4], b, ids), {}), (ValueError, (y, x, a[:, :1], b, ids), {}), (ValueError, (y, x, a[:2], b, ids), {}),
+        (ValueError, (y[:1], x, a, b, ids), {}), (ValueError, (y, x, a, b[..., :5], ids), {}), (TypeError, (y, x, a, b, ids.long()), {}),
+        (ValueError, (y, x, a, b, ids[:1]), {}), (TypeError, (y, x, a, b, ids, sc.double()), {}), (ValueError, (y, x, a, b, ids, sc[:2]), {}),
+        (ValueError, (y, x, a, b, ids), dict(cu_seqlens=cu)), (TypeError, (y[:1], x[:1], a, b, ids), dict(cu_seqlens=cu.long())),
+        (ValueError, (y[:1], x[:1], a, b, ids), dict(cu_seqlens=cu[:0])), (ValueError, (y[:1], x[:1], a, b, ids), dict(cu_seqlens=cu[:2])),
+        (ValueError, (y, x, a, b, ids), dict(out=y[..., :5])), (TypeError, (y, x, a, b, ids), dict(out=y.bfloat16())),
+        (ValueError, (w[..., 8:], w[..., :8], a, b, ids), dict(out=w[..., 2:8])),
+        (ValueError, (y, x, a, b, ids), dict(out=torch.zeros(6).expand(2, 3, 6))),
+    ]:
+        with pytest.raises(err):
+            G.low_rank_add(*args, **kw)
+    for err, args, kw in [
+        (TypeError, (x, a, b, ids, h, y), {}), (ValueError, (x, a, b, ids, h[..., :1], y), {}), (TypeError, (x, a, b, ids, h.bfloat16(), y), {}),
+        (ValueError, (x, a, b, ids, h, x), {}), (ValueError, (x, a, b, ids, h, y), dict(dx=x)), (ValueError, (x, a, b, ids, h, y), dict(dx=y)),
+    ]:
+        with pytest.raises(err):
+            G.low_rank_add_backward(*args, **kw)
