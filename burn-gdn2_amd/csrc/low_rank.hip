@@ -4,8 +4,8 @@
 //   dh = s_l dy b_l^T,  dx = dh a_l,  da_l = sum dh^T x,  db_l = s_l sum h^T dy
 //
 // Four kernels, each of which streams one wide tensor past matrix instructions:
-//   shrink  h or dh: rows of 16 MT by all ranks, the wide dimension split over the waves
-//           of a workgroup and over KS workgroups
+//   shrink  h or dh: rows of 16 MT by all ranks, the wide dimension split over the 4 or
+//           16 waves of a workgroup
 //   expand  out or dx: rows of 16 MT by 16 VC columns a wave, y read and out written once
 //   outer   da, db: ranks by 16 VC columns a wave, a block of one request's rows
 //   sums    those of an adapter's blocks, in order, in f64
@@ -167,20 +167,21 @@ struct ShrinkParams {
     Requests req;
     const void *x, *w; // [.., K]; [L, R, K]
     const float *scale;
-    float *h; // [KS][M][R]
+    float *h; // [M][P], zeros behind rank R
     int64_t xb, xt, wl, wr;
     int64_t K;
-    int R, KS;
+    int R, P;
 };
 
-template <typename T, int MT, int NR> __global__ __launch_bounds__(256) void shrink_kernel(ShrinkParams p) {
+template <typename T, int MT, int NR, int W> __global__ __launch_bounds__(64 * W) void shrink_kernel(ShrinkParams p) {
     typedef Mm<T> X;
-    constexpr int KV = X::KV, STEP = 4 * KV, CHUNK = 4 * STEP;
-    __shared__ floatx4 red[2][MT * NR][kWave];
+    constexpr int KV = X::KV, STEP = 4 * KV, U = 2, CHUNK = U * STEP;
+    constexpr bool AHEAD = W == 4; // the next chunk's loads in flight (16 waves overlap one another's)
+    __shared__ floatx4 red[W / 2][MT * NR][kWave];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
-    const int tile = blockIdx.x / p.KS, ks = blockIdx.x - tile * p.KS, r0 = blockIdx.y * NR * 16;
-    const Tile at = tile_at(p.req, tile, MT * 16);
+    const int r0 = blockIdx.y * NR * 16;
+    const Tile at = tile_at(p.req, blockIdx.x, MT * 16);
     if (at.rows <= 0) return;
     floatx4 acc[MT][NR];
 #pragma unroll
@@ -196,41 +197,51 @@ template <typename T, int MT, int NR> __global__ __launch_bounds__(256) void shr
 #pragma unroll
         for (int n = 0; n < NR; ++n)
             w[n] = static_cast<const T *>(p.w) + at.adapter * p.wl + min(r0 + 16 * n + i, p.R - 1) * p.wr + KV * g;
-        for (int64_t k0 = (int64_t)(ks * 4 + wave) * CHUNK; k0 < p.K; k0 += (int64_t)p.KS * 4 * CHUNK) {
-            if (k0 + CHUNK <= p.K) {
-                typename X::Op a[4][MT], b[4][NR];
+        typename X::Op a[U][MT], b[U][NR];
+        auto load = [&](int64_t k) {
 #pragma unroll
-                for (int s = 0; s < 4; ++s) {
+            for (int s = 0; s < U; ++s) {
 #pragma unroll
-                    for (int m = 0; m < MT; ++m) a[s][m] = loose<T, KV>(x[m] + k0 + s * STEP);
+                for (int m = 0; m < MT; ++m) a[s][m] = loose<T, KV>(x[m] + k + s * STEP);
 #pragma unroll
-                    for (int n = 0; n < NR; ++n) b[s][n] = loose<T, KV>(w[n] + k0 + s * STEP);
-                }
-#pragma unroll
-                for (int s = 0; s < 4; ++s)
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll
-                        for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a[s][m], b[s][n], acc[m][n]);
-            } else {
-                for (int64_t k = k0; k < p.K; k += STEP) {
-                    const int64_t left = p.K - k - KV * g;
-                    typename X::Op a[MT], b[NR];
-#pragma unroll
-                    for (int m = 0; m < MT; ++m) a[m] = loose_part<T, KV>(x[m] + k, left);
-#pragma unroll
-                    for (int n = 0; n < NR; ++n) b[n] = loose_part<T, KV>(w[n] + k, left);
-#pragma unroll
-                    for (int m = 0; m < MT; ++m)
-#pragma unroll
-                        for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a[m], b[n], acc[m][n]);
-                }
+                for (int n = 0; n < NR; ++n) b[s][n] = loose<T, KV>(w[n] + k + s * STEP);
             }
+        };
+        int64_t k = (int64_t)wave * CHUNK;
+        if (AHEAD && k + CHUNK <= p.K) load(k);
+        for (; k + CHUNK <= p.K; k += W * CHUNK) {
+            if constexpr (!AHEAD) load(k);
+            typename X::Op a1[U][MT], b1[U][NR];
+#pragma unroll
+            for (int s = 0; s < U; ++s) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) a1[s][m] = a[s][m];
+#pragma unroll
+                for (int n = 0; n < NR; ++n) b1[s][n] = b[s][n];
+            }
+            if (AHEAD && k + (W + 1) * CHUNK <= p.K) load(k + W * CHUNK);
+#pragma unroll
+            for (int s = 0; s < U; ++s)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a1[s][m], b1[s][n], acc[m][n]);
+        }
+        for (; k < p.K; k += STEP) { // (one wave's, and less than a chunk)
+            const int64_t left = p.K - k - KV * g;
+#pragma unroll
+            for (int m = 0; m < MT; ++m) a[0][m] = loose_part<T, KV>(x[m] + k, left);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) b[0][n] = loose_part<T, KV>(w[n] + k, left);
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a[0][m], b[0][n], acc[m][n]);
         }
     }
-    // the four waves' sums: 0 + 2 and 1 + 3, then those two
+    // the waves' sums: the upper half's onto the lower, and so on
 #pragma unroll
-    for (int half = 2; half >= 1; half /= 2) {
+    for (int half = W / 2; half >= 1; half /= 2) {
         if (wave >= half && wave < 2 * half)
 #pragma unroll
             for (int m = 0; m < MT; ++m)
@@ -242,11 +253,11 @@ template <typename T, int MT, int NR> __global__ __launch_bounds__(256) void shr
             for (int m = 0; m < MT; ++m)
 #pragma unroll
                 for (int n = 0; n < NR; ++n) acc[m][n] += red[wave][m * NR + n][lane];
-        __syncthreads();
+        if (half > 1) __syncthreads();
     }
     if (wave) return;
     const float s = p.scale && at.adapter >= 0 ? p.scale[at.adapter] : 1.f;
-    float *h = p.h + ((int64_t)ks * p.req.M + at.row) * p.R;
+    float *h = p.h + at.row * p.P;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -254,7 +265,7 @@ template <typename T, int MT, int NR> __global__ __launch_bounds__(256) void shr
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 const int row = 16 * m + 4 * g + q, r = r0 + 16 * n + i;
-                if (row < at.rows && r < p.R) h[(int64_t)row * p.R + r] = s * acc[m][n][q];
+                if (row < at.rows && r < p.P) h[(int64_t)row * p.P + r] = r < p.R ? s * acc[m][n][q] : 0.f;
             }
 }
 
@@ -262,79 +273,180 @@ template <typename T, int MT, int NR> __global__ __launch_bounds__(256) void shr
 
 struct ExpandParams {
     Requests req;
-    const float *h; // [KS][M][R]
+    const float *h; // [M][P], zeros behind rank R
     const void *w;  // [L, R, C]
     const void *y;  // or NULL
-    void *out;      // or NULL
+    void *out;
     const float *scale;
-    float *hidden; // the sum over KS, or NULL
+    float *hidden; // [M][R] h's copy for the caller, or NULL
     int64_t wl, wr, yb, yt, ob, ot;
     int64_t C;
-    int R, KS, groups; // workgroups over the columns
+    int R, P, groups, size; // workgroups over the columns; rows a tile
     int copies; // rows without an adapter are written too (out is not y's memory)
 };
 
-template <typename T, int MT> __global__ __launch_bounds__(256) void expand_kernel(ExpandParams p) {
+// Up to KR steps of ranks: the wave's columns of b stay in registers while it walks rows
+// of 16, the next ones' y and h in flight.
+template <typename T, int KR, bool WHOLE>
+__device__ __forceinline__ void expand_walk(const ExpandParams &p, const Tile &at, int64_t c0, bool keep, bool write) {
     typedef Mm<T> X;
     constexpr int KV = X::KV, VC = X::VC, STEP = 4 * KV;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int i = lane & 15, g = lane >> 4;
-    const int tile = blockIdx.x / p.groups, group = blockIdx.x - tile * p.groups;
-    const int64_t c0 = (int64_t)(group * 4 + wave) * 16 * VC;
-    if (c0 >= p.C) return;
-    const Tile at = tile_at(p.req, tile, MT * 16);
-    if (at.rows <= 0) return;
-    const int64_t c = c0 + VC * i, left = p.C - c;
-    const bool keep = p.hidden && group == 0 && wave == 0, write = p.out && (at.adapter >= 0 || p.copies);
-    if (!keep && !write) return;
-    const T *y = p.y ? static_cast<const T *>(p.y) + at.b * p.yb + at.t0 * p.yt + c : nullptr;
-    Raw<T, VC> old[MT][4];
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int64_t c = WHOLE ? min(c0 + VC * i, p.C - VC) : c0 + VC * i, left = p.C - c;
+    auto cols_at = [&](const T *q) { return WHOLE ? loose<T, VC>(q) : loose_part<T, VC>(q, left); };
+    typename X::Op cols[KR][VC];
+    const T *w = static_cast<const T *>(p.w) + at.adapter * p.wl + c;
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int s = 0; s < KR; ++s) {
+        Raw<T, VC> rows[KV];
+        const int r = s * STEP + KV * g;
+#pragma unroll
+        for (int k = 0; k < KV; ++k) rows[k] = cols_at(w + (int64_t)min(r + k, p.R - 1) * p.wr);
+        if ((s + 1) * STEP > p.R) // behind the last rank: zeros
+#pragma unroll
+            for (int k = 0; k < KV; ++k)
+                if (r + k >= p.R)
+#pragma unroll
+                    for (int t = 0; t < VC; ++t) rows[k][t] = (T)0.f;
+        X::turn(rows, cols[s]);
+    }
+    const T *y = p.y ? static_cast<const T *>(p.y) + at.b * p.yb + at.t0 * p.yt + c : nullptr;
+    T *out = static_cast<T *>(p.out) + at.b * p.ob + at.t0 * p.ot + c;
+    const float scale = p.scale ? p.scale[at.adapter] : 1.f;
+    Raw<T, VC> old[4];
+    float h[KR][KV];
+    auto load = [&](int m) {
+        const float *hm = p.h + (at.row + min(m + i, at.rows - 1)) * p.P;
+#pragma unroll
+        for (int s = 0; s < KR; ++s) {
+            const int r = s * STEP + KV * g;
+            load_n<float, KV>(hm + min(r, p.P - KV), h[s]);
+            if ((s + 1) * STEP > p.P && r >= p.P)
+#pragma unroll
+                for (int k = 0; k < KV; ++k) h[s][k] = 0.f;
+        }
+        if (y)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) old[q] = cols_at(y + min(m + 4 * g + q, at.rows - 1) * p.yt);
+    };
+    load(0);
+    for (int m = 0; m < at.rows; m += 16) {
+        typename X::Wide hw[KR];
+#pragma unroll
+        for (int s = 0; s < KR; ++s) {
+            hw[s] = X::wide(h[s]);
+            const int r = s * STEP + KV * g;
+            if (keep && m + i < at.rows) store_part<float, KV>(p.hidden + (at.row + m + i) * p.R + r, p.R - r, h[s]);
+        }
+        Raw<T, VC> was[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) was[q] = old[q];
+        if (m + 16 < at.rows) load(m + 16);
+        floatx4 acc[VC];
+#pragma unroll
+        for (int t = 0; t < VC; ++t) {
+            acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KR; ++s) acc[t] = X::mmw(hw[s], cols[s][t], acc[t]);
+        }
+        if (!write) continue;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
+            const int row = m + 4 * g + q;
+            if (row >= at.rows) continue;
+            float v[VC];
 #pragma unroll
-            for (int t = 0; t < VC; ++t) old[m][q][t] = (T)0.f;
-            const int row = 16 * m + 4 * g + q;
-            if (y && row < at.rows) old[m][q] = loose_part<T, VC>(y + row * p.yt, left);
+            for (int t = 0; t < VC; ++t) v[t] = __builtin_fmaf(scale, acc[t][q], y ? (float)was[q][t] : 0.f);
+            if constexpr (WHOLE) loose_store<T, VC>(out + row * p.ot, v);
+            else store_part<T, VC>(out + row * p.ot, left, v);
         }
+    }
+}
+
+// Rows without an adapter: y as it is, NaN and all, or zeros.
+template <typename T> __device__ __forceinline__ void expand_copy(const ExpandParams &p, const Tile &at, int64_t c0, bool keep) {
+    constexpr int VC = Mm<T>::VC;
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int64_t c = c0 + VC * i, left = p.C - c;
+    if (keep)
+        for (int64_t k = lane; k < (int64_t)at.rows * p.R; k += kWave) p.hidden[at.row * p.R + k] = 0.f;
+    if (!p.copies) return;
+    const T *y = p.y ? static_cast<const T *>(p.y) + at.b * p.yb + at.t0 * p.yt + c : nullptr;
+    T *out = static_cast<T *>(p.out) + at.b * p.ob + at.t0 * p.ot + c;
+    for (int row = g; row < at.rows; row += 4) {
+        float v[VC];
+#pragma unroll
+        for (int t = 0; t < VC; ++t) v[t] = 0.f;
+        if (y) load_part<T, VC>(y + row * p.yt, left, v);
+        store_part<T, VC>(out + row * p.ot, left, v);
+    }
+}
+
+// KR 0: any number of ranks, steps of them for rows of 32 at a time.
+// WHOLE: VC columns or more are left.  A lane whose columns would end behind the last
+// takes the last VC ones: what another lane of the wave takes too, with the same result.
+template <typename T, int MT, bool WHOLE>
+__device__ __forceinline__ void expand_tile(const ExpandParams &p, const Tile &at, int64_t c0, bool keep, bool write) {
+    typedef Mm<T> X;
+    constexpr int KV = X::KV, VC = X::VC, STEP = 4 * KV;
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int64_t c = WHOLE ? min(c0 + VC * i, p.C - VC) : c0 + VC * i, left = p.C - c;
+    auto cols_at = [&](const T *q) { return WHOLE ? loose<T, VC>(q) : loose_part<T, VC>(q, left); };
+    const T *w = static_cast<const T *>(p.w) + at.adapter * p.wl + c;
+    Raw<T, VC> rows[KV];
+    float h[MT][KV];
+    auto load = [&](int r0) { // (behind the last rank: zeros)
+        const int r = r0 + KV * g;
+#pragma unroll
+        for (int k = 0; k < KV; ++k) rows[k] = cols_at(w + (int64_t)min(r + k, p.R - 1) * p.wr);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+            load_n<float, KV>(p.h + (at.row + min(16 * m + i, at.rows - 1)) * p.P + min(r, p.P - KV), h[m]);
+        if (r0 + STEP > p.R) {
+#pragma unroll
+            for (int k = 0; k < KV; ++k)
+                if (r + k >= p.R)
+#pragma unroll
+                    for (int t = 0; t < VC; ++t) rows[k][t] = (T)0.f;
+            if (r >= p.P)
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int k = 0; k < KV; ++k) h[m][k] = 0.f;
+        }
+    };
+    load(0);
+    Raw<T, VC> old[MT][4];
+    if (write && p.y) {
+        const T *y = static_cast<const T *>(p.y) + at.b * p.yb + at.t0 * p.yt + c;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) old[m][q] = cols_at(y + min(16 * m + 4 * g + q, at.rows - 1) * p.yt);
+    }
     floatx4 acc[MT][VC];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int t = 0; t < VC; ++t) acc[m][t] = floatx4{0.f, 0.f, 0.f, 0.f};
-    float s = 1.f;
-    if (at.adapter >= 0) {
-        if (p.scale) s = p.scale[at.adapter];
-        const T *w = static_cast<const T *>(p.w) + at.adapter * p.wl + c;
-        for (int r0 = 0; r0 < p.R; r0 += STEP) {
+    for (int r0 = 0; r0 < p.R; r0 += STEP) {
+        typename X::Op cols[VC];
+        X::turn(rows, cols);
+        typename X::Wide hw[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            hw[m] = X::wide(h[m]);
             const int r = r0 + KV * g;
-            Raw<T, VC> rows[KV];
-#pragma unroll
-            for (int k = 0; k < KV; ++k) rows[k] = loose_part<T, VC>(w + (int64_t)min(r + k, p.R - 1) * p.wr, r + k < p.R ? left : 0);
-            typename X::Op cols[VC];
-            X::turn(rows, cols);
-#pragma unroll
-            for (int m = 0; m < MT; ++m) {
-                const int64_t place = (at.row + min(16 * m + i, at.rows - 1)) * p.R + r;
-                float h[KV];
-                load_part<float, KV>(p.h + place, p.R - r, h);
-                for (int k = 1; k < p.KS; ++k) {
-                    float more[KV];
-                    load_part<float, KV>(p.h + k * p.req.M * p.R + place, p.R - r, more);
-#pragma unroll
-                    for (int j = 0; j < KV; ++j) h[j] += more[j];
-                }
-                if (keep && 16 * m + i < at.rows) store_part<float, KV>(p.hidden + place, p.R - r, h);
-                const typename X::Wide hw = X::wide(h);
-#pragma unroll
-                for (int t = 0; t < VC; ++t) acc[m][t] = X::mmw(hw, cols[t], acc[m][t]);
-            }
+            if (keep && 16 * m + i < at.rows) store_part<float, KV>(p.hidden + (at.row + 16 * m + i) * p.R + r, p.R - r, h[m]);
         }
-    } else if (keep) {
-        for (int64_t k = lane; k < (int64_t)at.rows * p.R; k += kWave) p.hidden[at.row * p.R + k] = 0.f;
+        if (r0 + STEP < p.R) load(r0 + STEP);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int t = 0; t < VC; ++t) acc[m][t] = X::mmw(hw[m], cols[t], acc[m][t]);
     }
     if (!write) return;
+    const float s = p.scale ? p.scale[at.adapter] : 1.f;
     T *out = static_cast<T *>(p.out) + at.b * p.ob + at.t0 * p.ot + c;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -344,10 +456,31 @@ template <typename T, int MT> __global__ __launch_bounds__(256) void expand_kern
             if (row >= at.rows) continue;
             float v[VC];
 #pragma unroll
-            for (int t = 0; t < VC; ++t) // (rows without an adapter: as they are, NaN and all)
-                v[t] = at.adapter >= 0 ? __builtin_fmaf(s, acc[m][t][q], (float)old[m][q][t]) : (float)old[m][q][t];
-            store_part<T, VC>(out + row * p.ot, left, v);
+            for (int t = 0; t < VC; ++t) v[t] = __builtin_fmaf(s, acc[m][t][q], p.y ? (float)old[m][q][t] : 0.f);
+            if constexpr (WHOLE) loose_store<T, VC>(out + row * p.ot, v);
+            else store_part<T, VC>(out + row * p.ot, left, v);
         }
+}
+
+template <typename T, int KR> __global__ __launch_bounds__(256, 2) void expand_kernel(ExpandParams p) {
+    constexpr int VC = Mm<T>::VC;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int tile = blockIdx.x / p.groups, group = blockIdx.x - tile * p.groups;
+    const int64_t c0 = (int64_t)(group * 4 + wave) * 16 * VC;
+    if (c0 >= p.C && !(p.hidden && c0 == 0)) return;
+    const Tile at = tile_at(p.req, tile, p.size);
+    if (at.rows <= 0) return;
+    const bool keep = p.hidden && c0 == 0, write = at.adapter >= 0 || p.copies, whole = p.C - c0 >= VC;
+    if (!keep && !write) return;
+    if (at.adapter < 0 || p.R == 0) {
+        expand_copy<T>(p, at, c0, keep);
+    } else if constexpr (KR > 0) {
+        if (whole) expand_walk<T, KR, true>(p, at, c0, keep, write);
+        else expand_walk<T, KR, false>(p, at, c0, keep, write);
+    } else {
+        if (whole) expand_tile<T, 2, true>(p, at, c0, keep, write);
+        else expand_tile<T, 2, false>(p, at, c0, keep, write);
+    }
 }
 
 // -- outer -----------------------------------------------------------------------------
@@ -355,7 +488,8 @@ template <typename T, int MT> __global__ __launch_bounds__(256) void expand_kern
 struct OuterParams {
     Requests req;
     const void *z[2];  // x with dh for da, dy with h for db
-    const float *h[2]; // [M][R]
+    const float *h[2]; // [M][pitch]
+    int64_t pitch[2];
     float *part[2];    // [blocks][R][C]
     int64_t zb[2], zt[2], C[2];
     int tiles[2]; // column tiles
@@ -363,22 +497,21 @@ struct OuterParams {
     int R, rows;  // rows a block
 };
 
-template <typename T, int NR> __global__ __launch_bounds__(256) void outer_kernel(OuterParams p) {
+// Waves: WS shares of the ranks, 16 NR each, by 4 / WS shares of the rows.
+template <typename T, int NR, int WS, bool WHOLE>
+__device__ __forceinline__ void outer_tile(const OuterParams &p, const Tile &at, int block, int which, int64_t c0, int rs,
+                                           floatx4 (*red)[WS][NR * Mm<T>::VC][kWave]) {
     typedef Mm<T> X;
-    constexpr int KV = X::KV, VC = X::VC, STEP = 4 * KV;
-    __shared__ floatx4 red[2][NR * VC][kWave];
+    constexpr int KV = X::KV, VC = X::VC, STEP = 4 * KV, NS = 4 / WS;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int i = lane & 15, g = lane >> 4;
-    const int tiles = p.tiles[0] + p.tiles[1], block = blockIdx.x / tiles, ct = blockIdx.x - block * tiles;
-    const int which = ct >= p.tiles[0], r0 = blockIdx.y * NR * 16;
-    const Tile at = tile_at(p.req, block, p.rows);
-    const bool any = at.rows > 0 && at.adapter >= 0;
-    if (ct == 0 && r0 == 0 && threadIdx.x == 0) p.adapter[block] = any ? at.adapter : -1;
-    if (!any) return;
-    const int64_t C = p.C[which], c = (int64_t)(ct - which * p.tiles[0]) * 16 * VC + VC * i, left = C - c;
+    const int i = lane & 15, g = lane >> 4, ws = wave % WS, ms = wave / WS;
+    const int r0 = (rs * WS + ws) * NR * 16;
+    const int64_t C = p.C[which], c = WHOLE ? min(c0 + VC * i, C - VC) : c0 + VC * i, left = C - c;
     const T *z = static_cast<const T *>(p.z[which]) + at.b * p.zb[which] + at.t0 * p.zt[which] + c;
-    const int64_t zt = p.zt[which];
-    const float *h = p.h[which] + at.row * p.R;
+    const int64_t zt = p.zt[which], pitch = p.pitch[which];
+    const float *h[NR];
+#pragma unroll
+    for (int n = 0; n < NR; ++n) h[n] = p.h[which] + at.row * pitch + min(r0 + 16 * n + i, p.R - 1);
     floatx4 acc[NR][VC];
 #pragma unroll
     for (int n = 0; n < NR; ++n)
@@ -386,49 +519,54 @@ template <typename T, int NR> __global__ __launch_bounds__(256) void outer_kerne
         for (int t = 0; t < VC; ++t) acc[n][t] = floatx4{0.f, 0.f, 0.f, 0.f};
     Raw<T, VC> rows[KV];
     float hv[NR][KV];
-    auto load = [&](int m0) { // rows behind the last, ranks behind the last: zeros
+    auto load = [&](int m0) { // (ranks behind the last: the last one's again, not stored)
         const int m = m0 + KV * g;
 #pragma unroll
         for (int k = 0; k < KV; ++k) {
             const int row = min(m + k, at.rows - 1);
-            rows[k] = loose_part<T, VC>(z + row * zt, m + k < at.rows ? left : 0);
+            rows[k] = WHOLE ? loose<T, VC>(z + row * zt) : loose_part<T, VC>(z + row * zt, left);
 #pragma unroll
-            for (int n = 0; n < NR; ++n) {
-                const int r = r0 + 16 * n + i;
-                const float v = h[(int64_t)row * p.R + min(r, p.R - 1)];
-                hv[n][k] = m + k < at.rows ? v : 0.f;
-            }
+            for (int n = 0; n < NR; ++n) hv[n][k] = h[n][row * pitch];
         }
+        if (m0 + STEP > at.rows) // behind the last row: zeros
+#pragma unroll
+            for (int k = 0; k < KV; ++k)
+                if (m + k >= at.rows) {
+#pragma unroll
+                    for (int t = 0; t < VC; ++t) rows[k][t] = (T)0.f;
+#pragma unroll
+                    for (int n = 0; n < NR; ++n) hv[n][k] = 0.f;
+                }
     };
-    if (wave * STEP < at.rows) load(wave * STEP);
-    for (int m0 = wave * STEP; m0 < at.rows; m0 += 4 * STEP) {
+    if (ms * STEP < at.rows) load(ms * STEP);
+    for (int m0 = ms * STEP; m0 < at.rows; m0 += NS * STEP) {
         typename X::Op cols[VC];
         X::turn(rows, cols);
         typename X::Wide hw[NR];
 #pragma unroll
         for (int n = 0; n < NR; ++n) hw[n] = X::wide(hv[n]);
-        if (m0 + 4 * STEP < at.rows) load(m0 + 4 * STEP);
+        if (m0 + NS * STEP < at.rows) load(m0 + NS * STEP);
 #pragma unroll
         for (int n = 0; n < NR; ++n)
 #pragma unroll
             for (int t = 0; t < VC; ++t) acc[n][t] = X::mmw(hw[n], cols[t], acc[n][t]);
     }
 #pragma unroll
-    for (int half = 2; half >= 1; half /= 2) {
-        if (wave >= half && wave < 2 * half)
+    for (int half = NS / 2; half >= 1; half /= 2) {
+        if (ms >= half && ms < 2 * half)
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int t = 0; t < VC; ++t) red[wave - half][n * VC + t][lane] = acc[n][t];
+                for (int t = 0; t < VC; ++t) red[ms - half][ws][n * VC + t][lane] = acc[n][t];
         __syncthreads();
-        if (wave < half)
+        if (ms < half)
 #pragma unroll
             for (int n = 0; n < NR; ++n)
 #pragma unroll
-                for (int t = 0; t < VC; ++t) acc[n][t] += red[wave][n * VC + t][lane];
-        __syncthreads();
+                for (int t = 0; t < VC; ++t) acc[n][t] += red[ms][ws][n * VC + t][lane];
+        if (half > 1) __syncthreads();
     }
-    if (wave) return;
+    if (ms) return;
     float *part = p.part[which] + (int64_t)block * p.R * C + c;
 #pragma unroll
     for (int n = 0; n < NR; ++n)
@@ -439,8 +577,23 @@ template <typename T, int NR> __global__ __launch_bounds__(256) void outer_kerne
             float v[VC];
 #pragma unroll
             for (int t = 0; t < VC; ++t) v[t] = acc[n][t][q];
-            store_part<float, VC>(part + r * C, left, v);
+            if constexpr (WHOLE) loose_store<float, VC>(part + r * C, v);
+            else store_part<float, VC>(part + r * C, left, v);
         }
+}
+
+template <typename T, int NR, int WS> __global__ __launch_bounds__(256, 2) void outer_kernel(OuterParams p) {
+    constexpr int VC = Mm<T>::VC;
+    __shared__ floatx4 red[2 / WS][WS][NR * VC][kWave];
+    const int tiles = p.tiles[0] + p.tiles[1], block = blockIdx.x / tiles, ct = blockIdx.x - block * tiles;
+    const int which = ct >= p.tiles[0];
+    const Tile at = tile_at(p.req, block, p.rows);
+    const bool any = at.rows > 0 && at.adapter >= 0;
+    if (ct == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.adapter[block] = any ? at.adapter : -1;
+    if (!any) return;
+    const int64_t c0 = (int64_t)(ct - which * p.tiles[0]) * 16 * VC;
+    if (p.C[which] - c0 >= VC) outer_tile<T, NR, WS, true>(p, at, block, which, c0, blockIdx.y, red);
+    else outer_tile<T, NR, WS, false>(p, at, block, which, c0, blockIdx.y, red);
 }
 
 struct SumsParams {
@@ -453,31 +606,51 @@ struct SumsParams {
     int blocks;
 };
 
+// 256 values a workgroup: each of its waves adds every fourth of the adapter's blocks,
+// eight of them in flight.
 __global__ __launch_bounds__(256) void adapter_sums_kernel(SumsParams p) {
+    __shared__ double red[3][kWave][4];
     const int tiles = p.tiles[0] + p.tiles[1], l = blockIdx.x / tiles, ct = blockIdx.x - l * tiles;
-    const int which = ct >= p.tiles[0];
-    const int64_t n = p.n[which], e = ((int64_t)(ct - which * p.tiles[0]) * 256 + threadIdx.x) * 4;
-    const int64_t left = n - e;
+    const int which = ct >= p.tiles[0], lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t n = p.n[which], e = ((int64_t)(ct - which * p.tiles[0]) * kWave + lane) * 4, left = n - e;
+    const float *part = p.part[which] + e;
     double sum[4] = {0., 0., 0., 0.};
-    bool some = false;
     for (int b0 = 0; b0 < p.blocks; b0 += kWave) {
-        const int b = b0 + (int)(threadIdx.x & 63);
+        const int b = b0 + lane;
         uint64_t mine = __ballot(b < p.blocks && p.adapter[b < p.blocks ? b : 0] == l);
         while (mine) {
-            const int at = b0 + __builtin_ctzll(mine);
-            mine &= mine - 1;
-            some = true;
-            float v[4];
-            load_part<float, 4>(p.part[which] + at * n + e, left, v);
+            int at[8], count = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) sum[j] += v[j];
+            for (int k = 0; k < 8; ++k) at[k] = 0;
+            // (the same for every lane)
+#pragma unroll
+            for (int k = 0; k < 32; ++k) {
+                const int first = mine ? __builtin_ctzll(mine) : 0;
+                if (mine && (k & 3) == wave) at[k / 4] = b0 + first, count = k / 4 + 1;
+                mine &= mine - 1; // (0 stays 0)
+            }
+            float v[8][4];
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < count) load_part<float, 4>(part + at[k] * n, left, v[k]);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (k < count)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sum[j] += v[k][j];
         }
     }
-    if (left <= 0) return;
-    const double s = which && some && p.scale ? p.scale[l] : 1.;
+    if (wave)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) red[wave - 1][lane][j] = sum[j];
+    __syncthreads();
+    if (wave || left <= 0) return;
     float v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = (float)(s * sum[j]);
+    for (int j = 0; j < 4; ++j) {
+        const double t = (sum[j] + red[0][lane][j]) + (red[1][lane][j] + red[2][lane][j]);
+        v[j] = (float)(which && p.scale && t != 0. ? p.scale[l] * t : t); // (no rows: 0)
+    }
     store_part<float, 4>(p.out[which] + l * n + e, left, v);
 }
 
@@ -511,21 +684,9 @@ Requests requests_of(const gdn2_low_rank_args &a, const Shape &s, int size) {
     return r;
 }
 
-// Row tiles of 16 mt: the larger, the fewer times an adapter is read from the caches;
-// but no more than a request has, and while 128 tiles remain.
-int mt_of(const Shape &s) {
-    const int64_t mean = s.N > 0 ? up(s.M, s.N) : 1;
-    if (mean > 32 && s.tiles(64) >= 128) return 4;
-    return 1;
-}
-// Workgroups that share the wide dimension: while fewer than 512, and each wave has a
-// chunk of 128 (f32: 64).
-int ks_of(int64_t tiles, int64_t K, int element) {
-    const int64_t most = std::max<int64_t>(1, K / (4 * (element == 2 ? 128 : 64)));
-    int ks = 1;
-    while (ks < 8 && 2 * ks <= most && tiles * ks < 512) ks *= 2;
-    return ks;
-}
+// Row tiles of 16 mt in shrink: the larger, the fewer times an adapter is read from the
+// caches; but no more than a request has, and while 64 tiles remain.
+int mt_of(const Shape &s) { return s.N > 0 && up(s.M, s.N) > 32 && s.tiles(64) >= 64 ? 4 : 1; }
 int nr_of(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
 
 // Rows a block of the outer products: 1024 blocks by columns, while each has 128 rows or
@@ -543,27 +704,24 @@ bool sizes_ok(const gdn2_low_rank_args &a) {
            a.in_features < (1 << 24) && a.out_features < (1 << 24) && a.num_adapters < (1 << 24);
 }
 
-// Bytes of a forward's workspace: h of each share of the wide dimension.
-size_t hidden_bytes(const Shape &s, int64_t R, int ks) { return align256(sizeof(float) * (size_t)ks * (size_t)s.M * (size_t)R); }
+int64_t pitch_of(int64_t R) { return up(R, 16) * 16; }
+// Bytes of h.
+size_t hidden_bytes(const Shape &s, int64_t R) { return align256(sizeof(float) * (size_t)s.M * (size_t)pitch_of(R)); }
 
-struct Plan {
-    int mt, ks;
-    int64_t tiles, groups;
-};
-template <typename T> Plan plan_of(const Shape &s, int64_t K, int64_t C) {
-    Plan q{};
-    q.mt = mt_of(s);
-    q.tiles = s.tiles(16 * q.mt);
-    q.ks = C > 0 ? ks_of(q.tiles, K, sizeof(T)) : 1; // (expand joins the shares)
-    q.groups = up(C, 4 * 16 * Mm<T>::VC);
-    return q;
-}
-
-template <typename T> gdn2_status launch_shrink(const ShrinkParams &p, const Plan &q, hipStream_t s) {
-    const int nr = nr_of(p.R);
-    const dim3 grid((unsigned)(q.tiles * q.ks), (unsigned)up(p.R, 16 * nr));
-#define GDN2_RUN(MT, NR) hipLaunchKernelGGL((shrink_kernel<T, MT, NR>), grid, dim3(256), 0, s, p)
-    if (q.mt == 4) {
+template <typename T> gdn2_status launch_shrink(ShrinkParams p, const gdn2_low_rank_args &a, const Shape &sh, hipStream_t s) {
+    const int mt = mt_of(sh), nr = nr_of(p.R);
+    const int64_t tiles = sh.tiles(16 * mt);
+    const bool many = tiles >= 512;
+    p.req = requests_of(a, sh, 16 * mt);
+    const dim3 grid((unsigned)tiles, (unsigned)up(p.R, 16 * nr));
+    // (sixteen waves of the widest tile would not have the registers)
+#define GDN2_RUN(MT, NR)                                                                                 \
+    do {                                                                                                 \
+        constexpr int W = MT * NR == 16 ? 8 : 16;                                                        \
+        if (many) hipLaunchKernelGGL((shrink_kernel<T, MT, NR, 4>), grid, dim3(256), 0, s, p);           \
+        else hipLaunchKernelGGL((shrink_kernel<T, MT, NR, W>), grid, dim3(64 * W), 0, s, p);             \
+    } while (0)
+    if (mt == 4) {
         if (nr == 1) GDN2_RUN(4, 1);
         else if (nr == 2) GDN2_RUN(4, 2);
         else GDN2_RUN(4, 4);
@@ -577,12 +735,29 @@ template <typename T> gdn2_status launch_shrink(const ShrinkParams &p, const Pla
     return GDN2_OK;
 }
 
-template <typename T> gdn2_status launch_expand(const ExpandParams &p, const Plan &q, hipStream_t s) {
-    const dim3 grid((unsigned)(q.tiles * q.groups));
-    if (q.mt == 4) hipLaunchKernelGGL((expand_kernel<T, 4>), grid, dim3(256), 0, s, p);
-    else hipLaunchKernelGGL((expand_kernel<T, 1>), grid, dim3(256), 0, s, p);
+// Rows a tile in expand: 64 (32 where the ranks do not fit the registers), 16 for requests
+// so short.
+int expand_rows(const Shape &s, int64_t R) { return s.N > 0 && up(s.M, s.N) > 16 ? (R > 64 ? 32 : 64) : 16; }
+template <typename T> int64_t groups_of(int64_t C) { return std::max<int64_t>(1, up(C, 4 * 16 * Mm<T>::VC)); }
+
+template <typename T> gdn2_status launch_expand(ExpandParams p, const gdn2_low_rank_args &a, const Shape &sh, hipStream_t s) {
+    constexpr int STEP = 4 * Mm<T>::KV;
+    p.size = expand_rows(sh, p.R);
+    p.req = requests_of(a, sh, p.size);
+    p.groups = (int)groups_of<T>(p.C);
+    const dim3 grid((unsigned)(sh.tiles(p.size) * p.groups));
+#define GDN2_RUN(KR) hipLaunchKernelGGL((expand_kernel<T, KR>), grid, dim3(256), 0, s, p)
+    if (p.R <= STEP) GDN2_RUN(1);
+    else if (p.R <= 2 * STEP) GDN2_RUN(2);
+    else if (p.R <= 64) GDN2_RUN(64 / STEP);
+    else GDN2_RUN(0);
+#undef GDN2_RUN
     GDN2_HIP_CHECK(hipGetLastError());
     return GDN2_OK;
+}
+
+template <typename T> bool grids_ok(const Shape &sh, int64_t C, int64_t R) {
+    return sh.tiles(16 * mt_of(sh)) < (1 << 22) && sh.tiles(expand_rows(sh, R)) * groups_of<T>(C) < (1 << 24);
 }
 
 gdn2_status check(const gdn2_low_rank_args *a, const std::string &who) {
@@ -597,7 +772,6 @@ gdn2_status check(const gdn2_low_rank_args *a, const std::string &who) {
 bool workspace_ok(const void *p, size_t have, size_t need) {
     return !need || (p && have >= need && reinterpret_cast<uintptr_t>(p) % 256 == 0);
 }
-bool grid_ok(const Plan &q) { return q.tiles * std::max<int64_t>(q.groups, q.ks) < (1 << 24); }
 
 template <typename T> gdn2_status forward(const gdn2_low_rank_args *a, hipStream_t s, const char *name) {
     const std::string who = std::string(name) + ": ";
@@ -605,59 +779,50 @@ template <typename T> gdn2_status forward(const gdn2_low_rank_args *a, hipStream
     if (st != GDN2_OK) return st;
     const Shape sh = shape_of(*a);
     if (sh.M == 0) return GDN2_OK;
+    if (a->out_features == 0 && !a->hidden) return GDN2_OK;
     const int64_t D = a->in_features, O = a->out_features, R = a->rank;
     if ((D > 0 && R > 0 && a->num_adapters > 0 && (!a->x || !a->a)) || (O > 0 && (!a->y || !a->out || (R > 0 && a->num_adapters > 0 && !a->b))) ||
         (sh.N > 0 && !a->adapters))
         return fail(GDN2_EINVAL, who + "null pointer");
     if (O > 0 && a->out == a->y && ((a->batch > 1 && a->stride_out_b != a->stride_y_b) || (a->seq_len > 1 && a->stride_out_t != a->stride_y_t)))
         return fail(GDN2_EINVAL, who + "in place, the strides must be equal");
-    if (O == 0 && !a->hidden) return GDN2_OK;
-    const Plan q = plan_of<T>(sh, D, O);
-    if (!grid_ok(q)) return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
-    const bool direct = q.ks == 1 && a->hidden; // h needs no joining
-    const size_t need = R > 0 && !direct ? hidden_bytes(sh, R, q.ks) : 0;
-    if (!workspace_ok(a->workspace, a->workspace_bytes, need))
+    if (!grids_ok<T>(sh, O, R)) return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
+    if (!workspace_ok(a->workspace, a->workspace_bytes, R > 0 ? hidden_bytes(sh, R) : 0))
         return fail(GDN2_EINVAL, who + "workspace missing, too small or not 256-byte aligned");
-    float *h = direct ? a->hidden : static_cast<float *>(a->workspace);
-    const Requests req = requests_of(*a, sh, 16 * q.mt);
+    float *h = static_cast<float *>(a->workspace);
+    const int P = (int)pitch_of(R);
     if (R > 0) {
         ShrinkParams p{};
-        p.req = req;
         p.x = a->x; p.w = a->a; p.h = h;
         p.xb = a->stride_x_b; p.xt = a->stride_x_t; p.wl = a->stride_a_l; p.wr = a->stride_a_r;
-        p.K = D; p.R = (int)R; p.KS = q.ks;
-        if ((st = launch_shrink<T>(p, q, s)) != GDN2_OK) return st;
+        p.K = D; p.R = (int)R; p.P = P;
+        if ((st = launch_shrink<T>(p, *a, sh, s)) != GDN2_OK) return st;
     }
-    if (O == 0) return GDN2_OK;
     ExpandParams p{};
-    p.req = req;
-    p.h = h; p.w = a->b; p.y = a->y; p.out = a->out; p.scale = a->scale; p.hidden = direct || R == 0 ? nullptr : a->hidden;
+    p.h = h; p.w = a->b; p.y = a->y; p.out = a->out; p.scale = a->scale; p.hidden = R > 0 ? a->hidden : nullptr;
     p.wl = a->stride_b_l; p.wr = a->stride_b_r; p.yb = a->stride_y_b; p.yt = a->stride_y_t;
     p.ob = a->stride_out_b; p.ot = a->stride_out_t;
-    p.C = O; p.R = (int)R; p.KS = q.ks; p.groups = (int)q.groups;
+    p.C = O; p.R = (int)R; p.P = P;
     p.copies = a->out != a->y;
-    return launch_expand<T>(p, q, s);
+    return launch_expand<T>(p, *a, sh, s);
 }
 
 struct BwdPlan {
-    Plan q;
     int rows;
     int64_t blocks;
-    size_t h, one, ids, part[2], bytes;
+    size_t h, ids, part[2], bytes;
 };
 template <typename T> BwdPlan bwd_plan(const gdn2_low_rank_bwd_args &b) {
     const gdn2_low_rank_args &a = b.fwd;
     const Shape sh = shape_of(a);
     BwdPlan p{};
-    p.q = plan_of<T>(sh, a.out_features, a.in_features);
     const int64_t C[2] = {b.da ? a.in_features : 0, b.db ? a.out_features : 0};
     p.rows = block_rows(sh, C[0] + C[1], 16 * Mm<T>::VC);
     p.blocks = sh.tiles(p.rows);
-    p.h = hidden_bytes(sh, a.rank, p.q.ks);
-    p.one = p.q.ks > 1 ? hidden_bytes(sh, a.rank, 1) : 0;
+    p.h = hidden_bytes(sh, a.rank);
     p.ids = align256(sizeof(int) * (size_t)p.blocks);
     for (int i = 0; i < 2; ++i) p.part[i] = align256(sizeof(float) * (size_t)p.blocks * (size_t)a.rank * (size_t)C[i]);
-    p.bytes = p.h + p.one + p.ids + p.part[0] + p.part[1];
+    p.bytes = p.h + p.ids + p.part[0] + p.part[1];
     return p;
 }
 
@@ -669,12 +834,12 @@ template <typename T> gdn2_status backward(const gdn2_low_rank_bwd_args *b, hipS
     const Shape sh = shape_of(*a);
     const int64_t D = a->in_features, O = a->out_features, R = a->rank, L = a->num_adapters;
     const BwdPlan p = bwd_plan<T>(*b);
-    if (!grid_ok(p.q) || p.blocks * (up(D, 16 * Mm<T>::VC) + up(O, 16 * Mm<T>::VC)) >= (1 << 24))
+    if (!grids_ok<T>(sh, D, R) || p.blocks * (up(D, 16 * Mm<T>::VC) + up(O, 16 * Mm<T>::VC)) >= (1 << 24))
         return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
     SumsParams t{};
     t.n[0] = b->da ? R * D : 0;
     t.n[1] = b->db ? R * O : 0;
-    for (int i = 0; i < 2; ++i) t.tiles[i] = (int)up(t.n[i], 1024);
+    for (int i = 0; i < 2; ++i) t.tiles[i] = (int)up(t.n[i], 256);
     t.out[0] = b->da; t.out[1] = b->db; t.scale = a->scale;
     if (L * (t.tiles[0] + t.tiles[1]) >= (1 << 24)) return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
     if (sh.M > 0) {
@@ -685,48 +850,43 @@ template <typename T> gdn2_status backward(const gdn2_low_rank_bwd_args *b, hipS
         if (R > 0 && !workspace_ok(b->workspace, b->workspace_bytes, p.bytes))
             return fail(GDN2_EINVAL, who + "workspace missing, too small or not 256-byte aligned");
         char *ws = static_cast<char *>(b->workspace);
-        float *h = reinterpret_cast<float *>(ws);
-        float *dh = p.one ? reinterpret_cast<float *>(ws + p.h) : h;
-        ws += p.h + p.one;
+        float *dh = reinterpret_cast<float *>(ws);
+        ws += p.h;
         int *ids = reinterpret_cast<int *>(ws);
         ws += p.ids;
-        const bool want_dh = b->dx || b->da;
-        const Requests req = requests_of(*a, sh, 16 * p.q.mt);
-        if (R > 0 && want_dh) {
+        const int P = (int)pitch_of(R);
+        if (R > 0 && (b->dx || b->da)) {
             ShrinkParams k{};
-            k.req = req;
-            k.x = b->d_out; k.w = a->b; k.scale = a->scale; k.h = h;
+            k.x = b->d_out; k.w = a->b; k.scale = a->scale; k.h = dh;
             k.xb = b->stride_d_out_b; k.xt = b->stride_d_out_t; k.wl = a->stride_b_l; k.wr = a->stride_b_r;
-            k.K = O; k.R = (int)R; k.KS = p.q.ks;
-            if ((st = launch_shrink<T>(k, p.q, s)) != GDN2_OK) return st;
+            k.K = O; k.R = (int)R; k.P = P;
+            if ((st = launch_shrink<T>(k, *a, sh, s)) != GDN2_OK) return st;
         }
-        if (want_dh && (b->dx || p.one) && D > 0) {
+        if (b->dx && D > 0) {
             ExpandParams k{};
-            k.req = req;
-            k.h = h; k.w = a->a; k.y = b->accumulate_dx ? b->dx : nullptr; k.out = b->dx;
-            k.hidden = p.one && R > 0 ? dh : nullptr;
+            k.h = dh; k.w = a->a; k.y = b->accumulate_dx ? b->dx : nullptr; k.out = b->dx;
             k.wl = a->stride_a_l; k.wr = a->stride_a_r;
             k.yb = k.ob = b->stride_dx_b; k.yt = k.ot = b->stride_dx_t;
-            k.C = D; k.R = (int)R; k.KS = p.q.ks; k.groups = (int)p.q.groups;
+            k.C = D; k.R = (int)R; k.P = P;
             k.copies = !b->accumulate_dx;
-            if ((st = launch_expand<T>(k, p.q, s)) != GDN2_OK) return st;
+            if ((st = launch_expand<T>(k, *a, sh, s)) != GDN2_OK) return st;
         }
         if (R > 0 && (b->da || b->db)) {
             OuterParams k{};
             k.req = requests_of(*a, sh, p.rows);
             k.z[0] = a->x; k.z[1] = b->d_out;
-            k.h[0] = dh; k.h[1] = a->hidden;
+            k.h[0] = dh; k.h[1] = a->hidden; k.pitch[0] = P; k.pitch[1] = R;
             k.part[0] = reinterpret_cast<float *>(ws); k.part[1] = reinterpret_cast<float *>(ws + p.part[0]);
             k.zb[0] = a->stride_x_b; k.zt[0] = a->stride_x_t; k.zb[1] = b->stride_d_out_b; k.zt[1] = b->stride_d_out_t;
             k.C[0] = b->da ? D : 0; k.C[1] = b->db ? O : 0;
             for (int i = 0; i < 2; ++i) k.tiles[i] = (int)up(k.C[i], 16 * Mm<T>::VC);
             k.adapter = ids; k.R = (int)R; k.rows = p.rows;
-            const int nr = nr_of(R);
-            const dim3 grid((unsigned)(p.blocks * (k.tiles[0] + k.tiles[1])), (unsigned)up(R, 16 * nr));
+            // (more than 32 ranks: two waves' shares, for the registers)
+            const dim3 grid((unsigned)(p.blocks * (k.tiles[0] + k.tiles[1])), (unsigned)up(R, 64));
             if (grid.x > 0) {
-                if (nr == 1) hipLaunchKernelGGL((outer_kernel<T, 1>), grid, dim3(256), 0, s, k);
-                else if (nr == 2) hipLaunchKernelGGL((outer_kernel<T, 2>), grid, dim3(256), 0, s, k);
-                else hipLaunchKernelGGL((outer_kernel<T, 4>), grid, dim3(256), 0, s, k);
+                if (R <= 16) hipLaunchKernelGGL((outer_kernel<T, 1, 1>), grid, dim3(256), 0, s, k);
+                else if (R <= 32) hipLaunchKernelGGL((outer_kernel<T, 2, 1>), grid, dim3(256), 0, s, k);
+                else hipLaunchKernelGGL((outer_kernel<T, 2, 2>), grid, dim3(256), 0, s, k);
             }
             t.part[0] = k.part[0]; t.part[1] = k.part[1];
             t.adapter = ids; t.blocks = (int)p.blocks;
@@ -746,15 +906,10 @@ bool countable(const gdn2_low_rank_args &a) {
 }  // namespace
 }  // namespace gdn2
 
-// (the larger of the two types')
 extern "C" size_t gdn2_low_rank_add_workspace_bytes(const gdn2_low_rank_args *a) {
-    if (!a || !gdn2::countable(*a)) return 0;
-    const gdn2::Shape s = gdn2::shape_of(*a);
-    if (a->out_features == 0 && !a->hidden) return 0;
-    const int ks = std::max(gdn2::plan_of<float>(s, a->in_features, a->out_features).ks,
-                            gdn2::plan_of<gdn2::bf16>(s, a->in_features, a->out_features).ks);
-    return ks == 1 && a->hidden ? 0 : gdn2::hidden_bytes(s, a->rank, ks);
+    return a && gdn2::countable(*a) ? gdn2::hidden_bytes(gdn2::shape_of(*a), a->rank) : 0;
 }
+// (the larger of the two types')
 extern "C" size_t gdn2_low_rank_add_bwd_workspace_bytes(const gdn2_low_rank_bwd_args *b) {
     if (!b || !gdn2::countable(b->fwd)) return 0;
     return std::max(gdn2::bwd_plan<float>(*b).bytes, gdn2::bwd_plan<gdn2::bf16>(*b).bytes);
