@@ -4,7 +4,7 @@
 //   dh = s_l dy b_l^T,  dx = dh a_l,  da_l = sum dh^T x,  db_l = s_l sum h^T dy
 //
 // Four kernels, each of which streams one wide tensor past matrix instructions:
-//   shrink  h or dh: rows of 16 MT by all ranks, the wide dimension split over the 4 or
+//   shrink  h or dh: rows of 16 MT by all ranks, the wide dimension split over the 4 to
 //           16 waves of a workgroup
 //   expand  out or dx: rows of 16 MT by 16 VC columns a wave, y read and out written once
 //   outer   da, db: ranks by 16 VC columns a wave, a block of one request's rows
@@ -173,11 +173,15 @@ struct ShrinkParams {
     int R, P;
 };
 
-template <typename T, int MT, int NR, int W> __global__ __launch_bounds__(64 * W) void shrink_kernel(ShrinkParams p) {
+// A wave takes 256 bytes of each of its rows at a time, 16 lanes a row, and turns them
+// into operands through LDS of its own; the next ones' loads are in flight meanwhile.
+// (Operands loaded as they are used, 64 bytes of each of 16 rows a load, kept the same
+// tiles at 3.3 TB/s.)
+template <typename T, int MT, int NR, int W> __global__ __launch_bounds__(64 * W, W > 8 ? 4 : 2) void shrink_kernel(ShrinkParams p) {
     typedef Mm<T> X;
-    constexpr int KV = X::KV, STEP = 4 * KV, U = 2, CHUNK = U * STEP;
-    constexpr bool AHEAD = W == 4; // the next chunk's loads in flight (16 waves overlap one another's)
-    __shared__ floatx4 red[W / 2][MT * NR][kWave];
+    constexpr int KV = X::KV, STEP = 4 * KV, U = 4, CHUNK = U * STEP, PITCH = 17; // (16 bytes: a row's 16 and one)
+    constexpr int kStage = MT * 16 * PITCH, kSums = MT * NR * kWave * (W / 2);
+    __shared__ floatx4 lds[W * kStage > kSums ? W * kStage : kSums];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
     const int r0 = blockIdx.y * NR * 16;
@@ -190,70 +194,73 @@ template <typename T, int MT, int NR, int W> __global__ __launch_bounds__(64 * W
         for (int n = 0; n < NR; ++n) acc[m][n] = floatx4{0.f, 0.f, 0.f, 0.f};
     if (at.adapter >= 0) {
         // (rows behind the tile's last, ranks behind the last: the last one's again, not stored)
-        const T *x[MT], *w[NR];
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-            x[m] = static_cast<const T *>(p.x) + at.b * p.xb + (at.t0 + min(16 * m + i, at.rows - 1)) * p.xt + KV * g;
+        const T *x = static_cast<const T *>(p.x) + at.b * p.xb + at.t0 * p.xt, *w[NR];
 #pragma unroll
         for (int n = 0; n < NR; ++n)
             w[n] = static_cast<const T *>(p.w) + at.adapter * p.wl + min(r0 + 16 * n + i, p.R - 1) * p.wr + KV * g;
-        typename X::Op a[U][MT], b[U][NR];
-        auto load = [&](int64_t k) {
+        floatx4 *stage = lds + wave * kStage;
+        typename X::Op ahead[MT * 4], b[U][NR];
+        auto load_x = [&](int64_t k) {
 #pragma unroll
-            for (int s = 0; s < U; ++s) {
+            for (int j = 0; j < MT * 4; ++j) ahead[j] = loose<T, KV>(x + min(4 * j + g, at.rows - 1) * p.xt + k + KV * i);
+        };
+        auto load_w = [&](int64_t k, int s) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m) a[s][m] = loose<T, KV>(x[m] + k + s * STEP);
-#pragma unroll
-                for (int n = 0; n < NR; ++n) b[s][n] = loose<T, KV>(w[n] + k + s * STEP);
-            }
+            for (int n = 0; n < NR; ++n) b[s][n] = loose<T, KV>(w[n] + k + s * STEP);
         };
         int64_t k = (int64_t)wave * CHUNK;
-        if (AHEAD && k + CHUNK <= p.K) load(k);
+        if (k + CHUNK <= p.K) {
+            load_x(k);
+#pragma unroll
+            for (int s = 0; s < U; ++s) load_w(k, s);
+        }
         for (; k + CHUNK <= p.K; k += W * CHUNK) {
-            if constexpr (!AHEAD) load(k);
-            typename X::Op a1[U][MT], b1[U][NR];
+#pragma unroll
+            for (int j = 0; j < MT * 4; ++j) stage[(4 * j + g) * PITCH + i] = __builtin_bit_cast(floatx4, ahead[j]);
+            const bool more = k + (W + 1) * CHUNK <= p.K;
+            const int64_t next = more ? k + W * CHUNK : k; // (the last chunk's again, not used)
+            load_x(next);
+            __builtin_amdgcn_wave_barrier(); // (one wave's LDS operations are done in order)
 #pragma unroll
             for (int s = 0; s < U; ++s) {
 #pragma unroll
-                for (int m = 0; m < MT; ++m) a1[s][m] = a[s][m];
+                for (int m = 0; m < MT; ++m) {
+                    const typename X::Op a = __builtin_bit_cast(typename X::Op, stage[(16 * m + i) * PITCH + 4 * s + g]);
 #pragma unroll
-                for (int n = 0; n < NR; ++n) b1[s][n] = b[s][n];
+                    for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a, b[s][n], acc[m][n]);
+                }
+                load_w(next, s);
             }
-            if (AHEAD && k + (W + 1) * CHUNK <= p.K) load(k + W * CHUNK);
-#pragma unroll
-            for (int s = 0; s < U; ++s)
-#pragma unroll
-                for (int m = 0; m < MT; ++m)
-#pragma unroll
-                    for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a1[s][m], b1[s][n], acc[m][n]);
+            __builtin_amdgcn_wave_barrier();
         }
         for (; k < p.K; k += STEP) { // (one wave's, and less than a chunk)
             const int64_t left = p.K - k - KV * g;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) a[0][m] = loose_part<T, KV>(x[m] + k, left);
-#pragma unroll
             for (int n = 0; n < NR; ++n) b[0][n] = loose_part<T, KV>(w[n] + k, left);
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
+            for (int m = 0; m < MT; ++m) {
+                const typename X::Op a = loose_part<T, KV>(x + min(16 * m + i, at.rows - 1) * p.xt + k + KV * g, left);
 #pragma unroll
-                for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a[0][m], b[0][n], acc[m][n]);
+                for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a, b[0][n], acc[m][n]);
+            }
         }
     }
     // the waves' sums: the upper half's onto the lower, and so on
+    auto red = [&](int w, int n) -> floatx4 & { return lds[(w * MT * NR + n) * kWave + lane]; };
 #pragma unroll
     for (int half = W / 2; half >= 1; half /= 2) {
+        __syncthreads(); // what was here has been read
         if (wave >= half && wave < 2 * half)
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int n = 0; n < NR; ++n) red[wave - half][m * NR + n][lane] = acc[m][n];
+                for (int n = 0; n < NR; ++n) red(wave - half, m * NR + n) = acc[m][n];
         __syncthreads();
         if (wave < half)
 #pragma unroll
             for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int n = 0; n < NR; ++n) acc[m][n] += red[wave][m * NR + n][lane];
-        if (half > 1) __syncthreads();
+                for (int n = 0; n < NR; ++n) acc[m][n] += red(wave, m * NR + n);
     }
     if (wave) return;
     const float s = p.scale && at.adapter >= 0 ? p.scale[at.adapter] : 1.f;
@@ -685,8 +692,11 @@ Requests requests_of(const gdn2_low_rank_args &a, const Shape &s, int size) {
 }
 
 // Row tiles of 16 mt in shrink: the larger, the fewer times an adapter is read from the
-// caches; but no more than a request has, and while 64 tiles remain.
-int mt_of(const Shape &s) { return s.N > 0 && up(s.M, s.N) > 32 && s.tiles(64) >= 64 ? 4 : 1; }
+// caches; but no more than a request has, and while there are enough.
+int mt_of(const Shape &s) {
+    const int64_t mean = s.N > 0 ? up(s.M, s.N) : 1;
+    return mean > 32 && s.tiles(64) >= 512 ? 4 : mean > 16 && s.tiles(32) >= 256 ? 2 : 1;
+}
 int nr_of(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
 
 // Rows a block of the outer products: 1024 blocks by columns, while each has 128 rows or
@@ -711,25 +721,22 @@ size_t hidden_bytes(const Shape &s, int64_t R) { return align256(sizeof(float) *
 template <typename T> gdn2_status launch_shrink(ShrinkParams p, const gdn2_low_rank_args &a, const Shape &sh, hipStream_t s) {
     const int mt = mt_of(sh), nr = nr_of(p.R);
     const int64_t tiles = sh.tiles(16 * mt);
-    const bool many = tiles >= 512;
+    const bool few = tiles < 512;
     p.req = requests_of(a, sh, 16 * mt);
     const dim3 grid((unsigned)tiles, (unsigned)up(p.R, 16 * nr));
-    // (sixteen waves of the widest tile would not have the registers)
-#define GDN2_RUN(MT, NR)                                                                                 \
-    do {                                                                                                 \
-        constexpr int W = MT * NR == 16 ? 8 : 16;                                                        \
-        if (many) hipLaunchKernelGGL((shrink_kernel<T, MT, NR, 4>), grid, dim3(256), 0, s, p);           \
-        else hipLaunchKernelGGL((shrink_kernel<T, MT, NR, W>), grid, dim3(64 * W), 0, s, p);             \
+#define GDN2_RUN(MT, NR, W) hipLaunchKernelGGL((shrink_kernel<T, MT, NR, (W)>), grid, dim3(64 * (W)), 0, s, p)
+// (sixteen waves of 64 ranks would not have the registers)
+#define GDN2_RANKS(MT, W)                     \
+    do {                                      \
+        if (nr == 1) GDN2_RUN(MT, 1, W);      \
+        else if (nr == 2) GDN2_RUN(MT, 2, W); \
+        else GDN2_RUN(MT, 4, (W > 8 ? 8 : W)); \
     } while (0)
-    if (mt == 4) {
-        if (nr == 1) GDN2_RUN(4, 1);
-        else if (nr == 2) GDN2_RUN(4, 2);
-        else GDN2_RUN(4, 4);
-    } else {
-        if (nr == 1) GDN2_RUN(1, 1);
-        else if (nr == 2) GDN2_RUN(1, 2);
-        else GDN2_RUN(1, 4);
-    }
+    if (mt == 4) GDN2_RANKS(4, 4);
+    else if (mt == 2) GDN2_RANKS(2, 8);
+    else if (few) GDN2_RANKS(1, 16);
+    else GDN2_RANKS(1, 4);
+#undef GDN2_RANKS
 #undef GDN2_RUN
     GDN2_HIP_CHECK(hipGetLastError());
     return GDN2_OK;
