@@ -3,10 +3,11 @@
 //   h = x a_l^T (a [L, R, D]),  out = y + s_l h b_l (b [L, R, O])
 //   dh = s_l dy b_l^T,  dx = dh a_l,  da_l = sum dh^T x,  db_l = s_l sum h^T dy
 //
-// Four kernels, each of which streams one wide tensor past matrix instructions:
-//   shrink  h or dh: rows of 16 MT by all ranks, the wide dimension split over the 4 to
-//           16 waves of a workgroup
-//   expand  out or dx: rows of 16 MT by 16 VC columns a wave, y read and out written once
+// Kernels:
+//   adapt   up to 64 ranks: h and out (or dh and dx) of 16 or 32 rows.  The waves of a
+//           workgroup share the wide dimension of h, then the columns of out; h stays in
+//           LDS.  Each wide tensor is read or written once.
+//   shrink, expand  the same in two launches, for more ranks
 //   outer   da, db: ranks by 16 VC columns a wave, a block of one request's rows
 //   sums    those of an adapter's blocks, in order, in f64
 // A tile of rows lies in one request.  Packed requests (cu_seqlens) may take
@@ -34,6 +35,18 @@ namespace gdn2 {
 namespace {
 
 typedef uint32_t uintx4 __attribute__((ext_vector_type(4)));
+
+// A place `bytes` behind one that is the same for every lane: 32 bits a lane.  (What the
+// lane holds is made opaque, or the compiler forms the 64-bit sums ahead of the loops and
+// keeps two registers for each.)
+template <typename T> __device__ __forceinline__ const T *behind(const T *p, uint32_t &bytes) {
+    asm("" : "+v"(bytes));
+    return reinterpret_cast<const T *>(reinterpret_cast<const char *>(p) + bytes);
+}
+template <typename T> __device__ __forceinline__ T *behind(T *p, uint32_t &bytes) {
+    asm("" : "+v"(bytes));
+    return reinterpret_cast<T *>(reinterpret_cast<char *>(p) + bytes);
+}
 
 template <typename T> struct Mm;
 template <> struct Mm<float> {
@@ -112,17 +125,17 @@ struct Requests {
     int N, L;     // requests, adapters
     int per;      // without cu: tiles a request
 };
-struct Tile {
-    int64_t b, t0, row; // batch entry, first token, its place among all rows
-    int rows;           // <= 0: none
-    int adapter;        // -1: none
+struct Tile { // (the same for every lane)
+    int b, t0, row; // batch entry, first token, its place among all rows
+    int rows;       // <= 0: none
+    int adapter;    // -1: none
 };
 
 // Row 0, the offsets, the end of the rows: requests 1 .. N between rows of none.
-__device__ __forceinline__ int64_t bound_at(const Requests &r, int n) {
+__device__ __forceinline__ int bound_at(const Requests &r, int n) {
     if (n == 0) return 0;
-    if (n == r.N + 2) return r.M;
-    return min(max((int64_t)r.cu[n - 1], (int64_t)0), r.M);
+    if (n == r.N + 2) return (int)r.M;
+    return min(max(r.cu[n - 1], 0), (int)r.M);
 }
 
 // Of the wave's tile w (the same for every lane) of up to `size` rows.
@@ -133,9 +146,9 @@ __device__ __forceinline__ Tile tile_at(const Requests &r, int w, int size) {
     if (!r.cu) {
         n = w / r.per;
         t.b = n;
-        t.t0 = (int64_t)(w - n * r.per) * size;
-        t.row = n * r.T + t.t0;
-        t.rows = (int)min((int64_t)size, r.T - t.t0);
+        t.t0 = (w - n * r.per) * size; // (the last request's last tile: < 2^30 + 64)
+        t.row = n * (int)r.T + t.t0;
+        t.rows = min(size, (int)r.T - t.t0);
     } else {
         // the last n with bound / size + n <= w: 64 at a time
         int lo = 0, len = r.N + 2;
@@ -148,15 +161,16 @@ __device__ __forceinline__ Tile tile_at(const Requests &r, int w, int size) {
             len = step == 1 ? 1 : min(step, end - lo);
         }
         n = __builtin_amdgcn_readfirstlane(lo);
-        const int64_t first = bound_at(r, n);
-        t.t0 = first + (w - (first / size + n)) * (int64_t)size;
-        t.row = t.t0;
-        t.rows = (int)max((int64_t)0, min((int64_t)size, bound_at(r, n + 1) - t.t0));
-        if (t.t0 < 0) t.rows = 0; // (offsets that decrease)
+        const int first = __builtin_amdgcn_readfirstlane(bound_at(r, n));
+        const int64_t t0 = first + (int64_t)(w - (first / size + n)) * size;
+        const int64_t rows = min((int64_t)size, __builtin_amdgcn_readfirstlane(bound_at(r, n + 1)) - t0);
+        if (t0 < 0 || rows <= 0) return t; // (offsets that decrease; a slot without a tile)
+        t.t0 = t.row = (int)t0;
+        t.rows = (int)rows;
         if (n == 0 || n == r.N + 1) return t;
         --n;
     }
-    const int id = r.adapters[n];
+    const int id = __builtin_amdgcn_readfirstlane(r.adapters[n]);
     if (id >= 0 && id < r.L) t.adapter = id;
     return t;
 }
@@ -173,76 +187,76 @@ struct ShrinkParams {
     int R, P;
 };
 
-// A wave takes 256 bytes of each of its rows at a time, 16 lanes a row, and turns them
+constexpr int kStagePitch = 17; // (16 bytes: a row's 16 and one)
+
+// acc of wave 0: the tile's rows by 16 NR ranks from r0 on.  lds: W MT 16 kStagePitch or
+// MT NR 64 W / 2 of 16 bytes.  A wave takes 256 bytes of each of its rows at a time, 16 lanes a row, and turns them
 // into operands through LDS of its own; the next ones' loads are in flight meanwhile.
 // (Operands loaded as they are used, 64 bytes of each of 16 rows a load, kept the same
 // tiles at 3.3 TB/s.)
-template <typename T, int MT, int NR, int W> __global__ __launch_bounds__(64 * W, W > 8 ? 4 : 2) void shrink_kernel(ShrinkParams p) {
+template <typename T, int MT, int NR, int W>
+__device__ __forceinline__ void shrink_rows(floatx4 *lds, const void *px, int64_t xb, int64_t xt, const void *pw, int64_t wl, int64_t wr,
+                                            int64_t K, int R, int r0, const Tile &at, floatx4 (&acc)[MT][NR]) {
     typedef Mm<T> X;
-    constexpr int KV = X::KV, STEP = 4 * KV, U = 4, CHUNK = U * STEP, PITCH = 17; // (16 bytes: a row's 16 and one)
-    constexpr int kStage = MT * 16 * PITCH, kSums = MT * NR * kWave * (W / 2);
-    __shared__ floatx4 lds[W * kStage > kSums ? W * kStage : kSums];
+    constexpr int KV = X::KV, STEP = 4 * KV, U = 4, CHUNK = U * STEP, kStageW = MT * 16 * kStagePitch;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int i = lane & 15, g = lane >> 4;
-    const int r0 = blockIdx.y * NR * 16;
-    const Tile at = tile_at(p.req, blockIdx.x, MT * 16);
-    if (at.rows <= 0) return;
-    floatx4 acc[MT][NR];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
         for (int n = 0; n < NR; ++n) acc[m][n] = floatx4{0.f, 0.f, 0.f, 0.f};
-    if (at.adapter >= 0) {
-        // (rows behind the tile's last, ranks behind the last: the last one's again, not stored)
-        const T *x = static_cast<const T *>(p.x) + at.b * p.xb + at.t0 * p.xt, *w[NR];
+    // (rows behind the tile's last, ranks behind the last: the last one's again, not stored)
+    const T *x = static_cast<const T *>(px) + (int64_t)at.b * xb + (int64_t)at.t0 * xt;
+    const T *w = static_cast<const T *>(pw) + (int64_t)at.adapter * wl + (int64_t)r0 * wr;
+    uint32_t xo[MT * 4], wo[NR];
 #pragma unroll
-        for (int n = 0; n < NR; ++n)
-            w[n] = static_cast<const T *>(p.w) + at.adapter * p.wl + min(r0 + 16 * n + i, p.R - 1) * p.wr + KV * g;
-        floatx4 *stage = lds + wave * kStage;
-        typename X::Op ahead[MT * 4], b[U][NR];
-        auto load_x = [&](int64_t k) {
+    for (int j = 0; j < MT * 4; ++j) xo[j] = (uint32_t)(min(4 * j + g, at.rows - 1) * (uint32_t)xt + KV * i) * sizeof(T);
 #pragma unroll
-            for (int j = 0; j < MT * 4; ++j) ahead[j] = loose<T, KV>(x + min(4 * j + g, at.rows - 1) * p.xt + k + KV * i);
-        };
-        auto load_w = [&](int64_t k, int s) {
+    for (int n = 0; n < NR; ++n) wo[n] = (uint32_t)(min(16 * n + i, R - 1 - r0) * (uint32_t)wr + KV * g) * sizeof(T);
+    floatx4 *stage = lds + wave * kStageW;
+    typename X::Op ahead[MT * 4], b[U][NR];
+    auto load_x = [&](int64_t k) {
 #pragma unroll
-            for (int n = 0; n < NR; ++n) b[s][n] = loose<T, KV>(w[n] + k + s * STEP);
-        };
-        int64_t k = (int64_t)wave * CHUNK;
-        if (k + CHUNK <= p.K) {
-            load_x(k);
+        for (int j = 0; j < MT * 4; ++j) ahead[j] = loose<T, KV>(behind(x + k, xo[j]));
+    };
+    auto load_w = [&](int64_t k, int s) {
 #pragma unroll
-            for (int s = 0; s < U; ++s) load_w(k, s);
-        }
-        for (; k + CHUNK <= p.K; k += W * CHUNK) {
+        for (int n = 0; n < NR; ++n) b[s][n] = loose<T, KV>(behind(w + k + s * STEP, wo[n]));
+    };
+    int64_t k = (int64_t)wave * CHUNK;
+    if (k + CHUNK <= K) {
+        load_x(k);
 #pragma unroll
-            for (int j = 0; j < MT * 4; ++j) stage[(4 * j + g) * PITCH + i] = __builtin_bit_cast(floatx4, ahead[j]);
-            const bool more = k + (W + 1) * CHUNK <= p.K;
-            const int64_t next = more ? k + W * CHUNK : k; // (the last chunk's again, not used)
-            load_x(next);
-            __builtin_amdgcn_wave_barrier(); // (one wave's LDS operations are done in order)
+        for (int s = 0; s < U; ++s) load_w(k, s);
+    }
+    for (; k + CHUNK <= K; k += W * CHUNK) {
 #pragma unroll
-            for (int s = 0; s < U; ++s) {
+        for (int j = 0; j < MT * 4; ++j) stage[(4 * j + g) * kStagePitch + i] = __builtin_bit_cast(floatx4, ahead[j]);
+        const bool more = k + (W + 1) * CHUNK <= K;
+        const int64_t next = more ? k + W * CHUNK : k; // (the last chunk's again, not used)
+        load_x(next);
+        __builtin_amdgcn_wave_barrier(); // (one wave's LDS operations are done in order)
 #pragma unroll
-                for (int m = 0; m < MT; ++m) {
-                    const typename X::Op a = __builtin_bit_cast(typename X::Op, stage[(16 * m + i) * PITCH + 4 * s + g]);
-#pragma unroll
-                    for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a, b[s][n], acc[m][n]);
-                }
-                load_w(next, s);
-            }
-            __builtin_amdgcn_wave_barrier();
-        }
-        for (; k < p.K; k += STEP) { // (one wave's, and less than a chunk)
-            const int64_t left = p.K - k - KV * g;
-#pragma unroll
-            for (int n = 0; n < NR; ++n) b[0][n] = loose_part<T, KV>(w[n] + k, left);
+        for (int s = 0; s < U; ++s) {
 #pragma unroll
             for (int m = 0; m < MT; ++m) {
-                const typename X::Op a = loose_part<T, KV>(x + min(16 * m + i, at.rows - 1) * p.xt + k + KV * g, left);
+                const typename X::Op a = __builtin_bit_cast(typename X::Op, stage[(16 * m + i) * kStagePitch + 4 * s + g]);
 #pragma unroll
-                for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a, b[0][n], acc[m][n]);
+                for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a, b[s][n], acc[m][n]);
             }
+            load_w(next, s);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    for (; k < K; k += STEP) { // (one wave's, and less than a chunk)
+        const int64_t left = K - k - KV * g;
+#pragma unroll
+        for (int n = 0; n < NR; ++n) b[0][n] = loose_part<T, KV>(behind(w + k, wo[n]), left);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const typename X::Op a = loose_part<T, KV>(x + min(16 * m + i, at.rows - 1) * xt + k + KV * g, left);
+#pragma unroll
+            for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a, b[0][n], acc[m][n]);
         }
     }
     // the waves' sums: the upper half's onto the lower, and so on
@@ -262,9 +276,26 @@ template <typename T, int MT, int NR, int W> __global__ __launch_bounds__(64 * W
 #pragma unroll
                 for (int n = 0; n < NR; ++n) acc[m][n] += red(wave, m * NR + n);
     }
-    if (wave) return;
+}
+
+template <typename T, int MT, int NR, int W> __global__ __launch_bounds__(64 * W, 2) void shrink_kernel(ShrinkParams p) {
+    constexpr int kStage = W * MT * 16 * kStagePitch, kSums = MT * NR * kWave * (W / 2);
+    __shared__ floatx4 lds[kStage > kSums ? kStage : kSums];
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, r0 = blockIdx.y * NR * 16;
+    const Tile at = tile_at(p.req, blockIdx.x, MT * 16);
+    if (at.rows <= 0) return;
+    floatx4 acc[MT][NR];
+    if (at.adapter >= 0) {
+        shrink_rows<T, MT, NR, W>(lds, p.x, p.xb, p.xt, p.w, p.wl, p.wr, p.K, p.R, r0, at, acc);
+    } else {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NR; ++n) acc[m][n] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    if (threadIdx.x >= 64) return;
     const float s = p.scale && at.adapter >= 0 ? p.scale[at.adapter] : 1.f;
-    float *h = p.h + at.row * p.P;
+    float *h = p.h + (int64_t)at.row * p.P;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -278,6 +309,8 @@ template <typename T, int MT, int NR, int W> __global__ __launch_bounds__(64 * W
 
 // -- expand ----------------------------------------------------------------------------
 
+constexpr int kExpandRows = 32;
+
 struct ExpandParams {
     Requests req;
     const float *h; // [M][P], zeros behind rank R
@@ -288,98 +321,17 @@ struct ExpandParams {
     float *hidden; // [M][R] h's copy for the caller, or NULL
     int64_t wl, wr, yb, yt, ob, ot;
     int64_t C;
-    int R, P, groups, size; // workgroups over the columns; rows a tile
+    int R, P, groups; // workgroups over the columns
     int copies; // rows without an adapter are written too (out is not y's memory)
 };
 
-// Up to KR steps of ranks: the wave's columns of b stay in registers while it walks rows
-// of 16, the next ones' y and h in flight.
-template <typename T, int KR, bool WHOLE>
-__device__ __forceinline__ void expand_walk(const ExpandParams &p, const Tile &at, int64_t c0, bool keep, bool write) {
-    typedef Mm<T> X;
-    constexpr int KV = X::KV, VC = X::VC, STEP = 4 * KV;
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int64_t c = WHOLE ? min(c0 + VC * i, p.C - VC) : c0 + VC * i, left = p.C - c;
-    auto cols_at = [&](const T *q) { return WHOLE ? loose<T, VC>(q) : loose_part<T, VC>(q, left); };
-    typename X::Op cols[KR][VC];
-    const T *w = static_cast<const T *>(p.w) + at.adapter * p.wl + c;
-#pragma unroll
-    for (int s = 0; s < KR; ++s) {
-        Raw<T, VC> rows[KV];
-        const int r = s * STEP + KV * g;
-#pragma unroll
-        for (int k = 0; k < KV; ++k) rows[k] = cols_at(w + (int64_t)min(r + k, p.R - 1) * p.wr);
-        if ((s + 1) * STEP > p.R) // behind the last rank: zeros
-#pragma unroll
-            for (int k = 0; k < KV; ++k)
-                if (r + k >= p.R)
-#pragma unroll
-                    for (int t = 0; t < VC; ++t) rows[k][t] = (T)0.f;
-        X::turn(rows, cols[s]);
-    }
-    const T *y = p.y ? static_cast<const T *>(p.y) + at.b * p.yb + at.t0 * p.yt + c : nullptr;
-    T *out = static_cast<T *>(p.out) + at.b * p.ob + at.t0 * p.ot + c;
-    const float scale = p.scale ? p.scale[at.adapter] : 1.f;
-    Raw<T, VC> old[4];
-    float h[KR][KV];
-    auto load = [&](int m) {
-        const float *hm = p.h + (at.row + min(m + i, at.rows - 1)) * p.P;
-#pragma unroll
-        for (int s = 0; s < KR; ++s) {
-            const int r = s * STEP + KV * g;
-            load_n<float, KV>(hm + min(r, p.P - KV), h[s]);
-            if ((s + 1) * STEP > p.P && r >= p.P)
-#pragma unroll
-                for (int k = 0; k < KV; ++k) h[s][k] = 0.f;
-        }
-        if (y)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) old[q] = cols_at(y + min(m + 4 * g + q, at.rows - 1) * p.yt);
-    };
-    load(0);
-    for (int m = 0; m < at.rows; m += 16) {
-        typename X::Wide hw[KR];
-#pragma unroll
-        for (int s = 0; s < KR; ++s) {
-            hw[s] = X::wide(h[s]);
-            const int r = s * STEP + KV * g;
-            if (keep && m + i < at.rows) store_part<float, KV>(p.hidden + (at.row + m + i) * p.R + r, p.R - r, h[s]);
-        }
-        Raw<T, VC> was[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) was[q] = old[q];
-        if (m + 16 < at.rows) load(m + 16);
-        floatx4 acc[VC];
-#pragma unroll
-        for (int t = 0; t < VC; ++t) {
-            acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < KR; ++s) acc[t] = X::mmw(hw[s], cols[s][t], acc[t]);
-        }
-        if (!write) continue;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int row = m + 4 * g + q;
-            if (row >= at.rows) continue;
-            float v[VC];
-#pragma unroll
-            for (int t = 0; t < VC; ++t) v[t] = __builtin_fmaf(scale, acc[t][q], y ? (float)was[q][t] : 0.f);
-            if constexpr (WHOLE) loose_store<T, VC>(out + row * p.ot, v);
-            else store_part<T, VC>(out + row * p.ot, left, v);
-        }
-    }
-}
-
 // Rows without an adapter: y as it is, NaN and all, or zeros.
-template <typename T> __device__ __forceinline__ void expand_copy(const ExpandParams &p, const Tile &at, int64_t c0, bool keep) {
+template <typename T, typename P> __device__ __forceinline__ void copy_columns(const P &p, const Tile &at, int64_t c0) {
     constexpr int VC = Mm<T>::VC;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int64_t c = c0 + VC * i, left = p.C - c;
-    if (keep)
-        for (int64_t k = lane; k < (int64_t)at.rows * p.R; k += kWave) p.hidden[at.row * p.R + k] = 0.f;
-    if (!p.copies) return;
-    const T *y = p.y ? static_cast<const T *>(p.y) + at.b * p.yb + at.t0 * p.yt + c : nullptr;
-    T *out = static_cast<T *>(p.out) + at.b * p.ob + at.t0 * p.ot + c;
+    const T *y = p.y ? static_cast<const T *>(p.y) + (int64_t)at.b * p.yb + (int64_t)at.t0 * p.yt + c : nullptr;
+    T *out = static_cast<T *>(p.out) + (int64_t)at.b * p.ob + (int64_t)at.t0 * p.ot + c;
     for (int row = g; row < at.rows; row += 4) {
         float v[VC];
 #pragma unroll
@@ -388,18 +340,22 @@ template <typename T> __device__ __forceinline__ void expand_copy(const ExpandPa
         store_part<T, VC>(out + row * p.ot, left, v);
     }
 }
+template <typename T> __device__ __forceinline__ void expand_copy(const ExpandParams &p, const Tile &at, int64_t c0, bool keep) {
+    if (keep)
+        for (int64_t k = threadIdx.x & 63; k < (int64_t)at.rows * p.R; k += kWave) p.hidden[(int64_t)at.row * p.R + k] = 0.f;
+    if (p.copies) copy_columns<T>(p, at, c0);
+}
 
-// KR 0: any number of ranks, steps of them for rows of 32 at a time.
 // WHOLE: VC columns or more are left.  A lane whose columns would end behind the last
 // takes the last VC ones: what another lane of the wave takes too, with the same result.
 template <typename T, int MT, bool WHOLE>
-__device__ __forceinline__ void expand_tile(const ExpandParams &p, const Tile &at, int64_t c0, bool keep, bool write) {
+__device__ __forceinline__ void expand_tile(const ExpandParams &p, const Tile &at, int64_t c0, bool keep) {
     typedef Mm<T> X;
     constexpr int KV = X::KV, VC = X::VC, STEP = 4 * KV;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
     const int64_t c = WHOLE ? min(c0 + VC * i, p.C - VC) : c0 + VC * i, left = p.C - c;
     auto cols_at = [&](const T *q) { return WHOLE ? loose<T, VC>(q) : loose_part<T, VC>(q, left); };
-    const T *w = static_cast<const T *>(p.w) + at.adapter * p.wl + c;
+    const T *w = static_cast<const T *>(p.w) + (int64_t)at.adapter * p.wl + c;
     Raw<T, VC> rows[KV];
     float h[MT][KV];
     auto load = [&](int r0) { // (behind the last rank: zeros)
@@ -408,7 +364,7 @@ __device__ __forceinline__ void expand_tile(const ExpandParams &p, const Tile &a
         for (int k = 0; k < KV; ++k) rows[k] = cols_at(w + (int64_t)min(r + k, p.R - 1) * p.wr);
 #pragma unroll
         for (int m = 0; m < MT; ++m)
-            load_n<float, KV>(p.h + (at.row + min(16 * m + i, at.rows - 1)) * p.P + min(r, p.P - KV), h[m]);
+            load_n<float, KV>(p.h + (int64_t)(at.row + min(16 * m + i, at.rows - 1)) * p.P + min(r, p.P - KV), h[m]);
         if (r0 + STEP > p.R) {
 #pragma unroll
             for (int k = 0; k < KV; ++k)
@@ -424,8 +380,8 @@ __device__ __forceinline__ void expand_tile(const ExpandParams &p, const Tile &a
     };
     load(0);
     Raw<T, VC> old[MT][4];
-    if (write && p.y) {
-        const T *y = static_cast<const T *>(p.y) + at.b * p.yb + at.t0 * p.yt + c;
+    if (p.y) {
+        const T *y = static_cast<const T *>(p.y) + (int64_t)at.b * p.yb + (int64_t)at.t0 * p.yt + c;
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -444,7 +400,7 @@ __device__ __forceinline__ void expand_tile(const ExpandParams &p, const Tile &a
         for (int m = 0; m < MT; ++m) {
             hw[m] = X::wide(h[m]);
             const int r = r0 + KV * g;
-            if (keep && 16 * m + i < at.rows) store_part<float, KV>(p.hidden + (at.row + 16 * m + i) * p.R + r, p.R - r, h[m]);
+            if (keep && 16 * m + i < at.rows) store_part<float, KV>(p.hidden + (int64_t)(at.row + 16 * m + i) * p.R + r, p.R - r, h[m]);
         }
         if (r0 + STEP < p.R) load(r0 + STEP);
 #pragma unroll
@@ -452,9 +408,8 @@ __device__ __forceinline__ void expand_tile(const ExpandParams &p, const Tile &a
 #pragma unroll
             for (int t = 0; t < VC; ++t) acc[m][t] = X::mmw(hw[m], cols[t], acc[m][t]);
     }
-    if (!write) return;
     const float s = p.scale ? p.scale[at.adapter] : 1.f;
-    T *out = static_cast<T *>(p.out) + at.b * p.ob + at.t0 * p.ot + c;
+    T *out = static_cast<T *>(p.out) + (int64_t)at.b * p.ob + (int64_t)at.t0 * p.ot + c;
 #pragma unroll
     for (int m = 0; m < MT; ++m)
 #pragma unroll
@@ -469,25 +424,180 @@ __device__ __forceinline__ void expand_tile(const ExpandParams &p, const Tile &a
         }
 }
 
-template <typename T, int KR> __global__ __launch_bounds__(256, 2) void expand_kernel(ExpandParams p) {
+template <typename T> __global__ __launch_bounds__(256, 2) void expand_kernel(ExpandParams p) {
     constexpr int VC = Mm<T>::VC;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int tile = blockIdx.x / p.groups, group = blockIdx.x - tile * p.groups;
     const int64_t c0 = (int64_t)(group * 4 + wave) * 16 * VC;
     if (c0 >= p.C && !(p.hidden && c0 == 0)) return;
-    const Tile at = tile_at(p.req, tile, p.size);
+    const Tile at = tile_at(p.req, tile, kExpandRows);
     if (at.rows <= 0) return;
-    const bool keep = p.hidden && c0 == 0, write = at.adapter >= 0 || p.copies, whole = p.C - c0 >= VC;
-    if (!keep && !write) return;
-    if (at.adapter < 0 || p.R == 0) {
-        expand_copy<T>(p, at, c0, keep);
-    } else if constexpr (KR > 0) {
-        if (whole) expand_walk<T, KR, true>(p, at, c0, keep, write);
-        else expand_walk<T, KR, false>(p, at, c0, keep, write);
-    } else {
-        if (whole) expand_tile<T, 2, true>(p, at, c0, keep, write);
-        else expand_tile<T, 2, false>(p, at, c0, keep, write);
+    const bool keep = p.hidden && c0 == 0;
+    if (at.adapter < 0 || p.R == 0) expand_copy<T>(p, at, c0, keep);
+    else if (p.C - c0 >= VC) expand_tile<T, kExpandRows / 16, true>(p, at, c0, keep);
+    else expand_tile<T, kExpandRows / 16, false>(p, at, c0, keep);
+}
+
+// -- adapt: both at once, up to 64 ranks -----------------------------------------------
+
+struct AdaptParams {
+    Requests req;
+    const void *x, *w1; // [.., K]; [L, R, K]
+    const void *w2, *y; // [L, R, C]; y or NULL
+    void *out;          // or NULL
+    const float *scale;
+    float *hidden; // [M][pitch] h for the caller, or NULL
+    int64_t xb, xt, w1l, w1r, w2l, w2r, yb, yt, ob, ot, pitch;
+    int64_t K, C;
+    int R;
+    int copies;        // rows without an adapter are written too (out is not y's memory)
+    int scale_hidden;  // hidden times the scale (dh)
+};
+
+// h of a tile in LDS, as the second product's operands.
+template <typename T, int MT, int NR> struct Kept;
+template <int MT, int NR> struct Kept<float, MT, NR> {
+    static constexpr int KR = NR, PITCH = 16 * NR + 4;
+    static constexpr int BYTES = MT * 16 * PITCH * 4;
+    static __device__ __forceinline__ void put(void *lds, int row, int r, float v) { static_cast<float *>(lds)[row * PITCH + r] = v; }
+    static __device__ __forceinline__ Mm<float>::Wide get(const void *lds, int row, int r) {
+        return *reinterpret_cast<const Mm<float>::Op *>(static_cast<const float *>(lds) + row * PITCH + r);
     }
+};
+template <int MT, int NR> struct Kept<bf16, MT, NR> { // three planes of terms
+    static constexpr int KR = (NR + 1) / 2, PITCH = 32 * KR + 8, PLANE = MT * 16 * PITCH;
+    static constexpr int BYTES = 3 * PLANE * 2;
+    static __device__ __forceinline__ void put(void *lds, int row, int r, float v) {
+        uint16_t *to = static_cast<uint16_t *>(lds) + row * PITCH + r;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const uint32_t u = __builtin_bit_cast(uint32_t, v);
+            to[k * PLANE] = (uint16_t)(u >> 16);
+            v = fabsf(v) < __builtin_inff() ? v - __builtin_bit_cast(float, u & 0xFFFF0000u) : 0.f;
+        }
+    }
+    static __device__ __forceinline__ Mm<bf16>::Wide get(const void *lds, int row, int r) {
+        Mm<bf16>::Wide w;
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            w.t[k] = *reinterpret_cast<const Mm<bf16>::Op *>(static_cast<const uint16_t *>(lds) + k * PLANE + row * PITCH + r);
+        return w;
+    }
+};
+
+// One wave's 16 VC columns of a tile's rows.
+template <typename T, int MT, int NR, bool WHOLE>
+__device__ __forceinline__ void adapt_columns(const AdaptParams &p, const Tile &at, const void *kept, int64_t c0) {
+    typedef Mm<T> X;
+    typedef Kept<T, MT, NR> H;
+    constexpr int KV = X::KV, VC = X::VC, STEP = 4 * KV, KR = H::KR;
+    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+    const int c = WHOLE ? min(VC * i, (int)min(p.C - VC - c0, (int64_t)(16 * VC))) : VC * i; // from c0
+    const int64_t left = p.C - c0 - c;
+    auto cols_at = [&](const T *q) { return WHOLE ? loose<T, VC>(q) : loose_part<T, VC>(q, left); };
+    const T *w = static_cast<const T *>(p.w2) + (int64_t)at.adapter * p.w2l + c0;
+    typename X::Op cols[KR][VC];
+    Raw<T, VC> old[MT][4];
+    {
+        Raw<T, VC> rows[KR][KV];
+#pragma unroll
+        for (int s = 0; s < KR; ++s)
+#pragma unroll
+            for (int k = 0; k < KV; ++k) {
+                uint32_t o = (uint32_t)(min(s * STEP + KV * g + k, p.R - 1) * (uint32_t)p.w2r + c) * sizeof(T);
+                rows[s][k] = cols_at(behind(w, o));
+            }
+        if (p.y) {
+            const T *y = static_cast<const T *>(p.y) + (int64_t)at.b * p.yb + (int64_t)at.t0 * p.yt + c0;
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t o = (uint32_t)(min(16 * m + 4 * g + q, at.rows - 1) * (uint32_t)p.yt + c) * sizeof(T);
+                    old[m][q] = cols_at(behind(y, o));
+                }
+        }
+#pragma unroll
+        for (int s = 0; s < KR; ++s) {
+            if ((s + 1) * STEP > p.R) // behind the last rank: zeros
+#pragma unroll
+                for (int k = 0; k < KV; ++k)
+                    if (s * STEP + KV * g + k >= p.R)
+#pragma unroll
+                        for (int t = 0; t < VC; ++t) rows[s][k][t] = (T)0.f;
+            X::turn(rows[s], cols[s]);
+        }
+    }
+    T *out = static_cast<T *>(p.out) + (int64_t)at.b * p.ob + (int64_t)at.t0 * p.ot + c0;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+        if (16 * m >= at.rows) break;
+        typename X::Wide hw[KR];
+#pragma unroll
+        for (int s = 0; s < KR; ++s) hw[s] = H::get(kept, 16 * m + i, s * STEP + KV * g);
+        floatx4 acc[VC];
+#pragma unroll
+        for (int t = 0; t < VC; ++t) {
+            acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int s = 0; s < KR; ++s) acc[t] = X::mmw(hw[s], cols[s][t], acc[t]);
+        }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int row = 16 * m + 4 * g + q;
+            if (row >= at.rows) continue;
+            float v[VC];
+#pragma unroll
+            for (int t = 0; t < VC; ++t) v[t] = acc[t][q] + (p.y ? (float)old[m][q][t] : 0.f);
+            uint32_t o = (uint32_t)(row * (uint32_t)p.ot + c) * sizeof(T);
+            T *to = behind(out, o);
+            if constexpr (WHOLE) loose_store<T, VC>(to, v);
+            else store_part<T, VC>(to, left, v);
+        }
+    }
+}
+
+template <typename T, int MT, int NR, int W, int WPE> __global__ __launch_bounds__(64 * W, WPE) void adapt_kernel(AdaptParams p) {
+    typedef Mm<T> X;
+    typedef Kept<T, MT, NR> H;
+    constexpr int VC = X::VC, kStage = W * MT * 16 * kStagePitch * 16, kSums = MT * NR * kWave * (W / 2) * 16;
+    constexpr int kLds = (kStage > kSums ? kStage : kSums) > H::BYTES ? (kStage > kSums ? kStage : kSums) : H::BYTES;
+    __shared__ __attribute__((aligned(16))) char lds[kLds];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    const Tile at = tile_at(p.req, blockIdx.x, MT * 16);
+    if (at.rows <= 0) return;
+    if (at.adapter < 0) {
+        if (p.hidden)
+            for (int k = threadIdx.x; k < at.rows * p.R; k += 64 * W) p.hidden[(int64_t)(at.row + k / p.R) * p.pitch + k % p.R] = 0.f;
+        if (p.out && p.copies)
+            for (int64_t c0 = (int64_t)wave * 16 * VC; c0 < p.C; c0 += W * 16 * VC) copy_columns<T>(p, at, c0);
+        return;
+    }
+    floatx4 acc[MT][NR];
+    shrink_rows<T, MT, NR, W>(reinterpret_cast<floatx4 *>(lds), p.x, p.xb, p.xt, p.w1, p.w1l, p.w1r, p.K, p.R, 0, at, acc);
+    __syncthreads(); // the last sums have been read
+    if (wave == 0) {
+        const float s = p.scale ? p.scale[at.adapter] : 1.f;
+        // (bfloat16: a step of 32 ranks, of which 16 may be beyond the tiles: zeros)
+        constexpr int NZ = H::KR * 4 * X::KV / 16;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NZ; ++n)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int row = 16 * m + 4 * g + q, r = 16 * n + i;
+                    const float v = n < NR && r < p.R ? acc[m][n < NR ? n : 0][q] : 0.f;
+                    H::put(lds, row, r, s * v);
+                    if (p.hidden && row < at.rows && r < p.R) p.hidden[(int64_t)(at.row + row) * p.pitch + r] = p.scale_hidden ? s * v : v;
+                }
+    }
+    if (!p.out) return;
+    __syncthreads();
+    for (int64_t c0 = (int64_t)wave * 16 * VC; c0 < p.C; c0 += W * 16 * VC)
+        if (p.C - c0 >= VC) adapt_columns<T, MT, NR, true>(p, at, lds, c0);
+        else adapt_columns<T, MT, NR, false>(p, at, lds, c0);
 }
 
 // -- outer -----------------------------------------------------------------------------
@@ -514,11 +624,11 @@ __device__ __forceinline__ void outer_tile(const OuterParams &p, const Tile &at,
     const int i = lane & 15, g = lane >> 4, ws = wave % WS, ms = wave / WS;
     const int r0 = (rs * WS + ws) * NR * 16;
     const int64_t C = p.C[which], c = WHOLE ? min(c0 + VC * i, C - VC) : c0 + VC * i, left = C - c;
-    const T *z = static_cast<const T *>(p.z[which]) + at.b * p.zb[which] + at.t0 * p.zt[which] + c;
+    const T *z = static_cast<const T *>(p.z[which]) + (int64_t)at.b * p.zb[which] + (int64_t)at.t0 * p.zt[which] + c;
     const int64_t zt = p.zt[which], pitch = p.pitch[which];
     const float *h[NR];
 #pragma unroll
-    for (int n = 0; n < NR; ++n) h[n] = p.h[which] + at.row * pitch + min(r0 + 16 * n + i, p.R - 1);
+    for (int n = 0; n < NR; ++n) h[n] = p.h[which] + (int64_t)at.row * pitch + min(r0 + 16 * n + i, p.R - 1);
     floatx4 acc[NR][VC];
 #pragma unroll
     for (int n = 0; n < NR; ++n)
@@ -691,14 +801,6 @@ Requests requests_of(const gdn2_low_rank_args &a, const Shape &s, int size) {
     return r;
 }
 
-// Row tiles of 16 mt in shrink: the larger, the fewer times an adapter is read from the
-// caches; but no more than a request has, and while there are enough.
-int mt_of(const Shape &s) {
-    const int64_t mean = s.N > 0 ? up(s.M, s.N) : 1;
-    return mean > 32 && s.tiles(64) >= 512 ? 4 : mean > 16 && s.tiles(32) >= 256 ? 2 : 1;
-}
-int nr_of(int64_t R) { return R <= 16 ? 1 : R <= 32 ? 2 : 4; }
-
 // Rows a block of the outer products: 1024 blocks by columns, while each has 128 rows or
 // more and at most 4096.
 int block_rows(const Shape &s, int64_t columns, int tile_columns) {
@@ -714,57 +816,69 @@ bool sizes_ok(const gdn2_low_rank_args &a) {
            a.in_features < (1 << 24) && a.out_features < (1 << 24) && a.num_adapters < (1 << 24);
 }
 
+
 int64_t pitch_of(int64_t R) { return up(R, 16) * 16; }
 // Bytes of h.
 size_t hidden_bytes(const Shape &s, int64_t R) { return align256(sizeof(float) * (size_t)s.M * (size_t)pitch_of(R)); }
 
-template <typename T> gdn2_status launch_shrink(ShrinkParams p, const gdn2_low_rank_args &a, const Shape &sh, hipStream_t s) {
-    const int mt = mt_of(sh), nr = nr_of(p.R);
-    const int64_t tiles = sh.tiles(16 * mt);
-    const bool few = tiles < 512;
-    p.req = requests_of(a, sh, 16 * mt);
-    const dim3 grid((unsigned)tiles, (unsigned)up(p.R, 16 * nr));
-#define GDN2_RUN(MT, NR, W) hipLaunchKernelGGL((shrink_kernel<T, MT, NR, (W)>), grid, dim3(64 * (W)), 0, s, p)
-// (sixteen waves of 64 ranks would not have the registers)
-#define GDN2_RANKS(MT, W)                     \
-    do {                                      \
-        if (nr == 1) GDN2_RUN(MT, 1, W);      \
-        else if (nr == 2) GDN2_RUN(MT, 2, W); \
-        else GDN2_RUN(MT, 4, (W > 8 ? 8 : W)); \
-    } while (0)
-    if (mt == 4) GDN2_RANKS(4, 4);
-    else if (mt == 2) GDN2_RANKS(2, 8);
-    else if (few) GDN2_RANKS(1, 16);
-    else GDN2_RANKS(1, 4);
-#undef GDN2_RANKS
+constexpr int kFusedRank = 64; // ranks that adapt's tiles hold
+
+// Rows a tile of adapt: 32 for requests of more than 16 rows, while there are 128 of them.
+int adapt_rows(const Shape &s) { return s.N > 0 && up(s.M, s.N) > 16 && s.tiles(32) >= 128 ? 32 : 16; }
+
+template <typename T> gdn2_status launch_adapt(AdaptParams p, const gdn2_low_rank_args &a, const Shape &sh, hipStream_t s) {
+    const int size = adapt_rows(sh);
+    const int64_t tiles = sh.tiles(size);
+    p.req = requests_of(a, sh, size);
+#define GDN2_RUN(MT, NR, W, WPE) hipLaunchKernelGGL((adapt_kernel<T, MT, NR, W, WPE>), dim3((unsigned)tiles), dim3(64 * W), 0, s, p)
+    // (sixteen waves of 64 ranks would not have the registers)
+    if (size == 32 && tiles >= 512) {
+        if (p.R <= 16) GDN2_RUN(2, 1, 4, 3);
+        else if (p.R <= 32) GDN2_RUN(2, 2, 4, 3);
+        else GDN2_RUN(2, 4, 4, 2);
+    } else if (size == 32) {
+        if (p.R <= 16) GDN2_RUN(2, 1, 8, 2);
+        else if (p.R <= 32) GDN2_RUN(2, 2, 8, 2);
+        else GDN2_RUN(2, 4, 8, 2);
+    } else if (tiles >= 1024) {
+        if (p.R <= 16) GDN2_RUN(1, 1, 4, 4);
+        else if (p.R <= 32) GDN2_RUN(1, 2, 4, 4);
+        else GDN2_RUN(1, 4, 4, 2);
+    } else {
+        if (p.R <= 16) GDN2_RUN(1, 1, 16, 4);
+        else if (p.R <= 32) GDN2_RUN(1, 2, 16, 4);
+        else GDN2_RUN(1, 4, 8, 2);
+    }
 #undef GDN2_RUN
     GDN2_HIP_CHECK(hipGetLastError());
     return GDN2_OK;
 }
 
-// Rows a tile in expand: 64 (32 where the ranks do not fit the registers), 16 for requests
-// so short.
-int expand_rows(const Shape &s, int64_t R) { return s.N > 0 && up(s.M, s.N) > 16 ? (R > 64 ? 32 : 64) : 16; }
+// More ranks: 64 of them a workgroup in shrink.
+int shrink_rows_of(const Shape &s) { return s.N > 0 && up(s.M, s.N) > 32 && s.tiles(64) >= 512 ? 64 : 16; }
+template <typename T> gdn2_status launch_shrink(ShrinkParams p, const gdn2_low_rank_args &a, const Shape &sh, hipStream_t s) {
+    const int size = shrink_rows_of(sh);
+    p.req = requests_of(a, sh, size);
+    const dim3 grid((unsigned)sh.tiles(size), (unsigned)up(p.R, 64));
+    if (size == 64) hipLaunchKernelGGL((shrink_kernel<T, 4, 4, 4>), grid, dim3(256), 0, s, p);
+    else hipLaunchKernelGGL((shrink_kernel<T, 1, 4, 8>), grid, dim3(512), 0, s, p);
+    GDN2_HIP_CHECK(hipGetLastError());
+    return GDN2_OK;
+}
+
 template <typename T> int64_t groups_of(int64_t C) { return std::max<int64_t>(1, up(C, 4 * 16 * Mm<T>::VC)); }
 
 template <typename T> gdn2_status launch_expand(ExpandParams p, const gdn2_low_rank_args &a, const Shape &sh, hipStream_t s) {
-    constexpr int STEP = 4 * Mm<T>::KV;
-    p.size = expand_rows(sh, p.R);
-    p.req = requests_of(a, sh, p.size);
+    p.req = requests_of(a, sh, kExpandRows);
     p.groups = (int)groups_of<T>(p.C);
-    const dim3 grid((unsigned)(sh.tiles(p.size) * p.groups));
-#define GDN2_RUN(KR) hipLaunchKernelGGL((expand_kernel<T, KR>), grid, dim3(256), 0, s, p)
-    if (p.R <= STEP) GDN2_RUN(1);
-    else if (p.R <= 2 * STEP) GDN2_RUN(2);
-    else if (p.R <= 64) GDN2_RUN(64 / STEP);
-    else GDN2_RUN(0);
-#undef GDN2_RUN
+    hipLaunchKernelGGL((expand_kernel<T>), dim3((unsigned)(sh.tiles(kExpandRows) * p.groups)), dim3(256), 0, s, p);
     GDN2_HIP_CHECK(hipGetLastError());
     return GDN2_OK;
 }
 
 template <typename T> bool grids_ok(const Shape &sh, int64_t C, int64_t R) {
-    return sh.tiles(16 * mt_of(sh)) < (1 << 22) && sh.tiles(expand_rows(sh, R)) * groups_of<T>(C) < (1 << 24);
+    if (R > 0 && R <= kFusedRank) return sh.tiles(adapt_rows(sh)) < (1 << 22);
+    return sh.tiles(shrink_rows_of(sh)) < (1 << 23) && sh.tiles(kExpandRows) * groups_of<T>(C) < (1 << 24);
 }
 
 gdn2_status check(const gdn2_low_rank_args *a, const std::string &who) {
@@ -773,6 +887,11 @@ gdn2_status check(const gdn2_low_rank_args *a, const std::string &who) {
         return fail(GDN2_EINVAL, who + "negative dimension");
     if (a->cu_seqlens && (a->batch != 1 || a->num_seqs < 0))
         return fail(GDN2_EINVAL, who + "packed requests need a batch of 1");
+    for (const int64_t stride : {a->stride_x_b, a->stride_x_t, a->stride_y_b, a->stride_y_t, a->stride_out_b, a->stride_out_t,
+                                 a->stride_a_l, a->stride_a_r, a->stride_b_l, a->stride_b_r})
+        if (stride < 0) return fail(GDN2_EINVAL, who + "negative stride");
+    for (const int64_t stride : {a->stride_x_t, a->stride_y_t, a->stride_out_t, a->stride_a_r, a->stride_b_r})
+        if (stride >= (1 << 24)) return fail(GDN2_NOT_APPLICABLE, who + "rows too far apart");
     if (!sizes_ok(*a)) return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
     return GDN2_OK;
 }
@@ -794,6 +913,16 @@ template <typename T> gdn2_status forward(const gdn2_low_rank_args *a, hipStream
     if (O > 0 && a->out == a->y && ((a->batch > 1 && a->stride_out_b != a->stride_y_b) || (a->seq_len > 1 && a->stride_out_t != a->stride_y_t)))
         return fail(GDN2_EINVAL, who + "in place, the strides must be equal");
     if (!grids_ok<T>(sh, O, R)) return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
+    if (R > 0 && R <= kFusedRank) {
+        AdaptParams p{};
+        p.x = a->x; p.w1 = a->a; p.w2 = a->b; p.y = a->y; p.out = O > 0 ? a->out : nullptr; p.scale = a->scale; p.hidden = a->hidden;
+        p.xb = a->stride_x_b; p.xt = a->stride_x_t; p.w1l = a->stride_a_l; p.w1r = a->stride_a_r;
+        p.w2l = a->stride_b_l; p.w2r = a->stride_b_r; p.yb = a->stride_y_b; p.yt = a->stride_y_t;
+        p.ob = a->stride_out_b; p.ot = a->stride_out_t; p.pitch = R;
+        p.K = D; p.C = O; p.R = (int)R;
+        p.copies = a->out != a->y;
+        return launch_adapt<T>(p, *a, sh, s);
+    }
     if (!workspace_ok(a->workspace, a->workspace_bytes, R > 0 ? hidden_bytes(sh, R) : 0))
         return fail(GDN2_EINVAL, who + "workspace missing, too small or not 256-byte aligned");
     float *h = static_cast<float *>(a->workspace);
@@ -838,6 +967,9 @@ template <typename T> gdn2_status backward(const gdn2_low_rank_bwd_args *b, hipS
     const gdn2_low_rank_args *a = b ? &b->fwd : nullptr;
     gdn2_status st = check(a, who);
     if (st != GDN2_OK) return st;
+    if (b->stride_d_out_b < 0 || b->stride_d_out_t < 0 || b->stride_dx_b < 0 || b->stride_dx_t < 0)
+        return fail(GDN2_EINVAL, who + "negative stride");
+    if (b->stride_d_out_t >= (1 << 24) || b->stride_dx_t >= (1 << 24)) return fail(GDN2_NOT_APPLICABLE, who + "rows too far apart");
     const Shape sh = shape_of(*a);
     const int64_t D = a->in_features, O = a->out_features, R = a->rank, L = a->num_adapters;
     const BwdPlan p = bwd_plan<T>(*b);
@@ -862,14 +994,24 @@ template <typename T> gdn2_status backward(const gdn2_low_rank_bwd_args *b, hipS
         int *ids = reinterpret_cast<int *>(ws);
         ws += p.ids;
         const int P = (int)pitch_of(R);
-        if (R > 0 && (b->dx || b->da)) {
+        if (R > 0 && R <= kFusedRank) {
+            AdaptParams k{};
+            k.x = b->d_out; k.w1 = a->b; k.w2 = a->a; k.y = b->accumulate_dx ? b->dx : nullptr; k.out = D > 0 ? b->dx : nullptr;
+            k.scale = a->scale; k.hidden = b->da ? dh : nullptr; k.scale_hidden = 1;
+            k.xb = b->stride_d_out_b; k.xt = b->stride_d_out_t; k.w1l = a->stride_b_l; k.w1r = a->stride_b_r;
+            k.w2l = a->stride_a_l; k.w2r = a->stride_a_r; k.yb = k.ob = b->stride_dx_b; k.yt = k.ot = b->stride_dx_t; k.pitch = P;
+            k.K = O; k.C = D; k.R = (int)R;
+            k.copies = !b->accumulate_dx;
+            if ((k.out || k.hidden) && (st = launch_adapt<T>(k, *a, sh, s)) != GDN2_OK) return st;
+        }
+        if (R > kFusedRank && (b->dx || b->da)) {
             ShrinkParams k{};
             k.x = b->d_out; k.w = a->b; k.scale = a->scale; k.h = dh;
             k.xb = b->stride_d_out_b; k.xt = b->stride_d_out_t; k.wl = a->stride_b_l; k.wr = a->stride_b_r;
             k.K = O; k.R = (int)R; k.P = P;
             if ((st = launch_shrink<T>(k, *a, sh, s)) != GDN2_OK) return st;
         }
-        if (b->dx && D > 0) {
+        if ((R > kFusedRank || R == 0) && b->dx && D > 0) {
             ExpandParams k{};
             k.h = dh; k.w = a->a; k.y = b->accumulate_dx ? b->dx : nullptr; k.out = b->dx;
             k.wl = a->stride_a_l; k.wr = a->stride_a_r;
@@ -914,7 +1056,7 @@ bool countable(const gdn2_low_rank_args &a) {
 }  // namespace gdn2
 
 extern "C" size_t gdn2_low_rank_add_workspace_bytes(const gdn2_low_rank_args *a) {
-    return a && gdn2::countable(*a) ? gdn2::hidden_bytes(gdn2::shape_of(*a), a->rank) : 0;
+    return a && gdn2::countable(*a) && a->rank > gdn2::kFusedRank ? gdn2::hidden_bytes(gdn2::shape_of(*a), a->rank) : 0;
 }
 // (the larger of the two types')
 extern "C" size_t gdn2_low_rank_add_bwd_workspace_bytes(const gdn2_low_rank_bwd_args *b) {

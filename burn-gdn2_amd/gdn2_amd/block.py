@@ -371,8 +371,11 @@ def _adapters_check(x, a, b, adapters, scale, cu_seqlens, others) -> None:
             raise ValueError("scale must be [L]")
 
 
-def _rowed(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    return t if t is None or t.shape[-1] == 1 or t.stride(-1) == 1 else t.contiguous()
+def _rowed(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy, with contiguous channels and its rows no further apart than the
+    kernels take."""
+    near = t.dim() == 2 or t.shape[1] <= 1 or t.stride(1) < 1 << 24
+    return t if near and (t.shape[-1] == 1 or t.stride(-1) == 1) else t.contiguous()
 
 
 def _bt(t: Optional[torch.Tensor]) -> Tuple[int, int]:
@@ -380,7 +383,7 @@ def _bt(t: Optional[torch.Tensor]) -> Tuple[int, int]:
     if t is None:
         return 0, 0
     s = t.stride()
-    return (s[0], s[1]) if len(s) == 3 else (s[0], 0)
+    return (s[0], s[1] if t.shape[1] > 1 else 0) if len(s) == 3 else (s[0], 0)
 
 
 def _low_rank_args(x, a, b, y, out, adapters, scale, cu_seqlens, hidden):
@@ -388,7 +391,7 @@ def _low_rank_args(x, a, b, y, out, adapters, scale, cu_seqlens, hidden):
     L, R, D = a.shape
     return C.LowRankArgs(_p(x), _p(a), _p(b), _p(y), _p(out), _p(adapters), _p(cu_seqlens), _p(scale), _p(hidden), B, T, D,
                          b.shape[2], R, L, 0 if cu_seqlens is None else cu_seqlens.shape[0] - 1, *_bt(x), *_bt(y), *_bt(out),
-                         a.stride(0), a.stride(1), b.stride(0), b.stride(1), None, 0)
+                         a.stride(0), a.stride(1) if R > 1 else 0, b.stride(0), b.stride(1) if R > 1 else 0, None, 0)
 
 
 def low_rank_add(y, x, a, b, adapters, scale=None, cu_seqlens=None, return_hidden: bool = False, out=None, workspace=None):

@@ -157,8 +157,9 @@ GDN2_API gdn2_status gdn2_residual_norm_bwd_f32_bf16(const gdn2_residual_norm_bw
  * unspecified results, never an access out of bounds.
  * out may be y with the same strides, nothing else may overlap.
  * workspace: gdn2_low_rank_add_workspace_bytes(args) bytes, 256-byte aligned.
- * Limits (else GDN2_NOT_APPLICABLE): R <= 512; D, O, L, num_seqs < 2^24; B T < 2^30;
- * B T O < 2^36 for long requests, less for short ones.
+ * Limits (else GDN2_NOT_APPLICABLE): R <= 512; D, O, L, num_seqs < 2^24; B T < 2^30,
+ * and 2^26 for requests of up to 16 tokens; strides of tokens and ranks < 2^24 (none
+ * negative: GDN2_EINVAL).
  * ---------------------------------------------------------------------- */
 typedef struct gdn2_low_rank_args {
     const void *x, *a, *b, *y;

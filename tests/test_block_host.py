@@ -230,8 +230,8 @@ def test_low_rank_refusals_of_the_c_entry():
         assert fn(None, None) == C.GDN2_EINVAL
         for bad in (dict(batch=-1), dict(seq_len=-1), dict(in_features=-1), dict(out_features=-1), dict(rank=-1), dict(num_adapters=-1),
                     dict(x=None), dict(a=None), dict(b=None), dict(y=None), dict(out=None), dict(adapters=None),
-                    dict(cu_seqlens=256, num_seqs=1), dict(cu_seqlens=256, batch=1, num_seqs=-1), dict(workspace=None),
-                    dict(workspace=264), dict(workspace_bytes=8), dict(out=256, stride_out_t=8)):
+                    dict(cu_seqlens=256, num_seqs=1), dict(cu_seqlens=256, batch=1, num_seqs=-1), dict(rank=65, workspace=None),
+                    dict(rank=65, workspace=264), dict(rank=65, workspace_bytes=8), dict(out=256, stride_out_t=8)):
             assert fn(_lora(**bad), None) == C.GDN2_EINVAL, bad
             assert b"gdn2_low_rank_add" in L.gdn2_last_error()
         for big in (dict(rank=513), dict(in_features=1 << 24), dict(out_features=1 << 24), dict(batch=1 << 20, seq_len=1 << 20),
@@ -264,8 +264,8 @@ def test_low_rank_workspace_sizes():
     size = lambda **kw: L.gdn2_low_rank_add_workspace_bytes(_lora(**kw))  # noqa: E731
     assert L.gdn2_low_rank_add_workspace_bytes(None) == L.gdn2_low_rank_add_bwd_workspace_bytes(None) == 0
     assert size(batch=0) == size(rank=0) == size(rank=513) == size(seq_len=-1) == 0
-    # h in f32, rows of a multiple of 16 ranks
-    assert size(batch=8, seq_len=4096) == 4 * 8 * 4096 * 16 and size(batch=64, seq_len=1, rank=17) == 4 * 64 * 32
+    # more than 64 ranks: h in f32, rows of a multiple of 16
+    assert size(batch=8, seq_len=4096, rank=64) == 0 and size(batch=64, seq_len=1, rank=65) == 4 * 64 * 80
 
 
 def test_low_rank_refusals_in_python():
