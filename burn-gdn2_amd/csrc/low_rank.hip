@@ -460,6 +460,7 @@ template <int MT, int NR> struct Kept<float, MT, NR> {
     static constexpr int KR = NR, PITCH = 16 * NR + 4;
     static constexpr int BYTES = MT * 16 * PITCH * 4;
     static __device__ __forceinline__ void put(void *lds, int row, int r, float v) { static_cast<float *>(lds)[row * PITCH + r] = v; }
+    static __device__ __forceinline__ float value(const void *lds, int row, int r) { return static_cast<const float *>(lds)[row * PITCH + r]; }
     static __device__ __forceinline__ Mm<float>::Wide get(const void *lds, int row, int r) {
         return *reinterpret_cast<const Mm<float>::Op *>(static_cast<const float *>(lds) + row * PITCH + r);
     }
@@ -476,6 +477,13 @@ template <int MT, int NR> struct Kept<bf16, MT, NR> { // three planes of terms
             v = fabsf(v) < __builtin_inff() ? v - __builtin_bit_cast(float, u & 0xFFFF0000u) : 0.f;
         }
     }
+    static __device__ __forceinline__ float value(const void *lds, int row, int r) {
+        const uint16_t *from = static_cast<const uint16_t *>(lds) + row * PITCH + r;
+        float v = 0.f;
+#pragma unroll
+        for (int k = 2; k >= 0; --k) v += __builtin_bit_cast(float, (uint32_t)from[k * PLANE] << 16);
+        return v;
+    }
     static __device__ __forceinline__ Mm<bf16>::Wide get(const void *lds, int row, int r) {
         Mm<bf16>::Wide w;
 #pragma unroll
@@ -485,38 +493,50 @@ template <int MT, int NR> struct Kept<bf16, MT, NR> { // three planes of terms
     }
 };
 
-// One wave's 16 VC columns of a tile's rows.
-template <typename T, int MT, int NR, bool WHOLE>
+// A wave's columns of a tile's rows: 16 VC of every W times as many, the next ones' y
+// (and b, where the registers do) in flight.
+// (Fewer than VC columns behind the last whole tile are adapt_rest's.)
+template <typename T, int MT, int NR, int W>
 __device__ __forceinline__ void adapt_columns(const AdaptParams &p, const Tile &at, const void *kept, int64_t c0) {
     typedef Mm<T> X;
     typedef Kept<T, MT, NR> H;
-    constexpr int KV = X::KV, VC = X::VC, STEP = 4 * KV, KR = H::KR;
+    constexpr int KV = X::KV, VC = X::VC, STEP = 4 * KV, KR = H::KR, NEXT = W * 16 * VC;
+    constexpr bool AHEAD = sizeof(T) == 4 && NR <= 2;
     const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const int c = WHOLE ? min(VC * i, (int)min(p.C - VC - c0, (int64_t)(16 * VC))) : VC * i; // from c0
-    const int64_t left = p.C - c0 - c;
-    auto cols_at = [&](const T *q) { return WHOLE ? loose<T, VC>(q) : loose_part<T, VC>(q, left); };
-    const T *w = static_cast<const T *>(p.w2) + (int64_t)at.adapter * p.w2l + c0;
-    typename X::Op cols[KR][VC];
-    Raw<T, VC> old[MT][4];
-    {
-        Raw<T, VC> rows[KR][KV];
+    const T *w = static_cast<const T *>(p.w2) + (int64_t)at.adapter * p.w2l;
+    const T *y = p.y ? static_cast<const T *>(p.y) + (int64_t)at.b * p.yb + (int64_t)at.t0 * p.yt : nullptr;
+    T *out = static_cast<T *>(p.out) + (int64_t)at.b * p.ob + (int64_t)at.t0 * p.ot;
+    // a lane's columns from c0 on: where they would end behind the last, the last VC
+    auto place = [&](int64_t c0) { return min(VC * i, (int)min(p.C - VC - c0, (int64_t)(16 * VC))); };
+    Raw<T, VC> rows[KR][KV], old[MT][4];
+    auto load_w = [&](int64_t c0) {
+        const int c = place(c0);
 #pragma unroll
         for (int s = 0; s < KR; ++s)
 #pragma unroll
             for (int k = 0; k < KV; ++k) {
                 uint32_t o = (uint32_t)(min(s * STEP + KV * g + k, p.R - 1) * (uint32_t)p.w2r + c) * sizeof(T);
-                rows[s][k] = cols_at(behind(w, o));
+                const T *from = behind(w + c0, o);
+                rows[s][k] = loose<T, VC>(from);
             }
-        if (p.y) {
-            const T *y = static_cast<const T *>(p.y) + (int64_t)at.b * p.yb + (int64_t)at.t0 * p.yt + c0;
+    };
+    auto load_y = [&](int64_t c0, int m) {
+        const int c = place(c0);
 #pragma unroll
-            for (int m = 0; m < MT; ++m)
-#pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    uint32_t o = (uint32_t)(min(16 * m + 4 * g + q, at.rows - 1) * (uint32_t)p.yt + c) * sizeof(T);
-                    old[m][q] = cols_at(behind(y, o));
-                }
+        for (int q = 0; q < 4; ++q) {
+            uint32_t o = (uint32_t)(min(16 * m + 4 * g + q, at.rows - 1) * (uint32_t)p.yt + c) * sizeof(T);
+            const T *from = behind(y + c0, o);
+            old[m][q] = loose<T, VC>(from);
         }
+    };
+    auto more = [&](int64_t c0) { return c0 + VC <= p.C; };
+    if (!more(c0)) return;
+    load_w(c0);
+    if (y)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) load_y(c0, m);
+    do {
+        typename X::Op cols[KR][VC];
 #pragma unroll
         for (int s = 0; s < KR; ++s) {
             if ((s + 1) * STEP > p.R) // behind the last rank: zeros
@@ -527,33 +547,55 @@ __device__ __forceinline__ void adapt_columns(const AdaptParams &p, const Tile &
                         for (int t = 0; t < VC; ++t) rows[s][k][t] = (T)0.f;
             X::turn(rows[s], cols[s]);
         }
-    }
+        const bool next = more(c0 + NEXT);
+        if (AHEAD && next) load_w(c0 + NEXT);
+        const int c = place(c0);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            if (16 * m >= at.rows) break;
+            typename X::Wide hw[KR];
+#pragma unroll
+            for (int s = 0; s < KR; ++s) hw[s] = H::get(kept, 16 * m + i, s * STEP + KV * g);
+            floatx4 acc[VC];
+#pragma unroll
+            for (int t = 0; t < VC; ++t) {
+                acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int s = 0; s < KR; ++s) acc[t] = X::mmw(hw[s], cols[s][t], acc[t]);
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int row = 16 * m + 4 * g + q;
+                if (row >= at.rows) continue;
+                float v[VC];
+#pragma unroll
+                for (int t = 0; t < VC; ++t) v[t] = acc[t][q] + (y ? (float)old[m][q][t] : 0.f);
+                uint32_t o = (uint32_t)(row * (uint32_t)p.ot + c) * sizeof(T);
+                T *to = behind(out + c0, o);
+                loose_store<T, VC>(to, v);
+            }
+            if (y && next) load_y(c0 + NEXT, m);
+        }
+        c0 += NEXT;
+        if (!AHEAD && next) {
+            __builtin_amdgcn_sched_barrier(0); // (not ahead of the products: for the registers)
+            load_w(c0);
+        }
+    } while (more(c0));
+}
+
+// The few columns from c0 on, one value a lane at a time.
+template <typename T, int MT, int NR> __device__ __forceinline__ void adapt_rest(const AdaptParams &p, const Tile &at, const void *kept, int64_t c0) {
+    typedef Kept<T, MT, NR> H;
+    const int n = (int)(p.C - c0);
+    const T *w = static_cast<const T *>(p.w2) + (int64_t)at.adapter * p.w2l + c0;
+    const T *y = p.y ? static_cast<const T *>(p.y) + (int64_t)at.b * p.yb + (int64_t)at.t0 * p.yt + c0 : nullptr;
     T *out = static_cast<T *>(p.out) + (int64_t)at.b * p.ob + (int64_t)at.t0 * p.ot + c0;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) {
-        if (16 * m >= at.rows) break;
-        typename X::Wide hw[KR];
-#pragma unroll
-        for (int s = 0; s < KR; ++s) hw[s] = H::get(kept, 16 * m + i, s * STEP + KV * g);
-        floatx4 acc[VC];
-#pragma unroll
-        for (int t = 0; t < VC; ++t) {
-            acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int s = 0; s < KR; ++s) acc[t] = X::mmw(hw[s], cols[s][t], acc[t]);
-        }
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int row = 16 * m + 4 * g + q;
-            if (row >= at.rows) continue;
-            float v[VC];
-#pragma unroll
-            for (int t = 0; t < VC; ++t) v[t] = acc[t][q] + (p.y ? (float)old[m][q][t] : 0.f);
-            uint32_t o = (uint32_t)(row * (uint32_t)p.ot + c) * sizeof(T);
-            T *to = behind(out, o);
-            if constexpr (WHOLE) loose_store<T, VC>(to, v);
-            else store_part<T, VC>(to, left, v);
-        }
+    for (int e = threadIdx.x & 63; e < at.rows * n; e += kWave) {
+        const int row = e / n, c = e - row * n;
+        float sum = 0.f;
+        for (int r = 0; r < p.R; ++r) sum = __builtin_fmaf(H::value(kept, row, r), (float)w[r * p.w2r + c], sum);
+        out[row * p.ot + c] = (T)(sum + (y ? (float)y[row * p.yt + c] : 0.f));
     }
 }
 
@@ -595,9 +637,11 @@ template <typename T, int MT, int NR, int W, int WPE> __global__ __launch_bounds
     }
     if (!p.out) return;
     __syncthreads();
-    for (int64_t c0 = (int64_t)wave * 16 * VC; c0 < p.C; c0 += W * 16 * VC)
-        if (p.C - c0 >= VC) adapt_columns<T, MT, NR, true>(p, at, lds, c0);
-        else adapt_columns<T, MT, NR, false>(p, at, lds, c0);
+    adapt_columns<T, MT, NR, W>(p, at, lds, (int64_t)wave * 16 * VC);
+    // the last tile of columns, where it has less than a lane's: one wave's
+    const int64_t last = p.C / (16 * VC);
+    if (p.C - last * 16 * VC > 0 && p.C - last * 16 * VC < VC && wave == last % W)
+        adapt_rest<T, MT, NR>(p, at, lds, last * 16 * VC);
 }
 
 // -- outer -----------------------------------------------------------------------------
