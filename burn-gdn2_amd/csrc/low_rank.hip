@@ -867,18 +867,23 @@ size_t hidden_bytes(const Shape &s, int64_t R) { return align256(sizeof(float) *
 
 constexpr int kFusedRank = 64; // ranks that adapt's tiles hold
 
-// Rows a tile of adapt: 32 for requests of more than 16 rows, while there are 128 of them.
-int adapt_rows(const Shape &s) { return s.N > 0 && up(s.M, s.N) > 16 && s.tiles(32) >= 128 ? 32 : 16; }
+// Rows a tile of adapt: 32 for requests of more than 16 rows, while there are 128 of them
+// (of 64 ranks, bfloat16, 32767 x 2048: 128 us, in tiles of 16 rows 159 and of 64 135); 16
+// of up to 16 ranks, whose adapters cost little to read again, where they fill the card
+// (8 x 4096 x 2048 f32: 171 against 179).
+int adapt_rows(const Shape &s, int64_t R) {
+    if (s.N <= 0 || up(s.M, s.N) <= 16 || s.tiles(32) < 128) return 16;
+    return R <= 16 && s.tiles(16) >= 1024 ? 16 : 32;
+}
 
 template <typename T> gdn2_status launch_adapt(AdaptParams p, const gdn2_low_rank_args &a, const Shape &sh, hipStream_t s) {
-    const int size = adapt_rows(sh);
+    const int size = adapt_rows(sh, p.R);
     const int64_t tiles = sh.tiles(size);
     p.req = requests_of(a, sh, size);
 #define GDN2_RUN(MT, NR, W, WPE) hipLaunchKernelGGL((adapt_kernel<T, MT, NR, W, WPE>), dim3((unsigned)tiles), dim3(64 * W), 0, s, p)
     // (sixteen waves of 64 ranks would not have the registers)
     if (size == 32 && tiles >= 512) {
-        if (p.R <= 16) GDN2_RUN(2, 1, 4, 3);
-        else if (p.R <= 32) GDN2_RUN(2, 2, 4, 3);
+        if (p.R <= 32) GDN2_RUN(2, 2, 4, 3);
         else GDN2_RUN(2, 4, 4, 2);
     } else if (size == 32) {
         if (p.R <= 16) GDN2_RUN(2, 1, 8, 2);
@@ -921,7 +926,7 @@ template <typename T> gdn2_status launch_expand(ExpandParams p, const gdn2_low_r
 }
 
 template <typename T> bool grids_ok(const Shape &sh, int64_t C, int64_t R) {
-    if (R > 0 && R <= kFusedRank) return sh.tiles(adapt_rows(sh)) < (1 << 22);
+    if (R > 0 && R <= kFusedRank) return sh.tiles(adapt_rows(sh, R)) < (1 << 22);
     return sh.tiles(shrink_rows_of(sh)) < (1 << 23) && sh.tiles(kExpandRows) * groups_of<T>(C) < (1 << 24);
 }
 
