@@ -452,6 +452,7 @@ struct AdaptParams {
     int R;
     int copies;        // rows without an adapter are written too (out is not y's memory)
     int scale_hidden;  // hidden times the scale (dh)
+    int stream;        // out is too large for the caches
 };
 
 // h of a tile in LDS, as the second product's operands.
@@ -572,7 +573,7 @@ __device__ __forceinline__ void adapt_columns(const AdaptParams &p, const Tile &
                 for (int t = 0; t < VC; ++t) v[t] = acc[t][q] + (y ? (float)old[m][q][t] : 0.f);
                 uint32_t o = (uint32_t)(row * (uint32_t)p.ot + c) * sizeof(T);
                 T *to = behind(out + c0, o);
-                loose_store<T, VC>(to, v);
+                loose_store<T, VC>(to, v, p.stream);
             }
             if (y && next) load_y(c0 + NEXT, m);
         }
@@ -880,6 +881,7 @@ template <typename T> gdn2_status launch_adapt(AdaptParams p, const gdn2_low_ran
     const int size = adapt_rows(sh, p.R);
     const int64_t tiles = sh.tiles(size);
     p.req = requests_of(a, sh, size);
+    p.stream = (double)sh.M * (double)p.C * sizeof(T) >= kStreamBytes;
 #define GDN2_RUN(MT, NR, W, WPE) hipLaunchKernelGGL((adapt_kernel<T, MT, NR, W, WPE>), dim3((unsigned)tiles), dim3(64 * W), 0, s, p)
     // (sixteen waves of 64 ranks would not have the registers)
     if (size == 32 && tiles >= 512) {
