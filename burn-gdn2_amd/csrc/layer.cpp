@@ -25,6 +25,7 @@
 
 #include "blas.hpp"
 #include "common.hpp"
+#include "gdn2_block.h"
 #include "gdn2_layer.h"
 #include "kernels.hpp"
 
@@ -372,15 +373,71 @@ gdn2_status workspace(gdn2_layer &L, int64_t B, int64_t T, bool need_s0, Work *w
     return GDN2_OK;
 }
 
+// The requests' adapters of one call (NULL: none), and its rows.
+struct Adapted {
+    const gdn2_layer_adapters *set = nullptr;
+    int64_t B = 0, T = 0;
+};
+
+// Whether a Linear weight takes adapters: those whose product is one of the layer's own
+// launches (f_proj_1 and g_proj_1 are not).
+bool adaptable(int id) {
+    return id == P_Q || id == P_K || id == P_B || id == P_V || id == P_W || id == P_F0 || id == P_G0 || id == P_O;
+}
+
+// Adds what the adapters of weight `id` contribute to y = x W (columns from y on, rows ld_y apart).
+gdn2_status add_adapters(const gdn2_layer &L, const Adapted &ad, int id, const float *x, int64_t ld_x, float *y, int64_t ld_y,
+                         hipStream_t s) {
+    if (!ad.set) return GDN2_OK;
+    for (int i = 0; i < ad.set->count; ++i) {
+        const gdn2_layer_adapter &it = ad.set->items[i];
+        if (param_id(it.name) != id) continue;
+        int64_t rows, cols;
+        param_shape(L.cfg, id, &rows, &cols);
+        gdn2_low_rank_args a{};
+        a.x = x; a.a = it.a; a.b = it.b; a.y = y; a.out = y;
+        a.adapters = ad.set->ids; a.scale = ad.set->scale;
+        a.batch = ad.B; a.seq_len = ad.T; a.in_features = rows; a.out_features = cols; a.rank = it.rank;
+        a.num_adapters = ad.set->num_adapters;
+        a.stride_x_b = ad.T * ld_x; a.stride_x_t = ld_x;
+        a.stride_y_b = a.stride_out_b = ad.T * ld_y; a.stride_y_t = a.stride_out_t = ld_y;
+        a.stride_a_l = it.rank * rows; a.stride_a_r = rows; a.stride_b_l = it.rank * cols; a.stride_b_r = cols;
+        return gdn2_low_rank_add_f32(&a, s);
+    }
+    return GDN2_OK;
+}
+
+gdn2_status check_adapters(const gdn2_layer_adapters *ad, const char *name) {
+    if (!ad) return GDN2_OK;
+    const std::string who = name;
+    if (ad->count < 0 || ad->num_adapters < 0 || (ad->count > 0 && (!ad->items || !ad->ids)))
+        return fail(GDN2_EINVAL, who + ": invalid adapters");
+    bool seen[P_COUNT] = {};
+    for (int i = 0; i < ad->count; ++i) {
+        const gdn2_layer_adapter &it = ad->items[i];
+        const int id = param_id(it.name);
+        if (id < 0 || !adaptable(id))
+            return fail(GDN2_EINVAL, who + ": no adapters for " + (it.name ? it.name : "a weight without a name"));
+        if (seen[id]) return fail(GDN2_EINVAL, who + ": adapters for " + it.name + " twice");
+        seen[id] = true;
+        if (it.rank < 0 || (it.rank > 0 && ad->num_adapters > 0 && (!it.a || !it.b)))
+            return fail(GDN2_EINVAL, who + ": invalid adapters for " + it.name);
+        if (it.rank > 64) return fail(GDN2_NOT_APPLICABLE, who + ": adapters of more than 64 ranks");
+    }
+    return GDN2_OK;
+}
+
 // Linear layers of the input side: Y, F, G.
 // G holds the g_proj_1 bias only with_bias; the kernels that read G otherwise
 // add it themselves (one launch less per call).
 gdn2_status input_gemms(gdn2_layer &L, const float *x, int64_t M, const Work &wk, hipStream_t s,
-                        bool with_bias = false) {
+                        bool with_bias = false, const Adapted &ad = {}) {
     const Dims &d = L.d;
     gdn2_status st;
     if ((st = L.mm.run(false, false, M, L.ld_in, d.D, x, d.D, L.w_in, L.ld_in, wk.Y, L.ld_in, 0.0f, s, &L.sw_in)) != GDN2_OK)
         return st;
+    for (int id : {P_Q, P_K, P_B, P_V, P_W, P_F0, P_G0})
+        if ((st = add_adapters(L, ad, id, x, d.D, wk.Y + L.col_offset(id), L.ld_in, s)) != GDN2_OK) return st;
     if (lowrank_up_supported((int)d.V, M, wk.Y, L.ld_in, L.off_f0, L.off_g0)) { // a few rows (decode): one small launch for both
         LowRankParams lp{};
         lp.Y = wk.Y; lp.ldY = L.ld_in; lp.off_f0 = L.off_f0; lp.off_g0 = L.off_g0;
@@ -452,14 +509,15 @@ gdn2_status recurrence(gdn2_layer &L, int64_t B, int64_t T, int mode, const Work
 
 // Gated RMSNorm of wk.O into `normed` (wk.O itself when null), then out = normed W_o.
 gdn2_status output_side(gdn2_layer &L, int64_t M, bool norm, const Work &wk, float *out, hipStream_t s,
-                        float *normed = nullptr) {
+                        float *normed = nullptr, const Adapted &ad = {}) {
     const Dims &d = L.d;
     float *y = normed ? normed : wk.O;
     if (norm)
         GDN2_HIP_CHECK(launch_rmsnorm_gate(y, d.vd, wk.O, d.vd, wk.G, d.vd, L.p[P_G1_BIAS], L.p[P_O_NORM], M, (int)d.HV,
                                            (int)d.V,
                                            (float)L.cfg.norm_eps, s));
-    return L.mm.run(false, false, M, d.D, d.vd, y, d.vd, L.p[P_O], d.D, out, d.D, 0.0f, s, &L.sw_o);
+    const gdn2_status st = L.mm.run(false, false, M, d.D, d.vd, y, d.vd, L.p[P_O], d.D, out, d.D, 0.0f, s, &L.sw_o);
+    return st == GDN2_OK ? add_adapters(L, ad, P_O, y, d.vd, out, d.D, s) : st;
 }
 
 gdn2_status check_layer_call(const gdn2_layer *L, const float *x, int64_t B, int64_t T, const void *out,
@@ -706,14 +764,15 @@ extern "C" gdn2_status gdn2_layer_forward_train_f32(gdn2_layer *L, const float *
     return output_side(*L, M, true, wk, out, s);
 }
 
-extern "C" gdn2_status gdn2_layer_forward_f32(gdn2_layer *L, const float *x, int64_t B, int64_t T, gdn2_state *S,
-                                              float *out, gdn2_stream_t stream) {
-    gdn2_status st = check_layer_call(L, x, B, T, out, "gdn2_layer_forward_f32");
+static gdn2_status layer_forward(gdn2_layer *L, const float *x, int64_t B, int64_t T, gdn2_state *S, float *out,
+                                 const gdn2_layer_adapters *adapters, gdn2_stream_t stream, const char *who) {
+    gdn2_status st = check_layer_call(L, x, B, T, out, who);
     if (st != GDN2_OK) return st;
-    if (!S || S->layer != L) return fail(GDN2_EINVAL, "gdn2_layer_forward_f32: state missing or made for another layer");
+    if (!S || S->layer != L) return fail(GDN2_EINVAL, std::string(who) + ": state missing or made for another layer");
     if (S->batch != B)
-        return fail(GDN2_EINVAL, "gdn2_layer_forward_f32: state batch " + std::to_string(S->batch) +
-                                     " != input batch " + std::to_string(B));
+        return fail(GDN2_EINVAL, std::string(who) + ": state batch " + std::to_string(S->batch) + " != input batch " + std::to_string(B));
+    if ((st = check_adapters(adapters, who)) != GDN2_OK) return st;
+    const Adapted ad{adapters, B, T};
     if (T == 0) return GDN2_OK;
     hipStream_t s = (hipStream_t)stream;
     const Dims &d = L->d;
@@ -731,7 +790,7 @@ extern "C" gdn2_status gdn2_layer_forward_f32(gdn2_layer *L, const float *x, int
     const float *conv_in[3] = {S->conv[S->cur][0], S->conv[S->cur][1], S->conv[S->cur][2]};
     float *const *conv_out = S->conv[1 - S->cur];
     const bool has_cache = S->some;
-    if ((st = input_gemms(*L, x, M, wk, s)) != GDN2_OK) return st;
+    if ((st = input_gemms(*L, x, M, wk, s, false, ad)) != GDN2_OK) return st;
     if (T == 1 && d.K <= 256 && d.V <= 1024) {
         gdn2_layer_params lp{};
         lp.q_conv_w = L->p[P_QCONV]; lp.k_conv_w = L->p[P_KCONV]; lp.v_conv_w = L->p[P_VCONV];
@@ -759,7 +818,7 @@ extern "C" gdn2_status gdn2_layer_forward_f32(gdn2_layer *L, const float *x, int
         p.min_decay = (float)lp.min_decay; p.one_minus_min_decay = (float)(1.0 - lp.min_decay);
         p.norm_eps = (float)lp.norm_eps; p.scale = (float)std::pow((double)d.K, -0.5);
         GDN2_HIP_CHECK(launch_decode(p, s));
-        if ((st = output_side(*L, M, false, wk, out, s)) != GDN2_OK) return st;
+        if ((st = output_side(*L, M, false, wk, out, s, nullptr, ad)) != GDN2_OK) return st;
     } else {
         if ((st = project_epilogue(*L, B, T, has_cache ? conv_in : nullptr, wk, s)) != GDN2_OK) return st;
         if (sc) {
@@ -774,11 +833,22 @@ extern "C" gdn2_status gdn2_layer_forward_f32(gdn2_layer *L, const float *x, int
         }
         const int mode = T <= kFusedRecurrentMaxSeq ? GDN2_MODE_FUSED_RECURRENT : L->cfg.mode;
         if ((st = recurrence(*L, B, T, mode, wk, S->S, s)) != GDN2_OK) return st;
-        if ((st = output_side(*L, M, true, wk, out, s)) != GDN2_OK) return st;
+        if ((st = output_side(*L, M, true, wk, out, s, nullptr, ad)) != GDN2_OK) return st;
     }
     if (sc) S->cur = 1 - S->cur;
     S->some = true;
     return GDN2_OK;
+}
+
+extern "C" gdn2_status gdn2_layer_forward_f32(gdn2_layer *L, const float *x, int64_t B, int64_t T, gdn2_state *S,
+                                              float *out, gdn2_stream_t stream) {
+    return layer_forward(L, x, B, T, S, out, nullptr, stream, "gdn2_layer_forward_f32");
+}
+
+extern "C" gdn2_status gdn2_layer_forward_adapted_f32(gdn2_layer *L, const float *x, int64_t B, int64_t T, gdn2_state *S,
+                                                      float *out, const gdn2_layer_adapters *adapters,
+                                                      gdn2_stream_t stream) {
+    return layer_forward(L, x, B, T, S, out, adapters, stream, "gdn2_layer_forward_adapted_f32");
 }
 
 extern "C" gdn2_status gdn2_layer_project_f32(gdn2_layer *L, const float *x, int64_t B, int64_t T,

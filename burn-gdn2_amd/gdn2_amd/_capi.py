@@ -124,6 +124,15 @@ class LowRankBwdArgs(ctypes.Structure):
                 ("workspace", _fp), ("workspace_bytes", ctypes.c_size_t)]
 
 
+class LayerAdapter(ctypes.Structure):
+    _fields_ = [("name", ctypes.c_char_p), ("a", _fp), ("b", _fp), ("rank", _i64)]
+
+
+class LayerAdapters(ctypes.Structure):
+    _fields_ = [("items", ctypes.POINTER(LayerAdapter)), ("count", ctypes.c_int32), ("ids", _fp), ("scale", _fp),
+                ("num_adapters", _i64)]
+
+
 class GatedScanArgs(ctypes.Structure):
     _fields_ = [("g", _fp), ("v", _fp), ("w", _fp), ("state_in", _fp), ("state_out", _fp), ("out", _fp),
                 ("cu_seqlens", _fp),
@@ -199,7 +208,8 @@ EXPORTS = ("gdn2_last_error", "gdn2_hip_available", "gdn2_recurrent_step_f32", "
            "gdn2_state_numel", "gdn2_state_tensor", "gdn2_state_read", "gdn2_state_write", "gdn2_state_serialize",
            "gdn2_state_deserialize", "gdn2_layer_grads_create", "gdn2_layer_grads_destroy",
            "gdn2_layer_grads_zero", "gdn2_layer_grads_get", "gdn2_layer_backward_f32",
-           "gdn2_layer_saved_create", "gdn2_layer_saved_destroy", "gdn2_layer_forward_train_saved_f32")
+           "gdn2_layer_saved_create", "gdn2_layer_saved_destroy", "gdn2_layer_forward_train_saved_f32",
+           "gdn2_layer_forward_adapted_f32")
 
 _lib = None
 
@@ -313,6 +323,7 @@ def _declare_layer(L):
         "gdn2_layer_get_param": (i32, [vp, ctypes.c_char_p, fp, i64]),
         "gdn2_layer_forward_train_f32": (i32, [vp, fp, i64, i64, fp, vp]),
         "gdn2_layer_forward_f32": (i32, [vp, fp, i64, i64, vp, fp, vp]),
+        "gdn2_layer_forward_adapted_f32": (i32, [vp, fp, i64, i64, vp, fp, ctypes.POINTER(LayerAdapters), vp]),
         "gdn2_layer_project_f32": (i32, [vp, fp, i64, i64, vp, fp, fp, fp, fp, fp, fp, fp, vp]),
         "gdn2_state_create": (i32, [vp, i64, ctypes.POINTER(vp)]),
         "gdn2_state_destroy": (None, [vp]),

@@ -4,6 +4,8 @@ of include/gdn2_layer.h.
   Gdn2Config      src/config.rs:23-130 (fields, Default, validate)
   GatedDeltaNet2  src/module.rs:93-495 (new, forward, forward_train, project)
   Gdn2State       src/module.rs:30-63
+  Gdn2Adapters    low-rank adapters of many requests beside the Linear weights
+                  (no reference counterpart), for GatedDeltaNet2.forward
   Gdn2Grads       the parameter gradients that burn's autodiff returns
                   (tests/autodiff.rs:153-205), from GatedDeltaNet2.backward
 
@@ -302,6 +304,65 @@ class Gdn2Saved:
             pass
 
 
+class Gdn2Adapters:
+    """Low-rank adapters beside a layer's shared Linear weights: `weights` maps
+    "q_proj", "k_proj", "b_proj", "v_proj", "w_proj", "f_proj_0", "g_proj_0" or
+    "o_proj" to (a [L, R, in], b [L, R, out]), float32 device tensors (kept, not
+    copied, where contiguous; R at most 64, the same L for all), scale [L] or None
+    (1).  A request with adapter l sees the weight W + scale_l a_l^T b_l."""
+    NAMES = ("q_proj", "k_proj", "b_proj", "v_proj", "w_proj", "f_proj_0", "g_proj_0", "o_proj")
+
+    def __init__(self, layer: "GatedDeltaNet2", weights: dict, scale=None):
+        import torch
+
+        self._layer = layer
+        self._keep = []
+        self.num_adapters = None
+        items = []
+        for name, (a, b) in weights.items():
+            if name not in self.NAMES:
+                raise ValueError(f"no adapters for {name!r}; they go with {', '.join(self.NAMES)}")
+            rows, cols = param_shape(layer.config, name)
+            for t, n in ((a, rows), (b, cols)):
+                if t.dtype is not torch.float32 or not t.is_cuda:
+                    raise TypeError(f"{name}'s adapters must be float32 device tensors")
+                if t.dim() != 3 or t.shape[2] != n or t.shape[:2] != a.shape[:2]:
+                    raise ValueError(f"{name}'s adapters must be [L, R, {rows}] and [L, R, {cols}]")
+            if a.shape[1] > 64:
+                raise ValueError("adapters of more than 64 ranks")
+            if self.num_adapters not in (None, a.shape[0]):
+                raise ValueError("every weight needs the same number of adapters")
+            self.num_adapters = a.shape[0]
+            a, b = a.contiguous(), b.contiguous()
+            self._keep += [a, b]
+            items.append(C.LayerAdapter(name.encode(), a.data_ptr(), b.data_ptr(), a.shape[1]))
+        self.num_adapters = self.num_adapters or 0
+        if scale is not None:
+            if scale.dtype is not torch.float32 or not scale.is_cuda:
+                raise TypeError("scale must be a float32 device tensor")
+            if scale.shape != (self.num_adapters,):
+                raise ValueError("scale must be [L]")
+            scale = scale.contiguous()
+        self._scale = scale
+        if len({t.get_device() for t in (*self._keep, *([] if scale is None else [scale]))}) > 1:
+            raise ValueError("the adapters are on several devices")
+        self._items = (C.LayerAdapter * max(1, len(items)))(*items)
+        self._count = len(items)
+
+    def _args(self, ids, x) -> C.LayerAdapters:
+        import torch
+
+        if ids.dtype is not torch.int32 or not ids.is_contiguous():
+            raise TypeError("adapter_ids must be a contiguous int32 vector")
+        if ids.shape != (x.shape[0],):
+            raise ValueError(f"adapter_ids must be [{x.shape[0]}], one of each request")
+        for t in (ids, *self._keep, self._scale):
+            if t is not None and t.get_device() != x.get_device():
+                raise ValueError("the adapters and their ids must be on x's device")
+        return C.LayerAdapters(self._items, self._count, ids.data_ptr(), None if self._scale is None else self._scale.data_ptr(),
+                               self.num_adapters)
+
+
 def _forward_train_fn():
     import torch
 
@@ -403,18 +464,29 @@ class GatedDeltaNet2:
                                                                out.data_ptr(), saved._h, _stream()))
         return out
 
-    def forward(self, x, state: Optional[Gdn2State] = None):
+    def forward(self, x, state: Optional[Gdn2State] = None, adapters: Optional[Gdn2Adapters] = None, adapter_ids=None):
         """forward(x, &mut state, update_state = true) (src/module.rs:224-316).
         Returns (out [B, T, D], state); a None state is created empty and
-        filled, as the reference's `get_or_insert_with`."""
+        filled, as the reference's `get_or_insert_with`.  With `adapters` each
+        batch entry i also has the low-rank adapter adapter_ids[i] (int32 on the
+        device; none outside [0, L)): the same ids for the calls on one state."""
         import torch
 
         x = self._check_x(x)
+        if (adapters is None) != (adapter_ids is None):
+            raise ValueError("adapters and adapter_ids go together")
+        if adapters is not None and adapters._layer is not self:
+            raise ValueError("the adapters were made for another layer")
+        args = None if adapters is None else adapters._args(adapter_ids, x)
         if state is None:
             state = Gdn2State(self, x.shape[0])
         out = torch.empty_like(x)
-        C.check(C.lib().gdn2_layer_forward_f32(self._h, x.data_ptr(), x.shape[0], x.shape[1], state._h,
-                                               out.data_ptr(), _stream()))
+        if args is not None:
+            C.check(C.lib().gdn2_layer_forward_adapted_f32(self._h, x.data_ptr(), x.shape[0], x.shape[1], state._h,
+                                                           out.data_ptr(), ctypes.byref(args), _stream()))
+        else:
+            C.check(C.lib().gdn2_layer_forward_f32(self._h, x.data_ptr(), x.shape[0], x.shape[1], state._h,
+                                                   out.data_ptr(), _stream()))
         return out, state
 
     def project(self, x, state: Optional[Gdn2State] = None) -> Dict[str, "torch.Tensor"]:

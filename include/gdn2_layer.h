@@ -152,6 +152,32 @@ GDN2_API gdn2_status gdn2_layer_forward_train_f32(gdn2_layer *layer, const float
 GDN2_API gdn2_status gdn2_layer_forward_f32(gdn2_layer *layer, const float *x, int64_t batch, int64_t seq_len,
                                             gdn2_state *state, float *out, gdn2_stream_t stream);
 
+/* The same call for requests (batch entries) with low-rank adapters of their own beside
+ * the layer's shared Linear weights (no reference counterpart): request i's output is that
+ * of a layer whose weight `name` is W + scale[l] a_l^T b_l, l = ids[i], for every item.  An
+ * id outside [0, num_adapters) has none.  Prefill and decode, any T; calls that follow one
+ * another on a state take the same ids.
+ *   items  up to one of each of q_proj, k_proj, b_proj, v_proj, w_proj, f_proj_0, g_proj_0
+ *          and o_proj: a [L, rank, in], b [L, rank, out] contiguous in device memory, owned
+ *          by the caller (gdn2_low_rank_add_f32 of gdn2_block.h)
+ *   ids    device, int32, [batch];  scale  device, [num_adapters], or NULL (1)
+ * GDN2_NOT_APPLICABLE for more than 64 ranks. */
+typedef struct gdn2_layer_adapter {
+    const char *name;
+    const float *a, *b;
+    int64_t rank;
+} gdn2_layer_adapter;
+typedef struct gdn2_layer_adapters {
+    const gdn2_layer_adapter *items;
+    int32_t count;
+    const int32_t *ids;
+    const float *scale;
+    int64_t num_adapters;
+} gdn2_layer_adapters;
+GDN2_API gdn2_status gdn2_layer_forward_adapted_f32(gdn2_layer *layer, const float *x, int64_t batch, int64_t seq_len,
+                                                    gdn2_state *state, float *out, const gdn2_layer_adapters *adapters,
+                                                    gdn2_stream_t stream);
+
 /* project (src/module.rs:381-495): writes the recurrence's inputs q, k,
  * g, b, v, w [B, HV, T, V] and the gate signal [B, T, HV, V] (each
  * contiguous, caller-owned).  q, k, g, b are [B, H, T, K] under

@@ -295,3 +295,12 @@ def test_low_rank_refusals_in_python():
     ]:
         with pytest.raises(err):
             G.low_rank_add_backward(*args, **kw)
+
+
+def test_layer_adapters_of_the_c_entry():
+    """Invalid adapters come back before any launch (a layer is not needed to see that)."""
+    from gdn2_amd import _capi as C
+
+    L = C.lib()
+    assert L.gdn2_layer_forward_adapted_f32(None, 256, 1, 1, None, 512, None, None) == C.GDN2_EINVAL
+    assert b"gdn2_layer_forward_adapted_f32" in L.gdn2_last_error()
