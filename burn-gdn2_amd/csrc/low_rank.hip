@@ -248,13 +248,15 @@ __device__ __forceinline__ void shrink_rows(floatx4 *lds, const void *px, int64_
         }
         __builtin_amdgcn_wave_barrier();
     }
-    for (; k < K; k += STEP) { // (one wave's, and less than a chunk)
-        const int64_t left = K - k - KV * g;
+    // less than a chunk: a step each of the waves whose turn it is
+    const int64_t whole = K / CHUNK;
+    for (int64_t t = whole * CHUNK + ((wave + W - (int)(whole % W)) % W) * STEP; t < K; t += W * STEP) {
+        const int64_t left = K - t - KV * g;
 #pragma unroll
-        for (int n = 0; n < NR; ++n) b[0][n] = loose_part<T, KV>(behind(w + k, wo[n]), left);
+        for (int n = 0; n < NR; ++n) b[0][n] = loose_part<T, KV>(behind(w + t, wo[n]), left);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-            const typename X::Op a = loose_part<T, KV>(x + min(16 * m + i, at.rows - 1) * xt + k + KV * g, left);
+            const typename X::Op a = loose_part<T, KV>(x + min(16 * m + i, at.rows - 1) * xt + t + KV * g, left);
 #pragma unroll
             for (int n = 0; n < NR; ++n) acc[m][n] = X::mma(a, b[0][n], acc[m][n]);
         }
@@ -595,6 +597,7 @@ template <typename T, int MT, int NR> __device__ __forceinline__ void adapt_rest
     for (int e = threadIdx.x & 63; e < at.rows * n; e += kWave) {
         const int row = e / n, c = e - row * n;
         float sum = 0.f;
+#pragma unroll 8
         for (int r = 0; r < p.R; ++r) sum = __builtin_fmaf(H::value(kept, row, r), (float)w[r * p.w2r + c], sum);
         out[row * p.ot + c] = (T)(sum + (y ? (float)y[row * p.yt + c] : 0.f));
     }
@@ -846,12 +849,13 @@ Requests requests_of(const gdn2_low_rank_args &a, const Shape &s, int size) {
     return r;
 }
 
-// Rows a block of the outer products: 1024 blocks by columns, while each has 128 rows or
-// more and at most 4096.
+// Rows a block of the outer products: 256 blocks by columns, while each has 128 rows or
+// more and at most 4096 (4 x 2048 x 2048 bf16, 16 ranks: the whole backward 37.8 us; 512
+// of them 39.5, 1024 40.5: more to add up).
 int block_rows(const Shape &s, int64_t columns, int tile_columns) {
     const int64_t per = up(columns, tile_columns);
     int rows = 4096;
-    while (rows > 128 && s.tiles(rows) * per < 1024) rows /= 2;
+    while (rows > 128 && s.tiles(rows) * per < 256) rows /= 2;
     return rows;
 }
 
@@ -883,7 +887,7 @@ template <typename T> gdn2_status launch_adapt(AdaptParams p, const gdn2_low_ran
     p.req = requests_of(a, sh, size);
     p.stream = (double)sh.M * (double)p.C * sizeof(T) >= kStreamBytes;
 #define GDN2_RUN(MT, NR, W, WPE) hipLaunchKernelGGL((adapt_kernel<T, MT, NR, W, WPE>), dim3((unsigned)tiles), dim3(64 * W), 0, s, p)
-    // (sixteen waves of 64 ranks would not have the registers)
+    // more waves a tile where tiles are few (eight or sixteen: the same within 3 %)
     if (size == 32 && tiles >= 512) {
         if (p.R <= 32) GDN2_RUN(2, 2, 4, 3);
         else GDN2_RUN(2, 4, 4, 2);
@@ -896,8 +900,8 @@ template <typename T> gdn2_status launch_adapt(AdaptParams p, const gdn2_low_ran
         else if (p.R <= 32) GDN2_RUN(1, 2, 4, 4);
         else GDN2_RUN(1, 4, 4, 2);
     } else {
-        if (p.R <= 16) GDN2_RUN(1, 1, 16, 4);
-        else if (p.R <= 32) GDN2_RUN(1, 2, 16, 4);
+        if (p.R <= 16) GDN2_RUN(1, 1, 8, 4);
+        else if (p.R <= 32) GDN2_RUN(1, 2, 8, 4);
         else GDN2_RUN(1, 4, 8, 2);
     }
 #undef GDN2_RUN
