@@ -499,93 +499,101 @@ template <int MT, int NR> struct Kept<bf16, MT, NR> { // three planes of terms
 // A wave's columns of a tile's rows: 16 VC of every W times as many, the next ones' y
 // (and b, where the registers do) in flight.
 // (Fewer than VC columns behind the last whole tile are adapt_rest's.)
-template <typename T, int MT, int NR, int W>
-__device__ __forceinline__ void adapt_columns(const AdaptParams &p, const Tile &at, const void *kept, int64_t c0) {
+template <typename T, int MT, int NR, int W> struct Columns {
     typedef Mm<T> X;
     typedef Kept<T, MT, NR> H;
-    constexpr int KV = X::KV, VC = X::VC, STEP = 4 * KV, KR = H::KR, NEXT = W * 16 * VC;
-    constexpr bool AHEAD = sizeof(T) == 4 && NR <= 2;
-    const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-    const T *w = static_cast<const T *>(p.w2) + (int64_t)at.adapter * p.w2l;
-    const T *y = p.y ? static_cast<const T *>(p.y) + (int64_t)at.b * p.yb + (int64_t)at.t0 * p.yt : nullptr;
-    T *out = static_cast<T *>(p.out) + (int64_t)at.b * p.ob + (int64_t)at.t0 * p.ot;
-    // a lane's columns from c0 on: where they would end behind the last, the last VC
-    auto place = [&](int64_t c0) { return min(VC * i, (int)min(p.C - VC - c0, (int64_t)(16 * VC))); };
+    static constexpr int KV = X::KV, VC = X::VC, STEP = 4 * KV, KR = H::KR, NEXT = W * 16 * VC;
+    static constexpr bool AHEAD = sizeof(T) == 4 && NR <= 2;
+    const AdaptParams &p;
+    const Tile &at;
+    const int i, g;
+    const T *w, *y;
+    T *out;
     Raw<T, VC> rows[KR][KV], old[MT][4];
-    auto load_w = [&](int64_t c0) {
+
+    __device__ __forceinline__ Columns(const AdaptParams &p, const Tile &at)
+        : p(p), at(at), i(threadIdx.x & 15), g((threadIdx.x & 63) >> 4),
+          w(static_cast<const T *>(p.w2) + (int64_t)at.adapter * p.w2l),
+          y(p.y ? static_cast<const T *>(p.y) + (int64_t)at.b * p.yb + (int64_t)at.t0 * p.yt : nullptr),
+          out(static_cast<T *>(p.out) + (int64_t)at.b * p.ob + (int64_t)at.t0 * p.ot) {}
+
+    // a lane's columns from c0 on: where they would end behind the last, the last VC
+    __device__ __forceinline__ int place(int64_t c0) const { return min(VC * i, (int)min(p.C - VC - c0, (int64_t)(16 * VC))); }
+    __device__ __forceinline__ bool more(int64_t c0) const { return p.out && c0 + VC <= p.C; }
+    __device__ __forceinline__ void load_w(int64_t c0) {
         const int c = place(c0);
 #pragma unroll
         for (int s = 0; s < KR; ++s)
 #pragma unroll
             for (int k = 0; k < KV; ++k) {
                 uint32_t o = (uint32_t)(min(s * STEP + KV * g + k, p.R - 1) * (uint32_t)p.w2r + c) * sizeof(T);
-                const T *from = behind(w + c0, o);
-                rows[s][k] = loose<T, VC>(from);
+                rows[s][k] = loose<T, VC>(behind(w + c0, o));
             }
-    };
-    auto load_y = [&](int64_t c0, int m) {
+    }
+    __device__ __forceinline__ void load_y(int64_t c0, int m) {
         const int c = place(c0);
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             uint32_t o = (uint32_t)(min(16 * m + 4 * g + q, at.rows - 1) * (uint32_t)p.yt + c) * sizeof(T);
-            const T *from = behind(y + c0, o);
-            old[m][q] = loose<T, VC>(from);
+            old[m][q] = loose<T, VC>(behind(y + c0, o));
         }
-    };
-    auto more = [&](int64_t c0) { return c0 + VC <= p.C; };
-    if (!more(c0)) return;
-    load_w(c0);
-    if (y)
+    }
+    __device__ __forceinline__ void load(int64_t c0) {
+        if (!more(c0)) return;
+        load_w(c0);
+        if (y)
 #pragma unroll
-        for (int m = 0; m < MT; ++m) load_y(c0, m);
-    do {
-        typename X::Op cols[KR][VC];
+            for (int m = 0; m < MT; ++m) load_y(c0, m);
+    }
+    // (after load(c0))
+    __device__ __forceinline__ void run(const void *kept, int64_t c0) {
+        for (; more(c0); c0 += NEXT) {
+            typename X::Op cols[KR][VC];
 #pragma unroll
-        for (int s = 0; s < KR; ++s) {
-            if ((s + 1) * STEP > p.R) // behind the last rank: zeros
+            for (int s = 0; s < KR; ++s) {
+                if ((s + 1) * STEP > p.R) // behind the last rank: zeros
 #pragma unroll
-                for (int k = 0; k < KV; ++k)
-                    if (s * STEP + KV * g + k >= p.R)
+                    for (int k = 0; k < KV; ++k)
+                        if (s * STEP + KV * g + k >= p.R)
 #pragma unroll
-                        for (int t = 0; t < VC; ++t) rows[s][k][t] = (T)0.f;
-            X::turn(rows[s], cols[s]);
-        }
-        const bool next = more(c0 + NEXT);
-        if (AHEAD && next) load_w(c0 + NEXT);
-        const int c = place(c0);
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            if (16 * m >= at.rows) break;
-            typename X::Wide hw[KR];
-#pragma unroll
-            for (int s = 0; s < KR; ++s) hw[s] = H::get(kept, 16 * m + i, s * STEP + KV * g);
-            floatx4 acc[VC];
-#pragma unroll
-            for (int t = 0; t < VC; ++t) {
-                acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int s = 0; s < KR; ++s) acc[t] = X::mmw(hw[s], cols[s][t], acc[t]);
+                            for (int t = 0; t < VC; ++t) rows[s][k][t] = (T)0.f;
+                X::turn(rows[s], cols[s]);
             }
+            const bool next = more(c0 + NEXT);
+            if (AHEAD && next) load_w(c0 + NEXT);
+            const int c = place(c0);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                const int row = 16 * m + 4 * g + q;
-                if (row >= at.rows) continue;
-                float v[VC];
+            for (int m = 0; m < MT; ++m) {
+                if (16 * m >= at.rows) break;
+                typename X::Wide hw[KR];
 #pragma unroll
-                for (int t = 0; t < VC; ++t) v[t] = acc[t][q] + (y ? (float)old[m][q][t] : 0.f);
-                uint32_t o = (uint32_t)(row * (uint32_t)p.ot + c) * sizeof(T);
-                T *to = behind(out + c0, o);
-                loose_store<T, VC>(to, v, p.stream);
+                for (int s = 0; s < KR; ++s) hw[s] = H::get(kept, 16 * m + i, s * STEP + KV * g);
+                floatx4 acc[VC];
+#pragma unroll
+                for (int t = 0; t < VC; ++t) {
+                    acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int s = 0; s < KR; ++s) acc[t] = X::mmw(hw[s], cols[s][t], acc[t]);
+                }
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int row = 16 * m + 4 * g + q;
+                    if (row >= at.rows) continue;
+                    float v[VC];
+#pragma unroll
+                    for (int t = 0; t < VC; ++t) v[t] = acc[t][q] + (y ? (float)old[m][q][t] : 0.f);
+                    uint32_t o = (uint32_t)(row * (uint32_t)p.ot + c) * sizeof(T);
+                    loose_store<T, VC>(behind(out + c0, o), v, p.stream);
+                }
+                if (y && next) load_y(c0 + NEXT, m);
             }
-            if (y && next) load_y(c0 + NEXT, m);
+            if (!AHEAD && next) {
+                __builtin_amdgcn_sched_barrier(0); // (not ahead of the products: for the registers)
+                load_w(c0 + NEXT);
+            }
         }
-        c0 += NEXT;
-        if (!AHEAD && next) {
-            __builtin_amdgcn_sched_barrier(0); // (not ahead of the products: for the registers)
-            load_w(c0);
-        }
-    } while (more(c0));
-}
+    }
+};
 
 // The few columns from c0 on, one value a lane at a time.
 template <typename T, int MT, int NR> __device__ __forceinline__ void adapt_rest(const AdaptParams &p, const Tile &at, const void *kept, int64_t c0) {
@@ -640,8 +648,10 @@ template <typename T, int MT, int NR, int W, int WPE> __global__ __launch_bounds
                 }
     }
     if (!p.out) return;
+    Columns<T, MT, NR, W> columns(p, at);
+    columns.load((int64_t)wave * 16 * VC);
     __syncthreads();
-    adapt_columns<T, MT, NR, W>(p, at, lds, (int64_t)wave * 16 * VC);
+    columns.run(lds, (int64_t)wave * 16 * VC);
     // the last tile of columns, where it has less than a lane's: one wave's
     const int64_t last = p.C / (16 * VC);
     if (p.C - last * 16 * VC > 0 && p.C - last * 16 * VC < VC && wave == last % W)

@@ -438,11 +438,11 @@ struct SumParams {
     int64_t blocks, blocks_a_seg;
 };
 
-// The sums over workgroups: 64 columns of one result a workgroup, four a thread, in f64.
+// The sums over workgroups: 32 columns of one result a workgroup, four a thread, in f64.
 template <typename TB> __global__ __launch_bounds__(256) void residual_sums_kernel(SumParams p) {
-    __shared__ double red[16][64 + 1];
-    const int what = blockIdx.x / p.tiles, col = (threadIdx.x & 15) * 4, r = threadIdx.x >> 4;
-    const int c0 = (blockIdx.x - what * p.tiles) * 64, c = c0 + col, left = p.C - c;
+    __shared__ double red[32][32 + 1];
+    const int what = blockIdx.x / p.tiles, col = (threadIdx.x & 7) * 4, r = threadIdx.x >> 3;
+    const int c0 = (blockIdx.x - what * p.tiles) * 32, c = c0 + col, left = p.C - c;
     const float *part = what == 0 ? p.pre : what == 1 ? p.post : p.gate;
     if (!part) return;
     const int64_t b0 = what < 2 ? 0 : (what - 2) * p.blocks_a_seg, b1 = what < 2 ? p.blocks : b0 + p.blocks_a_seg;
@@ -452,14 +452,14 @@ template <typename TB> __global__ __launch_bounds__(256) void residual_sums_kern
         for (int j = 0; j < 4; ++j) sum[j] += v[j];
     };
     int64_t b = b0 + r;
-    for (; b + 7 * 16 < b1; b += 8 * 16) { // eight in flight
+    for (; b + 7 * 32 < b1; b += 8 * 32) { // eight in flight
         float v[8][4];
 #pragma unroll
-        for (int k = 0; k < 8; ++k) load_part<float, 4>(part + (b + 16 * k) * p.C + c, left, v[k]);
+        for (int k = 0; k < 8; ++k) load_part<float, 4>(part + (b + 32 * k) * p.C + c, left, v[k]);
 #pragma unroll
         for (int k = 0; k < 8; ++k) add(v[k]);
     }
-    for (; b < b1; b += 16) {
+    for (; b < b1; b += 32) {
         float v[4];
         load_part<float, 4>(part + b * p.C + c, left, v);
         add(v);
@@ -468,10 +468,10 @@ template <typename TB> __global__ __launch_bounds__(256) void residual_sums_kern
     for (int j = 0; j < 4; ++j) red[r][col + j] = sum[j];
     __syncthreads();
     const int t = threadIdx.x;
-    if (t >= 64 || c0 + t >= p.C) return;
+    if (t >= 32 || c0 + t >= p.C) return;
     double all = 0.;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) all += red[k][t];
+    for (int k = 0; k < 32; ++k) all += red[k][t];
     if (what == 0) p.dpre[c0 + t] = (float)all;
     else if (what == 1) p.dpost[c0 + t] = (float)all;
     else static_cast<TB *>(p.dgate)[(what - 2) * p.sgate + c0 + t] = (TB)(float)all;
@@ -664,7 +664,7 @@ gdn2_status backward(const gdn2_residual_norm_bwd_args *b, hipStream_t s, const 
     if (a->pre_weight || a->post_weight || gsum) {
         SumParams t{};
         t.C = p.C;
-        t.tiles = (p.C + 63) / 64;
+        t.tiles = (p.C + 31) / 32;
         t.blocks = M > 0 ? q.blocks : 0;
         t.blocks_a_seg = M > 0 ? q.per : 0;
         // (with no rows nothing of these is read)
