@@ -56,7 +56,14 @@ def test_sizes(gpu, ty, B, T, D, O, R, L):
 
 
 @pytest.mark.parametrize("ty", [F32, BF])
-@pytest.mark.parametrize("R", [1, 16, 40, 64])
+@pytest.mark.parametrize("B,T,R", [(1100, 5, 8), (1100, 5, 24), (1100, 5, 40), (2, 16500, 24), (2, 16500, 40), (1, 33000, 65)])
+def test_many_tiles(gpu, ty, B, T, R):
+    """Short and long requests that fill the card, by the number of ranks."""
+    check(gpu, make(B, T, 72, 70, R, 3, ty))
+
+
+@pytest.mark.parametrize("ty", [F32, BF])
+@pytest.mark.parametrize("R", [1, 16, 24, 40, 64])
 def test_long_requests(gpu, ty, R):
     """The tiles of 64 rows, ragged ends, several blocks of rows for an adapter."""
     check(gpu, make(3, 3001, 160, 144, R, 2, ty, seed=R))
