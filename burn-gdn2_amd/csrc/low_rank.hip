@@ -882,13 +882,15 @@ size_t hidden_bytes(const Shape &s, int64_t R) { return align256(sizeof(float) *
 
 constexpr int kFusedRank = 64; // ranks that adapt's tiles hold
 
-// Rows a tile of adapt: 32 for requests of more than 16 rows, while there are 128 of them
-// (of 64 ranks, bfloat16, 32767 x 2048: 128 us, in tiles of 16 rows 159 and of 64 135); 16
-// of up to 16 ranks, whose adapters cost little to read again, where they fill the card
-// (8 x 4096 x 2048 f32: 171 against 179).
+// Rows a tile of adapt: 32 where a request has more than 16 and the adapter's ranks cost
+// more to read again than tiles that fill the card: from 1024 such tiles on for 17 to 32
+// ranks (2048 features, f32: 182 us against 198 at 32768 rows, 99 against 95 at 16384),
+// from 256 on for more (64 ranks, bfloat16: 128 against 168 at 32767, 36 against 43 at
+// 8192, 27 against 24 at 4096).  Of up to 16 ranks 16 rows were never slower (f32: 159
+// against 180 at 32768, 26 against 33 at 4096).
 int adapt_rows(const Shape &s, int64_t R) {
-    if (s.N <= 0 || up(s.M, s.N) <= 16 || s.tiles(32) < 128) return 16;
-    return R <= 16 && s.tiles(16) >= 1024 ? 16 : 32;
+    if (R <= 16 || s.N <= 0 || up(s.M, s.N) <= 16) return 16;
+    return s.tiles(32) >= (R <= 32 ? 1024 : 256) ? 32 : 16;
 }
 
 template <typename T> gdn2_status launch_adapt(AdaptParams p, const gdn2_low_rank_args &a, const Shape &sh, hipStream_t s) {
@@ -897,15 +899,13 @@ template <typename T> gdn2_status launch_adapt(AdaptParams p, const gdn2_low_ran
     p.req = requests_of(a, sh, size);
     p.stream = (double)sh.M * (double)p.C * sizeof(T) >= kStreamBytes;
 #define GDN2_RUN(MT, NR, W, WPE) hipLaunchKernelGGL((adapt_kernel<T, MT, NR, W, WPE>), dim3((unsigned)tiles), dim3(64 * W), 0, s, p)
-    // more waves a tile where tiles are few (eight or sixteen: the same within 3 %)
-    if (size == 32 && tiles >= 512) {
+    // Eight waves a tile where tiles are few: their share of a chain of loads is shorter;
+    // four of them from 512 tiles of 16 rows on (16 ranks, 16384 bfloat16 rows: 46 us
+    // against 50; 64 ranks 81 and 92; 8192 f32 rows, 16 ranks: 47 and 46).
+    if (size == 32) {
         if (p.R <= 32) GDN2_RUN(2, 2, 4, 3);
         else GDN2_RUN(2, 4, 4, 2);
-    } else if (size == 32) {
-        if (p.R <= 16) GDN2_RUN(2, 1, 8, 2);
-        else if (p.R <= 32) GDN2_RUN(2, 2, 8, 2);
-        else GDN2_RUN(2, 4, 8, 2);
-    } else if (tiles >= 1024) {
+    } else if (tiles >= 512) {
         if (p.R <= 16) GDN2_RUN(1, 1, 4, 4);
         else if (p.R <= 32) GDN2_RUN(1, 2, 4, 4);
         else GDN2_RUN(1, 4, 4, 2);
@@ -919,8 +919,10 @@ template <typename T> gdn2_status launch_adapt(AdaptParams p, const gdn2_low_ran
     return GDN2_OK;
 }
 
-// More ranks: 64 of them a workgroup in shrink.
-int shrink_rows_of(const Shape &s) { return s.N > 0 && up(s.M, s.N) > 32 && s.tiles(64) >= 512 ? 64 : 16; }
+// More ranks: 64 of them a workgroup in shrink, and 64 rows where there are 512 tiles of
+// them (128 ranks, 8 x 4096 bfloat16 rows: 170 us of the whole call against 297; 8 x 1024
+// f32 rows 103 against 145; 64 requests of one or 16 of 33 rows: the same).
+int shrink_rows_of(const Shape &s) { return s.N > 0 && up(s.M, s.N) > 32 && s.tiles(64) >= 128 ? 64 : 16; }
 template <typename T> gdn2_status launch_shrink(ShrinkParams p, const gdn2_low_rank_args &a, const Shape &sh, hipStream_t s) {
     const int size = shrink_rows_of(sh);
     p.req = requests_of(a, sh, size);
