@@ -1,9 +1,9 @@
 // gdn2_dropout_*: y = x / (1 - p) or 0, by the words of philox.hpp.
 //
 // Rows that lie together, of a multiple of 8 channels, are one row (their counters
-// follow one another): a thread takes kSteps runs of 16 bytes, all loaded before the
-// first word is formed.  Other rows go in runs of VEC channels from each row's start,
-// the last one shorter; loads and stores need no alignment.
+// follow one another); a thread takes a run of 16 bytes.  Other rows go in runs of VEC
+// channels from each row's start, the last one shorter; loads and stores need no
+// alignment.
 #include <algorithm>
 #include <exception>
 #include <string>
@@ -16,43 +16,29 @@
 namespace gdn2 {
 namespace {
 
-constexpr int kSteps = 4;
-
 template <typename T, int VEC> __global__ __launch_bounds__(256) void dropout_flat_kernel(const T *x, T *y, int64_t n, Drop d) {
     drop_begin(d);
-    const int64_t first = ((int64_t)blockIdx.x * kSteps * 256 + threadIdx.x) * VEC;
-    Raw<T, VEC> r[kSteps];
+    const int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) * VEC;
+    if (i >= n) return;
+    const Raw<T, VEC> r = loose<T, VEC>(x + i);
+    float v[VEC];
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-        const int64_t i = first + (int64_t)s * 256 * VEC;
-        r[s] = loose<T, VEC>(x + (i < n ? i : 0));
-    }
-#pragma unroll
-    for (int s = 0; s < kSteps; ++s) {
-        const int64_t i = first + (int64_t)s * 256 * VEC;
-        float v[VEC];
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = (float)r[s][j];
-        drop_n<VEC>(d, (uint64_t)i / 4, d.scale, v);
-        if (i < n) loose_store<T, VEC>(y + i, v);
-    }
+    for (int j = 0; j < VEC; ++j) v[j] = (float)r[j];
+    drop_n<VEC>(d, (uint64_t)i / 4, d.scale, v);
+    loose_store<T, VEC>(y + i, v);
 }
 
 template <typename T, int VEC>
 __global__ __launch_bounds__(256) void dropout_rows_kernel(const T *x, T *y, uint32_t runs, uint32_t runs_a_row, int64_t C,
                                                            int64_t sx, int64_t sy, Drop d) {
     drop_begin(d);
-    const uint64_t quads = (uint64_t)(C + 3) / 4;
-#pragma unroll 1
-    for (int s = 0; s < kSteps; ++s) {
-        const uint64_t run = ((uint64_t)blockIdx.x * kSteps + s) * 256 + threadIdx.x;
-        if (run >= runs) return;
-        const uint32_t row = (uint32_t)run / runs_a_row, c = ((uint32_t)run - row * runs_a_row) * VEC;
-        float v[VEC];
-        load_part<T, VEC>(x + row * sx + c, C - c, v);
-        drop_n<VEC>(d, row * quads + c / 4, d.scale, v);
-        store_part<T, VEC>(y + row * sy + c, C - c, v);
-    }
+    const uint64_t quads = (uint64_t)(C + 3) / 4, run = (uint64_t)blockIdx.x * 256 + threadIdx.x;
+    if (run >= runs) return;
+    const uint32_t row = (uint32_t)run / runs_a_row, c = ((uint32_t)run - row * runs_a_row) * VEC;
+    float v[VEC];
+    row_part<T, VEC, false>(x + row * sx, c, (int)C, v);
+    drop_n<VEC>(d, row * quads + c / 4, d.scale, v);
+    store_part<T, VEC>(y + row * sy + c, C - c, v);
 }
 
 template <typename T> gdn2_status run(const void *x, void *y, int64_t rows, int64_t C, int64_t sx, int64_t sy,
@@ -69,7 +55,7 @@ template <typename T> gdn2_status run(const void *x, void *y, int64_t rows, int6
     if (C >= (int64_t(1) << 31) || rows >= (int64_t(1) << 40))
         return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
     if (C % 8 == 0 && (rows == 1 || (sx == C && sy == C))) {
-        const int64_t per = (int64_t)kSteps * 256 * VEC, n = rows * C;
+        const int64_t per = 256 * VEC, n = rows * C;
         const int64_t blocks = (n + per - 1) / per;
         if ((double)rows * (double)C >= 1e15 || blocks >= (1 << 24))
             return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
@@ -78,7 +64,7 @@ template <typename T> gdn2_status run(const void *x, void *y, int64_t rows, int6
     } else {
         if (quads >= 4294967040.) return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
         const int64_t runs_a_row = (C + VEC - 1) / VEC, runs = rows * runs_a_row;
-        hipLaunchKernelGGL((dropout_rows_kernel<T, VEC>), dim3((unsigned)((runs + kSteps * 256 - 1) / (kSteps * 256))), dim3(256), 0, s,
+        hipLaunchKernelGGL((dropout_rows_kernel<T, VEC>), dim3((unsigned)((runs + 255) / 256)), dim3(256), 0, s,
                            static_cast<const T *>(x), static_cast<T *>(y), (uint32_t)runs, (uint32_t)runs_a_row, C, sx, sy, d);
     }
     GDN2_HIP_CHECK(hipGetLastError());
