@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void dropout_rows_kernel(const T *x, T *y, uin
     if (run >= runs) return;
     const uint32_t row = (uint32_t)run / runs_a_row, c = ((uint32_t)run - row * runs_a_row) * VEC;
     float v[VEC];
-    row_part<T, VEC, false>(x + row * sx, c, (int)C, v);
+    load_part<T, VEC>(x + row * sx + c, C - c, v);
     drop_n<VEC>(d, row * quads + c / 4, d.scale, v);
     store_part<T, VEC>(y + row * sy + c, C - c, v);
 }

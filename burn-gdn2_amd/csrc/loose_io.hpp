@@ -55,30 +55,4 @@ template <typename T, int N, bool WHOLE = false> __device__ __forceinline__ void
     }
 }
 
-// Values c .. c + N - 1 of a row of C, zeros behind its last: without a branch, as the
-// row's last N, turned by as many as they start before c (only rows of less than N go
-// value by value).
-template <typename T, int N, bool WHOLE> __device__ __forceinline__ Raw<T, N> row_raw(const T *row, int c, int C) {
-    if (WHOLE || C < N) return loose_part<T, N, WHOLE>(row + c, C - c);
-    constexpr int WORDS = N * sizeof(T) / 4;
-    typedef uint32_t Words __attribute__((ext_vector_type(WORDS)));
-    const int from = min(c, C - N), bytes = min(c - from, N) * (int)sizeof(T);
-    const Raw<T, N> raw = loose<T, N>(row + from);
-    Words w = __builtin_bit_cast(Words, raw);
-    if constexpr (sizeof(T) == 2) {
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) w[i] = __builtin_amdgcn_alignbit(i + 1 < WORDS ? w[i + 1] : 0u, w[i], (bytes & 2) * 8);
-    }
-#pragma unroll
-    for (int by = 1; by <= WORDS; by *= 2)
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) w[i] = bytes & (4 * by) ? (i + by < WORDS ? w[i + by] : 0u) : w[i];
-    return __builtin_bit_cast(Raw<T, N>, w);
-}
-template <typename T, int N, bool WHOLE> __device__ __forceinline__ void row_part(const T *row, int c, int C, float *x) {
-    const Raw<T, N> v = row_raw<T, N, WHOLE>(row, c, C);
-#pragma unroll
-    for (int j = 0; j < N; ++j) x[j] = (float)v[j];
-}
-
 }  // namespace gdn2

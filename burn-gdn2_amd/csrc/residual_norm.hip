@@ -74,7 +74,7 @@ __device__ __forceinline__ void gate_of(int act, float z, float &a, float &d) {
 }
 
 template <int N, bool WHOLE> __device__ __forceinline__ void weights_n(const float *w, int c, int C, float *x) {
-    row_part<float, N, WHOLE>(w, c, C, x);
+    load_part<float, N, WHOLE>(w + c, C - c, x);
 }
 
 // Sums over the lanes of a row, to all of them.  WPR waves a row; `turn` alternates
@@ -141,16 +141,16 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void residual_norm_kerne
         {
             const TS *x = static_cast<const TS *>(p.x) + row_at(p.sx, m, p.S);
 #pragma unroll
-            for (int k = 0; k < NV; ++k) rx[k] = row_raw<TS, VEC, WHOLE>(x, at.c[k], p.C);
+            for (int k = 0; k < NV; ++k) rx[k] = loose_part<TS, VEC, WHOLE>(x + at.c[k], p.C - at.c[k]);
         }
         if (p.y) {
             const TB *y = static_cast<const TB *>(p.y) + row_at(p.sy, m, p.S);
 #pragma unroll
-            for (int k = 0; k < NV; ++k) ry[k] = row_raw<TB, VEC, WHOLE>(y, at.c[k], p.C);
+            for (int k = 0; k < NV; ++k) ry[k] = loose_part<TB, VEC, WHOLE>(y + at.c[k], p.C - at.c[k]);
             if (p.gate) {
                 const TB *g = static_cast<const TB *>(p.gate) + row_at(p.sgate, m, p.S);
 #pragma unroll
-                for (int k = 0; k < NV; ++k) rg[k] = row_raw<TB, VEC, WHOLE>(g, at.c[k], p.C);
+                for (int k = 0; k < NV; ++k) rg[k] = loose_part<TB, VEC, WHOLE>(g + at.c[k], p.C - at.c[k]);
             }
         }
         float r[NV][VEC], sy = 0.f, sr = 0.f;
@@ -227,12 +227,6 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void residual_norm_kerne
     }
 }
 
-// LEAN: with the branches that row_raw avoids, and fewer registers.
-template <typename T, int N, bool WHOLE, bool LEAN> __device__ __forceinline__ Raw<T, N> run_of(const T *row, int c, int C) {
-    if constexpr (LEAN) return loose_part<T, N, WHOLE>(row + c, C - c);
-    else return row_raw<T, N, WHOLE>(row, c, C);
-}
-
 // Sums of a workgroup's rows: lanes of the same channels, in a fixed order, to part.
 template <int VEC, int NV, int WPR, bool WHOLE> __device__ __forceinline__ void leave_sums(const Place<VEC, NV, WPR> &at, int C, int log_l,
                                                                                float (&v)[NV][VEC], float *part) {
@@ -266,7 +260,6 @@ template <int VEC, int NV, int WPR, bool WHOLE> __device__ __forceinline__ void 
 template <typename TS, typename TB, int VEC, int NV, int WPR, bool WHOLE, bool GSUM>
 __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void residual_norm_bwd_kernel(ResParams p) {
     __shared__ float red[2][WPR][1];
-    constexpr bool LEAN = NV * VEC == 16 && GSUM; // (or registers would not do)
     int turn = 0;
     const Place<VEC, NV, WPR> at(p.log_l);
     const int seg = blockIdx.x / p.blocks_a_seg, j0 = blockIdx.x - seg * p.blocks_a_seg;
@@ -303,30 +296,32 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void residual_norm_bwd_k
         if (p.dr)
 #pragma unroll
             for (int k = 0; k < NV; ++k)
-                r.d[k] = run_of<TS, VEC, WHOLE, LEAN>(static_cast<const TS *>(p.dr) + dr_at, at.c[k], p.C);
+                r.d[k] = loose_part<TS, VEC, WHOLE>(static_cast<const TS *>(p.dr) + dr_at + at.c[k], p.C - at.c[k]);
         if (p.pre) {
             const TB *dn = static_cast<const TB *>(p.dn) + row_at(p.sdn, r.m, p.S);
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
-                r.o[k] = run_of<TS, VEC, WHOLE, LEAN>(static_cast<const TS *>(p.out) + out_at, at.c[k], p.C);
-                r.n[k] = run_of<TB, VEC, WHOLE, LEAN>(dn, at.c[k], p.C);
+                r.o[k] = loose_part<TS, VEC, WHOLE>(static_cast<const TS *>(p.out) + out_at + at.c[k], p.C - at.c[k]);
+                r.n[k] = loose_part<TB, VEC, WHOLE>(dn + at.c[k], p.C - at.c[k]);
             }
         }
         if (p.post || p.gate) {
             const TB *y = static_cast<const TB *>(p.y) + row_at(p.sy, r.m, p.S);
 #pragma unroll
-            for (int k = 0; k < NV; ++k) r.y[k] = run_of<TB, VEC, WHOLE, LEAN>(y, at.c[k], p.C);
+            for (int k = 0; k < NV; ++k) r.y[k] = loose_part<TB, VEC, WHOLE>(y + at.c[k], p.C - at.c[k]);
         }
         if (p.gate) {
             const TB *g = static_cast<const TB *>(p.gate) + row_at(p.sgate, r.m, p.S);
 #pragma unroll
-            for (int k = 0; k < NV; ++k) r.g[k] = run_of<TB, VEC, WHOLE, LEAN>(g, at.c[k], p.C);
+            for (int k = 0; k < NV; ++k) r.g[k] = loose_part<TB, VEC, WHOLE>(g + at.c[k], p.C - at.c[k]);
         }
         r.sy = p.post ? p.stats[2 * r.m] : 0.f;
         r.sr = p.pre ? p.stats[2 * r.m + 1] : 0.f;
     };
     const int64_t step = (int64_t)p.blocks_a_seg * at.rows;
-    constexpr bool AHEAD = NV * VEC == 8; // (16 channels a lane would not have the registers)
+    // (16 channels a lane would not have the registers; ragged rows: 16760 x 1001 f32 119 us
+    // without it, 180 with it)
+    constexpr bool AHEAD = WHOLE && NV * VEC == 8;
     Row next;
     if constexpr (AHEAD) load(next, (int64_t)j0 * at.rows); // (every workgroup has a row)
     // (the trip count is the same for every thread: barriers)
