@@ -886,15 +886,19 @@ constexpr int kFusedRank = 64; // ranks that adapt's tiles hold
 // more to read again than tiles that fill the card: from 1024 such tiles on for 17 to 32
 // ranks (2048 features, f32: 182 us against 198 at 32768 rows, 99 against 95 at 16384),
 // from 256 on for more (64 ranks, bfloat16: 128 against 168 at 32767, 36 against 43 at
-// 8192, 27 against 24 at 4096).  Of up to 16 ranks 16 rows were never slower (f32: 159
-// against 180 at 32768, 26 against 33 at 4096).
-int adapt_rows(const Shape &s, int64_t R) {
-    if (R <= 16 || s.N <= 0 || up(s.M, s.N) <= 16) return 16;
-    return s.tiles(32) >= (R <= 32 ? 1024 : 256) ? 32 : 16;
+// 8192, 27 against 24 at 4096).  Of up to 16 ranks 16 rows (f32: 159 us against 180 at
+// 32768, 26 against 33 at 4096; bfloat16: the gradients 59 against 62 at 12288) but in
+// bfloat16, of half as many bytes a row, about where tiles of 32 come one to a compute unit
+// (36 against 37 at 6144, 38 against 41 at 8192).
+int adapt_rows(const Shape &s, int64_t R, size_t element) {
+    if (s.N <= 0 || up(s.M, s.N) <= 16) return 16;
+    const int64_t tiles = s.tiles(32);
+    if (R <= 16) return element == 2 && tiles >= 128 && tiles < 320 ? 32 : 16;
+    return tiles >= (R <= 32 ? 1024 : 256) ? 32 : 16;
 }
 
 template <typename T> gdn2_status launch_adapt(AdaptParams p, const gdn2_low_rank_args &a, const Shape &sh, hipStream_t s) {
-    const int size = adapt_rows(sh, p.R);
+    const int size = adapt_rows(sh, p.R, sizeof(T));
     const int64_t tiles = sh.tiles(size);
     p.req = requests_of(a, sh, size);
     p.stream = (double)sh.M * (double)p.C * sizeof(T) >= kStreamBytes;
@@ -903,7 +907,8 @@ template <typename T> gdn2_status launch_adapt(AdaptParams p, const gdn2_low_ran
     // four of them from 512 tiles of 16 rows on (16 ranks, 16384 bfloat16 rows: 46 us
     // against 50; 64 ranks 81 and 92; 8192 f32 rows, 16 ranks: 47 and 46).
     if (size == 32) {
-        if (p.R <= 32) GDN2_RUN(2, 2, 4, 3);
+        if (p.R <= 16) GDN2_RUN(2, 1, 8, 2);
+        else if (p.R <= 32) GDN2_RUN(2, 2, 4, 3);
         else GDN2_RUN(2, 4, 4, 2);
     } else if (tiles >= 512) {
         if (p.R <= 16) GDN2_RUN(1, 1, 4, 4);
@@ -944,7 +949,7 @@ template <typename T> gdn2_status launch_expand(ExpandParams p, const gdn2_low_r
 }
 
 template <typename T> bool grids_ok(const Shape &sh, int64_t C, int64_t R) {
-    if (R > 0 && R <= kFusedRank) return sh.tiles(adapt_rows(sh, R)) < (1 << 22);
+    if (R > 0 && R <= kFusedRank) return sh.tiles(adapt_rows(sh, R, sizeof(T))) < (1 << 22);
     return sh.tiles(shrink_rows_of(sh)) < (1 << 23) && sh.tiles(kExpandRows) * groups_of<T>(C) < (1 << 24);
 }
 
