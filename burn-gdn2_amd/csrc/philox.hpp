@@ -1,9 +1,10 @@
 // The random words of dropout: Philox-4x32 with 7 rounds (J. K. Salmon, M. A. Moraes,
 // R. O. Dror, D. E. Shaw, "Parallel random numbers: as easy as 1, 2, 3", 2011), the
 // counter a 64-bit number, the key the seed.  A round is two products of 32 x 32 bits
-// into 64, which issue at a quarter of the rate of a sum: 7 rounds cost about 100
-// cycles of a SIMD for 64 elements, where their 4 bytes of bfloat16 in and out take it
-// 110 at 6 TB/s; the 10 rounds of the paper's safety margin would bound the pass.
+// into 64, which issue at a quarter of the rate of a sum: 7 rounds for 4 elements take
+// about as long as the memory does for their 4 bytes of bfloat16 in and out (32768 x
+// 2048: 45 us, 43 the bytes at a copy's rate), and so overlap with it; 10, the paper's
+// safety margin, would bound the pass.
 #pragma once
 
 #include <cmath>

@@ -6,10 +6,20 @@
 //   b = sigma drop(d),  dgate = b p act'(gate),  q = b act(gate)
 //   dpost = sum q yn,  f = q post,  dy = sy (f - yn mean(f yn))
 //
-// A row stays in the registers of its lanes, 8 channels a lane (16 in the widest
-// rows): up to 512 channels the 2^log_l lanes of a part of a wave, up to 2048 the four
+// A row stays in the registers of its lanes, 8 channels a lane (16 above 4096 channels):
+// up to 512 channels the 2^log_l lanes of a part of a wave, up to 2048 the four
 // waves of a workgroup, up to 8192 eight.  So each operand is read once and each
 // result written once, and the two means of a row are sums over its lanes.
+//
+// Bound: HBM.  Forward: 32768 x 2048 bfloat16 with a gate 124 us, 5.4 TB/s (129 at 4096
+// channels, where 16 a lane took 138; 126 at 8192); 8192 x 2048 with an f32 stream and
+// dropout 41 to 43 us, 4.8.  Backward: 8192 x 2048 bfloat16 with gate and dropout 53 us
+// and 5 for the weights' sums, 4.7 TB/s together; its instructions (generator, gate, two
+// norms) take about 35 us of a SIMD, which overlap with the bytes only in part.  Of 4096 channels
+// 64 us (16 a lane: 106), of 8192 93.  Rows that are no multiple of 8 bfloat16 (4 f32) go
+// by a form with a branch a run, since each row ends in the middle of one: 32768 x 321
+// bfloat16 80 us, of 320 57.  (Without branches, a row's last whole run turned to its place:
+// 87; its values all loaded first: 88.)
 //
 // The backward's workgroups walk the rows of one gate row (all rows, or a sample's
 // where the gate is a sample's) with their sums for the weights in registers: at most
@@ -281,7 +291,8 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void residual_norm_bwd_k
         if (p.pre) weights_n<VEC, WHOLE>(p.pre, at.c[k], p.C, wpre[k]);
         if (p.post) weights_n<VEC, WHOLE>(p.post, at.c[k], p.C, wpost[k]);
     }
-    // A row's operands, the next one's in flight while this one's are used.
+    // A row's operands, the next one's in flight while this one's are used (8192 x 2048
+    // bfloat16, gated, with dropout: 57 us, without 66).
     struct Row {
         Raw<TS, VEC> o[NV], d[NV];
         Raw<TB, VEC> n[NV], y[NV], g[NV];
@@ -501,8 +512,8 @@ Held held_of(int64_t C, int vec) {
 }
 
 // Workgroups for each gate row of the backward: 768 in all, three a compute unit, while
-// each has rows (8192 x 2048 bf16: 59.7 us; 1024: 60.2, 512: 61; 4 x 1999 x 320 f32: 27.8,
-// 35 and 27.5), and enough that no f32 sum runs over more than kMostRows.
+// each has rows (8192 x 2048 bfloat16: 59.7 us; 1024: 60.2, 512: 61; 4 x 1999 x 320 f32:
+// 27.8, 35 and 27.5), and enough that no f32 sum runs over more than kMostRows.
 int64_t blocks_of(int64_t seg_rows, int64_t segs, const Held &h) {
     const int64_t most = (seg_rows + h.rows - 1) / h.rows;
     const int64_t least = (seg_rows + (int64_t)h.rows * kMostRows - 1) / ((int64_t)h.rows * kMostRows);
@@ -634,7 +645,8 @@ gdn2_status backward(const gdn2_residual_norm_bwd_args *b, hipStream_t s, const 
     const BwdPlan q = plan_of(*a, VEC);
     const bool gsum = gate_summed(*a);
     ResParams p = params_of(*a);
-    if (q.blocks >= (1 << 22)) return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
+    const int64_t wgs = (2 + (gsum ? (a->gate_rows == GDN2_GATE_SAMPLE ? a->samples : 1) : 0)) * (int64_t)((p.C + 31) / 32);
+    if (q.blocks >= (1 << 22) || wgs >= (1 << 24)) return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
     if (M > 0) {
         if (q.bytes && (!b->workspace || b->workspace_bytes < q.bytes || reinterpret_cast<uintptr_t>(b->workspace) % 256))
             return fail(GDN2_EINVAL, who + "workspace missing, too small or not 256-byte aligned");
@@ -675,8 +687,6 @@ gdn2_status backward(const gdn2_residual_norm_bwd_args *b, hipStream_t s, const 
         t.post = M > 0 ? p.part_post : reinterpret_cast<const float *>(a->post_weight);
         t.gate = gsum ? (M > 0 ? p.part_gate : static_cast<const float *>(a->gate)) : nullptr;
         t.dpre = b->dpre; t.dpost = b->dpost; t.dgate = b->dgate; t.sgate = b->stride_dgate_n;
-        const int64_t wgs = (2 + (gsum ? (a->gate_rows == GDN2_GATE_SAMPLE ? a->samples : 1) : 0)) * (int64_t)t.tiles;
-        if (wgs >= (1 << 24)) return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
         hipLaunchKernelGGL((residual_sums_kernel<TB>), dim3((unsigned)wgs), dim3(256), 0, s, t);
     }
     GDN2_HIP_CHECK(hipGetLastError());

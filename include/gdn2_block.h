@@ -120,6 +120,8 @@ GDN2_API gdn2_status gdn2_residual_norm_f32_bf16(const gdn2_residual_norm_args *
  * dx may be d_out and dy may be d_normed with the same strides; nothing else may
  * overlap.  Sums over rows run in a fixed order: in f32 over at most 128 of them,
  * those in f64.
+ * Limits besides (else GDN2_NOT_APPLICABLE): N S < 2^28; where samples have a gate each,
+ * N < 2^21 and N ceil(C / 32) < 2^23.
  * workspace: gdn2_residual_norm_bwd_workspace_bytes(args) bytes, 256-byte aligned. */
 typedef struct gdn2_residual_norm_bwd_args {
     gdn2_residual_norm_args fwd;
@@ -157,9 +159,10 @@ GDN2_API gdn2_status gdn2_residual_norm_bwd_f32_bf16(const gdn2_residual_norm_bw
  * unspecified results, never an access out of bounds.
  * out may be y with the same strides, nothing else may overlap.
  * workspace: gdn2_low_rank_add_workspace_bytes(args) bytes, 256-byte aligned.
- * Limits (else GDN2_NOT_APPLICABLE): R <= 512; D, O, L, num_seqs < 2^24; B T < 2^30,
- * and 2^26 for requests of up to 16 tokens; strides of tokens and ranks < 2^24 (none
- * negative: GDN2_EINVAL).
+ * Limits (else GDN2_NOT_APPLICABLE): R <= 512; D, O, L, num_seqs < 2^24; fewer than 2^22
+ * tiles of 16 rows of one request (B ceil(T / 16); packed: T / 16 + num_seqs + 2), which
+ * for R > 64 and R = 0 by ceil(O / 256) are fewer than 2^24; strides of tokens and ranks < 2^24
+ * (none negative: GDN2_EINVAL).
  * ---------------------------------------------------------------------- */
 typedef struct gdn2_low_rank_args {
     const void *x, *a, *b, *y;
@@ -190,6 +193,8 @@ GDN2_API gdn2_status gdn2_low_rank_add_bf16(const gdn2_low_rank_args *args, gdn2
  *          all rows of an adapter's requests, 0 for one without any; in a fixed order,
  *          in f32 over at most 4096 rows, those in f64
  * Nothing may overlap.
+ * Limits besides, the forward's for D in place of O (else GDN2_NOT_APPLICABLE):
+ * (B T / 4096 + requests + 2) ((D + O) / 64 + 2) < 2^23, L R (D + O) < 2^31.
  * workspace: gdn2_low_rank_add_bwd_workspace_bytes(args) bytes, 256-byte aligned. */
 typedef struct gdn2_low_rank_bwd_args {
     gdn2_low_rank_args fwd;

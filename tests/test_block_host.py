@@ -124,6 +124,35 @@ def test_residual_refusals_of_the_c_entry():
         assert bwd(dict(channels=0)) == C.GDN2_OK
 
 
+def test_sizes_at_the_limits_of_the_c_entries():
+    """Refused before anything runs, and no sooner than the header says (there the next
+    check, of the workspace or a pointer, refuses)."""
+    from gdn2_amd import _capi as C
+
+    L = C.lib()
+    for fn in (L.gdn2_residual_norm_bwd_f32, L.gdn2_residual_norm_bwd_bf16, L.gdn2_residual_norm_bwd_f32_bf16):
+
+        def bwd(**kw):
+            b = C.ResidualNormBwdArgs()
+            b.fwd = _res(gate=256, **kw)
+            b.d_out = b.dx = b.dy = b.dgate = 256
+            return fn(ctypes.byref(b), None)
+
+        one = dict(gate_rows=C.GATE_SAMPLE)
+        assert bwd(samples=1 << 16, rows=2, channels=8192, **one) == C.GDN2_NOT_APPLICABLE
+        assert bwd(samples=(1 << 15) - 1, rows=2, channels=8192, **one) == C.GDN2_EINVAL
+        assert bwd(samples=1 << 22, rows=1, channels=64, **one) == C.GDN2_NOT_APPLICABLE
+        assert bwd(samples=(1 << 21) - 1, rows=100, channels=64, **one) == C.GDN2_EINVAL
+        assert bwd(samples=1, rows=1 << 29, channels=2048, gate_rows=C.GATE_ALL) == C.GDN2_NOT_APPLICABLE
+        assert bwd(samples=1, rows=(1 << 28) - 1, channels=2048, gate_rows=C.GATE_ALL) == C.GDN2_EINVAL
+    for fn in (L.gdn2_low_rank_add_f32, L.gdn2_low_rank_add_bf16):
+        for rank in (16, 64):
+            assert fn(_lora(batch=1 << 22, seq_len=1, rank=rank), None) == C.GDN2_NOT_APPLICABLE
+            assert fn(_lora(batch=1 << 21, seq_len=33, rank=rank), None) == C.GDN2_NOT_APPLICABLE
+        assert fn(_lora(batch=(1 << 20) - 1, seq_len=64, rank=128, out_features=1024, workspace=None), None) == C.GDN2_EINVAL
+        assert fn(_lora(batch=1 << 20, seq_len=64, rank=128, out_features=4096, workspace=None), None) == C.GDN2_NOT_APPLICABLE
+
+
 def test_residual_workspace_sizes():
     from gdn2_amd import _capi as C
 
