@@ -31,8 +31,8 @@
 // of loads and its adapter's 0.5 MB from L2.  64 f32 rows, an adapter of 16 ranks each:
 // 13 us, a chain of latencies (offsets or adapter, x and a, the waves' sums, b and y).
 // Gradients at 4 x 2048 bfloat16 rows, 16 ranks: 20 us dh and dx, 14 the products, 4
-// the sums.  Without effect: tiles in the order of the XCDs (211 for 169 us), chunks that
-// start elsewhere in each workgroup, x's operands straight from memory.
+// the sums.  Slower: tiles in the order of the XCDs (211 us for 169).  The same: chunks
+// that start elsewhere in each workgroup, x's operands straight from memory.
 #include <algorithm>
 #include <exception>
 #include <string>
