@@ -77,6 +77,14 @@ def test_sizes(gpu, ty, M, C):
 
 
 @pytest.mark.parametrize("ty", list(TYPES))
+@pytest.mark.parametrize("C", [2100, 2051, 4096, 4104])
+@pytest.mark.parametrize("shared", [False, True])
+def test_wide_rows(gpu, ty, C, shared):
+    """More rows than workgroups, of channels that eight waves hold."""
+    check(gpu, make(1602, C, ty, N=2, gate_shape=(2, 1, C) if shared else None), 1602, C, p=0.1)
+
+
+@pytest.mark.parametrize("ty", list(TYPES))
 @pytest.mark.parametrize("post,pre,gate", [(a, b, c) for a in (False, True) for b in (False, True) for c in (False, True)])
 @pytest.mark.parametrize("p", [0.0, 0.3])
 def test_forms(gpu, ty, post, pre, gate, p):
