@@ -642,11 +642,12 @@ gdn2_status backward(const gdn2_residual_norm_bwd_args *b, hipStream_t s, const 
     }
     if (!sizes_ok(*a)) return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
     constexpr int VEC = vec_of<TS, TB>();
-    const BwdPlan q = plan_of(*a, VEC);
-    const bool gsum = gate_summed(*a);
+    const BwdPlan q = M > 0 ? plan_of(*a, VEC) : BwdPlan{};
+    const bool gsum = gate_summed(*a) && (a->gate_rows == GDN2_GATE_ALL || a->samples > 0); // (no samples: no rows of dgate)
     ResParams p = params_of(*a);
     const int64_t wgs = (2 + (gsum ? (a->gate_rows == GDN2_GATE_SAMPLE ? a->samples : 1) : 0)) * (int64_t)((p.C + 31) / 32);
     if (q.blocks >= (1 << 22) || wgs >= (1 << 24)) return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
+    if (M == 0 && !a->pre_weight && !a->post_weight && !gsum) return GDN2_OK;
     if (M > 0) {
         if (q.bytes && (!b->workspace || b->workspace_bytes < q.bytes || reinterpret_cast<uintptr_t>(b->workspace) % 256))
             return fail(GDN2_EINVAL, who + "workspace missing, too small or not 256-byte aligned");

@@ -1,0 +1,31 @@
+"""What the block operators do at their edges without a GPU: empty batches and sizes
+whose products pass 64 bits.  No call here gets as far as a launch."""
+import ctypes
+
+from gdn2_amd import _capi as C
+
+
+def _res(**kw):
+    a = C.ResidualNormArgs()
+    for k, v in dict(dict(x=256, y=256, out=256, samples=2, rows=3, channels=8, eps=1e-5, residual_scale=1.0,
+                          branch_scale=1.0), **kw).items():
+        setattr(a, k, v)
+    return a
+
+
+def _res_bwd(fwd, **kw):
+    b = C.ResidualNormBwdArgs()
+    b.fwd = _res(**fwd)
+    for k, v in dict(dict(d_out=256, dx=256, dy=256), **kw).items():
+        setattr(b, k, v)
+    return ctypes.byref(b)
+
+
+def test_residual_backward_of_no_samples():
+    """A gate a sample and no samples: an empty dgate, and nothing to launch."""
+    L = C.lib()
+    for fn in (L.gdn2_residual_norm_bwd_f32, L.gdn2_residual_norm_bwd_bf16, L.gdn2_residual_norm_bwd_f32_bf16):
+        for rows in (0, 3):
+            assert fn(_res_bwd(dict(gate=256, gate_rows=C.GATE_SAMPLE, samples=0, rows=rows), dgate=256), None) == C.GDN2_OK
+        assert fn(_res_bwd(dict(samples=0)), None) == C.GDN2_OK
+    assert L.gdn2_residual_norm_bwd_workspace_bytes(_res_bwd(dict(gate=256, gate_rows=C.GATE_SAMPLE, samples=0), dgate=256)) == 0

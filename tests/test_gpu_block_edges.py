@@ -1,0 +1,37 @@
+"""The block operators' edges on the device: C entries without rows, sums whose terms
+differ much in size, large shapes of constant rows."""
+import ctypes
+
+import pytest
+import torch
+
+import block_testutil as K
+
+pytestmark = pytest.mark.gpu
+F32, BF = torch.float32, torch.bfloat16
+
+
+@pytest.mark.parametrize("ty", ["f32", "bf16", "f32_bf16"])
+@pytest.mark.parametrize("samples,rows", [(0, 3), (0, 0), (2, 0)])
+@pytest.mark.parametrize("gate_rows", [0, 1, 2])
+def test_residual_backward_entry_without_rows(gpu, ty, samples, rows, gate_rows):
+    """The weights' gradients, and those of gates that no row takes, are zeros."""
+    from gdn2_amd import _capi as C
+
+    n = 40
+    w, dpre, dpost = (torch.full((n,), 9.0, device=gpu) for _ in range(3))
+    gate, dgate, some = (torch.full((4, n), 9.0, dtype=F32 if ty == "f32" else BF, device=gpu) for _ in range(3))
+    b = C.ResidualNormBwdArgs()
+    for k, v in dict(y=some, gate=gate, post_weight=w, pre_weight=w, out=some).items():
+        setattr(b.fwd, k, v.data_ptr())
+    for k, v in dict(samples=samples, rows=rows, channels=n, stride_gate_n=n, eps=1e-5, residual_scale=1.0, branch_scale=1.0,
+                     gate_rows=gate_rows).items():
+        setattr(b.fwd, k, v)
+    for k, v in dict(dx=some, dy=some, dgate=dgate, dpost=dpost, dpre=dpre).items():
+        setattr(b, k, v.data_ptr())
+    b.stride_dgate_n = n
+    assert getattr(C.lib(), "gdn2_residual_norm_bwd_" + ty)(ctypes.byref(b), torch.cuda.current_stream().cuda_stream) == C.GDN2_OK
+    torch.cuda.synchronize()
+    assert (dpre == 0).all() and (dpost == 0).all() and (some == 9).all()
+    written = {0: 0, 1: samples, 2: 1}[gate_rows]
+    assert (dgate[:written] == 0).all() and (dgate[written:] == 9).all()
