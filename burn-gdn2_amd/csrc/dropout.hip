@@ -59,10 +59,11 @@ template <typename T> gdn2_status run(const void *x, void *y, int64_t rows, int6
     if (C >= (int64_t(1) << 31) || rows >= (int64_t(1) << 40))
         return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
     if (C % 8 == 0 && (rows == 1 || (sx == C && sy == C))) {
-        const int64_t per = 256 * VEC, n = rows * C;
-        const int64_t blocks = (n + per - 1) / per;
-        if ((double)rows * (double)C >= 1e15 || blocks >= (1 << 24))
+        const int64_t per = 256 * VEC;
+        // (fewer than 2^24 workgroups, 2^32 threads; in doubles: the product may pass 64 bits)
+        if ((double)rows * (double)C > ((1 << 24) - 1) * (double)per)
             return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
+        const int64_t n = rows * C, blocks = (n + per - 1) / per;
         hipLaunchKernelGGL((dropout_flat_kernel<T, VEC>), dim3((unsigned)blocks), dim3(256), 0, s, static_cast<const T *>(x),
                            static_cast<T *>(y), n, d);
     } else {

@@ -547,7 +547,7 @@ gdn2_status check(const gdn2_residual_norm_args *a, const std::string &who, bool
     if (!(a->eps >= 0.)) return fail(GDN2_EINVAL, who + "eps must not be negative");
     if (!a->y && (a->gate || a->post_weight || a->dropout.p != 0.))
         return fail(GDN2_EINVAL, who + "a gate, a weight or dropout without y");
-    if (a->channels == 0 || (!bwd && a->samples * a->rows == 0)) {
+    if (a->channels == 0 || (!bwd && (a->samples == 0 || a->rows == 0))) {
         *nothing = true;
         return GDN2_OK;
     }
@@ -634,13 +634,14 @@ gdn2_status backward(const gdn2_residual_norm_bwd_args *b, hipStream_t s, const 
     if (!b->dpre != !a->pre_weight || !b->dpost != !a->post_weight)
         return fail(GDN2_EINVAL, who + "a weight and its gradient go together");
     if (!b->dgate != !a->gate || !b->dy != !a->y) return fail(GDN2_EINVAL, who + "y, gate and their gradients go together");
-    const int64_t M = a->samples * a->rows;
-    if (M > 0) {
+    const bool some = a->samples > 0 && a->rows > 0;
+    if (some) {
         if (!b->d_normed != !a->pre_weight) return fail(GDN2_EINVAL, who + "d_normed and pre_weight go together");
         if (a->pre_weight && !a->out) return fail(GDN2_EINVAL, who + "null pointer");
         if (!a->stats && (a->pre_weight || a->post_weight)) return fail(GDN2_EINVAL, who + "stats missing");
     }
     if (!sizes_ok(*a)) return fail(GDN2_NOT_APPLICABLE, who + "sizes above the kernels' limits");
+    const int64_t M = a->samples * a->rows; // (below 2^30)
     constexpr int VEC = vec_of<TS, TB>();
     const BwdPlan q = M > 0 ? plan_of(*a, VEC) : BwdPlan{};
     const bool gsum = gate_summed(*a) && (a->gate_rows == GDN2_GATE_ALL || a->samples > 0); // (no samples: no rows of dgate)

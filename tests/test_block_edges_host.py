@@ -29,3 +29,22 @@ def test_residual_backward_of_no_samples():
             assert fn(_res_bwd(dict(gate=256, gate_rows=C.GATE_SAMPLE, samples=0, rows=rows), dgate=256), None) == C.GDN2_OK
         assert fn(_res_bwd(dict(samples=0)), None) == C.GDN2_OK
     assert L.gdn2_residual_norm_bwd_workspace_bytes(_res_bwd(dict(gate=256, gate_rows=C.GATE_SAMPLE, samples=0), dgate=256)) == 0
+
+
+def test_sizes_whose_product_passes_64_bits():
+    """2^32 samples of 2^32 rows are not none."""
+    L = C.lib()
+    for fn in (L.gdn2_residual_norm_f32, L.gdn2_residual_norm_bf16, L.gdn2_residual_norm_f32_bf16):
+        for samples, rows in ((1 << 32, 1 << 32), (1 << 62, 4), (1 << 33, 1 << 30)):
+            assert fn(_res(samples=samples, rows=rows), None) == C.GDN2_NOT_APPLICABLE
+    for fn in (L.gdn2_residual_norm_bwd_f32, L.gdn2_residual_norm_bwd_bf16, L.gdn2_residual_norm_bwd_f32_bf16):
+        assert fn(_res_bwd(dict(samples=1 << 32, rows=1 << 32)), None) == C.GDN2_NOT_APPLICABLE
+    for fn in (L.gdn2_dropout_f32, L.gdn2_dropout_bf16):
+        assert fn(256, 512, 1 << 39, 1 << 30, 1 << 30, 1 << 30, C.Dropout(0.5, 0, 0, None), None) == C.GDN2_NOT_APPLICABLE
+    big = dict(batch=1 << 32, seq_len=1 << 32)
+    for fn in (L.gdn2_low_rank_add_f32, L.gdn2_low_rank_add_bf16):
+        a = C.LowRankArgs()
+        for k, v in dict(x=256, a=256, b=256, y=256, out=512, adapters=256, in_features=8, out_features=8, rank=2, num_adapters=2,
+                         **big).items():
+            setattr(a, k, v)
+        assert fn(a, None) == C.GDN2_NOT_APPLICABLE
