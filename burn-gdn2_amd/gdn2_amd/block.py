@@ -28,7 +28,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import _capi as C
-from .mixer import _SUFFIX, _contig, _call, _device, _p, _workspace
+from .mixer import _SUFFIX, _contig, _call, _device, _p, _same_layout, _workspace
 from .ops import _stream_of
 
 _U64 = (1 << 64) - 1
@@ -59,7 +59,7 @@ def _clash(a: Optional[torch.Tensor], b: Optional[torch.Tensor]) -> bool:
     (a0, a1), (b0, b1) = _span(a), _span(b)
     if a1 <= b0 or b1 <= a0:
         return False
-    if a.shape == b.shape and a.stride() == b.stride() and a.element_size() == b.element_size():
+    if a.shape == b.shape and _same_layout(a, b) and a.element_size() == b.element_size():
         n, e = a.shape[-1], a.element_size()
         rows = [s for m, s in zip(a.shape[:-1], a.stride()[:-1]) if m > 1]
         row = math.gcd(*rows) if rows else 0
@@ -88,7 +88,7 @@ def _takes(name: str, t: torch.Tensor, like: torch.Tensor, dtype, own: Optional[
         raise ValueError(f"{name} must have the operand's shape")
     if t.numel() and (t.shape[-1] != 1 and t.stride(-1) != 1 or not _rows_apart(t)):
         raise ValueError(f"{name}'s channels must be contiguous and its rows apart")
-    if own is not None and t.data_ptr() == own.data_ptr() and t.stride() == own.stride():
+    if own is not None and t.data_ptr() == own.data_ptr() and _same_layout(t, own):
         own = None
     if any(_clash(t, o) for o in (own, *others)):
         raise ValueError(f"{name} must not share memory with another operand")

@@ -2,6 +2,9 @@
 whose products pass 64 bits.  No call here gets as far as a launch."""
 import ctypes
 
+import pytest
+import torch
+
 from gdn2_amd import _capi as C
 
 
@@ -48,3 +51,29 @@ def test_sizes_whose_product_passes_64_bits():
                          **big).items():
             setattr(a, k, v)
         assert fn(a, None) == C.GDN2_NOT_APPLICABLE
+
+
+def _one(t, *strides):
+    """t's memory by other strides of its dimensions of one."""
+    return t.as_strided(t.shape, strides)
+
+
+def test_strides_of_dimensions_of_one_do_not_count():
+    """In place is in place, and other columns of the same rows are other columns (these
+    operands are not on a device: the next check refuses)."""
+    import gdn2_amd as G
+
+    x, y, w = torch.zeros(64, 1, 8), torch.zeros(64, 1, 8), torch.zeros(8)
+    out, normed = _one(x, 8, 512, 1), _one(y, 8, 3, 1)
+    one = torch.zeros(5, 1)
+    buf = torch.zeros(4, 1, 32)
+    left, right = buf[..., :8], _one(buf[..., 8:], 32, 77, 1)[..., :8]
+    ids, a = torch.zeros(64, dtype=torch.int32), torch.zeros(1, 2, 8)
+    for f, args, kw in ((G.dropout, (x, 0.5), dict(out=out)), (G.dropout, (one, 0.5), dict(out=_one(one, 1, 9))),
+                        (G.residual_norm, (x, y), dict(out=out)), (G.residual_norm, (x, y, None, w, w), dict(out=out, normed=normed)),
+                        (G.residual_norm, (left, torch.zeros(4, 1, 8)), dict(out=right)),
+                        (G.low_rank_add, (y, x, a, a, ids), dict(out=normed))):
+        with pytest.raises(TypeError, match="device"):
+            f(*args, **kw)
+    with pytest.raises(ValueError):  # still refused: another place of the same memory
+        G.dropout(buf[..., :8], 0.5, out=_one(buf[..., 4:], 32, 5, 1)[..., :8])

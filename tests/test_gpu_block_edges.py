@@ -35,3 +35,24 @@ def test_residual_backward_entry_without_rows(gpu, ty, samples, rows, gate_rows)
     assert (dpre == 0).all() and (dpost == 0).all() and (some == 9).all()
     written = {0: 0, 1: samples, 2: 1}[gate_rows]
     assert (dgate[:written] == 0).all() and (dgate[written:] == 9).all()
+
+
+@pytest.mark.parametrize("ty", [F32, BF])
+def test_in_place_by_other_strides_of_dimensions_of_one(gpu, ty):
+    import gdn2_amd as G
+
+    g = torch.Generator().manual_seed(3)
+    rnd = lambda *s: torch.randn(*s, generator=g).to(ty).to(gpu)  # noqa: E731
+    x, y, a, b = rnd(64, 1, 40), rnd(64, 1, 40), rnd(3, 4, 40), rnd(3, 4, 40)
+    w, ids = torch.rand(40, generator=g).to(gpu), (torch.arange(64, dtype=torch.int32) % 4).to(gpu)
+    one = lambda t: t.as_strided(t.shape, (40, 512, 1))  # noqa: E731
+    ref = G.dropout(x, 0.5, 3)
+    t = x.clone()
+    assert torch.equal(G.dropout(t, 0.5, 3, out=one(t)), ref) and torch.equal(t, ref)
+    ref = G.residual_norm(x, y, None, w, w)
+    t, u = x.clone(), y.clone()
+    got = G.residual_norm(t, u, None, w, w, out=one(t), normed=one(u))
+    assert all(torch.equal(p, q) for p, q in zip(got, ref)) and torch.equal(t, ref[0]) and torch.equal(u, ref[1])
+    ref = G.low_rank_add(y, x, a, b, ids)
+    t = y.clone()
+    assert torch.equal(G.low_rank_add(t, x, a, b, ids, out=one(t)), ref) and torch.equal(t, ref)
