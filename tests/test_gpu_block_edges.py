@@ -56,3 +56,36 @@ def test_in_place_by_other_strides_of_dimensions_of_one(gpu, ty):
     ref = G.low_rank_add(y, x, a, b, ids)
     t = y.clone()
     assert torch.equal(G.low_rank_add(t, x, a, b, ids, out=one(t)), ref) and torch.equal(t, ref)
+
+
+@pytest.mark.parametrize("C,M", [(8, 2 ** 29 + 300), (520, 2 ** 21 + 5), (2056, 2 ** 21 + 5)])
+def test_residual_norm_over_more_rows_than_a_launch(gpu, C, M):
+    """A second turn of the workgroups' row loop, and places past 2^32 elements: the bits of
+    calls on those rows alone, and in the backward the sums over all rows."""
+    import gdn2_amd as G
+
+    g = torch.Generator(device=gpu).manual_seed(C)
+    rnd = lambda: torch.empty(M, C, dtype=BF, device=gpu).normal_(generator=g)  # noqa: E731
+    x, y = rnd(), rnd()
+    post, pre = (0.5 + torch.rand(C, generator=g, device=gpu) for _ in range(2))
+    a = (None, post, pre, 1e-5, "none", 0.8, 0.5, 0.1, 7)
+    out, normed, stats = G.residual_norm(x, y, *a, offset=11, return_stats=True)
+    spans = [slice(r, min(r + 9, M)) for r in (0, M // 2, 2 ** 32 // C, M - 310, M - 9)]
+    for at in spans:
+        ref = G.residual_norm(x[at], y[at], *a, offset=11 + at.start * (C // 4), return_stats=True)
+        assert all(torch.equal(p[at], q) for p, q in zip((out, normed, stats), ref))
+    if M >= 2 ** 28:  # (the backward's limit)
+        return
+    del normed
+    b = (None, post, pre, "none", 0.8, 0.5, 0.1, 7)
+    got = G.residual_norm_backward(out, y, stats, x, y, *b, offset=11)  # (x and y stand for the results' gradients)
+    for at in spans:
+        ref = G.residual_norm_backward(out[at], y[at], stats[at], x[at], y[at], *b, offset=11 + at.start * (C // 4))
+        assert all(torch.equal(got[k][at], ref[k]) for k in ("dx", "dy"))
+    want = torch.zeros(C, dtype=K.F64, device=gpu)
+    size = torch.zeros_like(want)
+    for r in range(0, M, 2 ** 17):
+        t = y[r:r + 2 ** 17].double() * out[r:r + 2 ** 17].double() * stats[r:r + 2 ** 17, 1:].double()
+        want += t.sum(0)
+        size += t.abs().sum(0)
+    K.near(got["dpre"], want.cpu(), ((128 + 3) * K.U * size).cpu())
