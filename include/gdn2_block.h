@@ -119,7 +119,7 @@ GDN2_API gdn2_status gdn2_residual_norm_f32_bf16(const gdn2_residual_norm_args *
  *   dpost, dpre  [C]; NULL iff the weight is
  * dx may be d_out and dy may be d_normed with the same strides; nothing else may
  * overlap.  Sums over rows run in a fixed order: in f32 over at most 128 of them,
- * those in f64.
+ * those in f64 (of a workgroup's rows, rounded to f32, and of all workgroups).
  * Limits besides (else GDN2_NOT_APPLICABLE): N S < 2^28; where samples have a gate each,
  * N < 2^21 and N ceil(C / 32) < 2^23.
  * workspace: gdn2_residual_norm_bwd_workspace_bytes(args) bytes, 256-byte aligned. */

@@ -89,3 +89,26 @@ def test_residual_norm_over_more_rows_than_a_launch(gpu, C, M):
         want += t.sum(0)
         size += t.abs().sum(0)
     K.near(got["dpre"], want.cpu(), ((128 + 3) * K.U * size).cpu())
+
+
+@pytest.mark.parametrize("ty", [F32, BF])
+@pytest.mark.parametrize("C", [8, 24, 40, 320, 512])
+def test_column_sums_of_narrow_rows(gpu, ty, C):
+    """The rows that a workgroup holds at once (256 of 8 channels, 4 of 512) are added in 64
+    bits: one of 2^24, ones, and as many rows again with -2^24 among zeros.  Each lane has
+    one row; a workgroup's sum is rounded to f32, half a step of 2^24 (1) off at most."""
+    import gdn2_amd as G
+
+    lanes = 1
+    while lanes * 8 < C:
+        lanes *= 2
+    n = 256 // lanes
+    v = torch.zeros(2 * n, C, dtype=ty, device=gpu)
+    v[0], v[1:n - 1], v[n] = 2.0 ** 24, 1, -2.0 ** 24
+    one, w = torch.ones_like(v), torch.ones(C, device=gpu)
+    stats = torch.ones(2 * n, 2, device=gpu)
+    got = G.residual_norm_backward(one, one, stats, None, v, pre_weight=w)["dpre"]
+    assert float((got - (n - 2)).abs().max()) <= 1
+    r = G.residual_norm_backward(one, one, stats, v, None, torch.ones(C, dtype=ty, device=gpu), w)
+    for k in ("dpost", "dgate"):
+        assert float((r[k].float() - (n - 2)).abs().max()) <= 1, k
