@@ -897,13 +897,16 @@ constexpr int kFusedRank = 64; // ranks that adapt's tiles hold
 // ranks (2048 features, f32: 182 us against 198 at 32768 rows, 99 against 95 at 16384),
 // from 256 on for more (64 ranks, bfloat16: 128 against 168 at 32767, 36 against 43 at
 // 8192, 27 against 24 at 4096).  Of up to 16 ranks 16 rows (f32: 159 us against 180 at
-// 32768, 26 against 33 at 4096; bfloat16: the gradients 59 against 62 at 12288) but in
-// bfloat16, of half as many bytes a row, about where tiles of 32 come one to a compute unit
-// (36 against 37 at 6144, 38 against 41 at 8192).
+// 32768, 26 against 33 at 4096) but in bfloat16, of half as many bytes a row, where tiles of
+// 32 come at most one to a compute unit (the registers of its form allow one there) and tiles
+// of 16 come more than one: 128 to 256 tiles of 32 (the gradients at 160, 192 and 256: 31.8,
+// 33.5 and 39.0 us, of 16 rows 34.2, 35.9 and 40.7; the forward 23.0, 22.9 and 29.1 against
+// 23.2, 23.9 and 27.2; at 64 and 128 both the same; from 257 on, where a second round
+// follows, 51.9 against 46.7 and 40.8 against 34.9).
 int adapt_rows(const Shape &s, int64_t R, size_t element) {
     if (s.N <= 0 || up(s.M, s.N) <= 16) return 16;
     const int64_t tiles = s.tiles(32);
-    if (R <= 16) return element == 2 && tiles >= 128 && tiles < 320 ? 32 : 16;
+    if (R <= 16) return element == 2 && tiles >= 128 && tiles <= 256 ? 32 : 16;
     return tiles >= (R <= 32 ? 1024 : 256) ? 32 : 16;
 }
 

@@ -50,7 +50,8 @@ def check(gpu, B, T, D, O, R, ty, L=2, cu=None):
 @pytest.mark.parametrize("B,T", [
     (1, 1000),   # 16 rows a tile, eight waves
     (600, 13),   # ... four waves, short requests
-    (1, 8200),   # 257 tiles of 32 rows, 513 of 16
+    (1, 6150),   # 193 tiles of 32 rows
+    (1, 8200),   # 257 of 32, 513 of 16
     (1, 10300),  # 322 of 32
     (3, 11000)])  # 1032 of 32
 @pytest.mark.parametrize("R", [16, 24, 64])
