@@ -920,8 +920,9 @@ template <typename T> gdn2_status launch_adapt(AdaptParams p, const gdn2_low_ran
     // four of them from 512 tiles of 16 rows on (16 ranks, 16384 bfloat16 rows: 46 us
     // against 50; 64 ranks 81 and 92; 8192 f32 rows, 16 ranks: 47 and 46).
     if (size == 32) {
-        if (p.R <= 16) GDN2_RUN(2, 1, 8, 2);
-        else if (p.R <= 32) GDN2_RUN(2, 2, 4, 3);
+        if (p.R <= 16) {
+            if constexpr (sizeof(T) == 2) GDN2_RUN(2, 1, 8, 2); // (f32: never of so few ranks)
+        } else if (p.R <= 32) GDN2_RUN(2, 2, 4, 3);
         else GDN2_RUN(2, 4, 4, 2);
     } else if (tiles >= 512) {
         if (p.R <= 16) GDN2_RUN(1, 1, 4, 4);
