@@ -68,6 +68,13 @@ struct ResParams {
 // (v_rcp_f32 is within one unit in the last place)
 __device__ __forceinline__ float sigmoid_f(float z) { return __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * z)); }
 
+// 1 / sqrt(v), v >= 0 (v_rsq_f32 takes a subnormal v, which eps = 0 allows, as 0)
+__device__ __forceinline__ float rstd_f(float v) {
+    const bool tiny = v < 0x1p-126f;
+    const float r = __builtin_amdgcn_rsqf(tiny ? v * 0x1p48f : v);
+    return tiny ? r * 0x1p24f : r;
+}
+
 // a = act(z), d = act'(z)
 __device__ __forceinline__ void gate_of(int act, float z, float &a, float &d) {
     if (act == GDN2_GATE_NONE) {
@@ -178,7 +185,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void residual_norm_kerne
 #pragma unroll
                     for (int j = 0; j < VEC; ++j) sum[0] = __builtin_fmaf((float)ry[k][j], (float)ry[k][j], sum[0]);
                 row_sum<WPR, 1>(sum, p.log_l, red, turn);
-                sy = __builtin_amdgcn_rsqf(__builtin_fmaf(sum[0], p.inv_c, p.eps));
+                sy = rstd_f(__builtin_fmaf(sum[0], p.inv_c, p.eps));
             }
 #pragma unroll
             for (int k = 0; k < NV; ++k) {
@@ -221,7 +228,7 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR) void residual_norm_kerne
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) sum[0] = __builtin_fmaf(r[k][j], r[k][j], sum[0]);
             row_sum<WPR, 1>(sum, p.log_l, red, turn);
-            sr = __builtin_amdgcn_rsqf(__builtin_fmaf(sum[0], p.inv_c, p.eps));
+            sr = rstd_f(__builtin_fmaf(sum[0], p.inv_c, p.eps));
             TB *normed = static_cast<TB *>(p.normed) + row_at(p.snormed, m, p.S);
 #pragma unroll
             for (int k = 0; k < NV; ++k) {

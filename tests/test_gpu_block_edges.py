@@ -112,3 +112,24 @@ def test_column_sums_of_narrow_rows(gpu, ty, C):
     r = G.residual_norm_backward(one, one, stats, v, None, torch.ones(C, dtype=ty, device=gpu), w)
     for k in ("dpost", "dgate"):
         assert float((r[k].float() - (n - 2)).abs().max()) <= 1, k
+
+
+@pytest.mark.parametrize("C", [96, 2048])
+@pytest.mark.parametrize("size", [1.2e-19, 1e-19, 1e-20, 2.0 ** -70])
+def test_rows_whose_squares_are_subnormal(gpu, C, size):
+    """Without eps: both statistics are finite.  A square, and the mean, are each off by half
+    of 2^-149 at most, halved by the root; the rest as in block_testutil."""
+    import gdn2_amd as G
+
+    x = torch.full((3, C), size, device=gpu)
+    x[1] *= -1
+    x[2] = 0
+    w = torch.ones(C, device=gpu)
+    got, n, stats = G.residual_norm(torch.zeros_like(x), x, None, w, w, eps=0.0, return_stats=True)
+    rel = 2.0 ** -150 / size ** 2 + 25 * K.U
+    assert float((stats[:2, 0].double() * x[0, 0].double() - 1).abs().max()) <= rel
+    assert float((got[:2].double() - torch.tensor([[1.0], [-1.0]], device=gpu)).abs().max()) <= rel
+    assert stats[2, 0].isinf() and got[2].isnan().all()  # 1 / 0, and 0 times it
+    _, n, stats = G.residual_norm(x, pre_weight=w, eps=0.0, return_stats=True)
+    assert float((stats[:2, 1].double() * x[0, 0].double() - 1).abs().max()) <= rel
+    assert float((n[:2].double() - torch.tensor([[1.0], [-1.0]], device=gpu)).abs().max()) <= rel
