@@ -278,6 +278,9 @@ def residual_norm(x, y=None, gate=None, post_weight=None, pre_weight=None, eps: 
                                *_sizes(x), *_ns(x), *_ns(y), *_gate_ns(gate, kind), *_ns(o), *_ns(n), eps, residual_scale,
                                branch_scale, _GATES[activation], kind, drop)
         _call(getattr(C.lib(), "gdn2_residual_norm" + _TYPES[x.dtype, branch]), a, index)
+    elif stats is not None and stats.numel():  # rows of no channels: the mean of nothing
+        for i, taken in enumerate((post_weight is not None, pre_weight is not None)):
+            stats[..., i] = math.nan if taken else 0.0
     o = out if out is not None else _seen(o, shape)
     n = normed if normed is not None else _seen(n, shape)
     return (o, n, stats) if return_stats else (o, n)

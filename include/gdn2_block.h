@@ -71,7 +71,7 @@ GDN2_API gdn2_status gdn2_dropout_bf16(const void *x, void *y, int64_t rows, int
  * (not wanted) only with it.
  * stats [N, S, 2] contiguous, or NULL: rstd(y) and rstd(r), which the backward
  * takes; 0 for a norm that is not taken.  rstd(r) and n are of r before its
- * rounding.
+ * rounding.  Without channels nothing is written.
  * out may be x and normed may be y, with the same strides; nothing else may
  * overlap.
  * _f32, _bf16: all of them; _f32_bf16: x and out f32; y, gate and normed bf16.

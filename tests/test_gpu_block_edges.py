@@ -133,3 +133,20 @@ def test_rows_whose_squares_are_subnormal(gpu, C, size):
     _, n, stats = G.residual_norm(x, pre_weight=w, eps=0.0, return_stats=True)
     assert float((stats[:2, 1].double() * x[0, 0].double() - 1).abs().max()) <= rel
     assert float((n[:2].double() - torch.tensor([[1.0], [-1.0]], device=gpu)).abs().max()) <= rel
+
+
+@pytest.mark.parametrize("post,pre", [(True, True), (False, True), (True, False), (False, False)])
+def test_statistics_of_rows_of_no_channels(gpu, post, pre):
+    """NaN, the mean of nothing, for a norm that is taken, else 0: never what memory held."""
+    import gdn2_amd as G
+
+    x, w = torch.empty(2, 3, 0, device=gpu), torch.empty(0, device=gpu)
+    for _ in range(3):
+        del_me = torch.full((12,), 7.0, device=gpu)  # what the allocator gives out next
+        del del_me
+        o, n, st = G.residual_norm(x, x, None, w if post else None, w if pre else None, return_stats=True)
+        assert st.shape == (2, 3, 2) and o.shape == x.shape
+        for i, taken in enumerate((post, pre)):
+            assert st[..., i].isnan().all() if taken else (st[..., i] == 0).all()
+    r = G.residual_norm_backward(o, x, st, o, o if pre else None, None, w if post else None, w if pre else None)
+    assert r["dx"].shape == r["dy"].shape == x.shape
