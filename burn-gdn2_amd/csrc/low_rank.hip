@@ -800,9 +800,11 @@ __global__ __launch_bounds__(256) void adapter_sums_kernel(SumsParams p) {
     const int64_t n = p.n[which], e = ((int64_t)(ct - which * p.tiles[0]) * kWave + lane) * 4, left = n - e;
     const float *part = p.part[which] + e;
     double sum[4] = {0., 0., 0., 0.};
+    bool any = false; // (the same in every wave)
     for (int b0 = 0; b0 < p.blocks; b0 += kWave) {
         const int b = b0 + lane;
         uint64_t mine = __ballot(b < p.blocks && p.adapter[b < p.blocks ? b : 0] == l);
+        any |= mine != 0;
         while (mine) {
             int at[8], count = 0;
 #pragma unroll
@@ -834,7 +836,7 @@ __global__ __launch_bounds__(256) void adapter_sums_kernel(SumsParams p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const double t = (sum[j] + red[0][lane][j]) + (red[1][lane][j] + red[2][lane][j]);
-        v[j] = (float)(which && p.scale && t != 0. ? p.scale[l] * t : t); // (no rows: 0)
+        v[j] = (float)(which && p.scale && any ? p.scale[l] * t : t); // (no rows: 0)
     }
     store_part<float, 4>(p.out[which] + l * n + e, left, v);
 }

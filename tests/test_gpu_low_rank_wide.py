@@ -137,3 +137,25 @@ def test_infinite_products(gpu, ty, R):
     keep = torch.ones(2, 20, dtype=torch.bool, device=gpu)
     keep[0, 2] = False
     assert got["dx"][keep].isfinite().all()
+
+
+@pytest.mark.parametrize("ty", [F32, BF])
+@pytest.mark.parametrize("R", [8, 100])
+def test_scales_that_are_not_finite(gpu, ty, R):
+    """db is the scale times a sum, of zero too; an adapter without requests has zeros,
+    whatever its scale."""
+    import gdn2_amd as G
+
+    t = make(gpu, 3, 40, 96, 80, R, 3, ty)
+    t["ids"].copy_(torch.tensor([0, 2, 0]))
+    t["d_out"][..., 3] = 0
+    hidden = torch.randn(3, 40, R, device=gpu)
+    grads = lambda: G.low_rank_add_backward(t["x"], t["a"], t["b"], t["ids"], hidden, t["d_out"], t["scale"])  # noqa: E731
+    ref = grads()
+    t["scale"][0], t["scale"][1] = float("inf"), float("nan")
+    got = grads()
+    want = ref["db"].sign() * float("inf")
+    want[:, :, 3] = float("nan")
+    assert torch.equal(got["db"][0].nan_to_num(nan=7.0), want[0].nan_to_num(nan=7.0))
+    assert (got["db"][1] == 0).all() and (got["da"][1] == 0).all()
+    assert all(torch.equal(got[k][2], ref[k][2]) for k in ("da", "db")) and torch.equal(got["dx"][1], ref["dx"][1])
