@@ -528,8 +528,8 @@ Held held_of(int64_t C, int vec) {
 }
 
 // Workgroups for each gate row of the backward: 768 in all, three a compute unit, while
-// each has rows (8192 x 2048 bfloat16: 59.7 us; 1024: 60.2, 512: 61; 4 x 1999 x 320 f32:
-// 27.8, 35 and 27.5), and enough that no f32 sum runs over more than kMostRows.
+// each has rows (8192 x 2048 bfloat16: 57.4 us; 1024: 58.0, 512: 60.0; 4 x 1999 x 320 f32:
+// 27.5, 30.0 and 27.8), and enough that no f32 sum runs over more than kMostRows.
 int64_t blocks_of(int64_t seg_rows, int64_t segs, const Held &h) {
     const int64_t most = (seg_rows + h.rows - 1) / h.rows;
     const int64_t least = (seg_rows + (int64_t)h.rows * kMostRows - 1) / ((int64_t)h.rows * kMostRows);

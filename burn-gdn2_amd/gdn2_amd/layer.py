@@ -309,8 +309,8 @@ class Gdn2Adapters:
     "q_proj", "k_proj", "b_proj", "v_proj", "w_proj", "f_proj_0", "g_proj_0" or
     "o_proj" to (a [L, R, in], b [L, R, out]), float32 device tensors (kept, not
     copied, where contiguous; R at most 64, the same L for all), scale [L] or None
-    (1).  A request with adapter l sees the weight W + scale_l a_l^T b_l.  A captured
-    graph reads the tensors at every replay: keep this object as long as the graph."""
+    (1).  A request with adapter l sees the weight W + scale_l a_l^T b_l (in
+    `forward`; `forward_train` and `backward` take no adapters).  A captured graph reads the tensors at every replay: keep this object as long as the graph."""
     NAMES = ("q_proj", "k_proj", "b_proj", "v_proj", "w_proj", "f_proj_0", "g_proj_0", "o_proj")
 
     def __init__(self, layer: "GatedDeltaNet2", weights: dict, scale=None):

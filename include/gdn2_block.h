@@ -48,8 +48,9 @@ typedef struct gdn2_dropout {
  * holds).  x, y: rows of C channels, `stride_x` and `stride_y` apart.  y may be x with
  * the same stride and must not overlap it otherwise.  The gradient of x for dy is
  * the same call on dy.
- * Limits (else GDN2_NOT_APPLICABLE): C < 2^31, rows ceil(C / 4) < 2^32 unless C
- * is a multiple of 8 and the rows lie together. */
+ * Limits (else GDN2_NOT_APPLICABLE): C < 2^31, rows < 2^40; where C is a multiple of 8
+ * and the rows lie together, rows C <= 2^34 - 2^10 in f32 and 2^35 - 2^11 in bf16;
+ * elsewhere rows ceil(C / 4) < 2^32 - 2^8. */
 GDN2_API gdn2_status gdn2_dropout_f32(const void *x, void *y, int64_t rows, int64_t channels, int64_t stride_x,
                                       int64_t stride_y, const gdn2_dropout *drop, gdn2_stream_t stream);
 GDN2_API gdn2_status gdn2_dropout_bf16(const void *x, void *y, int64_t rows, int64_t channels, int64_t stride_x,
@@ -122,7 +123,10 @@ GDN2_API gdn2_status gdn2_residual_norm_f32_bf16(const gdn2_residual_norm_args *
  * those in f64 (of a workgroup's rows, rounded to f32, and of all workgroups).
  * Limits besides (else GDN2_NOT_APPLICABLE): N S < 2^28; where samples have a gate each,
  * N < 2^21 and N ceil(C / 32) < 2^23.
- * workspace: gdn2_residual_norm_bwd_workspace_bytes(args) bytes, 256-byte aligned. */
+ * workspace: gdn2_residual_norm_bwd_workspace_bytes(args) bytes, 256-byte aligned: a row
+ * of C f32 a workgroup for each weight and for a gate that rows share.  Workgroups: up to
+ * 768, more only for more than 98304 rows; where samples have a gate each, at least one a
+ * sample (32768 samples of two rows of 2048 channels, both weights: 805 MB). */
 typedef struct gdn2_residual_norm_bwd_args {
     gdn2_residual_norm_args fwd;
     const void *d_out, *d_normed;

@@ -161,7 +161,8 @@ GDN2_API gdn2_status gdn2_layer_forward_f32(gdn2_layer *layer, const float *x, i
  *          and o_proj: a [L, rank, in], b [L, rank, out] contiguous in device memory, owned
  *          by the caller (gdn2_low_rank_add_f32 of gdn2_block.h)
  *   ids    device, int32, [batch];  scale  device, [num_adapters], or NULL (1)
- * GDN2_NOT_APPLICABLE for more than 64 ranks. */
+ * GDN2_NOT_APPLICABLE for more than 64 ranks.  The training calls and
+ * gdn2_layer_backward_f32 take no adapters. */
 typedef struct gdn2_layer_adapter {
     const char *name;
     const float *a, *b;

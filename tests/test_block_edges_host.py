@@ -77,3 +77,13 @@ def test_strides_of_dimensions_of_one_do_not_count():
             f(*args, **kw)
     with pytest.raises(ValueError):  # still refused: another place of the same memory
         G.dropout(buf[..., :8], 0.5, out=_one(buf[..., 4:], 32, 5, 1)[..., :8])
+
+
+def test_limits_of_dropout():
+    """Rows that lie together: from 2^24 workgroups of 1024 (f32) or 2048 (bf16) elements on."""
+    L = C.lib()
+    half = C.Dropout(0.5, 0, 0, None)
+    for fn, per in ((L.gdn2_dropout_f32, 1024), (L.gdn2_dropout_bf16, 2048)):
+        for rows, ch in (((1 << 24) * per // 2048, 2048), (((1 << 24) - 1) * per // 8 + 1, 8), ((1 << 40), 8)):
+            assert fn(256, 512, rows, ch, ch, ch, half, None) == C.GDN2_NOT_APPLICABLE
+        assert fn(256, 512, (1 << 32) - 256, 4, 8, 8, half, None) == C.GDN2_NOT_APPLICABLE  # counters of rows apart
